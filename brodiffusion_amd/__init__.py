@@ -25,6 +25,8 @@ from .ops import (  # noqa: F401
     headnorm_rope,
     add_inplace_row_bias,
     add_inplace_vec,
+    add_rms_norm,
+    add_rms_norm_int8,
     attention_map_avg,
     fused_linear_geglu,
     fused_linear_geglu_int8w,
@@ -34,7 +36,9 @@ from .ops import (  # noqa: F401
     linear_attention_relu_forward,
     linear_attention_relu_forward_static_scratch,
     linear_attention_relu_forward_channel_major,
+    linear_act,
     linear_batched,
+    quantize_rows_int8,
     qwen_rope_positions,
     rms_norm_rows,
     rope_apply,
@@ -51,5 +55,5 @@ __all__ = [
     "flash_attention_windowed_forward", "gqa_attention_masked", "joint_attention",
     "linear_attention_relu_forward", "linear_attention_relu_forward_static_scratch", "linear_attention_relu_forward_channel_major", "rope_apply", "flash_attention_qkvo_forward", "flash_attention_q_with_kv_cached_forward",
     "flash_attention_project_kv", "flash_attention_scratch_bytes", "linear_batched", "headnorm_rope", "flash_attention_varlen_forward", "flash_attention_qkvo_int8w_fp16", "flash_attention_q_with_kv_cached_int8w_fp16",
-    "flash_attention_project_kv_int8w_fp16", "linear_forward_batched_int8w_fp16", "fused_linear_geglu", "fused_linear_geglu_int8w", "add_inplace_vec", "add_inplace_row_bias", "joint_attention_traced", "cross_attention_forward_with_attn", "mha_forward", "attention_map_avg", "scale_rows", "rope_apply_perhead", "rms_norm_rows", "sana_self_attention", "sdpa_forward", "set_sdpa_kernel_choice",
+    "flash_attention_project_kv_int8w_fp16", "linear_forward_batched_int8w_fp16", "fused_linear_geglu", "fused_linear_geglu_int8w", "add_inplace_vec", "add_inplace_row_bias", "joint_attention_traced", "cross_attention_forward_with_attn", "mha_forward", "attention_map_avg", "scale_rows", "rope_apply_perhead", "rms_norm_rows", "add_rms_norm", "add_rms_norm_int8", "quantize_rows_int8", "linear_act", "sana_self_attention", "sdpa_forward", "set_sdpa_kernel_choice",
 ]

@@ -21,6 +21,7 @@ MI_LINEAR_ATTN_STATIC_SCRATCH_BYTES = 16 * 1024 * 1024
 MI_LINEAR_ATTN_FORM_BY_SIZE = 0
 MI_LINEAR_ATTN_FORM_THREE_LAUNCHES = 1
 MI_LINEAR_ATTN_FORM_ONE_LAUNCH = 2
+MI_ACT_NONE, MI_ACT_GELU, MI_ACT_GELU_TANH, MI_ACT_SILU = 0, 1, 2, 3
 MI_LAYOUT_TOKEN_MAJOR = 0
 MI_LAYOUT_CHANNEL_MAJOR = 1
 
@@ -142,6 +143,35 @@ class MiLinearArgs(C.Structure):
     ]
 
 
+class MiAddRmsNormArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("gain", C.c_void_p),
+        ("sum_out", C.c_void_p), ("out", C.c_void_p), ("out_q", C.c_void_p), ("out_scales", C.c_void_p),
+        ("rows", C.c_int32), ("cols", C.c_int32),
+        ("x_row_stride", C.c_int64), ("residual_row_stride", C.c_int64), ("sum_row_stride", C.c_int64),
+        ("out_row_stride", C.c_int64), ("q_row_stride", C.c_int64), ("eps", C.c_float), ("stream", C.c_void_p),
+    ]
+
+
+class MiQuantizeRowsArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("x", C.c_void_p), ("out_q", C.c_void_p), ("out_scales", C.c_void_p),
+        ("rows", C.c_int32), ("cols", C.c_int32), ("x_row_stride", C.c_int64), ("q_row_stride", C.c_int64), ("stream", C.c_void_p),
+    ]
+
+
+class MiLinearActArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+        ("rows", C.c_int32), ("in_features", C.c_int32), ("out_features", C.c_int32),
+        ("x_row_stride", C.c_int64), ("w_row_stride", C.c_int64), ("residual_row_stride", C.c_int64), ("y_row_stride", C.c_int64),
+        ("x_scales", C.c_void_p), ("w_scales", C.c_void_p), ("activation", C.c_int32), ("stream", C.c_void_p),
+    ]
+
+
 class MiAttnBlockArgs(C.Structure):
     _fields_ = [
         ("struct_size", C.c_uint32), ("dtype", C.c_int32),
@@ -209,6 +239,9 @@ def lib() -> C.CDLL:
         L.mi_rms_norm_forward.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.c_float,
                                           C.c_int32, C.c_void_p]
         L.mi_rms_norm_pair_forward.argtypes = [C.c_void_p] * 6 + [C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.c_float, C.c_int32, C.c_void_p]
+        L.mi_add_rms_norm_forward.argtypes = [C.POINTER(MiAddRmsNormArgs)]
+        L.mi_quantize_rows_forward.argtypes = [C.POINTER(MiQuantizeRowsArgs)]
+        L.mi_linear_act_forward.argtypes = [C.POINTER(MiLinearActArgs)]
         L.mi_flash_attention_scratch_bytes.argtypes = [C.c_int32] * 5
         L.mi_flash_attention_scratch_bytes.restype = C.c_size_t
         L.mi_attn_block_scratch_bytes.argtypes = [C.POINTER(MiAttnBlockArgs)]

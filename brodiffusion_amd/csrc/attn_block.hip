@@ -42,7 +42,7 @@ int check_common(const mi_attn_block_args* a, const char* op, BlockDims& d, bool
 }
 
 LinearProblem problem(const void* x, const void* w, const void* bias, void* y, long M, int N, int K, const float* w_scale = nullptr) {
-    LinearProblem p;
+    LinearProblem p{};
     p.x = x; p.w = w; p.bias = bias; p.y = y;
     p.w_scale = w_scale;
     p.M = static_cast<int>(M); p.N = N; p.K = K;

@@ -154,6 +154,11 @@ struct LinearProblem {
     const float* w_scale;   // non-null: w is INT8 (N, K) with one FP32 scale per row, Y = (X Wq^T) * scale + bias
     int M, N, K;
     long ldx, ldw, ldy;
+    // What launch_linear_act adds: Y = act(X W^T [* w_scale] [* x_scale] + bias) + residual.
+    const void* residual;   // (M, N) of the type of Y, or null
+    const float* x_scale;   // non-null: x and w are INT8 with a scale per row each; K, ldx and ldw are then in pairs of elements (two bytes)
+    long ldr;
+    int act;                // MI_ACT_*
 };
 constexpr int kMaxLinearProblems = 3;
 struct LinearBatch { LinearProblem p[kMaxLinearProblems]; };
@@ -165,6 +170,9 @@ int launch_linear(const LinearBatch& batch, int n_problems, int dtype, hipStream
 bool linear_pipe_takes(const LinearBatch& batch, int n_problems, bool geglu);
 int launch_linear_pipe(const LinearBatch& batch, int n_problems, int dtype, bool geglu, hipStream_t stream);
 int launch_linear_dma(const LinearBatch& batch, int n_problems, int dtype, hipStream_t stream);
+// One problem with an epilogue (linear_act.hip); its form with tiles through registers (linear.hip).
+int launch_linear_act(const LinearProblem& p, int dtype, hipStream_t stream);
+int launch_linear_act_tiles(const LinearProblem& p, int dtype, hipStream_t stream);
 
 // Cross-attention to cached keys with its query projection in the same launch (sdpa_small.hip): p.q is not read, q projects batch * Lq
 // rows to H * head_dim columns (q.y is not written).

@@ -92,10 +92,12 @@ __device__ __forceinline__ void store_tile_int8(const u32x2 (&raw)[ROWS / 32], c
 // GEGLU with W8 (2 N scales): the reference composes this one from its INT8-weight linear layer and a GEGLU pass over a
 // 16-bit (M, 2 N) buffer (src/fused_transformer.cu:360-396); here the two halves are rounded to T at the same point,
 // in registers, so the result is the composition's without the buffer.
-template <typename T, int BM, int BN, bool GEGLU, bool W8, int WM = 2, int WN = 2>
+// ACT: the epilogue of launch_linear_act; A: the operands' type where it is not that of Y.
+template <typename T, int BM, int BN, bool GEGLU, bool W8, int WM = 2, int WN = 2, typename A = T, bool ACT = false>
 struct TileMath {
-    using M = Mma<T>;
-    using V4 = typename M::v4;
+    using M = Mma<A>;
+    using V4 = typename Mma<T>::v4;
+    using Sum = typename M::sum16;
     static constexpr int NT = 64 * WM * WN;                       // threads: WM x WN wavefronts over tokens x features
     static constexpr int TM = BM / (32 * WM), TN = BN / (32 * WN);  // 32 x 32 blocks per wavefront along tokens / features
     static_assert(!GEGLU || TN == 2, "the GEGLU form pairs the two feature blocks of a wavefront");
@@ -109,13 +111,13 @@ struct TileMath {
         const int lane = tid & 63, wave = tid >> 6;
         lq = lane & 31; lh = lane >> 5; wm = wave % WM; wn = wave / WM;
     }
-    static __device__ __forceinline__ void clear(f32x16 (&acc)[TN][TM]) {
+    static __device__ __forceinline__ void clear(Sum (&acc)[TN][TM]) {
 #pragma unroll
         for (int a = 0; a < TN; ++a)
 #pragma unroll
             for (int b = 0; b < TM; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+                for (int e = 0; e < 16; ++e) acc[a][b][e] = 0;
     }
     // The bias of this lane's features of the tile at feature n0, requested long before the epilogue (there each of these
     // loads would be a memory latency of its own). Straight-line code: lanes without a bias read the first bytes of W and
@@ -136,7 +138,7 @@ struct TileMath {
             }
     }
     // the four k-substeps of 16 of one step for every 32 x 32 block of this wavefront, operands from the LDS tile pair at `cur`
-    __device__ __forceinline__ void multiply(f32x16 (&acc)[TN][TM], const char* cur) const {
+    __device__ __forceinline__ void multiply(Sum (&acc)[TN][TM], const char* cur) const {
         const char* xs = cur + (wm * TM * 32 + lq) * kRowBytes + lh * 16;
         const char* ws = cur + X_BYTES + (wn * TN * 32 + lq) * kRowBytes + lh * 16;
 #pragma unroll
@@ -156,9 +158,40 @@ struct TileMath {
     // The results leave through LDS (`stage`, kOutBytes, not in use by anything else): a lane holds 4 features of one token
     // per group, and written from there a wavefront's store instruction would touch 32 rows of Y with 16 bytes each.
     // Staged, consecutive threads write consecutive 16-byte pieces of a row.
-    __device__ __forceinline__ void write_tile(const f32x16 (&acc)[TN][TM], const V4 (&braw)[TN][4], const LinearProblem& p, char* stage,
+    __device__ __forceinline__ void write_tile(const Sum (&acc)[TN][TM], const V4 (&braw)[TN][4], const LinearProblem& p, char* stage,
                                                int m0, int n0) const {
-        if constexpr (GEGLU) {
+        if constexpr (ACT) {
+            // The residual is read here, each value by the lane that adds it, ahead of the barrier behind which the work group writes
+            // the tile: y may be the residual.
+            constexpr bool A8 = std::is_same_v<A, Int8>;
+#pragma unroll
+            for (int b = 0; b < TM; ++b) {
+                const int token = min(m0 + (wm * TM + b) * 32 + lq, p.M - 1);
+                const float sx = A8 ? p.x_scale[token] : 1.f;
+#pragma unroll
+                for (int a = 0; a < TN; ++a)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int feat = (wn * TN + a) * 32 + 8 * g + 4 * lh, f = min(n0 + feat, p.N - 4);
+                        float v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float sum = static_cast<float>(acc[a][b][4 * g + i]), bias = static_cast<float>(braw[a][g][i]);
+                            v[i] = A8 || W8 ? scaled_acc(sum, sx * p.w_scale[f + i], bias) : sum + bias;
+                        }
+                        with_activation(p.act, [&](auto act) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] = act(v[i]);
+                        });
+                        V4 r{};
+                        if (p.residual != nullptr) r = *reinterpret_cast<const V4*>(static_cast<const T*>(p.residual) + static_cast<long>(token) * p.ldr + f);
+                        V4 o;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[i] = static_cast<T>(v[i] + static_cast<float>(r[i]));
+                        *reinterpret_cast<V4*>(stage + ((wm * TM + b) * 32 + lq) * kOutRow + feat * 2) = o;
+                    }
+            }
+        } else if constexpr (GEGLU) {
             // acc[0] = value, acc[1] = gate of features n0 + wn*32 + 8g + 4*lh + i
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -234,9 +267,9 @@ struct TileMath {
 };
 
 // One work group per output tile, one contraction step prefetched while the previous one is multiplied.
-template <typename T, int BM, int BN, bool GEGLU = false, bool W8 = false>
+template <typename T, int BM, int BN, bool GEGLU = false, bool W8 = false, typename A = T, bool ACT = false>
 __global__ __launch_bounds__(kThreads) void linear_kernel(const LinearBatch batch) {
-    using TM_ = TileMath<T, BM, BN, GEGLU, W8>;
+    using TM_ = TileMath<T, BM, BN, GEGLU, W8, 2, 2, A, ACT>;
     constexpr int TM = TM_::TM, TN = TM_::TN, BN_OUT = TM_::BN_OUT, X_BYTES = TM_::X_BYTES, W_BYTES = TM_::W_BYTES;
     static_assert(TM_::kOutBytes <= 2 * (X_BYTES + W_BYTES), "the staged output fits the operand buffers");
     extern __shared__ __attribute__((aligned(16))) char lds[];  // [2][X tile ; W tile]
@@ -252,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void linear_kernel(const LinearBatch batc
     const char* xg = static_cast<const char*>(p.x);
     const char* wg = static_cast<const char*>(p.w);
 
-    f32x16 acc[TN][TM];
+    typename TM_::Sum acc[TN][TM];
     TM_::clear(acc);
     typename TM_::V4 braw[TN][4];
     tm.request_bias(braw, p, n0);
@@ -292,7 +325,7 @@ __global__ __launch_bounds__(kThreads) void linear_kernel(const LinearBatch batc
     tm.write_tile(acc, braw, p, lds, m0, n0);
 }
 
-template <typename T, int BM, int BN, bool GEGLU = false, bool W8 = false>
+template <typename T, int BM, int BN, bool GEGLU = false, bool W8 = false, typename A = T, bool ACT = false>
 int launch_tiles(const LinearBatch& batch, int n_problems, hipStream_t st) {
     constexpr int BN_OUT = GEGLU ? BN / 2 : BN;
     int max_tiles = 0;
@@ -304,7 +337,7 @@ int launch_tiles(const LinearBatch& batch, int n_problems, hipStream_t st) {
     static_assert(lds <= 160 * 1024, "operand ring exceeds the LDS of a compute unit");
     // (launched by name: a launch through a pointer variable is dropped by this compiler when the host code is built with
     // -fsanitize=undefined)
-    const void* const kern = reinterpret_cast<const void*>(&linear_kernel<T, BM, BN, GEGLU, W8>);
+    const void* const kern = reinterpret_cast<const void*>(&linear_kernel<T, BM, BN, GEGLU, W8, A, ACT>);
     if (lds > 64 * 1024) {
         static thread_local bool raised = false;
         if (!raised) {
@@ -312,7 +345,7 @@ int launch_tiles(const LinearBatch& batch, int n_problems, hipStream_t st) {
             raised = true;
         }
     }
-    hipLaunchKernelGGL((linear_kernel<T, BM, BN, GEGLU, W8>), dim3(max_tiles, n_problems), dim3(kThreads), lds, st, batch);
+    hipLaunchKernelGGL((linear_kernel<T, BM, BN, GEGLU, W8, A, ACT>), dim3(max_tiles, n_problems), dim3(kThreads), lds, st, batch);
     MI_HIP_CHECK(hipGetLastError());
     return 0;
 }
@@ -337,7 +370,21 @@ int launch_t(const LinearBatch& batch, int n_problems, hipStream_t st, bool gegl
     return w8 ? launch_tiles<T, 64, 64, false, true>(batch, n_problems, st) : launch_tiles<T, 64, 64>(batch, n_problems, st);
 }
 
+template <typename T>
+int launch_act(const LinearBatch& b, hipStream_t st) {
+    const bool big = static_cast<long>((b.p[0].M + 127) / 128) * ((b.p[0].N + 127) / 128) >= 2L * device_cu_count();      // (as in launch_t)
+    if (b.p[0].x_scale != nullptr) return big ? launch_tiles<T, 128, 128, false, false, Int8, true>(b, 1, st) : launch_tiles<T, 64, 64, false, false, Int8, true>(b, 1, st);
+    if (b.p[0].w_scale != nullptr) return big ? launch_tiles<T, 128, 128, false, true, T, true>(b, 1, st) : launch_tiles<T, 64, 64, false, true, T, true>(b, 1, st);
+    return big ? launch_tiles<T, 128, 128, false, false, T, true>(b, 1, st) : launch_tiles<T, 64, 64, false, false, T, true>(b, 1, st);
+}
+
 }  // namespace gemm
+
+int launch_linear_act_tiles(const LinearProblem& p, int dtype, hipStream_t st) {
+    LinearBatch b{};
+    b.p[0] = p;
+    return dtype == MI_DTYPE_BF16 ? gemm::launch_act<__bf16>(b, st) : gemm::launch_act<_Float16>(b, st);
+}
 
 int launch_linear(const LinearBatch& batch, int n_problems, int dtype, hipStream_t st, bool geglu) {
     if (geglu && n_problems != 1) return fail("linear: the GEGLU form takes one problem per launch");

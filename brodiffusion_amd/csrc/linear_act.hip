@@ -1,0 +1,53 @@
+// Y = act(X W^T [* w_scales] [* x_scales] + bias) + residual: the linear layer with its epilogue, for 16-bit operands, INT8 weights
+// (W8A16) and INT8 operands (W8A8).
+#include "internal.h"
+
+namespace mi {
+
+int launch_linear_act(const LinearProblem& p, int dtype, hipStream_t st) { return launch_linear_act_tiles(p, dtype, st); }
+
+namespace {
+
+int linear_act(const mi_linear_act_args& a) {
+    const char* op = "mi_linear_act_forward";
+    if (a.dtype != MI_DTYPE_BF16 && a.dtype != MI_DTYPE_F16) return fail("%s: dtype %d is neither MI_DTYPE_F16 nor MI_DTYPE_BF16", op, a.dtype);
+    if (a.rows < 0 || a.in_features <= 0 || a.out_features <= 0) return fail("%s: %d rows, %d x %d features", op, a.rows, a.in_features, a.out_features);
+    if (a.activation < MI_ACT_NONE || a.activation > MI_ACT_SILU) return fail("%s: activation %d is none of MI_ACT_*", op, a.activation);
+    const bool a8 = a.x_scales != nullptr;
+    if (a8 && !a.w_scales) return fail("%s: INT8 rows need INT8 weights (w_scales)", op);
+    const int step = a8 ? 16 : 8;
+    if (a.in_features % step || a.out_features % 8) return fail("%s: in_features %d must be a multiple of %d, out_features %d of 8", op, a.in_features, step, a.out_features);
+    // 128 * 128 * in_features stays below 2^31
+    if (a8 && a.in_features > 131056) return fail("%s: in_features %d exceed the 131056 whose INT32 sums are exact", op, a.in_features);
+    if (a.rows == 0) return 0;
+    if (!a.x || !a.w || !a.y) return fail("%s: null operand", op);
+    LinearProblem p{};
+    p.x = a.x; p.w = a.w; p.bias = a.bias; p.y = a.y; p.residual = a.residual;
+    p.w_scale = a.w_scales; p.x_scale = a.x_scales; p.act = a.activation;
+    p.M = a.rows; p.N = a.out_features; p.K = a.in_features;
+    p.ldx = a.x_row_stride ? a.x_row_stride : a.in_features;
+    p.ldw = a.w_row_stride ? a.w_row_stride : a.in_features;
+    p.ldy = a.y_row_stride ? a.y_row_stride : a.out_features;
+    p.ldr = a.residual_row_stride ? a.residual_row_stride : a.out_features;
+    if (p.ldx % step || p.ldw % step || p.ldy % 8 || p.ldr % 8) return fail("%s: row strides must be multiples of 8 elements (INT8 rows and their weights: of 16)", op);
+    if (p.ldx < p.K || p.ldw < p.K || p.ldy < p.N || (p.residual && p.ldr < p.N)) return fail("%s: a row stride is smaller than the row", op);
+    uintptr_t al = 0;
+    for (const void* q : {p.x, p.w, p.bias, p.residual, static_cast<const void*>(p.y)}) al |= reinterpret_cast<uintptr_t>(q);
+    if (al & 15u) return fail("%s: operands must be 16-byte aligned", op);
+    if ((reinterpret_cast<uintptr_t>(p.x_scale) | reinterpret_cast<uintptr_t>(p.w_scale)) & 3u) return fail("%s: scales must be 4-byte aligned", op);
+    if (p.residual && !(p.residual == p.y && p.ldr == p.ldy) && operands_overlap(p.residual, p.ldr, 0, p.y, p.ldy, 0, 1, p.M, p.N))
+        return fail("%s: y overlaps the residual", op);
+    if (static_cast<long>((p.M + 31) / 32) * ((p.N + 31) / 32) > 0x7ffffff0L) return fail("%s: problem too large for one launch", op);
+    if (a8) { p.K /= 2; p.ldx /= 2; p.ldw /= 2; }      // rows of pairs (LinearProblem::x_scale)
+    return launch_linear_act(p, a.dtype, resolve_stream(a.stream));
+}
+
+}  // namespace
+}  // namespace mi
+
+extern "C" int mi_linear_act_forward(const mi_linear_act_args* a) {
+    mi::clear_error();
+    if (!a) return mi::fail("mi_linear_act_forward: null args");
+    if (a->struct_size != sizeof(*a)) return mi::fail("mi_linear_act_forward: struct_size %u != %zu (header mismatch)", a->struct_size, sizeof(*a));
+    return mi::linear_act(*a);
+}

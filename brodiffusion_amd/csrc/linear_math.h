@@ -14,10 +14,16 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+// Operands as 16-byte pieces of rows: 8 values of a 16-bit type, or 16 INT8. Products of either kind take the same bytes in the same time.
+struct Int8 {};
 template <typename T> struct Mma;
 template <> struct Mma<__bf16> {
     using v8 = bf16x8;
+    using sum4 = f32x4;
+    using sum16 = f32x16;
     using v4 = bf16x4;
     static __device__ __forceinline__ f32x16 run(v8 a, v8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -28,6 +34,8 @@ template <> struct Mma<__bf16> {
 };
 template <> struct Mma<_Float16> {
     using v8 = f16x8;
+    using sum4 = f32x4;
+    using sum16 = f32x16;
     using v4 = f16x4;
     static __device__ __forceinline__ f32x16 run(v8 a, v8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -35,6 +43,14 @@ template <> struct Mma<_Float16> {
     static __device__ __forceinline__ f32x4 run16(v8 a, v8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
+};
+
+template <> struct Mma<Int8> {
+    using v8 = i32x4;
+    using sum4 = i32x4;
+    using sum16 = i32x16;
+    static __device__ __forceinline__ i32x16 run(v8 a, v8 b, i32x16 c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ i32x4 run16(v8 a, v8 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
 
 // x * Phi(x), the erf form of GELU (gelu_exact_scalar, src/fused_transformer.cu:89-92), branch free. With z = |x| / sqrt 2,
@@ -71,6 +87,21 @@ __device__ __forceinline__ float scaled_acc(float acc, float scale, float bias) 
     float r = __builtin_fmaf(acc, scale, bias);
     asm volatile("" : "+v"(r));
     return r;
+}
+
+// x / (1 + exp(-x)); exp(-x) = inf far on the left gives -0
+__device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504f)); }
+// The tanh form of GELU, x (1 + tanh u) / 2 with u = sqrt(2 / pi) (x + 0.044715 x^3), as x / (1 + exp(-2 u)): the constants are
+// -2 sqrt(2 / pi) log2 e and 0.044715 times that. Where x^3 overflows the factor is 0 or 1, as it should be.
+__device__ __forceinline__ float gelu_tanh(float x) {
+    const float u = x * __builtin_fmaf(x * x, -0.102943237f, -2.30220818f);
+    return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u));
+}
+// f(activation function) for the one that `kind` names, which is the same for the whole launch: one branch around a lane's values
+template <typename F> __device__ __forceinline__ void with_activation(int kind, F f) {
+    if (kind == MI_ACT_GELU) f([](float x) { return gelu_erf(x); });
+    else if (kind == MI_ACT_GELU_TANH) f([](float x) { return gelu_tanh(x); });
+    else if (kind == MI_ACT_SILU) f([](float x) { return silu(x); });
 }
 
 // 8 INT8 weights -> 8 values of T, exactly

@@ -287,6 +287,89 @@ void linear_forward_batched_int8w_fp16(const Tensor& W_int8, const Tensor& scale
 }
 
 namespace {
+void fit(Tensor& t, int rows, int cols, Dtype dt, Device dev) {
+    if (t.data == nullptr || t.rows != rows || t.cols != cols || t.dtype != dt) t.resize(rows, cols, dt, dev);
+}
+const float* scales_ptr(const char* op, const Tensor* s, const char* name, int n) {
+    if (s == nullptr) return nullptr;
+    need_gpu(op, *s);
+    if (s->dtype != Dtype::FP32 || s->size() != static_cast<std::size_t>(n)) fail(std::string(op) + ": " + name + " must hold " + std::to_string(n) + " FP32 values");
+    return static_cast<const float*>(s->data);
+}
+void add_rms_norm_impl(const char* op, const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out, Tensor* scales) {
+    need_gpu(op, X); need_gpu(op, gain);
+    if (gain.dtype != X.dtype || gain.size() != static_cast<std::size_t>(X.cols)) fail(std::string(op) + ": gain must hold one value of X's dtype per column");
+    mi_add_rms_norm_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.dtype = dtype_code(op, X.dtype);
+    a.x = X.data; a.gain = gain.data; a.eps = eps;
+    a.rows = X.rows; a.cols = X.cols;
+    if (residual != nullptr) {
+        need_gpu(op, *residual);
+        if (residual->dtype != X.dtype || residual->rows != X.rows || residual->cols != X.cols) fail(std::string(op) + ": the residual must have X's shape and dtype");
+        fit(sum, X.rows, X.cols, X.dtype, X.device);
+        a.residual = residual->data; a.sum_out = sum.data;
+    }
+    fit(out, X.rows, X.cols, scales ? Dtype::INT8 : X.dtype, X.device);
+    if (scales != nullptr) {
+        fit(*scales, X.rows, 1, Dtype::FP32, X.device);
+        a.out_q = out.data; a.out_scales = static_cast<float*>(scales->data);
+    } else {
+        a.out = out.data;
+    }
+    check(op, mi_add_rms_norm_forward(&a));
+}
+}  // namespace
+
+void linear_act(const Tensor& X, const Tensor* x_scales, const Tensor& W, const Tensor* w_scales, const Tensor* bias, Activation activation,
+                const Tensor* residual, Tensor& Y) {
+    const char* op = "linear_act";
+    need_gpu(op, X); need_gpu(op, W);
+    const Dtype dt = x_scales == nullptr ? X.dtype : residual ? residual->dtype : bias ? bias->dtype : Y.dtype;
+    if (x_scales != nullptr && w_scales == nullptr) fail(std::string(op) + ": INT8 rows need INT8 weights (w_scales)");
+    if (X.dtype != (x_scales ? Dtype::INT8 : dt) || W.dtype != (w_scales ? Dtype::INT8 : dt)) fail(std::string(op) + ": X and W must be INT8 where they have scales, of Y's dtype otherwise");
+    if (W.cols != X.cols) fail(std::string(op) + ": X and W must have the same columns");
+    mi_linear_act_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.dtype = dtype_code(op, dt);
+    a.x_scales = scales_ptr(op, x_scales, "x_scales", X.rows);
+    a.w_scales = scales_ptr(op, w_scales, "w_scales", W.rows);
+    a.bias = bias_ptr(op, bias, "bias", dt, W.rows);
+    if (residual != nullptr) {
+        need_gpu(op, *residual);
+        if (residual->dtype != dt || residual->rows != X.rows || residual->cols != W.rows) fail(std::string(op) + ": the residual must have Y's shape and dtype");
+        a.residual = residual->data;
+    }
+    fit(Y, X.rows, W.rows, dt, X.device);
+    a.x = X.data; a.w = W.data; a.y = Y.data;
+    a.rows = X.rows; a.in_features = X.cols; a.out_features = W.rows;
+    a.activation = static_cast<int>(activation);
+    check(op, mi_linear_act_forward(&a));
+}
+
+void add_rms_norm(const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out) {
+    add_rms_norm_impl("add_rms_norm", X, residual, gain, eps, sum, out, nullptr);
+}
+void add_rms_norm_int8(const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out, Tensor& scales) {
+    add_rms_norm_impl("add_rms_norm_int8", X, residual, gain, eps, sum, out, &scales);
+}
+void quantize_rows_int8(const Tensor& X, Tensor& out, Tensor& scales) {
+    const char* op = "quantize_rows_int8";
+    need_gpu(op, X);
+    mi_quantize_rows_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.dtype = dtype_code(op, X.dtype);
+    fit(out, X.rows, X.cols, Dtype::INT8, X.device);
+    fit(scales, X.rows, 1, Dtype::FP32, X.device);
+    a.x = X.data; a.out_q = out.data; a.out_scales = static_cast<float*>(scales.data);
+    a.rows = X.rows; a.cols = X.cols;
+    check(op, mi_quantize_rows_forward(&a));
+}
+
+namespace {
 struct Scales { const Tensor* q; const Tensor* k; const Tensor* v; const Tensor* o; };
 void qkvo_impl(const char* op, const Tensor& X, const Tensor* Ctx, const Tensor& Wq, const Tensor* bq, const Tensor& Wk,
                const Tensor* bk, const Tensor& Wv, const Tensor* bv, const Tensor& Wo, const Tensor* bo, const float* d_mask,

@@ -61,6 +61,20 @@ void linear_attention_relu_forward_channel_major(const Tensor& Q, const Tensor& 
 // Y = X W^T + bias, W (out_features, in_features); bias may be null.
 void linear_batched(const Tensor& W, const Tensor* bias, const Tensor& X, Tensor& Y);
 
+// Y = act(X W^T [* w_scales] [* x_scales] + bias) + residual (mi_linear_act_forward). With w_scales (W.rows FP32 values) W is INT8; with
+// x_scales (X.rows) X is INT8 too, as quantize_rows_int8 and add_rms_norm_int8 write it, and Y gets the dtype of the residual, the bias,
+// or, without either, the one that it has. bias, residual and the scales may be null; residual may be Y itself.
+enum class Activation { None = MI_ACT_NONE, Gelu = MI_ACT_GELU, GeluTanh = MI_ACT_GELU_TANH, Silu = MI_ACT_SILU };
+void linear_act(const Tensor& X, const Tensor* x_scales, const Tensor& W, const Tensor* w_scales, const Tensor* bias, Activation activation,
+                const Tensor* residual, Tensor& Y);
+
+// h = X + residual (null: X, and `sum` is left alone) and the RMS normalisation of its rows: `out` of X's dtype, or INT8 rows with an
+// FP32 scale each (mi_add_rms_norm_forward). `sum` and `out` may be X or the residual. quantize_rows_int8: rows as they are
+// (mi_quantize_rows_forward).
+void add_rms_norm(const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out);
+void add_rms_norm_int8(const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out, Tensor& scales);
+void quantize_rows_int8(const Tensor& X, Tensor& out, Tensor& scales);
+
 // Attention with its projections (the U-Net spatial transformer's operators). Weights are (out_features, in_features),
 // biases may be null, Ctx == nullptr is self-attention. The projections and the attention output live in a scratch
 // tensor owned by the calling thread, grown on demand and kept (no allocation after warm-up, as the reference's

@@ -16,6 +16,7 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -40,6 +41,9 @@ struct Lib {
     decltype(&mi_add_inplace) add_inplace;
     decltype(&mi_rms_norm_forward) rms_norm;
     decltype(&mi_rms_norm_pair_forward) rms_norm_pair;
+    decltype(&mi_add_rms_norm_forward) add_rms_norm;
+    decltype(&mi_quantize_rows_forward) quantize_rows;
+    decltype(&mi_linear_act_forward) linear_act;
     decltype(&mi_attn_block_scratch_bytes) block_scratch_bytes;
     decltype(&mi_flash_attention_qkvo_forward) qkvo;
     decltype(&mi_flash_attention_q_with_kv_cached_forward) kv_cached;
@@ -240,6 +244,157 @@ NATIVE(rms_norm, 4)
     void* const stream = current_stream();
     run("rms_norm_rows", [&] { return L.rms_norm(px, pg, py, rows, cols, x_rs, y_rs, eps, dt, stream); });
     return given(a[3], y);
+NATIVE_END
+
+// ── 8-bit rows and the linear layer with an epilogue ──
+// rows along all axes but the last: contiguous, or 2-D with any row stride; returns the stride
+int64_t row_stride(const Tensor& t, at::ScalarType dt) {
+    need(t.scalar_type() == dt && t.dim() >= 1 && t.size(-1) > 0);
+    if (t.is_contiguous()) return t.size(-1);
+    need(t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1));
+    return t.stride(0);
+}
+// `o` of x's leading sizes with `cols` columns, or a new one
+Tensor rows_like(PyObject* o, const Tensor& x, int64_t cols, at::ScalarType dt) {
+    auto sizes = x.sizes().vec();
+    sizes.back() = cols;
+    if (none(o)) return at::empty(sizes, x.options().dtype(dt));
+    const Tensor& t = tensor(o);
+    need(t.sizes() == at::IntArrayRef(sizes));
+    return t;
+}
+Tensor scales_like(PyObject* o, const Tensor& x) {
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    if (none(o)) return at::empty(lead, x.options().dtype(at::kFloat));
+    const Tensor& t = tensor(o);
+    need(t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == x.numel() / x.size(-1));
+    return t;
+}
+PyObject* tuple_of(std::initializer_list<PyObject*> items) {     // takes the references
+    PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(items.size()));
+    Py_ssize_t i = 0;
+    for (PyObject* o : items) {
+        if (t && o) PyTuple_SET_ITEM(t, i++, o);
+        else Py_XDECREF(o);
+    }
+    if (t && i != static_cast<Py_ssize_t>(items.size())) { Py_DECREF(t); return nullptr; }
+    return t;
+}
+
+// X, residual, gain, eps, sum_out, out, scales, int8, op
+NATIVE(add_rms_norm, 9)
+    const Tensor &x = tensor(a[0]), &g = tensor(a[2]);
+    const bool int8 = truth(a[7]);
+    mi_add_rms_norm_args p;
+    std::memset(&p, 0, sizeof(p));
+    p.struct_size = sizeof(p);
+    p.dtype = dtype_code(x);
+    p.x_row_stride = row_stride(x, x.scalar_type());
+    need(g.scalar_type() == x.scalar_type() && g.numel() == x.size(-1) && g.is_contiguous());
+    Tensor sum = x;
+    if (none(a[1])) need(none(a[4]));
+    else {
+        const Tensor& r = tensor(a[1]);
+        need(r.sizes() == x.sizes());
+        p.residual = r.data_ptr(); p.residual_row_stride = row_stride(r, x.scalar_type());
+        sum = rows_like(a[4], x, x.size(-1), x.scalar_type());
+        p.sum_out = sum.data_ptr(); p.sum_row_stride = row_stride(sum, x.scalar_type());
+    }
+    const at::ScalarType dt = int8 ? at::kChar : x.scalar_type();
+    const Tensor y = rows_like(a[5], x, x.size(-1), dt);
+    const int64_t y_rs = row_stride(y, dt);
+    Tensor scales;
+    if (int8) {
+        scales = scales_like(a[6], x);
+        p.out_q = y.data_ptr(); p.q_row_stride = y_rs; p.out_scales = static_cast<float*>(scales.data_ptr());
+    } else {
+        need(none(a[6]));
+        p.out = y.data_ptr(); p.out_row_stride = y_rs;
+    }
+    p.x = x.data_ptr(); p.gain = g.data_ptr(); p.eps = static_cast<float>(number(a[3]));
+    p.rows = rows32(x.numel() / x.size(-1)); p.cols = rows32(x.size(-1));
+    p.stream = current_stream();
+    run(name_of(a[8]), [&] { return L.add_rms_norm(&p); });
+    PyObject* const h = none(a[1]) ? given(a[0], x) : given(a[4], sum);
+    if (int8) return tuple_of({h, given(a[5], y), given(a[6], scales)});
+    return tuple_of({h, given(a[5], y)});
+NATIVE_END
+
+// X, out, scales
+NATIVE(quantize_rows, 3)
+    const Tensor& x = tensor(a[0]);
+    mi_quantize_rows_args p;
+    std::memset(&p, 0, sizeof(p));
+    p.struct_size = sizeof(p);
+    p.dtype = dtype_code(x);
+    p.x_row_stride = row_stride(x, x.scalar_type());
+    const Tensor y = rows_like(a[1], x, x.size(-1), at::kChar), scales = scales_like(a[2], x);
+    p.q_row_stride = row_stride(y, at::kChar);
+    p.x = x.data_ptr(); p.out_q = y.data_ptr(); p.out_scales = static_cast<float*>(scales.data_ptr());
+    p.rows = rows32(x.numel() / x.size(-1)); p.cols = rows32(x.size(-1));
+    p.stream = current_stream();
+    run("quantize_rows_int8", [&] { return L.quantize_rows(&p); });
+    return tuple_of({given(a[1], y), given(a[2], scales)});
+NATIVE_END
+
+int activation_of(PyObject* o) {
+    need(PyUnicode_Check(o));
+    static const char* const names[] = {"none", "gelu", "gelu_tanh", "silu"};      // by MI_ACT_*
+    for (int i = 0; i < 4; ++i)
+        if (PyUnicode_CompareWithASCIIString(o, names[i]) == 0) return i;
+    throw Decline{};
+}
+// X, W, bias, activation, residual, x_scales, w_scales, dtype, out
+NATIVE(linear_act, 9)
+    const Tensor &x = tensor(a[0]), &w = tensor(a[1]);
+    mi_linear_act_args p;
+    std::memset(&p, 0, sizeof(p));
+    p.struct_size = sizeof(p);
+    p.activation = activation_of(a[3]);
+    const bool w8 = !none(a[6]), a8 = !none(a[5]);
+    need(w.dim() == 2 && x.dim() >= 1 && x.size(-1) == w.size(1) && (w8 || !a8));
+    at::ScalarType dt = x.scalar_type();
+    if (none(a[7])) {
+        if (a8) {       // (the type of the first of these that there is)
+            PyObject* const first = !none(a[8]) ? a[8] : !none(a[4]) ? a[4] : a[2];
+            need(!none(first));
+            dt = tensor(first).scalar_type();
+        }
+    } else {
+        need(THPDtype_Check(a[7]));
+        const at::ScalarType asked = reinterpret_cast<THPDtype*>(a[7])->scalar_type;
+        need(a8 || asked == dt);
+        dt = asked;
+    }
+    need(dt == at::kBFloat16 || dt == at::kHalf);
+    p.dtype = dt == at::kBFloat16 ? MI_DTYPE_BF16 : MI_DTYPE_F16;
+    const int64_t n_out = w.size(0), rows = x.numel() / (x.size(-1) > 0 ? x.size(-1) : 1);
+    p.x_row_stride = row_stride(x, a8 ? at::kChar : dt);
+    p.w_row_stride = row_stride(w, w8 ? at::kChar : dt);
+    need(n_out > 0);
+    p.bias = bias_ptr(a[2], dt, n_out);
+    if (w8) {
+        const Tensor& s = tensor(a[6]);
+        need(s.scalar_type() == at::kFloat && s.numel() == n_out && s.is_contiguous());
+        p.w_scales = f32(s);
+    }
+    if (a8) {
+        const Tensor& s = tensor(a[5]);
+        need(s.scalar_type() == at::kFloat && s.numel() == rows && s.is_contiguous());
+        p.x_scales = f32(s);
+    }
+    const Tensor y = rows_like(a[8], x, n_out, dt);
+    p.y_row_stride = row_stride(y, dt);
+    if (!none(a[4])) {
+        const Tensor& r = tensor(a[4]);
+        need(r.sizes() == y.sizes());
+        p.residual = r.data_ptr(); p.residual_row_stride = row_stride(r, dt);
+    }
+    p.x = x.data_ptr(); p.w = w.data_ptr(); p.y = y.data_ptr();
+    p.rows = rows32(rows); p.in_features = rows32(w.size(1)); p.out_features = rows32(n_out);
+    p.stream = current_stream();
+    run("linear_act", [&] { return L.linear_act(&p); });
+    return given(a[8], y);
 NATIVE_END
 
 // ── RoPE ──
@@ -633,7 +788,8 @@ PyObject* bind(PyObject*, PyObject* args) {
     get(L.rms_norm_pair, "mi_rms_norm_pair_forward"); get(L.block_scratch_bytes, "mi_attn_block_scratch_bytes");
     get(L.qkvo, "mi_flash_attention_qkvo_forward"); get(L.kv_cached, "mi_flash_attention_q_with_kv_cached_forward");
     get(L.la_workspace_bytes, "mi_linear_attn_workspace_bytes"); get(L.la_scratch_bytes, "mi_linear_attn_scratch_bytes");
-    get(L.linear_attn, "mi_linear_attn_relu_forward");
+    get(L.linear_attn, "mi_linear_attn_relu_forward"); get(L.add_rms_norm, "mi_add_rms_norm_forward");
+    get(L.quantize_rows, "mi_quantize_rows_forward"); get(L.linear_act, "mi_linear_act_forward");
     if (!ok) return PyErr_Format(PyExc_RuntimeError, "%s does not export every function of mi_attention.h: build the library again", path);
     Py_INCREF(lend);
     Py_XSETREF(lend_scratch, lend);
@@ -642,7 +798,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(linear), FAST(geglu), FAST(add_inplace), FAST(rms_norm), FAST(rope), FAST(headnorm_rope),
+PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(linear), FAST(geglu), FAST(add_inplace), FAST(rms_norm), FAST(add_rms_norm), FAST(quantize_rows), FAST(linear_act), FAST(rope), FAST(headnorm_rope),
                          FAST(sdpa), FAST(joint), FAST(attn_block), FAST(mha), FAST(linear_attn), FAST(sana), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native host path of brodiffusion_amd.ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -19,6 +19,7 @@ Names, argument order and error behaviour follow the brotensor operators the ref
                                                                              src/unet_blocks.cpp:311-317
     flash_attention_project_kv(ctx, Wk, bk, Wv, bv, K_out, V_out)            src/unet.cpp:476-480
     linear_batched(W, bias, X, Y)                                            include/brodiffusion/detail/compute.h:52
+    add_rms_norm, add_rms_norm_int8, quantize_rows_int8, linear_act          no counterpart: 8-bit rows and projections with an epilogue
     fused_linear_geglu(X, W, b, Y), add_inplace_vec(Y, X), add_inplace_row_bias(Y, bias)
                                                                              include/brodiffusion/fused_transformer.h:20-61
 
@@ -1111,6 +1112,161 @@ def rms_norm_rows(X, gain, eps: float, out: Optional[torch.Tensor] = None):
         _fail(op, "out must have X's shape and dtype")
     capi.check(capi.lib().mi_rms_norm_forward(X.data_ptr(), gain.data_ptr(), out.data_ptr(), X.shape[0], X.shape[1], X.stride(0),
                                               out.stride(0), eps, dt, _stream()), op)
+    return out
+
+
+def _rows_of(op: str, t, name: str, dtype, shape=None):
+    """A tensor whose last axis is the columns and whose others are rows: contiguous, or 2-D with any row stride. Returns (rows, row stride)."""
+    _dev(op, t)
+    if t.dtype != dtype:
+        _fail(op, f"{name} has dtype {t.dtype}, expected {dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        _fail(op, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dim() < 1 or t.shape[-1] == 0:
+        _fail(op, f"{name} must have columns")
+    if t.is_contiguous():
+        return t.numel() // t.shape[-1], t.shape[-1]
+    if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        _fail(op, f"{name} must be contiguous, or (rows, cols) and contiguous along columns")
+    return t.shape[0], t.stride(0)
+
+
+def _scales_of(op: str, t, name: str, n: int) -> int:
+    _dev(op, t)
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        _fail(op, f"{name} must hold {n} contiguous float32 values")
+    return t.data_ptr()
+
+
+def _add_rms_norm(op: str, X, residual, gain, eps: float, sum_out, out, scales, int8: bool):
+    r = _native.add_rms_norm(X, residual, gain, eps, sum_out, out, scales, int8, op)
+    if r is not None:
+        return r
+    _dev(op, X, residual, gain, sum_out, out, scales)
+    a = capi.MiAddRmsNormArgs()
+    a.struct_size = C.sizeof(a)
+    a.dtype = _dtype_code(op, X)
+    a.rows, a.x_row_stride = _rows_of(op, X, "X", X.dtype)
+    a.cols = X.shape[-1]
+    if gain.dtype != X.dtype or gain.numel() != X.shape[-1] or not gain.is_contiguous():
+        _fail(op, "gain must hold one value of X's dtype per column")
+    a.x, a.gain, a.eps = X.data_ptr(), gain.data_ptr(), eps
+    if residual is None:
+        if sum_out is not None:
+            _fail(op, "sum_out without a residual")
+        sum_out = X
+    else:
+        if sum_out is None:
+            sum_out = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+        a.residual, a.residual_row_stride = residual.data_ptr(), _rows_of(op, residual, "residual", X.dtype, X.shape)[1]
+        a.sum_out, a.sum_row_stride = sum_out.data_ptr(), _rows_of(op, sum_out, "sum_out", X.dtype, X.shape)[1]
+    if out is None:
+        out = torch.empty(X.shape, dtype=torch.int8 if int8 else X.dtype, device=X.device)
+    stride = _rows_of(op, out, "out", torch.int8 if int8 else X.dtype, X.shape)[1]
+    if int8:
+        if scales is None:
+            scales = torch.empty(X.shape[:-1], dtype=torch.float32, device=X.device)
+        a.out_q, a.q_row_stride, a.out_scales = out.data_ptr(), stride, _scales_of(op, scales, "scales", a.rows)
+    else:
+        a.out, a.out_row_stride = out.data_ptr(), stride
+    a.stream = _stream()
+    capi.check(capi.lib().mi_add_rms_norm_forward(C.byref(a)), op)
+    return (sum_out, out, scales) if int8 else (sum_out, out)
+
+
+def add_rms_norm(X, residual, gain, eps: float, sum_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """(h, y): h = X + residual, rounded to X's dtype, and y = h * rsqrt(mean(h^2) + eps) * gain over the last axis: add_inplace_vec and
+    rms_norm_rows in one pass (mi_add_rms_norm_forward). residual None: h is X itself. X (..., cols), residual of its shape, gain (cols),
+    all of one dtype; sum_out and out may be X or residual."""
+    return _add_rms_norm("add_rms_norm", X, residual, gain, eps, sum_out, out, None, False)
+
+
+def add_rms_norm_int8(X, residual, gain, eps: float, sum_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                      scales: Optional[torch.Tensor] = None):
+    """(h, q, scales): as add_rms_norm with the normalised rows as INT8 and one FP32 scale each, y = q * scales[..., None]: the x and
+    x_scales of linear_act. With z = h * gain in FP32, q is 127 z / max|z| of its row to the nearest integer, exactly; a row of zeros has
+    scale 0, one that is not finite scale NaN and q = 0. scales has X's leading shape."""
+    return _add_rms_norm("add_rms_norm_int8", X, residual, gain, eps, sum_out, out, scales, True)
+
+
+def quantize_rows_int8(X, out: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
+    """(q, scales): X (..., cols) of float16 / bfloat16 as INT8 with one FP32 scale per row, q = 127 X / max|X| of its row to the nearest
+    integer, exactly, scales = max|X| / 127 (mi_quantize_rows_forward): the x and x_scales of linear_act."""
+    op = "quantize_rows_int8"
+    r = _native.quantize_rows(X, out, scales)
+    if r is not None:
+        return r
+    _dev(op, X, out, scales)
+    a = capi.MiQuantizeRowsArgs()
+    a.struct_size = C.sizeof(a)
+    a.dtype = _dtype_code(op, X)
+    a.rows, a.x_row_stride = _rows_of(op, X, "X", X.dtype)
+    a.cols = X.shape[-1]
+    if out is None:
+        out = torch.empty(X.shape, dtype=torch.int8, device=X.device)
+    if scales is None:
+        scales = torch.empty(X.shape[:-1], dtype=torch.float32, device=X.device)
+    a.x, a.out_q, a.q_row_stride = X.data_ptr(), out.data_ptr(), _rows_of(op, out, "out", torch.int8, X.shape)[1]
+    a.out_scales = _scales_of(op, scales, "scales", a.rows)
+    a.stream = _stream()
+    capi.check(capi.lib().mi_quantize_rows_forward(C.byref(a)), op)
+    return out, scales
+
+
+_ACTIVATIONS = {"none": capi.MI_ACT_NONE, "gelu": capi.MI_ACT_GELU, "gelu_tanh": capi.MI_ACT_GELU_TANH, "silu": capi.MI_ACT_SILU}
+
+
+def linear_act(X, W, bias=None, *, activation: str = "none", residual: Optional[torch.Tensor] = None, x_scales: Optional[torch.Tensor] = None,
+               w_scales: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None):
+    """act(X W^T [* w_scales] [* x_scales] + bias) + residual, one rounding at the end (mi_linear_act_forward). X (..., in_features),
+    W (out_features, in_features), bias (out_features), residual (..., out_features). activation: "none", "gelu" (erf), "gelu_tanh", "silu".
+    With w_scales (out_features) W is INT8; with x_scales (one per row) X is INT8 too, as add_rms_norm_int8 and quantize_rows_int8 return it, and
+    `dtype` says what the result (and bias, residual) is: float16 or bfloat16. `out` may be the residual itself."""
+    op = "linear_act"
+    r = _native.linear_act(X, W, bias, activation, residual, x_scales, w_scales, dtype, out)
+    if r is not None:
+        return r
+    _dev(op, X, W, bias, residual, x_scales, w_scales, out)
+    if activation not in _ACTIVATIONS:
+        _fail(op, f"activation {activation!r} is none of {', '.join(_ACTIVATIONS)}")
+    if W.dim() != 2 or X.dim() < 1 or X.shape[-1] != W.shape[1]:
+        _fail(op, f"X is {tuple(X.shape)}, W is {tuple(W.shape)}")
+    if x_scales is not None and w_scales is None:
+        _fail(op, "INT8 rows need INT8 weights (w_scales)")
+    if x_scales is None:
+        if dtype is not None and dtype != X.dtype:
+            _fail(op, f"dtype {dtype} is not X's, {X.dtype}")
+        dtype = X.dtype
+    elif dtype is None:
+        given = next((t for t in (out, residual, bias) if t is not None), None)
+        if given is None:
+            _fail(op, "INT8 rows without bias, residual and out need a dtype")
+        dtype = given.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        _fail(op, f"dtype {dtype} not supported (float16 / bfloat16)")
+    n_out = W.shape[0]
+    shape = (*X.shape[:-1], n_out)
+    a = capi.MiLinearActArgs()
+    a.struct_size = C.sizeof(a)
+    a.dtype = capi.MI_DTYPE_BF16 if dtype == torch.bfloat16 else capi.MI_DTYPE_F16
+    a.rows, a.x_row_stride = _rows_of(op, X, "X", torch.int8 if x_scales is not None else dtype)
+    if _rows_of(op, W, "W", torch.int8 if w_scales is not None else dtype)[0] != n_out:
+        _fail(op, "W must be (out_features, in_features)")
+    a.w_row_stride = W.stride(0) if n_out > 1 else W.shape[1]
+    a.in_features, a.out_features = W.shape[1], n_out
+    a.bias = _bias(op, bias, "bias", dtype, n_out)
+    if w_scales is not None:
+        a.w_scales = _scales_of(op, w_scales, "w_scales", n_out)
+    if x_scales is not None:
+        a.x_scales = _scales_of(op, x_scales, "x_scales", a.rows)
+    if residual is not None:
+        a.residual, a.residual_row_stride = residual.data_ptr(), _rows_of(op, residual, "residual", dtype, shape)[1]
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=X.device)
+    a.x, a.w, a.y, a.y_row_stride = X.data_ptr(), W.data_ptr(), out.data_ptr(), _rows_of(op, out, "out", dtype, shape)[1]
+    a.activation = _ACTIVATIONS[activation]
+    a.stream = _stream()
+    capi.check(capi.lib().mi_linear_act_forward(C.byref(a)), op)
     return out
 
 

@@ -438,6 +438,79 @@ MI_API int mi_rms_norm_forward(const void* x, const void* gain, void* out, int32
 MI_API int mi_rms_norm_pair_forward(const void* x0, const void* gain0, void* out0, const void* x1, const void* gain1, void* out1, int32_t rows,
                                     int32_t cols, int64_t x_row_stride, int64_t out_row_stride, float eps, int32_t dtype, void* stream);
 
+/* ── rows in front of a projection, 8-bit rows ─────────────────────────────
+ * h = T(x + residual), FP32 addition and one rounding to the tensor type T (residual NULL: h = x); then of the rows h
+ *   out:                 T(h * rsqrt(mean over c of h^2 + eps) * gain), FP32 in between, one rounding;
+ *   out_q, out_scales:   the same row as 8-bit integers and one FP32 scale, out_q[r][c] * out_scales[r] in place of `out`. With
+ *                        z = h * gain in FP32 and a = max over c of |z|: out_q = 127 z / a rounded to the nearest integer, exactly
+ *                        (ties to even, so within -127 .. 127), out_scales = a * rsqrt(...) / 127. A row of zeros has scale 0; a row with
+ *                        a value that is not finite has scale NaN and integers 0.
+ * The residual stream's step between two projections of a transformer block: mi_add_inplace and mi_rms_norm_forward (whose results it
+ * gives, to rounding) in one pass, with the 8-bit operand of mi_linear_act_forward as its output where that is wanted. At least one of
+ * out and out_q; out_q and out_scales together; sum_out (h itself) only with a residual and optional. The mean square is an FP32 sum, as
+ * in mi_rms_norm_forward: a row whose sum of squares exceeds FP32 becomes zeros.
+ * cols a multiple of 8, at most 65536; strides in elements (0 = dense), multiples of 8; 16-bit tensors 16-byte aligned, out_q 8-byte
+ * aligned. sum_out and out may each be x or residual (same pointer and stride); outputs share no other memory with each other or an
+ * input. */
+typedef struct mi_add_rms_norm_args {
+    uint32_t struct_size;
+    int32_t dtype;
+    const void* x;           /* (rows, cols) */
+    const void* residual;    /* (rows, cols) or NULL */
+    const void* gain;        /* (cols) of `dtype` */
+    void* sum_out;           /* (rows, cols) or NULL */
+    void* out;               /* (rows, cols) or NULL */
+    void* out_q;             /* INT8 (rows, cols) or NULL */
+    float* out_scales;       /* (rows) or NULL */
+    int32_t rows, cols;
+    int64_t x_row_stride, residual_row_stride, sum_row_stride, out_row_stride, q_row_stride;
+    float eps;
+    void* stream;
+} mi_add_rms_norm_args;
+MI_API int mi_add_rms_norm_forward(const mi_add_rms_norm_args* args);
+/* Rows as they are to 8-bit integers with one FP32 scale each: the above with z = x and out_scales = a / 127 (the operand of the second
+ * product of an MLP, between mi_linear_act_forward and mi_linear_act_forward). */
+typedef struct mi_quantize_rows_args {
+    uint32_t struct_size;
+    int32_t dtype;
+    const void* x;           /* (rows, cols) */
+    void* out_q;             /* INT8 (rows, cols) */
+    float* out_scales;       /* (rows) */
+    int32_t rows, cols;
+    int64_t x_row_stride, q_row_stride;
+    void* stream;
+} mi_quantize_rows_args;
+MI_API int mi_quantize_rows_forward(const mi_quantize_rows_args* args);
+
+/* ── linear layer with an epilogue ─────────────────────────────────────────
+ * Y = act(X W^T [* w_scales] [* x_scales] + bias) + residual, everything behind the product in FP32, one rounding to `dtype`.
+ * Three kinds of operands:
+ *   x, w of `dtype`                               sums in FP32
+ *   x of `dtype`, w INT8 with w_scales            (W8A16) sums in FP32 of exactly widened weights
+ *   x INT8 with x_scales, w INT8 with w_scales    (W8A8) sums in INT32, exact: x as mi_quantize_rows_forward and
+ *                                                 mi_add_rms_norm_forward write it, one scale per row; in_features at most 131056
+ * act: MI_ACT_*, GELU with erf, GELU_TANH = x / (1 + exp(-2 sqrt(2 / pi) (x + 0.044715 x^3))), SILU = x / (1 + exp(-x)).
+ * in_features and out_features are multiples of 8 (W8A8: in_features of 16); strides in elements (0 = dense), multiples of 8 (INT8 x and
+ * its w: of 16); pointers 16-byte aligned. y may be `residual` itself (same pointer and stride) and shares no memory with
+ * another operand; partial overlap with the residual is refused. rows may be 0. */
+enum { MI_ACT_NONE = 0, MI_ACT_GELU = 1, MI_ACT_GELU_TANH = 2, MI_ACT_SILU = 3 };
+typedef struct mi_linear_act_args {
+    uint32_t struct_size;
+    int32_t dtype;           /* of bias, residual, y, and of x and w where they have no scales */
+    const void* x;           /* (rows, in_features) */
+    const void* w;           /* (out_features, in_features) */
+    const void* bias;        /* (out_features) or NULL */
+    const void* residual;    /* (rows, out_features) or NULL */
+    void* y;                 /* (rows, out_features) */
+    int32_t rows, in_features, out_features;
+    int64_t x_row_stride, w_row_stride, residual_row_stride, y_row_stride;
+    const float* x_scales;   /* NULL, or (rows): x is INT8 */
+    const float* w_scales;   /* NULL, or (out_features): w is INT8 */
+    int32_t activation;      /* MI_ACT_* */
+    void* stream;
+} mi_linear_act_args;
+MI_API int mi_linear_act_forward(const mi_linear_act_args* args);
+
 /* ── attention with its projections ────────────────────────────────────────
  * The three operators the U-Net spatial transformer calls (src/unet_blocks.cpp:255-327,
  * src/unet.cpp:470-480; also the VAE mid blocks, src/vae.cpp:268):
