@@ -15,7 +15,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libmi_attention.so")
-SOURCES = ["capi.hip", "sdpa_fwd.hip", "sdpa_small.hip", "sdpa_flow.hip", "sdpa_wide.hip", "sdpa_wide_long.hip", "rope.hip", "linear_attn.hip", "linear.hip", "linear_pipe.hip", "linear_dma.hip", "attn_block.hip", "attn_map.hip", "elementwise.hip", "rows_int8.hip", "linear_act.hip", "probe.hip"]
+SOURCES = ["capi.hip", "sdpa_fwd.hip", "sdpa_small.hip", "sdpa_flow.hip", "sdpa_wide.hip", "sdpa_wide_long.hip", "rope.hip", "linear_attn.hip", "linear.hip", "linear_pipe.hip", "linear_dma.hip", "attn_block.hip", "attn_map.hip", "elementwise.hip", "rows_int8.hip", "linear_act.hip", "linear_act_16.hip", "linear_act_w8.hip", "linear_act_int8.hip", "probe.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-fvisibility=hidden",
@@ -27,8 +27,8 @@ FLAGS = [
     "-fno-honor-nans",
     "-Wall", "-Wno-unused-value", "-Wno-unknown-pragmas",
 ]
-# flags of one source alone; the reason stands at its top
-SOURCE_FLAGS = {"linear_pipe.hip": ["-falign-loops=64"]}
+# flags of the sources with the ring kernel; the reason stands at the top of linear_pipe.h
+SOURCE_FLAGS = {s: ["-falign-loops=64"] for s in ("linear_pipe.hip", "linear_act_16.hip", "linear_act_w8.hip", "linear_act_int8.hip")}
 
 
 def _compile(src: str, obj_dir: str, save_temps: bool) -> str:

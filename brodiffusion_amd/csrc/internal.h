@@ -170,8 +170,12 @@ int launch_linear(const LinearBatch& batch, int n_problems, int dtype, hipStream
 bool linear_pipe_takes(const LinearBatch& batch, int n_problems, bool geglu);
 int launch_linear_pipe(const LinearBatch& batch, int n_problems, int dtype, bool geglu, hipStream_t stream);
 int launch_linear_dma(const LinearBatch& batch, int n_problems, int dtype, hipStream_t stream);
-// One problem with an epilogue (linear_act.hip); its form with tiles through registers (linear.hip).
+// One problem with an epilogue (linear_act.hip): on the rings, by its kind of operands (linear_act_16.hip, _w8, _int8), and with tiles through
+// registers (linear.hip).
 int launch_linear_act(const LinearProblem& p, int dtype, hipStream_t stream);
+int launch_linear_act_16(const LinearProblem& p, int dtype, hipStream_t stream);
+int launch_linear_act_w8(const LinearProblem& p, int dtype, hipStream_t stream);
+int launch_linear_act_int8(const LinearProblem& p, int dtype, hipStream_t stream);
 int launch_linear_act_tiles(const LinearProblem& p, int dtype, hipStream_t stream);
 
 // Cross-attention to cached keys with its query projection in the same launch (sdpa_small.hip): p.q is not read, q projects batch * Lq

@@ -1,0 +1,37 @@
+// The linear layer with an epilogue, 16-bit operands: which instance of linear_pipe.h or linear_dma.h a launch takes (the forms and their
+// rule are those of the layer without one, linear_forms.h).
+#include "linear_dma.h"
+#include "linear_pipe.h"
+
+namespace mi {
+namespace gemm {
+namespace {
+
+template <typename T>
+int launch_form(const LinearBatch& b, hipStream_t st) {
+    switch (pick_form(kPlain, kPlainForms, b, 1, device_cu_count())) {
+        case k32x32: return launch_pipe<T, false, false, 1, 1, 1, 1, 6, 2, T, true>(b, 1, st);
+        case k64x32: return launch_pipe<T, false, false, 2, 1, 1, 1, 6, 2, T, true>(b, 1, st);
+        case k64x64: return launch_pipe<T, false, false, 2, 2, 1, 1, 4, 4, T, true>(b, 1, st);
+        case k64x96: return launch_pipe<T, false, false, 2, 3, 1, 1, 5, 4, T, true>(b, 1, st);
+        case k128x64_load: return launch_pipe<T, false, false, 2, 2, 2, 1, 3, 4, T, true>(b, 1, st);
+        case k128x96: return launch_pipe<T, false, false, 2, 3, 2, 1, 4, 4, T, true>(b, 1, st);
+        case k128x64: return launch_pipe<T, false, false, 2, 2, 2, 1, 3, 0, T, true>(b, 1, st);
+        case k128x128: return launch_pipe<T, false, false, 2, 2, 2, 2, 3, 4, T, true>(b, 1, st);
+        case k128x128_2: return launch_pipe<T, false, false, 2, 2, 2, 2, 2, 0, T, true>(b, 1, st);
+        case k192x128: return launch_pipe<T, false, false, 2, 4, 3, 1, 4, 0, T, true>(b, 1, st);
+        case k256x128: return launch_pipe<T, false, false, 4, 2, 2, 2, 3, 0, T, true>(b, 1, st);
+        default: return gemm_dma::launch_t<T, T, true>(b, 1, st);
+    }
+}
+
+}  // namespace
+}  // namespace gemm
+
+int launch_linear_act_16(const LinearProblem& p, int dtype, hipStream_t st) {
+    LinearBatch b{};
+    b.p[0] = p;
+    return dtype == MI_DTYPE_BF16 ? gemm::launch_form<__bf16>(b, st) : gemm::launch_form<_Float16>(b, st);
+}
+
+}  // namespace mi
