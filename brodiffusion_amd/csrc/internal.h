@@ -177,6 +177,9 @@ int launch_linear_act_16(const LinearProblem& p, int dtype, hipStream_t stream);
 int launch_linear_act_w8(const LinearProblem& p, int dtype, hipStream_t stream);
 int launch_linear_act_int8(const LinearProblem& p, int dtype, hipStream_t stream);
 int launch_linear_act_tiles(const LinearProblem& p, int dtype, hipStream_t stream);
+// ... and for few rows (linear_few.hip): whether that kernel takes a problem, and the launch.
+bool linear_few_takes(const LinearProblem& p);
+int launch_linear_few(const LinearProblem& p, int dtype, hipStream_t stream);
 
 // Cross-attention to cached keys with its query projection in the same launch (sdpa_small.hip): p.q is not read, q projects batch * Lq
 // rows to H * head_dim columns (q.y is not written).
