@@ -140,8 +140,10 @@ __global__ void __launch_bounds__(kThreads, 2) linear_dma_kernel(const LinearBat
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = typename M::sum4{0, 0, 0, 0};
 
-    const int nb = p.K / kBlock;      // blocks
+    const int nb = ACT ? (p.K + kBlock - 1) / kBlock : p.K / kBlock;      // blocks
+    const int in_last = ACT ? p.K - (nb - 1) * kBlock : kBlock;           // contraction elements of the last one
     const int nt = 2 * nb;         // half-steps
+    // (ACT: at least three blocks, so that the last one is not among the two of the prologue; its forms take contractions from 512 on)
     // prologue: blocks 0 and 1 requested, block 0 in LDS (block 1 has landed by the first close_half; waiting for it here too
     // made every work group of the launch wait for twice the bytes before its first product)
     dma_block(0);
@@ -160,6 +162,24 @@ __global__ void __launch_bounds__(kThreads, 2) linear_dma_kernel(const LinearBat
         constexpr int S = decltype(set_tag)::value;
         const int nxt = (t >> 1) + 2;
         const bool more = nxt < nb;
+        if constexpr (ACT) {       // a partial last block (linear_pipe.h): its loads and its fragments
+            if (in_last < kBlock && nxt == nb - 1) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int piece = (lane & 7) ^ ((8 * (4 * wave + u) + (lane >> 3)) >> 1 & 7);
+                    if (8 * piece >= in_last) (S == 0 ? woff : xoff)[u] -= piece * 16;
+                }
+            }
+            if (in_last < kBlock && (t >> 1) == nb - 1) {
+                const bool there = 8 * (4 * S + lg) < in_last;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) xf[S][j] = there ? xf[S][j] : V8{};
+                if constexpr (!A8) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) wf[S][i] = there ? wf[S][i] : V8{};
+                }
+            }
+        }
         [&]<int... Q>(std::integer_sequence<int, Q...>) {
             ([&] {
                 // (two token blocks at a time, each feature block meets both in a row)
@@ -205,31 +225,6 @@ __global__ void __launch_bounds__(kThreads, 2) linear_dma_kernel(const LinearBat
         for (int j = 0; j < 4; ++j) xs[j] = p.x_scale[min(m0 + wm * 64 + 16 * j + lr, p.M - 1)];
     }
     if constexpr (ACT) {
-        // the contraction elements behind the whole blocks, straight from memory; pieces past the end count as zeros
-        if (p.K > nb * kBlock) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if (nb * kBlock + 32 * c >= p.K) continue;
-                const int first = nb * kBlock + 32 * c + 8 * lg;
-                const bool there = first < p.K;
-                const long at = there ? first : 0;
-                V8 xt[4], wt[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    xt[j] = *reinterpret_cast<const V8*>(static_cast<const unsigned char*>(p.x) + (static_cast<long>(min(m0 + wm * 64 + 16 * j + lr, p.M - 1)) * p.ldx + at) * 2);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    wt[i] = *reinterpret_cast<const V8*>(static_cast<const unsigned char*>(p.w) + (static_cast<long>(min(n0 + wn * 128 + 16 * i + lr, p.N - 1)) * p.ldw + at) * 2);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) xt[j] = there ? xt[j] : V8{};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    wt[i] = there ? wt[i] : V8{};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = M::run16(wt[i], xt[j], acc[i][j]);
-                }
-            }
-        }
         // the residual's tile goes where the tile of Y will be staged (the rings are used up: the last half-step ended at a barrier)
         if (p.residual != nullptr) {
             const unsigned char* const rg = static_cast<const unsigned char*>(p.residual) + min(n0 + (tid & 31) * 8, p.N - 8) * 2L;

@@ -103,8 +103,9 @@ struct PipeGeo {
     static_assert((S - 1) * MI < 64, "outstanding loads fit the counter");
 };
 
-// ACT: Y = act(X W^T [* w_scale] [* x_scale] + bias) + residual, contractions of any number of 16-byte pieces (the last, partial stage goes
-// from memory to registers behind the ring). A: the type of the operands where it is not that of Y (Int8: both, K and the strides in
+// ACT: Y = act(X W^T [* w_scale] [* x_scale] + bias) + residual, contractions of any number of 16-byte pieces: of a partial last stage
+// the pieces past the end are loaded as copies of the row's first piece of that stage and blanked in registers (what is multiplied by
+// zero must be finite, so in both operands where they can hold anything else). A: the type of the operands where it is not that of Y (Int8: both, K and the strides in
 // pairs of elements; a stage is then 128 contraction elements in the same bytes).
 template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false>
 __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(const PipeArgs args) {
@@ -177,9 +178,30 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
         if (j < G::MX) dma(xoff[j < G::MX ? j : 0], xg, lds_base + slot + (lw + G::LW * j) * 1024);
         else dma(woff[j < G::MX ? 0 : j - G::MX], wg, lds_base + slot + G::X_BYTES + (lw + G::LW * (j - G::MX)) * 1024);
     };
+    // ACT: how many contraction elements the last stage holds, and the stage that xg and wg stand on
+    const int stages = ACT ? (p.K + kBK - 1) / kBK : 0;
+    const int in_last = ACT ? p.K - (stages - 1) * kBK : kBK;
+    int loading = 0;
+    auto shorten = [&]() {
+#pragma unroll
+        for (int u = 0; u < G::MX; ++u) {
+            const int r = 8 * (lw + G::LW * u) + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
+            if (8 * piece >= in_last) xoff[u] -= piece * 16;
+        }
+#pragma unroll
+        for (int u = 0; u < G::MW; ++u) {
+            const int r = W8 ? 16 * (lw + G::LW * u) + (lane >> 2) : 8 * (lw + G::LW * u) + (lane >> 3);
+            const int piece = W8 ? (lane & 3) ^ ((r >> 2) & 3) : (lane & 7) ^ ((r >> 1) & 7);
+            if ((W8 ? 16 : 8) * piece >= in_last) woff[u] -= piece * 16;
+        }
+    };
+    if (ACT && stages == 1) shorten();
     auto next_stage = [&]() {
         xg += kBK * 2;
         wg += W8 ? kBK : kBK * 2;
+        if constexpr (ACT) {
+            if (++loading == stages - 1 && in_last < kBK) shorten();
+        }
     };
     // Waits until at most `stages` of this wavefront's stages are in flight and its LDS reads have returned, then meets the others.
     auto wait_barrier = [&](int stages) {
@@ -297,7 +319,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     using Half1 = std::integral_constant<int, 1>;
     using Mid = std::integral_constant<int, MI / 2>;
     using All = std::integral_constant<int, MI>;
-    const int n = p.K / kBK;                          // whole stages; at least one without ACT
+    const int n = ACT ? stages : p.K / kBK;
     unsigned cur = 0, prev = (S - 1) * G::STAGE;      // ring slots of stages t and t - 1
     // Step t. D0: the second part of stage t + S - 1 is loaded, into the slot of stage t - 1; D1: the first part of stage t + S,
     // into the slot of stage t.
@@ -329,26 +351,22 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
                 next_stage();
                 slot = slot + G::STAGE == S * G::STAGE ? 0u : slot + G::STAGE;
             };
-            if (!ACT || n > 0) {
-                for (int s = 0; s < ahead; ++s) load_stage();
-                if (ahead == S) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((S - 1) * MI) : "memory");
-                else wait_barrier(ahead - 1);
-                int t = 0;
-                for (; t < n - S; ++t) {       // stage t + 1 has landed, the slot of stage t is free
-                    wait_barrier(S - 2);
-                    load_stage();
-                }
-                for (; t < n - 1; ++t) wait_barrier(n - 2 - t);
+            for (int s = 0; s < ahead; ++s) load_stage();
+            if (ahead == S) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((S - 1) * MI) : "memory");
+            else wait_barrier(ahead - 1);
+            int t = 0;
+            for (; t < n - S; ++t) {       // stage t + 1 has landed, the slot of stage t is free
+                wait_barrier(S - 2);
+                load_stage();
             }
+            for (; t < n - 1; ++t) wait_barrier(n - 2 - t);
             if (ACT && p.residual != nullptr) __syncthreads();
             __syncthreads();
             __syncthreads();
             return;
         }
-        if (!ACT || n > 0) {
-            asm volatile("s_barrier" ::: "memory");      // stage 0 has landed
-            read_half(Half0{}, 0);
-        }
+        asm volatile("s_barrier" ::: "memory");      // stage 0 has landed
+        read_half(Half0{}, 0);
         for (int t = 0; t < n - 1; ++t) {
             const unsigned nxt = cur + G::STAGE == S * G::STAGE ? 0u : cur + G::STAGE;
             multiply_half(Half0{}, std::true_type{}, cur, Half0{}, Half0{}, 0u);
@@ -359,7 +377,6 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
             __builtin_amdgcn_sched_barrier(0);
             cur = nxt;
         }
-    } else if (ACT && n == 0) {
     } else if (n < S) {   // everything fits the ring
         for (int s = 0; s < n; ++s) {
 #pragma unroll
@@ -390,11 +407,28 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     // put 215 to 356 of them in scratch, each reload behind a wait for the DMA as well (GEGLU, fp16, us with the branch / without:
     // 2048 x 640 -> 2 x 2560 28.7 / 20.0, INT8 36.0 / 20.9; 4096 x 320 -> 2 x 1280 23.0 / 14.1, INT8 29.5 / 15.2; 1024 x 1280 ->
     // 2 x 5120 41.2 / 32.5, INT8 48.8 / 32.9).
-    if (!ACT || n > 0) {
-        multiply_half(Half0{}, std::true_type{}, cur, Half0{}, Half0{}, 0u);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply_half(Half1{}, std::false_type{}, 0u, Half0{}, Half0{}, 0u);
-    }
+    // (ACT: the pieces of the last stage that are past the end of the contraction)
+    auto blank_half = [&](auto half_tag) {
+        constexpr int H = decltype(half_tag)::value;
+        if constexpr (ACT) {
+            if (in_last == kBK) return;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const bool there = 8 * ((KS * H + k) * (64 / BS) + lg) < in_last;
+#pragma unroll
+                for (int b = 0; b < TB; ++b) xf[H][k * TB + b] = there ? xf[H][k * TB + b] : V8{};
+                if constexpr (!W8 && !A8) {
+#pragma unroll
+                    for (int a = 0; a < FB; ++a) wf[H][k * FB + a] = there ? wf[H][k * FB + a] : WRaw{};
+                }
+            }
+        }
+    };
+    blank_half(Half0{});
+    multiply_half(Half0{}, std::true_type{}, cur, Half0{}, Half0{}, 0u);
+    __builtin_amdgcn_sched_barrier(0);
+    blank_half(Half1{});
+    multiply_half(Half1{}, std::false_type{}, 0u, Half0{}, Half0{}, 0u);
 
     constexpr int PPR = BN_OUT / 8;   // 16-byte pieces per staged row
     constexpr int PIECES = BM * PPR / G::NT, RSTEP = G::NT / PPR;
@@ -407,38 +441,6 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
             const unsigned char* const rg = static_cast<const unsigned char*>(p.residual) + min(n0 + piece * 8, p.N - 8) * 2L;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) out[i] = *reinterpret_cast<const u32x4*>(rg + static_cast<long>(min(m0 + row + i * RSTEP, p.M - 1)) * p.ldr_b);
-        }
-        // the contraction elements behind the whole stages, straight from memory: pieces past the end count as zeros
-        if (p.K > n * kBK) {
-#pragma unroll
-            for (int c = 0; c < 2 * KS; ++c) {
-                const int first = n * kBK + 8 * (c * (64 / BS) + lg);
-                const bool there = first < p.K;
-                if (n * kBK + 8 * c * (64 / BS) >= p.K) continue;
-                const long at = there ? first : 0;
-                V8 xt[TB];
-                WRaw wt[FB];
-#pragma unroll
-                for (int b = 0; b < TB; ++b)
-                    xt[b] = *reinterpret_cast<const V8*>(static_cast<const unsigned char*>(p.x) + static_cast<long>(min(m0 + wm * TM * 32 + BS * b + lr, p.M - 1)) * p.ldx_b + at * 2);
-#pragma unroll
-                for (int a = 0; a < FB; ++a)
-                    wt[a] = *reinterpret_cast<const WRaw*>(static_cast<const unsigned char*>(p.w) + static_cast<long>(min(n0 + wn * TN * 32 + BS * a + lr, p.N - 1)) * p.ldw_b + at * (W8 ? 1 : 2));
-#pragma unroll
-                for (int b = 0; b < TB; ++b) xt[b] = there ? xt[b] : V8{};
-#pragma unroll
-                for (int a = 0; a < FB; ++a) {
-                    wt[a] = there ? wt[a] : WRaw{};
-                    V8 w;
-                    if constexpr (W8) w = widen<T>(wt[a]);
-                    else w = wt[a];
-#pragma unroll
-                    for (int b = 0; b < TB; ++b) {
-                        if constexpr (ONE) acc[a][b] = M::run(w, xt[b], acc[a][b]);
-                        else acc[a][b] = M::run16(w, xt[b], acc[a][b]);
-                    }
-                }
-            }
         }
     }
 

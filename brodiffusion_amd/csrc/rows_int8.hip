@@ -12,7 +12,7 @@
 //
 // Bound: HBM. Each row is read once, held in registers between its sums and what is written, and nothing else passes through memory.
 // A lane holds N 16-byte chunks; a row belongs to W wavefronts (one: sums by lane exchanges alone, four rows in a work group; more:
-// one exchange through LDS behind a barrier).
+// one exchange through LDS behind a barrier). 4608 rows of 6144: 41.8 us = 5.4 TB/s, a large copy's rate here; to 8 bits 37.9 us (5.2 TB/s).
 #include "internal.h"
 
 namespace mi {
@@ -175,15 +175,23 @@ int launch_chunks(const RowsArgs& a, hipStream_t st) {
         case 2: return launch_rows<T, 2, W, NORM>(a, st);
         case 3: return launch_rows<T, 3, W, NORM>(a, st);
         case 4: return launch_rows<T, 4, W, NORM>(a, st);
-        case 5: case 6: return launch_rows<T, 6, W, NORM>(a, st);
-        default: return launch_rows<T, 8, W, NORM>(a, st);
+        default:
+            if constexpr (W == 16) return launch_rows<T, 8, W, NORM>(a, st);
+            return fail("rows: no kernel for %d columns", a.cols);      // (not asked for below)
     }
 }
 
+// Wavefronts per row. Where rows fill the GPU (4 for each compute unit) up to 3 chunks per lane: fewer lanes have none, fewer meet at the barrier;
+// where they do not, a row is a chain of latencies and 2 chunks per lane shorten it. Measured (us, 8-bit norm, 1 / 2 / 4 / 8 / 16 wavefronts):
+//   4608 rows of 2240 19.9 / 17.6 / 20.1 / 21.9 / -, of 6144 - / 41.7 / 37.9 / 40.1 / 52.1; 2048 of 16384 - / - / 51.9 / 53.4 / 59.7
+//   333 rows of 2240 5.9 / 5.0 / 4.5 / 4.4 / -; 1 row of 6144 - / 5.3 / 3.9 / 3.8 / 4.0, of 16384 - / - / 6.7 / 5.6 / 5.3
 template <typename T, bool NORM>
 int launch_width(const RowsArgs& a, hipStream_t st) {
-    if (a.cols <= 64 * 8 * 8) return launch_chunks<T, 1, NORM>(a, st);
-    if (a.cols <= 256 * 8 * 8) return launch_chunks<T, 4, NORM>(a, st);
+    const int chunks = a.cols / 8, each = a.rows >= 4 * device_cu_count() ? 3 : 2;
+    if (chunks <= 64 * each) return launch_chunks<T, 1, NORM>(a, st);
+    if (chunks <= 128 * each) return launch_chunks<T, 2, NORM>(a, st);
+    if (chunks <= 256 * each) return launch_chunks<T, 4, NORM>(a, st);
+    if (chunks <= 512 * (each == 3 ? 4 : 2)) return launch_chunks<T, 8, NORM>(a, st);
     return launch_chunks<T, 16, NORM>(a, st);
 }
 
