@@ -189,9 +189,10 @@ int launch(const LinearProblem& p, hipStream_t st) {
 // How a problem stands to the GPU. narrow: up to 8 features per compute unit, so that work groups of 8 features are what there is to spread;
 // wide: over 32; brief: not narrow, with a contraction of at most 4 KB of W's row, of which a wavefront gets a step or two.
 struct Shape {
+    int cu;
     bool narrow, wide, brief;
     Shape(const LinearProblem& p, int kind) {
-        const int cu = device_cu_count();
+        cu = device_cu_count();
         narrow = p.N <= 8 * cu;
         wide = p.N > 32 * cu;
         brief = !narrow && p.K * (kind == kWeights8 ? 1L : 2L) <= 4096;
@@ -199,18 +200,40 @@ struct Shape {
 };
 int kind_of(const LinearProblem& p) { return p.x_scale ? kBoth8 : p.w_scale ? kWeights8 : kSixteen; }
 
+// Three or four blocks of R features per work group, by which of them the busiest compute unit has less: 6144 features are 256 work groups of 24 or
+// 192 of 32 (us, three / four blocks, 6144 x 16384: 16-bit 16 rows 39.2 / 42.8, W8A16 20 rows 26.7 / 30.7, W8A8 16 rows 20.4 / 24.3).
+template <int R> bool three_blocks(const LinearProblem& p, int cu) {
+    auto share = [&](int blocks) { return (p.N + R * blocks * cu - 1) / (R * blocks * cu) * blocks; };
+    return share(3) <= share(4);
+}
+
 template <typename T, int KIND>
 int launch_rows(const LinearProblem& p, hipStream_t st) {
     const Shape s(p, KIND);
+    // four wavefronts with two steps on their way each where there are work groups enough, else eight (with one, where a step is many loads)
+    const bool many = p.N > 16 * s.cu;
     if (p.M <= 4) {
         if constexpr (KIND != kBoth8) if (s.brief) return launch<T, KIND, 4, 4, 1, 1, 8>(p, st);
         return launch<T, KIND, 4, 2, 1, 2, 8>(p, st);
     }
-    if (p.M <= 8 && !s.brief && !(s.wide && KIND == kWeights8)) return launch<T, KIND, 4, 2, 2, 2, 8>(p, st);
-    if (p.M <= 16 && s.narrow) return launch<T, KIND, 4, 2, 4, 2, 8>(p, st);
-    if (s.narrow) return launch<T, KIND, 4, 2, 8, 1, KIND == kWeights8 ? 4 : 8>(p, st);
-    if constexpr (KIND != kBoth8) if (p.M <= 16) return launch<T, KIND, 2, 4, 2, 2, 4>(p, st);
-    if constexpr (KIND == kWeights8) return p.M <= 24 ? launch<T, KIND, 2, 4, 3, 1, 8>(p, st) : launch<T, KIND, 2, 4, 4, 1, 8>(p, st);
+    if (s.narrow) {
+        if (p.M <= 8) return launch<T, KIND, 4, 2, 2, 2, 8>(p, st);
+        if (p.M <= 16) return launch<T, KIND, 4, 2, 4, 2, 8>(p, st);
+        return launch<T, KIND, 4, 2, 8, 1, KIND == kWeights8 ? 4 : 8>(p, st);
+    }
+    if (p.M <= 8) {
+        if (!many) return three_blocks<4>(p, s.cu) ? launch<T, KIND, 4, 3, 2, 2, 8>(p, st) : launch<T, KIND, 4, 4, 2, 2, 8>(p, st);
+        return three_blocks<4>(p, s.cu) ? launch<T, KIND, 4, 3, 2, 2, 4>(p, st) : launch<T, KIND, 4, 4, 2, 2, 4>(p, st);
+    }
+    if (p.M <= 16) {
+        if (!many) return launch<T, KIND, 2, 2, 2, 2, 8>(p, st);
+        return three_blocks<8>(p, s.cu) ? launch<T, KIND, 2, 3, 2, 2, 4>(p, st) : launch<T, KIND, 2, 4, 2, 2, 4>(p, st);
+    }
+    if (!many) return p.M <= 24 ? launch<T, KIND, 2, 2, 3, 1, 8>(p, st) : launch<T, KIND, 2, 2, 4, 1, 8>(p, st);
+    if constexpr (KIND != kBoth8) {
+        if (p.M <= 24) return three_blocks<8>(p, s.cu) ? launch<T, KIND, 2, 3, 3, 2, 4>(p, st) : launch<T, KIND, 2, 4, 3, 2, 4>(p, st);
+        return three_blocks<8>(p, s.cu) ? launch<T, KIND, 2, 3, 4, 2, 4>(p, st) : launch<T, KIND, 2, 4, 4, 2, 4>(p, st);
+    }
     return fail("linear: no kernel for %d rows", p.M);      // (linear_few_takes leaves these to others)
 }
 
@@ -227,19 +250,20 @@ int launch_kind(const LinearProblem& p, hipStream_t st) {
 }  // namespace gemm
 
 // Up to which number of rows this kernel is the faster one, by both sides' times (us, this kernel / the rings of linear_pipe.h, bf16, weights of
-// 600 MB in turn; features x contraction):
-//   narrow      1152 x 4608: 16-bit 8 rows 4.4 / 9.9, 32 7.2 / 9.9; W8A16 4.0 / 15.4, 7.5 / 15.3; W8A8 32 5.3 / 6.6
-//   brief       4608 x 1152: 16-bit 1 row 4.2 / 4.4, 8 4.8 / 4.4; W8A16 20 5.1 / 5.9, 32 6.1 / 5.9; W8A8 1 4.5 / 3.9
-//   otherwise   6144 x 16384: 16-bit 8 38.8 / 43.6, 16 42.8 / 43.6, 24 45.4 / 43.9; W8A16 16 28.2 / 48.8, 32 37.8 / 49.0, 40 58.3 / 50.8;
-//               W8A8 8 19.9 / 23.1, 16 24.5 / 23.1
-//   wide        16384 x 6144: 16-bit 16 39.7 / 42.1, 20 42.1 / 43.1; W8A16 16 24.2 / 23.7, 20 29.4 / 25.4; W8A8 4 20.1 / 19.8, 8 21.8 / 19.8
+// up to 600 MB in turn; features x contraction):
+//   narrow      1152 x 4608: 16-bit 8 rows 4.4 / 9.9, 32 7.2 / 9.8; W8A16 4.0 / 15.3, 7.5 / 15.3; W8A8 32 5.3 / 6.9
+//   brief       4608 x 1152: 16-bit 4 rows 4.2 / 4.4, 8 5.1 / 4.4; W8A16 24 5.8 / 5.9, 32 6.3 / 5.9; W8A8 1 5.0 / 4.0;
+//               8192 x 2048: 16-bit 1 row 7.6 / 6.9; W8A16 24 7.3 / 8.6; W8A8 1 5.3 / 5.2
+//   otherwise   6144 x 16384: 16-bit 16 39.8 / 43.6, 32 45.4 / 45.9; W8A16 16 24.4 / 48.9, 32 32.4 / 48.1; W8A8 16 20.6 / 23, 20 22.2 / 23.1;
+//               6144 x 6144: 16-bit 32 19.8 / 20.3; W8A16 15.1 / 20.1; W8A8 16 9.0 / 9.2, 20 10.1 / 9.2; 2240 x 6720: W8A8 32 7.6 / 8.7
+//   wide        16384 x 6144: 16-bit 24 41.6 / 43.2, 32 45.9 / 45.1; W8A16 4 21.2 / 21.8, 16 24.3 / 23.8; W8A8 16 19.8 / 19.8
 bool linear_few_takes(const LinearProblem& p) {
     const int kind = gemm::kind_of(p);
     const gemm::Shape s(p, kind);
     if (s.narrow) return p.M <= 32;
-    if (kind == gemm::kSixteen) return p.M <= (s.brief ? 4 : 16);
-    if (kind == gemm::kWeights8) return p.M <= (s.wide ? 16 : s.brief ? 24 : 32);
-    return !s.brief && p.M <= (s.wide ? 4 : 8);
+    if (kind == gemm::kSixteen) return s.brief ? p.M <= 4 && p.N <= 24 * s.cu : p.M <= (s.wide ? 24 : 32);
+    if (kind == gemm::kWeights8) return p.M <= (s.wide ? 8 : s.brief ? 24 : 32);
+    return !s.brief && p.M <= (p.N <= 16 * s.cu ? 32 : 16);
 }
 
 int launch_linear_few(const LinearProblem& p, int dtype, hipStream_t st) {
