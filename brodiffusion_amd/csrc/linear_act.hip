@@ -6,9 +6,8 @@ namespace mi {
 
 int launch_linear_act(const LinearProblem& p, int dtype, hipStream_t st) {
     if (linear_few_takes(p)) return launch_linear_few(p, dtype, st);
-    // what the rings do not take: tiles that 32-bit byte offsets do not reach, INT8 weights whose rows are not whole 16-byte pieces
-    if (p.ldx * 2 * 256 >= (1L << 31) || p.ldw * 2 * 256 >= (1L << 31) || (p.w_scale && !p.x_scale && (p.ldw % 16 != 0 || p.K % 16 != 0)))
-        return launch_linear_act_tiles(p, dtype, st);
+    // what the rings do not take: tiles that 32-bit byte offsets do not reach
+    if (p.ldx * 2 * 256 >= (1L << 31) || p.ldw * 2 * 256 >= (1L << 31)) return launch_linear_act_tiles(p, dtype, st);
     if (p.x_scale) return launch_linear_act_int8(p, dtype, st);
     return p.w_scale ? launch_linear_act_w8(p, dtype, st) : launch_linear_act_16(p, dtype, st);
 }

@@ -85,7 +85,7 @@ __device__ __forceinline__ DivMod div_mod(int x, int d, unsigned inv) {
     return {static_cast<int>(q), static_cast<int>(r)};
 }
 
-template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL>
+template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, int WL = 16>
 struct PipeGeo {
     static constexpr int NW = WM * WN, NT = 64 * NW;
     static constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
@@ -93,11 +93,11 @@ struct PipeGeo {
     static constexpr int WROW = W8 ? 64 : 128;                    // bytes of a W row in a stage
     static constexpr int X_BYTES = BM * 128, W_BYTES = BN * WROW, STAGE = X_BYTES + W_BYTES;
     static constexpr int LW = NL ? NL : NW;                       // wavefronts that load
-    static constexpr int MX = X_BYTES / 1024 / LW, MW = W_BYTES / 1024 / LW;   // DMA instructions of such a one per stage
+    static constexpr int MX = X_BYTES / 1024 / LW, MW = W_BYTES / (64 * WL) / LW;   // DMA instructions of such a one per stage
     static constexpr int MI = MX + MW;
     static constexpr int OUT_ROW = BN_OUT * 2 + 16;
     static constexpr int LDS = S * STAGE > BM * OUT_ROW ? S * STAGE : BM * OUT_ROW;
-    static_assert(MX * LW * 1024 == X_BYTES && MW * LW * 1024 == W_BYTES, "the same DMA duty for every loading wavefront");
+    static_assert(MX * LW * 1024 == X_BYTES && MW * LW * 64 * WL == W_BYTES, "the same DMA duty for every loading wavefront");
     static_assert(!GEGLU || TN == 2, "the GEGLU form pairs the two feature blocks of a wavefront");
     static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
     static_assert((S - 1) * MI < 64, "outstanding loads fit the counter");
@@ -106,15 +106,17 @@ struct PipeGeo {
 // ACT: Y = act(X W^T [* w_scale] [* x_scale] + bias) + residual, contractions of any number of 16-byte pieces: of a partial last stage
 // the pieces past the end are loaded as copies of the row's first piece of that stage and blanked in registers (what is multiplied by
 // zero must be finite, so in both operands where they can hold anything else). A: the type of the operands where it is not that of Y (Int8: both, K and the strides in
-// pairs of elements; a stage is then 128 contraction elements in the same bytes).
-template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false>
+// pairs of elements; a stage is then 128 contraction elements in the same bytes). WL: bytes that a lane loads of W at a time, 4 where the
+// rows of INT8 weights lie on 8-byte addresses only (contractions that are no multiple of 16).
+template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16>
 __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(const PipeArgs args) {
-    using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL>;
+    using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL, WL>;
     using M = Mma<A>;
     using V8 = typename M::v8;
     using V4 = typename Mma<T>::v4;
     constexpr bool A8 = std::is_same_v<A, Int8>;
     static_assert(!ACT || !GEGLU, "the GEGLU form has its own epilogue");
+    static_assert(WL == 16 || (W8 && ACT && WL == 4), "whole pieces, or words of INT8 weights");
     constexpr int BM = G::BM, BN = G::BN, BN_OUT = G::BN_OUT, MI = G::MI;
     // one block of INT8 weights per wavefront: v_mfma_f32_32x32x16 (see the top)
     constexpr bool ONE = W8 && TM == 1 && TN == 1;
@@ -162,6 +164,11 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     }
 #pragma unroll
     for (int u = 0; u < G::MW; ++u) {
+        if constexpr (WL == 4) {       // 4 rows of 16 words; the pieces are swizzled as everywhere
+            const int r = 4 * (lw + G::LW * u) + (lane >> 4);
+            woff[u] = static_cast<unsigned>(min(r, p.N - 1 - n0)) * p.ldw_b + (((lane >> 2 & 3) ^ ((r >> 2) & 3)) * 4 + (lane & 3)) * 4u;
+            continue;
+        }
         const int r = W8 ? 16 * (lw + G::LW * u) + (lane >> 2) : 8 * (lw + G::LW * u) + (lane >> 3);
         const unsigned piece = W8 ? (lane & 3) ^ ((r >> 2) & 3) : (lane & 7) ^ ((r >> 1) & 7);
         // GEGLU: 32-row groups of the tile alternate between the value and the gate rows of the same features
@@ -176,6 +183,8 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     // pieces [J0, J1) of this wavefront's share of a stage; xg / wg stand on that stage
     auto dma_piece = [&](int j, unsigned slot) {
         if (j < G::MX) dma(xoff[j < G::MX ? j : 0], xg, lds_base + slot + (lw + G::LW * j) * 1024);
+        else if constexpr (WL == 4)
+            asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(woff[j < G::MX ? 0 : j - G::MX]), "s"(wg), "{m0}"(lds_base + slot + G::X_BYTES + (lw + G::LW * (j - G::MX)) * 256) : "memory");
         else dma(woff[j < G::MX ? 0 : j - G::MX], wg, lds_base + slot + G::X_BYTES + (lw + G::LW * (j - G::MX)) * 1024);
     };
     // ACT: how many contraction elements the last stage holds, and the stage that xg and wg stand on
@@ -190,6 +199,11 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
         }
 #pragma unroll
         for (int u = 0; u < G::MW; ++u) {
+            if constexpr (WL == 4) {
+                const int r = 4 * (lw + G::LW * u) + (lane >> 4), word = ((lane >> 2 & 3) ^ ((r >> 2) & 3)) * 4 + (lane & 3);
+                if (4 * word >= in_last) woff[u] -= word * 4;
+                continue;
+            }
             const int r = W8 ? 16 * (lw + G::LW * u) + (lane >> 2) : 8 * (lw + G::LW * u) + (lane >> 3);
             const int piece = W8 ? (lane & 3) ^ ((r >> 2) & 3) : (lane & 7) ^ ((r >> 1) & 7);
             if ((W8 ? 16 : 8) * piece >= in_last) woff[u] -= piece * 16;
@@ -538,9 +552,9 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     }
 }
 
-template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false>
+template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16>
 int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st) {
-    using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL>;
+    using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL, WL>;
     auto tiles_m = [&](int i) { return (batch.p[i].M + G::BM - 1) / G::BM; };
     auto tiles_n = [&](int i) { return (batch.p[i].N + G::BN_OUT - 1) / G::BN_OUT; };
     long tiles = 0;
@@ -549,7 +563,7 @@ int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st) {
     if (G::LDS > 64 * 1024) {
         static thread_local bool raised = false;
         if (!raised) {
-            MI_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT>),
+            MI_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS));
             raised = true;
         }
@@ -575,7 +589,7 @@ int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st) {
         p.inv_panel = inverse(p.panel_tiles); p.inv_width = inverse(p.width); p.inv_last = inverse(p.last_width);
         first += tiles_m(i) * tiles_n(i);
     }
-    hipLaunchKernelGGL((linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT>), dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(G::NT + 64 * NL), G::LDS, st, args);
+    hipLaunchKernelGGL((linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL>), dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(G::NT + 64 * NL), G::LDS, st, args);
     MI_HIP_CHECK(hipGetLastError());
     return 0;
 }
