@@ -62,6 +62,7 @@ def build(save_temps: bool = False, verbose: bool = False) -> str:
 HOST_DIR = os.path.join(HERE, "host")
 HOST_LIB = os.path.join(LIB_DIR, "libbrodiffusion_amd_host.so")
 HOST_TEST = os.path.join(LIB_DIR, "test_host_ops")
+BLOCK_TEST = os.path.join(LIB_DIR, "test_block_half")
 SPLIT_TEST = os.path.join(LIB_DIR, "test_split_geo")
 FORMS_LIB = os.path.join(LIB_DIR, "liblinear_forms_test.so")
 WAITING_LIB = os.path.join(LIB_DIR, "libwaiting_test.so")
@@ -81,12 +82,13 @@ def build_host(with_test: bool = True, verbose: bool = False) -> str:
         raise RuntimeError("host library build failed")
     if with_test:
         oracle_dir = os.path.join(ROOT, "oracle")
-        cmd = [*common, os.path.join(ROOT, "tests", "cpp", "test_host_ops.cpp"), "-o", HOST_TEST, *rpath,
-               "-Wl,-rpath,$ORIGIN/../../oracle", "-L" + oracle_dir, "-lbrodiffusion_amd_host", "-lmi_attention", "-loracle"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            sys.stderr.write(r.stdout + r.stderr)
-            raise RuntimeError("host test build failed")
+        for source, exe in (("test_host_ops.cpp", HOST_TEST), ("test_block_half.cpp", BLOCK_TEST)):
+            cmd = [*common, os.path.join(ROOT, "tests", "cpp", source), "-o", exe, *rpath,
+                   "-Wl,-rpath,$ORIGIN/../../oracle", "-L" + oracle_dir, "-lbrodiffusion_amd_host", "-lmi_attention", "-loracle"]
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if r.returncode != 0:
+                sys.stderr.write(r.stdout + r.stderr)
+                raise RuntimeError("host test build failed")
     if with_test:
         # host-only check of the launch-planning arithmetic shared by host and device code (needs the HIP headers: hipcc)
         cmd = [HIPCC, "-std=c++20", "-O1", "-Wall", "--offload-host-only", "-x", "hip", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC,

@@ -254,8 +254,10 @@ __global__ void __launch_bounds__(kThreads, 2) linear_dma_kernel(const LinearBat
             float sw[4];
             if constexpr (A8) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    sw[e] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(src + 4 * (e >> 1), __builtin_bit_cast(int, scale2[e & 1])));
+                for (int e = 0; e < 4; ++e) {
+                    const float held = scale2[e & 1];      // (a bit cast of the element itself takes the vector's first)
+                    sw[e] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(src + 4 * (e >> 1), __builtin_bit_cast(int, held)));
+                }
             }
             f32x4 v[4];
 #pragma unroll

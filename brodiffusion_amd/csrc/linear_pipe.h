@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     constexpr bool A8 = std::is_same_v<A, Int8>;
     static_assert(!ACT || !GEGLU, "the GEGLU form has its own epilogue");
     static_assert(WL == 16 || (W8 && ACT && WL == 4), "whole pieces, or words of INT8 weights");
-    constexpr int BM = G::BM, BN = G::BN, BN_OUT = G::BN_OUT, MI = G::MI;
+    constexpr int BM = G::BM, BN_OUT = G::BN_OUT, MI = G::MI;
     // one block of INT8 weights per wavefront: v_mfma_f32_32x32x16 (see the top)
     constexpr bool ONE = W8 && TM == 1 && TN == 1;
     constexpr int BS = ONE ? 32 : 16, FB = TN * 32 / BS, TB = TM * 32 / BS;      // rows of a block; feature and token blocks of a wavefront
@@ -438,25 +438,25 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
             }
         }
     };
-    blank_half(Half0{});
-    multiply_half(Half0{}, std::true_type{}, cur, Half0{}, Half0{}, 0u);
-    __builtin_amdgcn_sched_barrier(0);
-    blank_half(Half1{});
-    multiply_half(Half1{}, std::false_type{}, 0u, Half0{}, Half0{}, 0u);
-
     constexpr int PPR = BN_OUT / 8;   // 16-byte pieces per staged row
     constexpr int PIECES = BM * PPR / G::NT, RSTEP = G::NT / PPR;
     static_assert(BM * PPR % G::NT == 0 && G::NT % PPR == 0, "the same pieces for every thread, one below the other");
     u32x4 out[PIECES];
     if constexpr (ACT) {
         const int row = tid / PPR, piece = tid % PPR;
-        // the residual's pieces that this thread will write again as pieces of Y
+        // the residual's pieces that this thread will write again as pieces of Y, on their way during the last stage (no load of the ring
+        // is waited for any more)
         if (p.residual != nullptr) {
             const unsigned char* const rg = static_cast<const unsigned char*>(p.residual) + min(n0 + piece * 8, p.N - 8) * 2L;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) out[i] = *reinterpret_cast<const u32x4*>(rg + static_cast<long>(min(m0 + row + i * RSTEP, p.M - 1)) * p.ldr_b);
         }
     }
+    blank_half(Half0{});
+    multiply_half(Half0{}, std::true_type{}, cur, Half0{}, Half0{}, 0u);
+    __builtin_amdgcn_sched_barrier(0);
+    blank_half(Half1{});
+    multiply_half(Half1{}, std::false_type{}, 0u, Half0{}, Half0{}, 0u);
 
     __syncthreads();   // the ring is used up
     // ── epilogue: acc[a][b][i] is feature n0 + wn TN 32 + 16 a + 4 lg + i of token m0 + wm TM 32 + 16 b + lr; the tile
