@@ -283,6 +283,7 @@ PyObject* tuple_of(std::initializer_list<PyObject*> items) {     // takes the re
 
 // X, residual, gain, eps, sum_out, out, scales, int8, op
 NATIVE(add_rms_norm, 9)
+    need(L.add_rms_norm != nullptr);
     const Tensor &x = tensor(a[0]), &g = tensor(a[2]);
     const bool int8 = truth(a[7]);
     mi_add_rms_norm_args p;
@@ -322,6 +323,7 @@ NATIVE_END
 
 // X, out, scales
 NATIVE(quantize_rows, 3)
+    need(L.quantize_rows != nullptr);
     const Tensor& x = tensor(a[0]);
     mi_quantize_rows_args p;
     std::memset(&p, 0, sizeof(p));
@@ -346,6 +348,7 @@ int activation_of(PyObject* o) {
 }
 // X, W, bias, activation, residual, x_scales, w_scales, dtype, out
 NATIVE(linear_act, 9)
+    need(L.linear_act != nullptr);
     const Tensor &x = tensor(a[0]), &w = tensor(a[1]);
     mi_linear_act_args p;
     std::memset(&p, 0, sizeof(p));
@@ -788,9 +791,10 @@ PyObject* bind(PyObject*, PyObject* args) {
     get(L.rms_norm_pair, "mi_rms_norm_pair_forward"); get(L.block_scratch_bytes, "mi_attn_block_scratch_bytes");
     get(L.qkvo, "mi_flash_attention_qkvo_forward"); get(L.kv_cached, "mi_flash_attention_q_with_kv_cached_forward");
     get(L.la_workspace_bytes, "mi_linear_attn_workspace_bytes"); get(L.la_scratch_bytes, "mi_linear_attn_scratch_bytes");
-    get(L.linear_attn, "mi_linear_attn_relu_forward"); get(L.add_rms_norm, "mi_add_rms_norm_forward");
-    get(L.quantize_rows, "mi_quantize_rows_forward"); get(L.linear_act, "mi_linear_act_forward");
+    get(L.linear_attn, "mi_linear_attn_relu_forward");
     if (!ok) return PyErr_Format(PyExc_RuntimeError, "%s does not export every function of mi_attention.h: build the library again", path);
+    // (a library without these binds all the same: their calls decline, and the Python code says what is missing)
+    get(L.add_rms_norm, "mi_add_rms_norm_forward"); get(L.quantize_rows, "mi_quantize_rows_forward"); get(L.linear_act, "mi_linear_act_forward");
     Py_INCREF(lend);
     Py_XSETREF(lend_scratch, lend);
     bound = true;
