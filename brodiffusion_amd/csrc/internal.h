@@ -172,10 +172,11 @@ int launch_linear_pipe(const LinearBatch& batch, int n_problems, int dtype, bool
 int launch_linear_dma(const LinearBatch& batch, int n_problems, int dtype, hipStream_t stream);
 // One problem with an epilogue (linear_act.hip): on the rings, by its kind of operands (linear_act_16.hip, _w8, _int8), and with tiles through
 // registers (linear.hip).
-int launch_linear_act(const LinearProblem& p, int dtype, hipStream_t stream);
-int launch_linear_act_16(const LinearProblem& p, int dtype, hipStream_t stream);
-int launch_linear_act_w8(const LinearProblem& p, int dtype, hipStream_t stream);
-int launch_linear_act_int8(const LinearProblem& p, int dtype, hipStream_t stream);
+struct LinearScratch { void* p; size_t bytes; };      // what the caller lent: a call that could use more does without
+int launch_linear_act(const LinearProblem& p, int dtype, const LinearScratch& lent, hipStream_t stream);
+int launch_linear_act_16(const LinearProblem& p, int dtype, const LinearScratch& lent, hipStream_t stream);
+int launch_linear_act_w8(const LinearProblem& p, int dtype, const LinearScratch& lent, hipStream_t stream);
+int launch_linear_act_int8(const LinearProblem& p, int dtype, const LinearScratch& lent, hipStream_t stream);
 int launch_linear_act_tiles(const LinearProblem& p, int dtype, hipStream_t stream);
 // ... and for few rows (linear_few.hip): whether that kernel takes a problem, and the launch.
 bool linear_few_takes(const LinearProblem& p);

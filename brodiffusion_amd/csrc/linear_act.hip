@@ -1,21 +1,25 @@
 // Y = act(X W^T [* w_scales] [* x_scales] + bias) + residual: the linear layer with its epilogue, for 16-bit operands, INT8 weights
 // (W8A16) and INT8 operands (W8A8).
-#include "internal.h"
+#include "linear_forms.h"
 
 namespace mi {
 
-int launch_linear_act(const LinearProblem& p, int dtype, hipStream_t st) {
+namespace {
+// what the rings take: tiles that 32-bit byte offsets reach
+bool rings_take(const LinearProblem& p) { return p.ldx * 2 * 256 < (1L << 31) && p.ldw * 2 * 256 < (1L << 31); }
+}  // namespace
+
+int launch_linear_act(const LinearProblem& p, int dtype, const LinearScratch& lent, hipStream_t st) {
     if (linear_few_takes(p)) return launch_linear_few(p, dtype, st);
-    // what the rings do not take: tiles that 32-bit byte offsets do not reach
-    if (p.ldx * 2 * 256 >= (1L << 31) || p.ldw * 2 * 256 >= (1L << 31)) return launch_linear_act_tiles(p, dtype, st);
-    if (p.x_scale) return launch_linear_act_int8(p, dtype, st);
-    return p.w_scale ? launch_linear_act_w8(p, dtype, st) : launch_linear_act_16(p, dtype, st);
+    if (!rings_take(p)) return launch_linear_act_tiles(p, dtype, st);
+    if (p.x_scale) return launch_linear_act_int8(p, dtype, lent, st);
+    return p.w_scale ? launch_linear_act_w8(p, dtype, lent, st) : launch_linear_act_16(p, dtype, lent, st);
 }
 
 namespace {
 
-int linear_act(const mi_linear_act_args& a) {
-    const char* op = "mi_linear_act_forward";
+// The problem of a call, checked. 1: there is one, 0: no rows, -1: refused.
+int problem_of(const mi_linear_act_args& a, const char* op, LinearProblem& p) {
     if (a.dtype != MI_DTYPE_BF16 && a.dtype != MI_DTYPE_F16) return fail("%s: dtype %d is neither MI_DTYPE_F16 nor MI_DTYPE_BF16", op, a.dtype);
     if (a.rows < 0 || a.in_features <= 0 || a.out_features <= 0) return fail("%s: %d rows, %d x %d features", op, a.rows, a.in_features, a.out_features);
     if (a.activation < MI_ACT_NONE || a.activation > MI_ACT_SILU) return fail("%s: activation %d is none of MI_ACT_*", op, a.activation);
@@ -27,7 +31,6 @@ int linear_act(const mi_linear_act_args& a) {
     if (a8 && a.in_features > 131056) return fail("%s: in_features %d exceed the 131056 whose INT32 sums are exact", op, a.in_features);
     if (a.rows == 0) return 0;
     if (!a.x || !a.w || !a.y) return fail("%s: null operand", op);
-    LinearProblem p{};
     p.x = a.x; p.w = a.w; p.bias = a.bias; p.y = a.y; p.residual = a.residual;
     p.w_scale = a.w_scales; p.x_scale = a.x_scales; p.act = a.activation;
     p.M = a.rows; p.N = a.out_features; p.K = a.in_features;
@@ -45,15 +48,39 @@ int linear_act(const mi_linear_act_args& a) {
         return fail("%s: y overlaps the residual", op);
     if (static_cast<long>((p.M + 31) / 32) * ((p.N + 31) / 32) > 0x7ffffff0L) return fail("%s: problem too large for one launch", op);
     if (a8) { p.K /= 2; p.ldx /= 2; p.ldw /= 2; }      // rows of pairs (LinearProblem::x_scale)
-    return launch_linear_act(p, a.dtype, resolve_stream(a.stream));
+    return 1;
+}
+
+size_t scratch_bytes(const LinearProblem& p) {
+    if (linear_few_takes(p) || !rings_take(p)) return 0;
+    LinearBatch b{};
+    b.p[0] = p;
+    const bool w8 = p.w_scale && !p.x_scale;
+    const gemm::Parts s = w8 ? gemm::pick_parts(gemm::kPlainW8, gemm::kPlainW8Forms, gemm::kSplitW8, b, device_cu_count())
+                             : gemm::pick_parts(gemm::kPlain, gemm::kPlainForms, gemm::kSplitPlain, b, device_cu_count());
+    return s.splits > 1 ? static_cast<size_t>(gemm::part_bytes((w8 ? gemm::kPlainW8 : gemm::kPlain)[s.form], p, s.splits)) : 0;
 }
 
 }  // namespace
 }  // namespace mi
 
-extern "C" int mi_linear_act_forward(const mi_linear_act_args* a) {
+extern "C" {
+
+int mi_linear_act_forward(const mi_linear_act_args* a) {
+    const char* op = "mi_linear_act_forward";
     mi::clear_error();
-    if (!a) return mi::fail("mi_linear_act_forward: null args");
-    if (a->struct_size != sizeof(*a)) return mi::fail("mi_linear_act_forward: struct_size %u != %zu (header mismatch)", a->struct_size, sizeof(*a));
-    return mi::linear_act(*a);
+    if (!a) return mi::fail("%s: null args", op);
+    if (a->struct_size != sizeof(*a)) return mi::fail("%s: struct_size %u != %zu (header mismatch)", op, a->struct_size, sizeof(*a));
+    if (reinterpret_cast<uintptr_t>(a->scratch) & 15u) return mi::fail("%s: scratch must be 16-byte aligned", op);
+    mi::LinearProblem p{};
+    const int rc = mi::problem_of(*a, op, p);
+    return rc <= 0 ? rc : mi::launch_linear_act(p, a->dtype, {a->scratch, a->scratch ? a->scratch_bytes : 0}, mi::resolve_stream(a->stream));
 }
+
+size_t mi_linear_act_scratch_bytes(const mi_linear_act_args* a) {
+    mi::LinearProblem p{};
+    if (!a || a->struct_size != sizeof(*a) || mi::problem_of(*a, "mi_linear_act_scratch_bytes", p) != 1) return 0;
+    return mi::scratch_bytes(p);
+}
+
+}  // extern "C"

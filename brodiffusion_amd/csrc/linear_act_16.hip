@@ -8,8 +8,8 @@ namespace gemm {
 namespace {
 
 template <typename T>
-int launch_form(const LinearBatch& b, hipStream_t st) {
-    switch (pick_form(kPlain, kPlainForms, b, 1, device_cu_count())) {
+int launch_form(const LinearBatch& b, int form, hipStream_t st) {
+    switch (form) {
         case k32x32: return launch_pipe<T, false, false, 1, 1, 1, 1, 6, 2, T, true>(b, 1, st);
         case k64x32: return launch_pipe<T, false, false, 2, 1, 1, 1, 6, 2, T, true>(b, 1, st);
         case k64x64: return launch_pipe<T, false, false, 2, 2, 1, 1, 4, 4, T, true>(b, 1, st);
@@ -24,14 +24,30 @@ int launch_form(const LinearBatch& b, hipStream_t st) {
         default: return gemm_dma::launch_t<T, T, true>(b, 1, st);
     }
 }
+// ... in several parts (the forms of kSplitPlain)
+template <typename T>
+int launch_split(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
+    switch (s.form) {
+        case k32x32: return launch_pipe<T, false, false, 1, 1, 1, 1, 6, 2, T, true, 16, true>(b, 1, st, s.splits, parts);
+        case k64x64: return launch_pipe<T, false, false, 2, 2, 1, 1, 4, 4, T, true, 16, true>(b, 1, st, s.splits, parts);
+        case k128x64_load: return launch_pipe<T, false, false, 2, 2, 2, 1, 3, 4, T, true, 16, true>(b, 1, st, s.splits, parts);
+        default: return launch_pipe<T, false, false, 2, 2, 2, 2, 3, 4, T, true, 16, true>(b, 1, st, s.splits, parts);
+    }
+}
+template <typename T>
+int launch_any(const LinearBatch& b, const LinearScratch& lent, hipStream_t st) {
+    const Parts s = pick_parts(kPlain, kPlainForms, kSplitPlain, b, device_cu_count());
+    if (s.splits > 1 && lent.bytes >= static_cast<size_t>(part_bytes(kPlain[s.form], b.p[0], s.splits))) return launch_split<T>(b, s, lent.p, st);
+    return launch_form<T>(b, pick_form(kPlain, kPlainForms, b, 1, device_cu_count()), st);
+}
 
 }  // namespace
 }  // namespace gemm
 
-int launch_linear_act_16(const LinearProblem& p, int dtype, hipStream_t st) {
+int launch_linear_act_16(const LinearProblem& p, int dtype, const LinearScratch& lent, hipStream_t st) {
     LinearBatch b{};
     b.p[0] = p;
-    return dtype == MI_DTYPE_BF16 ? gemm::launch_form<__bf16>(b, st) : gemm::launch_form<_Float16>(b, st);
+    return dtype == MI_DTYPE_BF16 ? gemm::launch_any<__bf16>(b, lent, st) : gemm::launch_any<_Float16>(b, lent, st);
 }
 
 }  // namespace mi

@@ -76,7 +76,13 @@ struct PipeArgs {
     PipeProblem p[kMaxLinearProblems];
     int first[kMaxLinearProblems];       // first tile of a problem
     int n_tiles, chunk;
+    int splits;                          // ACT instances: work groups that share a tile's contraction (blockIdx.y), and where each leaves its
+    void* parts;                         // sums (PipeParts) if there are several
 };
+// The sums of a tile's parts: per tile and part, every multiplying wavefront's groups of 4 features x BS tokens, 64 lanes of 16 bytes each.
+template <int NW, int GROUPS> __device__ __forceinline__ long part_of(int tile, int splits, int split, int wave, int group, int lane) {
+    return (((static_cast<long>(tile) * splits + split) * NW + wave) * GROUPS + group) * 64 + lane;
+}
 // x / d and x % d for x < 2^32; inv = floor(2^32 / d), one less for d = 1: the estimate is at most one short
 struct DivMod { int q, r; };
 __device__ __forceinline__ DivMod div_mod(int x, int d, unsigned inv) {
@@ -188,8 +194,18 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
         else dma(woff[j < G::MX ? 0 : j - G::MX], wg, lds_base + slot + G::X_BYTES + (lw + G::LW * (j - G::MX)) * 1024);
     };
     // ACT: how many contraction elements the last stage holds, and the stage that xg and wg stand on
-    const int stages = ACT ? (p.K + kBK - 1) / kBK : 0;
-    const int in_last = ACT ? p.K - (stages - 1) * kBK : kBK;
+    int stages = 0, in_last = kBK;
+    if constexpr (ACT) {
+        stages = (p.K + kBK - 1) / kBK;
+        in_last = p.K - (stages - 1) * kBK;
+        if (args.splits > 1) {      // (this part's stages; the divisions are left to those launches)
+            const int all = stages, part = static_cast<int>(blockIdx.y), from = part * all / args.splits, to = (part + 1) * all / args.splits;
+            stages = to - from;
+            if (to < all) in_last = kBK;
+            xg += static_cast<long>(from) * (kBK * 2);
+            wg += static_cast<long>(from) * (W8 ? kBK : kBK * 2);
+        }
+    }
     int loading = 0;
     auto shorten = [&]() {
 #pragma unroll
@@ -374,6 +390,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
                 load_stage();
             }
             for (; t < n - 1; ++t) wait_barrier(n - 2 - t);
+            if (ACT && args.splits > 1) return;
             if (ACT && p.residual != nullptr) __syncthreads();
             __syncthreads();
             __syncthreads();
@@ -446,7 +463,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
         const int row = tid / PPR, piece = tid % PPR;
         // the residual's pieces that this thread will write again as pieces of Y, on their way during the last stage (no load of the ring
         // is waited for any more)
-        if (p.residual != nullptr) {
+        if (p.residual != nullptr && args.splits == 1) {
             const unsigned char* const rg = static_cast<const unsigned char*>(p.residual) + min(n0 + piece * 8, p.N - 8) * 2L;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) out[i] = *reinterpret_cast<const u32x4*>(rg + static_cast<long>(min(m0 + row + i * RSTEP, p.M - 1)) * p.ldr_b);
@@ -458,6 +475,22 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     blank_half(Half1{});
     multiply_half(Half1{}, std::false_type{}, 0u, Half0{}, Half0{}, 0u);
 
+    if constexpr (ACT) {
+        if (args.splits > 1) {
+            using Sum = typename M::sum4;
+            Sum* const parts = static_cast<Sum*>(args.parts);
+#pragma unroll
+            for (int a = 0; a < FB * NG; ++a)
+#pragma unroll
+                for (int b = 0; b < TB; ++b) {
+                    Sum v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = acc[a / NG][b][4 * (a % NG) + i];
+                    parts[part_of<G::NW, FB * NG * TB>(tile, args.splits, blockIdx.y, wave, a * TB + b, lane)] = v;
+                }
+            return;
+        }
+    }
     __syncthreads();   // the ring is used up
     // ── epilogue: acc[a][b][i] is feature n0 + wn TN 32 + 16 a + 4 lg + i of token m0 + wm TM 32 + 16 b + lr; the tile
     //    leaves through LDS as 16-byte pieces of rows of Y ──
@@ -552,8 +585,53 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     }
 }
 
-template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16>
-int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st) {
+// Adds the parts of every tile in their order and finishes the layer: a wavefront per group of 4 features x BS tokens.
+template <typename T, bool W8, int WM, int WN, int TM, int TN, typename A>
+__global__ void __launch_bounds__(256) linear_join_kernel(const PipeArgs args) {
+    constexpr bool A8 = std::is_same_v<A, Int8>, ONE = W8 && TM == 1 && TN == 1;
+    constexpr int BS = ONE ? 32 : 16, FB = TN * 32 / BS, TB = TM * 32 / BS, NG = ONE ? 4 : 1, GROUPS = FB * NG * TB, NW = WM * WN;
+    using V4 = typename Mma<T>::v4;
+    using Sum = typename Mma<A>::sum4;
+    const PipeProblem& p = args.p[0];
+    const int lane = threadIdx.x & 63, lr = lane % BS, lg = lane / BS;
+    const int id = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6);
+    const int group = id % GROUPS, wave = id / GROUPS % NW, tile = id / (GROUPS * NW);
+    if (tile >= args.n_tiles) return;
+    // (tiles are numbered as in linear_pipe_kernel)
+    const int panel = tile / p.panel_tiles, in_panel = tile % p.panel_tiles, width = panel == p.n_panels - 1 ? p.last_width : p.width;
+    const int token = in_panel / width * (WM * TM * 32) + wave % WM * TM * 32 + BS * (group % TB) + lr;
+    const int feature = (panel * p.width + in_panel % width) * (WN * TN * 32) + wave / WM * TN * 32 + BS / NG * (group / TB) + 4 * lg;
+    if (token >= p.M || feature >= p.N) return;
+    const Sum* const parts = static_cast<const Sum*>(args.parts);
+    Sum sum = parts[part_of<NW, GROUPS>(tile, args.splits, 0, wave, group, lane)];
+    for (int s = 1; s < args.splits; ++s) {
+        const Sum next = parts[part_of<NW, GROUPS>(tile, args.splits, s, wave, group, lane)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += next[i];
+    }
+    V4 bias{}, res{};
+    if (p.bias) bias = *reinterpret_cast<const V4*>(static_cast<const T*>(p.bias) + feature);
+    if (p.residual) res = *reinterpret_cast<const V4*>(static_cast<const unsigned char*>(p.residual) + static_cast<long>(token) * p.ldr_b + feature * 2L);
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float b = static_cast<float>(bias[i]), s = static_cast<float>(sum[i]);
+        if constexpr (A8) v[i] = scaled_acc(s, p.x_scale[token] * p.w_scale[feature + i], b);
+        else if constexpr (W8) v[i] = scaled_acc(s, p.w_scale[feature + i], b);
+        else v[i] = s + b;
+    }
+    with_activation(p.act, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = act(v[i]);
+    });
+    V4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = static_cast<T>(v[i] + static_cast<float>(res[i]));
+    *reinterpret_cast<V4*>(static_cast<unsigned char*>(p.y) + static_cast<long>(token) * p.ldy_b + feature * 2L) = o;
+}
+
+template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16, bool JOIN = false>
+int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st, int splits = 1, void* parts = nullptr) {
     using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL, WL>;
     auto tiles_m = [&](int i) { return (batch.p[i].M + G::BM - 1) / G::BM; };
     auto tiles_n = [&](int i) { return (batch.p[i].N + G::BN_OUT - 1) / G::BN_OUT; };
@@ -571,6 +649,8 @@ int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st) {
     auto inverse = [](int d) { return d == 1 ? 0xffffffffu : static_cast<unsigned>((1ull << 32) / static_cast<unsigned>(d)); };
     PipeArgs args{};
     args.n_tiles = static_cast<int>(tiles);
+    args.splits = splits;
+    args.parts = parts;
     args.chunk = (args.n_tiles + 7) / 8;
     int first = 0;
     for (int i = 0; i < kMaxLinearProblems; ++i) {
@@ -589,8 +669,13 @@ int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st) {
         p.inv_panel = inverse(p.panel_tiles); p.inv_width = inverse(p.width); p.inv_last = inverse(p.last_width);
         first += tiles_m(i) * tiles_n(i);
     }
-    hipLaunchKernelGGL((linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL>), dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(G::NT + 64 * NL), G::LDS, st, args);
+    hipLaunchKernelGGL((linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL>), dim3(static_cast<unsigned>((tiles + 7) / 8 * 8), ACT ? splits : 1), dim3(G::NT + 64 * NL), G::LDS, st, args);
     MI_HIP_CHECK(hipGetLastError());
+    if constexpr (JOIN) {
+        const long waves = tiles * G::BM * G::BN / 256;      // of 4 features x 64 lanes
+        hipLaunchKernelGGL((linear_join_kernel<T, W8, WM, WN, TM, TN, A>), dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, st, args);
+        MI_HIP_CHECK(hipGetLastError());
+    }
     return 0;
 }
 

@@ -346,6 +346,13 @@ void linear_act(const Tensor& X, const Tensor* x_scales, const Tensor& W, const 
     a.x = X.data; a.w = W.data; a.y = Y.data;
     a.rows = X.rows; a.in_features = X.cols; a.out_features = W.rows;
     a.activation = static_cast<int>(activation);
+    struct LinearActScratch;
+    Tensor& scratch = per_stream<Tensor, LinearActScratch>();
+    if (const std::size_t need = mi_linear_act_scratch_bytes(&a); need > 0) {
+        if (scratch.data == nullptr || scratch.bytes() < need) scratch.resize(1, static_cast<int>((need + 3) / 4), Dtype::FP32, Device::GPU);
+        a.scratch = scratch.data;
+        a.scratch_bytes = scratch.bytes();
+    }
     check(op, mi_linear_act_forward(&a));
 }
 

@@ -44,6 +44,7 @@ struct Lib {
     decltype(&mi_add_rms_norm_forward) add_rms_norm;
     decltype(&mi_quantize_rows_forward) quantize_rows;
     decltype(&mi_linear_act_forward) linear_act;
+    decltype(&mi_linear_act_scratch_bytes) linear_act_scratch_bytes;
     decltype(&mi_attn_block_scratch_bytes) block_scratch_bytes;
     decltype(&mi_flash_attention_qkvo_forward) qkvo;
     decltype(&mi_flash_attention_q_with_kv_cached_forward) kv_cached;
@@ -348,7 +349,7 @@ int activation_of(PyObject* o) {
 }
 // X, W, bias, activation, residual, x_scales, w_scales, dtype, out
 NATIVE(linear_act, 9)
-    need(L.linear_act != nullptr);
+    need(L.linear_act != nullptr && L.linear_act_scratch_bytes != nullptr);
     const Tensor &x = tensor(a[0]), &w = tensor(a[1]);
     mi_linear_act_args p;
     std::memset(&p, 0, sizeof(p));
@@ -396,6 +397,12 @@ NATIVE(linear_act, 9)
     p.x = x.data_ptr(); p.w = w.data_ptr(); p.y = y.data_ptr();
     p.rows = rows32(rows); p.in_features = rows32(w.size(1)); p.out_features = rows32(n_out);
     p.stream = current_stream();
+    // (from the allocator, per call: its memory is this stream's until the call is done, and a captured graph's own)
+    Tensor scratch;
+    if (const size_t bytes = L.linear_act_scratch_bytes(&p)) {
+        scratch = at::empty({static_cast<int64_t>(bytes)}, y.options().dtype(at::kByte));
+        p.scratch = scratch.data_ptr(); p.scratch_bytes = bytes;
+    }
     run("linear_act", [&] { return L.linear_act(&p); });
     return given(a[8], y);
 NATIVE_END
@@ -795,6 +802,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     if (!ok) return PyErr_Format(PyExc_RuntimeError, "%s does not export every function of mi_attention.h: build the library again", path);
     // (a library without these binds all the same: their calls decline, and the Python code says what is missing)
     get(L.add_rms_norm, "mi_add_rms_norm_forward"); get(L.quantize_rows, "mi_quantize_rows_forward"); get(L.linear_act, "mi_linear_act_forward");
+    get(L.linear_act_scratch_bytes, "mi_linear_act_scratch_bytes");
     Py_INCREF(lend);
     Py_XSETREF(lend_scratch, lend);
     bound = true;

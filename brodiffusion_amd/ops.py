@@ -1266,6 +1266,11 @@ def linear_act(X, W, bias=None, *, activation: str = "none", residual: Optional[
     a.x, a.w, a.y, a.y_row_stride = X.data_ptr(), W.data_ptr(), out.data_ptr(), _rows_of(op, out, "out", dtype, shape)[1]
     a.activation = _ACTIVATIONS[activation]
     a.stream = _stream()
+    # (from the allocator, per call: its memory is this stream's until the call is done, and a captured graph's own)
+    need = int(capi.lib().mi_linear_act_scratch_bytes(C.byref(a)))
+    if need > 0:
+        scratch = torch.empty(need, dtype=torch.uint8, device=X.device)
+        a.scratch, a.scratch_bytes = scratch.data_ptr(), need
     capi.check(capi.lib().mi_linear_act_forward(C.byref(a)), op)
     return out
 

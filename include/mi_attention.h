@@ -507,9 +507,17 @@ typedef struct mi_linear_act_args {
     const float* x_scales;   /* NULL, or (rows): x is INT8 */
     const float* w_scales;   /* NULL, or (out_features): w is INT8 */
     int32_t activation;      /* MI_ACT_* */
+    void* scratch;           /* device, 16-byte aligned, or NULL: with mi_linear_act_scratch_bytes(args) bytes a launch of few output tiles and a
+                                long contraction gives each tile to several work groups, which leave their sums here for a second
+                                small launch to add in a fixed order. The next call on the stream may use it again; calls that can overlap
+                                on the GPU (two streams, two captured graphs replayed together) must not share one */
+    size_t scratch_bytes;
     void* stream;
 } mi_linear_act_args;
 MI_API int mi_linear_act_forward(const mi_linear_act_args* args);
+/* Bytes of scratch that this call would use (the scratch fields are ignored): 0 where it would not, or is one that is refused. With less the
+ * call does without; results agree to rounding (INT8 rows: the sums are exact either way, so bit for bit). */
+MI_API size_t mi_linear_act_scratch_bytes(const mi_linear_act_args* args);
 
 /* ── attention with its projections ────────────────────────────────────────
  * The three operators the U-Net spatial transformer calls (src/unet_blocks.cpp:255-327,
