@@ -83,25 +83,29 @@ inline int pick_form(const LinearBatch& batch, int n_problems, bool geglu, int n
 }
 
 // ── several work groups for a tile's contraction (the layer with an epilogue, where the caller lends memory for their sums) ──
-// Parts leave FP32 or INT32 sums, a second launch adds them and finishes the layer: about 4 us and the bytes of the parts, written and read at
+// Parts leave FP32 or INT32 sums, a second launch adds them and finishes the layer: 3 to 4 us and the bytes of the parts, written and read at
 // 4 TB/s. Paid where few tiles have a long contraction (us, one part / several, 16-bit; rows x features x contraction): 46 x 368 x 15984 29.5 / 10.8
 // (8 parts of 32 x 32 tiles), 382 x 352 x 14856 28.8 / 20.0 (6 of 64 x 64), 436 x 1200 x 6472 33.1 / 21.9 (6 of 128 x 128); not for 40 x 320 x 1280
-// 5.7 / 6.4 or 1031 x 1152 x 4608 19.8 / 22.0. Taken where the rule below expects a tenth less.
+// 5.7 / 6.4 or 1031 x 1152 x 4608 19.8 / 22.0. Taken where the rule below expects a twentieth less; over 140 such problems of 33 to 1500 rows the time
+// was 0.76 (16-bit), 0.54 (W8A16) and 0.83 (W8A8) of one part's on average, at worst 1.26 (49 x 2616 x 10544 W8A8 12.5 -> 15.6).
 struct Parts { int form, splits; };
 constexpr int kSplitPlain[] = {k32x32, k64x64, k128x64_load, k128x128};
 constexpr int kSplitW8[] = {k8_32x32, k8_64x64, k8_128x64, k8_128x96};
 inline long tiles_of(const Form& f, const LinearProblem& p) { return static_cast<long>((p.M + f.bm - 1) / f.bm) * ((p.N + f.bn_out - 1) / f.bn_out); }
 inline long part_bytes(const Form& f, const LinearProblem& p, int splits) { return tiles_of(f, p) * splits * f.bm * f.bn_out * 4; }
+// Rows that do not begin on 128-byte lines make a stage's pieces of a row two lines instead of one and its step longer (436 x 1200 x 6472
+// 33 us on 64 x 64 tiles, 18 by the constants above); steps of INT8 weights are long for their widening, whatever the lines.
 inline Parts pick_parts(const Form* forms, int n_forms, const int (&split_forms)[4], const LinearBatch& b, int n_cu) {
     const LinearProblem& p = b.p[0];
-    const double steps = p.K / 64;
+    const bool lines = (p.w_scale && !p.x_scale) || (p.ldx * 2 % 128 == 0 && p.ldw * 2 % 128 == 0);
+    const double steps = p.K / 64 * (lines ? 1.0 : 1.25);
     auto cost = [&](const Form& f, int splits) {
         const double m = static_cast<double>((tiles_of(f, p) * splits + n_cu - 1) / n_cu), s = steps / splits;
-        return f.phi + s * f.lam + (m - 1) * (s * f.tau + f.eps) + (splits > 1 ? 4.0 + 2.0 * part_bytes(f, p, splits) / 4e6 : 0.0);
+        return f.phi + s * f.lam + (m - 1) * (s * f.tau + f.eps) + (splits > 1 ? 3.0 + 2.0 * part_bytes(f, p, splits) / 4e6 : 0.0);
     };
     const int whole = pick_form(forms, n_forms, b, 1, n_cu);
     Parts best{whole, 1};
-    double best_cost = 0.9 * cost(forms[whole], 1);
+    double best_cost = 0.95 * cost(forms[whole], 1);
     for (int f : split_forms)
         for (int splits : {2, 3, 4, 6, 8, 12, 16}) {
             if (splits * 4 > p.K / 64) break;

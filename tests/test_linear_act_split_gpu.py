@@ -50,6 +50,8 @@ def test_parts(kind, M, N, K, form, splits):
     # (whole stages, a partial last one, INT8 weights on 8-byte rows; twice the contraction of INT8 operands is the same stages)
     for more in (0, 8, 40):
         k = 2 * (K + more) if kind == "w8a8" else K + more
+        splits = _parts(M, N, K + more, kind == "w8")[1]       # (rows off 128-byte lines: more parts)
+        assert splits > 1
         c = make(M + N + K + more, kind, M, N, k, "bf16" if more else "fp16", residual=more != 8)
         act = ("none", "gelu", "silu")[more % 3]
         wide = torch.full((M + 1, N), 7.0, dtype=c["dt"], device="cuda")
