@@ -148,6 +148,15 @@ inline bool operands_overlap(const void* a, long a_rs, long a_bs, const void* b,
     return column < len || column > a_rs - len;
 }
 
+// Whether two operands of `rows` rows share a byte. Equal strides: by column; otherwise by their whole ranges.
+inline bool rows_share(const void* a, long a_rs, long a_len, const void* b, long b_rs, long b_len, long rows) {
+    const long apart = static_cast<long>(reinterpret_cast<intptr_t>(a)) - static_cast<long>(reinterpret_cast<intptr_t>(b));     // from b to a
+    if (apart >= (rows - 1) * b_rs + b_len || apart + (rows - 1) * a_rs + a_len <= 0) return false;
+    if (a_rs != b_rs) return true;
+    const long column = (apart % a_rs + a_rs) % a_rs;      // a's first byte in b's rows
+    return column < b_len || column > a_rs - a_len;
+}
+
 // One Y = X W^T + bias problem: X (M, K), W (N, K), Y (M, N), bias (N) or null; strides in elements.
 struct LinearProblem {
     const void* x; const void* w; const void* bias; void* y;

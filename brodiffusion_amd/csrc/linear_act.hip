@@ -46,6 +46,10 @@ int problem_of(const mi_linear_act_args& a, const char* op, LinearProblem& p) {
     if ((reinterpret_cast<uintptr_t>(p.x_scale) | reinterpret_cast<uintptr_t>(p.w_scale)) & 3u) return fail("%s: scales must be 4-byte aligned", op);
     if (p.residual && !(p.residual == p.y && p.ldr == p.ldy) && operands_overlap(p.residual, p.ldr, 0, p.y, p.ldy, 0, 1, p.M, p.N))
         return fail("%s: y overlaps the residual", op);
+    const long x_bytes = a8 ? 1 : 2, w_bytes = a.w_scales ? 1 : 2;
+    if (rows_share(p.y, 2 * p.ldy, 2L * p.N, p.x, x_bytes * p.ldx, x_bytes * p.K, p.M)) return fail("%s: y overlaps x", op);
+    const char *const w0 = static_cast<const char*>(p.w), *const y0 = static_cast<const char*>(p.y);
+    if (y0 < w0 + w_bytes * ((p.N - 1) * p.ldw + p.K) && w0 < y0 + 2 * ((p.M - 1) * p.ldy + p.N)) return fail("%s: y overlaps w", op);
     if (static_cast<long>((p.M + 31) / 32) * ((p.N + 31) / 32) > 0x7ffffff0L) return fail("%s: problem too large for one launch", op);
     if (a8) { p.K /= 2; p.ldx /= 2; p.ldw /= 2; }      // rows of pairs (LinearProblem::x_scale)
     return 1;

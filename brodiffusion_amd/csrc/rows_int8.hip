@@ -200,15 +200,6 @@ int launch(const RowsArgs& a, int dtype, bool norm, hipStream_t st) {
     return norm ? launch_width<_Float16, true>(a, st) : launch_width<_Float16, false>(a, st);
 }
 
-// Whether two operands of `rows` rows share a byte. Equal strides: by column; otherwise by their whole ranges.
-bool share(const void* a, long a_rs, long a_len, const void* b, long b_rs, long b_len, long rows) {
-    const long apart = static_cast<long>(reinterpret_cast<intptr_t>(a)) - static_cast<long>(reinterpret_cast<intptr_t>(b));     // from b to a
-    if (apart >= (rows - 1) * b_rs + b_len || apart + (rows - 1) * a_rs + a_len <= 0) return false;
-    if (a_rs != b_rs) return true;
-    const long column = (apart % a_rs + a_rs) % a_rs;      // a's first byte in b's rows
-    return column < b_len || column > a_rs - a_len;
-}
-
 struct Operand { const char* name; const void* p; long rs, len; };      // bytes
 
 int check_rows(const char* op, int dtype, int rows, int cols) {
@@ -231,10 +222,10 @@ int check_operands(const char* op, int rows, int cols, const Operand* ins, int n
         const Operand& o = outs[i];
         if (o.p == nullptr) continue;
         for (int j = 0; j < n_in; ++j)
-            if (ins[j].p != nullptr && !(o.p == ins[j].p && o.rs == ins[j].rs && o.len == ins[j].len) && share(o.p, o.rs, o.len, ins[j].p, ins[j].rs, ins[j].len, rows))
+            if (ins[j].p != nullptr && !(o.p == ins[j].p && o.rs == ins[j].rs && o.len == ins[j].len) && rows_share(o.p, o.rs, o.len, ins[j].p, ins[j].rs, ins[j].len, rows))
                 return fail("%s: %s overlaps %s", op, o.name, ins[j].name);
         for (int j = 0; j < i; ++j)
-            if (outs[j].p != nullptr && share(o.p, o.rs, o.len, outs[j].p, outs[j].rs, outs[j].len, rows)) return fail("%s: %s overlaps %s", op, o.name, outs[j].name);
+            if (outs[j].p != nullptr && rows_share(o.p, o.rs, o.len, outs[j].p, outs[j].rs, outs[j].len, rows)) return fail("%s: %s overlaps %s", op, o.name, outs[j].name);
     }
     return 0;
 }

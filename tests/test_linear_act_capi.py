@@ -73,7 +73,8 @@ REFUSED = [
         (dict(x_scales=0x60000, w_scales=0x70000, in_features=72), "multiple of 16"), (dict(x_scales=0x60000, w_scales=0x70000, in_features=131072), "131056"),
         (dict(x_scales=0x60000, w_scales=0x70000, x_row_stride=72), "row strides"), (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"),
         (dict(x_row_stride=60), "row strides"), (dict(x_row_stride=56), "smaller"), (dict(residual_row_stride=32), "smaller"), (dict(bias=0x30008), "16-byte"),
-        (dict(w_scales=0x60002), "4-byte"), (dict(y=0x40010), "overlaps the residual"), (dict(y=0x40000, y_row_stride=48), "overlaps the residual")]),
+        (dict(w_scales=0x60002), "4-byte"), (dict(y=0x40010), "overlaps the residual"), (dict(y=0x40000, y_row_stride=48), "overlaps the residual"),
+        (dict(y=0x10020), "overlaps x"), (dict(y=0x20100), "overlaps w"), (dict(y=0x10100, x_row_stride=96, residual=None), "overlaps x")]),
 ]
 
 
