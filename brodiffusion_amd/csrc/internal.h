@@ -157,6 +157,13 @@ inline bool rows_share(const void* a, long a_rs, long a_len, const void* b, long
     return column < b_len || column > a_rs - a_len;
 }
 
+// Whether two runs of bytes share one; null: not there
+inline bool runs_share(const void* a, long a_len, const void* b, long b_len) {
+    const char *const p = static_cast<const char*>(a), *const q = static_cast<const char*>(b);
+    return p && q && p < q + b_len && q < p + a_len;
+}
+constexpr long kMostStride = 1L << 40;      // of rows, in elements: offsets stay within 64 bits whatever the rows
+
 // One Y = X W^T + bias problem: X (M, K), W (N, K), Y (M, N), bias (N) or null; strides in elements.
 struct LinearProblem {
     const void* x; const void* w; const void* bias; void* y;

@@ -25,6 +25,8 @@ int problem_of(const mi_linear_act_args& a, const char* op, LinearProblem& p) {
     if (a.activation < MI_ACT_NONE || a.activation > MI_ACT_SILU) return fail("%s: activation %d is none of MI_ACT_*", op, a.activation);
     const bool a8 = a.x_scales != nullptr;
     if (a8 && !a.w_scales) return fail("%s: INT8 rows need INT8 weights (w_scales)", op);
+    // (tile and step indices are 32-bit)
+    if (a.rows > 1 << 30 || a.in_features > 1 << 30 || a.out_features > 1 << 30) return fail("%s: more than 2^30 rows or features are not supported", op);
     const int step = a8 ? 16 : 8;
     if (a.in_features % step || a.out_features % 8) return fail("%s: in_features %d must be a multiple of %d, out_features %d of 8", op, a.in_features, step, a.out_features);
     // 128 * 128 * in_features stays below 2^31
@@ -40,6 +42,8 @@ int problem_of(const mi_linear_act_args& a, const char* op, LinearProblem& p) {
     p.ldr = a.residual_row_stride ? a.residual_row_stride : a.out_features;
     if (p.ldx % step || p.ldw % step || p.ldy % 8 || p.ldr % 8) return fail("%s: row strides must be multiples of 8 elements (INT8 rows and their weights: of 16)", op);
     if (p.ldx < p.K || p.ldw < p.K || p.ldy < p.N || (p.residual && p.ldr < p.N)) return fail("%s: a row stride is smaller than the row", op);
+    for (long s : {p.ldx, p.ldw, p.ldy, p.ldr})
+        if (s > kMostStride) return fail("%s: a row stride exceeds 2^40 elements", op);
     uintptr_t al = 0;
     for (const void* q : {p.x, p.w, p.bias, p.residual, static_cast<const void*>(p.y)}) al |= reinterpret_cast<uintptr_t>(q);
     if (al & 15u) return fail("%s: operands must be 16-byte aligned", op);
@@ -48,8 +52,10 @@ int problem_of(const mi_linear_act_args& a, const char* op, LinearProblem& p) {
         return fail("%s: y overlaps the residual", op);
     const long x_bytes = a8 ? 1 : 2, w_bytes = a.w_scales ? 1 : 2;
     if (rows_share(p.y, 2 * p.ldy, 2L * p.N, p.x, x_bytes * p.ldx, x_bytes * p.K, p.M)) return fail("%s: y overlaps x", op);
-    const char *const w0 = static_cast<const char*>(p.w), *const y0 = static_cast<const char*>(p.y);
-    if (y0 < w0 + w_bytes * ((p.N - 1) * p.ldw + p.K) && w0 < y0 + 2 * ((p.M - 1) * p.ldy + p.N)) return fail("%s: y overlaps w", op);
+    const long y_run = 2 * ((p.M - 1) * p.ldy + p.N);      // (from the first byte to the last: what is no rows of y's number is held against all of it)
+    if (runs_share(p.y, y_run, p.w, w_bytes * ((p.N - 1) * p.ldw + p.K))) return fail("%s: y overlaps w", op);
+    if (runs_share(p.y, y_run, p.bias, 2L * p.N)) return fail("%s: y overlaps the bias", op);
+    if (runs_share(p.y, y_run, p.w_scale, 4L * p.N) || runs_share(p.y, y_run, p.x_scale, 4L * p.M)) return fail("%s: y overlaps scales", op);
     if (static_cast<long>((p.M + 31) / 32) * ((p.N + 31) / 32) > 0x7ffffff0L) return fail("%s: problem too large for one launch", op);
     if (a8) { p.K /= 2; p.ldx /= 2; p.ldw /= 2; }      // rows of pairs (LinearProblem::x_scale)
     return 1;

@@ -216,6 +216,7 @@ int check_operands(const char* op, int rows, int cols, const Operand* ins, int n
             const long bytes = o.len / cols;
             if (o.p == nullptr || bytes == 0) continue;
             if (o.rs % (8 * bytes) != 0 || o.rs < o.len) return fail("%s: the row stride of %s must be a multiple of 8 elements and at least cols", op, o.name);
+            if (o.rs > bytes * kMostStride) return fail("%s: the row stride of %s exceeds 2^40 elements", op, o.name);
             if (reinterpret_cast<uintptr_t>(o.p) % (8 * bytes) != 0) return fail("%s: %s must be %ld-byte aligned", op, o.name, 8 * bytes);
         }
     for (int i = 0; i < n_out; ++i) {
@@ -256,10 +257,12 @@ int mi_add_rms_norm_forward(const mi_add_rms_norm_args* a) {
     auto stride = [&](int64_t s) { return s ? static_cast<long>(s) : n; };
     mi::RowsArgs r{a->x, a->residual, a->gain, a->sum_out, a->out, a->out_q, a->out_scales, a->rows, a->cols,
                    stride(a->x_row_stride), stride(a->residual_row_stride), stride(a->sum_row_stride), stride(a->out_row_stride), stride(a->q_row_stride), a->eps};
-    // (gain and scales: rows of nothing but themselves, one behind the other)
+    // (scales: rows of nothing but themselves, one behind the other)
     const mi::Operand ins[] = {{"x", r.x, 2 * r.x_rs, 2 * n}, {"residual", r.residual, 2 * r.r_rs, 2 * n}};
     const mi::Operand outs[] = {{"sum_out", r.sum, 2 * r.s_rs, 2 * n}, {"out", r.out, 2 * r.o_rs, 2 * n}, {"out_q", r.q, r.q_rs, n}, {"out_scales", r.scales, 4, 4}};
     if (mi::check_operands(op, a->rows, a->cols, ins, 2, outs, 4)) return -1;
+    for (const mi::Operand& o : outs)
+        if (mi::runs_share(o.p, (a->rows - 1) * o.rs + o.len, r.gain, 2 * n)) return fail("%s: %s overlaps gain", op, o.name);
     return mi::launch(r, a->dtype, true, mi::resolve_stream(a->stream));
 }
 

@@ -3,7 +3,10 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <unordered_map>
+#include <utility>
+#include <vector>
 
 namespace bdamd {
 namespace {
@@ -290,6 +293,11 @@ namespace {
 void fit(Tensor& t, int rows, int cols, Dtype dt, Device dev) {
     if (t.data == nullptr || t.rows != rows || t.cols != cols || t.dtype != dt) t.resize(rows, cols, dt, dev);
 }
+// An output that has to be made, and so may not be an operand: what is resized loses what it holds
+void own_tensor(const char* op, const char* name, const Tensor* out, std::initializer_list<const Tensor*> others) {
+    for (const Tensor* t : others)
+        if (t == out) fail(std::string(op) + ": " + name + " is another operand too");
+}
 const float* scales_ptr(const char* op, const Tensor* s, const char* name, int n) {
     if (s == nullptr) return nullptr;
     need_gpu(op, *s);
@@ -298,6 +306,12 @@ const float* scales_ptr(const char* op, const Tensor* s, const char* name, int n
 }
 void add_rms_norm_impl(const char* op, const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out, Tensor* scales) {
     need_gpu(op, X); need_gpu(op, gain);
+    if (residual != nullptr) own_tensor(op, "sum", &sum, {&gain, &out, scales});
+    if (scales == nullptr) own_tensor(op, "out", &out, {&gain});
+    else {
+        own_tensor(op, "out", &out, {&X, residual, &gain, scales});
+        own_tensor(op, "scales", scales, {&X, residual, &gain});
+    }
     if (gain.dtype != X.dtype || gain.size() != static_cast<std::size_t>(X.cols)) fail(std::string(op) + ": gain must hold one value of X's dtype per column");
     mi_add_rms_norm_args a;
     std::memset(&a, 0, sizeof(a));
@@ -326,6 +340,7 @@ void linear_act(const Tensor& X, const Tensor* x_scales, const Tensor& W, const 
                 const Tensor* residual, Tensor& Y) {
     const char* op = "linear_act";
     need_gpu(op, X); need_gpu(op, W);
+    own_tensor(op, "Y", &Y, {&X, x_scales, &W, w_scales, bias});
     const Dtype dt = x_scales == nullptr ? X.dtype : residual ? residual->dtype : bias ? bias->dtype : Y.dtype;
     if (x_scales != nullptr && w_scales == nullptr) fail(std::string(op) + ": INT8 rows need INT8 weights (w_scales)");
     if (X.dtype != (x_scales ? Dtype::INT8 : dt) || W.dtype != (w_scales ? Dtype::INT8 : dt)) fail(std::string(op) + ": X and W must be INT8 where they have scales, of Y's dtype otherwise");
@@ -346,12 +361,18 @@ void linear_act(const Tensor& X, const Tensor* x_scales, const Tensor& W, const 
     a.x = X.data; a.w = W.data; a.y = Y.data;
     a.rows = X.rows; a.in_features = X.cols; a.out_features = W.rows;
     a.activation = static_cast<int>(activation);
-    struct LinearActScratch;
-    Tensor& scratch = per_stream<Tensor, LinearActScratch>();
+    // (outgrown scratch is kept, a captured graph may still write to it; each is twice the one before, so that together they are less than the last)
+    struct LinearActScratch { std::vector<Tensor> grown; };
+    auto& scratch = per_stream<LinearActScratch, LinearActScratch>().grown;
     if (const std::size_t need = mi_linear_act_scratch_bytes(&a); need > 0) {
-        if (scratch.data == nullptr || scratch.bytes() < need) scratch.resize(1, static_cast<int>((need + 3) / 4), Dtype::FP32, Device::GPU);
-        a.scratch = scratch.data;
-        a.scratch_bytes = scratch.bytes();
+        if (scratch.empty() || scratch.back().bytes() < need) {
+            const std::size_t bytes = scratch.empty() ? need : std::max(need, 2 * scratch.back().bytes());
+            Tensor next;
+            next.resize(1, static_cast<int>((bytes + 3) / 4), Dtype::FP32, Device::GPU);
+            scratch.push_back(std::move(next));
+        }
+        a.scratch = scratch.back().data;
+        a.scratch_bytes = scratch.back().bytes();
     }
     check(op, mi_linear_act_forward(&a));
 }
@@ -365,6 +386,8 @@ void add_rms_norm_int8(const Tensor& X, const Tensor* residual, const Tensor& ga
 void quantize_rows_int8(const Tensor& X, Tensor& out, Tensor& scales) {
     const char* op = "quantize_rows_int8";
     need_gpu(op, X);
+    own_tensor(op, "out", &out, {&X, &scales});
+    own_tensor(op, "scales", &scales, {&X});
     mi_quantize_rows_args a;
     std::memset(&a, 0, sizeof(a));
     a.struct_size = sizeof(a);

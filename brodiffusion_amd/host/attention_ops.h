@@ -63,13 +63,15 @@ void linear_batched(const Tensor& W, const Tensor* bias, const Tensor& X, Tensor
 
 // Y = act(X W^T [* w_scales] [* x_scales] + bias) + residual (mi_linear_act_forward). With w_scales (W.rows FP32 values) W is INT8; with
 // x_scales (X.rows) X is INT8 too, as quantize_rows_int8 and add_rms_norm_int8 write it, and Y gets the dtype of the residual, the bias,
-// or, without either, the one that it has. bias, residual and the scales may be null; residual may be Y itself.
+// or, without either, the one that it has. bias, residual and the scales may be null; residual may be Y itself. Sums of split contractions
+// go through scratch of the calling thread and its stream, allocated on first use: warm up before a capture, and replay graphs captured on
+// one stream one after the other.
 enum class Activation { None = MI_ACT_NONE, Gelu = MI_ACT_GELU, GeluTanh = MI_ACT_GELU_TANH, Silu = MI_ACT_SILU };
 void linear_act(const Tensor& X, const Tensor* x_scales, const Tensor& W, const Tensor* w_scales, const Tensor* bias, Activation activation,
                 const Tensor* residual, Tensor& Y);
 
 // h = X + residual (null: X, and `sum` is left alone) and the RMS normalisation of its rows: `out` of X's dtype, or INT8 rows with an
-// FP32 scale each (mi_add_rms_norm_forward). `sum` and `out` may be X or the residual. quantize_rows_int8: rows as they are
+// FP32 scale each (mi_add_rms_norm_forward). `sum` and a 16-bit `out` may be X or the residual. quantize_rows_int8: rows as they are
 // (mi_quantize_rows_forward).
 void add_rms_norm(const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out);
 void add_rms_norm_int8(const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out, Tensor& scales);

@@ -491,8 +491,8 @@ MI_API int mi_quantize_rows_forward(const mi_quantize_rows_args* args);
  *                                                 mi_add_rms_norm_forward write it, one scale per row; in_features at most 131056
  * act: MI_ACT_*, GELU with erf, GELU_TANH = x / (1 + exp(-2 sqrt(2 / pi) (x + 0.044715 x^3))), SILU = x / (1 + exp(-x)).
  * in_features and out_features are multiples of 8 (W8A8: in_features of 16); strides in elements (0 = dense), multiples of 8 (INT8 x and
- * its w: of 16); pointers 16-byte aligned. y may be `residual` itself (same pointer and stride); a call whose y shares other memory with the residual,
- * x or w is refused. rows may be 0. */
+ * its w: of 16); pointers 16-byte aligned. y may be `residual` itself (same pointer and stride); a call whose y shares other memory with an
+ * operand is refused, and so are more than 2^30 rows or features. rows may be 0. */
 enum { MI_ACT_NONE = 0, MI_ACT_GELU = 1, MI_ACT_GELU_TANH = 2, MI_ACT_SILU = 3 };
 typedef struct mi_linear_act_args {
     uint32_t struct_size;

@@ -119,6 +119,17 @@ static void test_half(int rows) {
     // into the residual itself
     bt::linear_act(q2, &s2, w2.q, &w2.scales, &b2, bt::Activation::None, &h, h);
     CHECK(h.to_host_bytes() == y.to_host_bytes());
+    // an output that is an operand: refused before anything is resized
+    CHECK(throws_with([&] { bt::add_rms_norm_int8(x, &r, gain, 1e-6f, h, x, s); }, "out is another operand"));
+    CHECK(throws_with([&] { bt::add_rms_norm_int8(x, &r, gain, 1e-6f, q, q, s); }, "sum is another operand"));
+    CHECK(throws_with([&] { bt::add_rms_norm(x, &r, gain, 1e-6f, h, gain); }, "out is another operand"));
+    CHECK(throws_with([&] { bt::quantize_rows_int8(u, u, s2); }, "out is another operand"));
+    CHECK(throws_with([&] { bt::linear_act(u, nullptr, w2.q, &w2.scales, nullptr, bt::Activation::None, nullptr, u); }, "Y is another operand"));
+    CHECK(values(x) == vx && gain.cols == D && u.cols == F);
+    // 16-bit outputs in place
+    Tensor x1 = normal_bf16(11 + rows, rows, D), r1 = normal_bf16(12 + rows, rows, D);
+    bt::add_rms_norm(x1, &r1, gain, 1e-6f, r1, x1);
+    CHECK(values(r1) == vh && values(x1) == vn);
     CHECK(throws_with([&] { bt::linear_act(q2, &s2, w2.q, nullptr, &b2, bt::Activation::None, &h, y); }, "INT8 weights"));
     CHECK(throws_with([&] { bt::linear_act(q2, &s2, w1.q, &w1.scales, nullptr, bt::Activation::None, &h, y); }, "same columns"));
     CHECK(throws_with([&] { bt::linear_act(q2, &s, w2.q, &w1.scales, &b2, bt::Activation::None, &h, y); }, "w_scales"));

@@ -63,7 +63,9 @@ REFUSED = [
         (dict(sum_out=0x50000), "out overlaps sum_out"), (dict(out=0x10010), "out overlaps x"), (dict(sum_out=0x20080), "sum_out overlaps residual"),
         (dict(out_q=0x10000, out_scales=0x60000), "out_q overlaps x"), (dict(out_q=0x60000, out_scales=0x60040), "out_scales overlaps out_q"),
         (dict(out_q=0x60004, out_scales=0x70000), "8-byte aligned"), (dict(out_q=0x60000, out_scales=0x70002), "4-byte"),
-        (dict(out_q=0x60000, out_scales=0x70000, q_row_stride=60), "row stride of out_q")]),
+        (dict(out_q=0x60000, out_scales=0x70000, q_row_stride=60), "row stride of out_q"), (dict(out=0x30000), "out overlaps gain"),
+        (dict(sum_out=0x2ff80), "sum_out overlaps gain"), (dict(out_q=0x60000, out_scales=0x30010), "out_scales overlaps gain"),
+        (dict(x_row_stride=1 << 41), "exceeds 2^40")]),
     ("mi_quantize_rows_forward", _rows, [
         (dict(struct_size=8), "struct_size"), (dict(dtype=0), "dtype"), (dict(cols=4), "multiple of 8"), (dict(x=None), "null"), (dict(out_q=None), "null"),
         (dict(out_scales=None), "null"), (dict(out_q=0x10040), "overlaps"), (dict(x_row_stride=60), "row stride")]),
@@ -74,7 +76,10 @@ REFUSED = [
         (dict(x_scales=0x60000, w_scales=0x70000, x_row_stride=72), "row strides"), (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"),
         (dict(x_row_stride=60), "row strides"), (dict(x_row_stride=56), "smaller"), (dict(residual_row_stride=32), "smaller"), (dict(bias=0x30008), "16-byte"),
         (dict(w_scales=0x60002), "4-byte"), (dict(y=0x40010), "overlaps the residual"), (dict(y=0x40000, y_row_stride=48), "overlaps the residual"),
-        (dict(y=0x10020), "overlaps x"), (dict(y=0x20100), "overlaps w"), (dict(y=0x10100, x_row_stride=96, residual=None), "overlaps x")]),
+        (dict(y=0x10020), "overlaps x"), (dict(y=0x20100), "overlaps w"), (dict(y=0x10100, x_row_stride=96, residual=None), "overlaps x"),
+        (dict(y=0x30010), "overlaps the bias"), (dict(y=0x5ff00, w_scales=0x60000), "overlaps scales"),
+        (dict(y=0x50000, x_scales=0x50004, w_scales=0x70000), "overlaps scales"), (dict(in_features=(1 << 30) + 8), "2^30"),
+        (dict(rows=(1 << 30) + 1), "2^30"), (dict(out_features=(1 << 30) + 8), "2^30"), (dict(w_row_stride=1 << 41), "exceeds 2^40")]),
 ]
 
 
