@@ -63,12 +63,8 @@ int problem_of(const mi_linear_act_args& a, const char* op, LinearProblem& p) {
 
 size_t scratch_bytes(const LinearProblem& p) {
     if (linear_few_takes(p) || !rings_take(p)) return 0;
-    LinearBatch b{};
-    b.p[0] = p;
-    const bool w8 = p.w_scale && !p.x_scale;
-    const gemm::Parts s = w8 ? gemm::pick_parts(gemm::kPlainW8, gemm::kPlainW8Forms, gemm::kSplitW8, b, device_cu_count())
-                             : gemm::pick_parts(gemm::kPlain, gemm::kPlainForms, gemm::kSplitPlain, b, device_cu_count());
-    return s.splits > 1 ? static_cast<size_t>(gemm::part_bytes((w8 ? gemm::kPlainW8 : gemm::kPlain)[s.form], p, s.splits)) : 0;
+    const gemm::Parts s = gemm::pick_parts(p, device_cu_count());
+    return s.splits > 1 ? static_cast<size_t>(gemm::part_bytes(gemm::table_of(p).forms[s.form], p, s.splits)) : 0;
 }
 
 }  // namespace

@@ -34,11 +34,34 @@ int launch_split(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
         default: return launch_pipe<T, false, false, 2, 2, 2, 2, 3, 4, Int8, true, 16, true>(b, 1, st, s.splits, parts);
     }
 }
+// ... of rows that do not begin on lines (kOff), in one part or, with memory for them, several
+template <typename T, bool JOIN>
+int launch_off(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
+    switch (s.form) {
+        case kOff32x32: return launch_pipe<T, false, false, 1, 1, 1, 1, 6, 2, Int8, true, 16, JOIN>(b, 1, st, s.splits, parts);
+        case kOff64x64_row: return launch_pipe<T, false, false, 2, 2, 1, 1, 5, 4, Int8, true, 16, JOIN, true>(b, 1, st, s.splits, parts);
+        case kOff128x64_row: return launch_pipe<T, false, false, 2, 2, 2, 1, 4, 4, Int8, true, 16, JOIN, true>(b, 1, st, s.splits, parts);
+        case kOff128x128_row: return launch_pipe<T, false, false, 2, 2, 2, 2, 4, 4, Int8, true, 16, JOIN, true>(b, 1, st, s.splits, parts);
+    }
+    if constexpr (!JOIN) switch (s.form) {
+        case kOff64x32: return launch_pipe<T, false, false, 2, 1, 1, 1, 6, 2, Int8, true>(b, 1, st);
+        case kOff64x32_row: return launch_pipe<T, false, false, 2, 1, 1, 1, 6, 2, Int8, true, 16, false, true>(b, 1, st);
+        case kOff64x96_row: return launch_pipe<T, false, false, 2, 3, 1, 1, 5, 4, Int8, true, 16, false, true>(b, 1, st);
+        case kOff128x96_row: return launch_pipe<T, false, false, 2, 3, 2, 1, 4, 4, Int8, true, 16, false, true>(b, 1, st);
+        case kOff192x128_row: return launch_pipe<T, false, false, 2, 4, 3, 1, 4, 0, Int8, true, 16, false, true>(b, 1, st);
+        case kOff256x256: return gemm_dma::launch_t<T, gemm::Int8, true>(b, 1, st);
+    }
+    return fail("linear: no kernel for form %d", s.form);      // (not asked for)
+}
 template <typename T>
 int launch_any(const LinearBatch& b, const LinearScratch& lent, hipStream_t st) {
-    const Parts s = pick_parts(kPlain, kPlainForms, kSplitPlain, b, device_cu_count());
-    if (s.splits > 1 && lent.bytes >= static_cast<size_t>(part_bytes(kPlain[s.form], b.p[0], s.splits))) return launch_split<T>(b, s, lent.p, st);
-    return launch_form<T>(b, pick_form(kPlain, kPlainForms, b, 1, device_cu_count()), st);
+    const LinearProblem& p = b.p[0];
+    const FormTable& table = table_of(p);
+    const bool off = off_lines(p);
+    const Parts s = pick_parts(p, device_cu_count());
+    if (s.splits > 1 && lent.bytes >= static_cast<size_t>(part_bytes(table.forms[s.form], p, s.splits))) return off ? launch_off<T, true>(b, s, lent.p, st) : launch_split<T>(b, s, lent.p, st);
+    const int form = s.splits > 1 ? pick_form(table.forms, table.n, b, 1, device_cu_count()) : s.form;
+    return off ? launch_off<T, false>(b, {form, 1}, nullptr, st) : launch_form<T>(b, form, st);
 }
 
 }  // namespace

@@ -31,9 +31,9 @@ int launch_split(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
 }
 template <typename T, int WL>
 int launch_words(const LinearBatch& b, const LinearScratch& lent, hipStream_t st) {
-    const Parts s = pick_parts(kPlainW8, kPlainW8Forms, kSplitW8, b, device_cu_count());
+    const Parts s = pick_parts(b.p[0], device_cu_count());
     if (s.splits > 1 && lent.bytes >= static_cast<size_t>(part_bytes(kPlainW8[s.form], b.p[0], s.splits))) return launch_split<T, WL>(b, s, lent.p, st);
-    return launch_form<T, WL>(b, pick_form(kPlainW8, kPlainW8Forms, b, 1, device_cu_count()), st);
+    return launch_form<T, WL>(b, s.splits > 1 ? pick_form(kPlainW8, kPlainW8Forms, b, 1, device_cu_count()) : s.form, st);
 }
 template <typename T>
 int launch_any(const LinearBatch& b, const LinearScratch& lent, hipStream_t st) {

@@ -35,13 +35,13 @@ struct Form {
     float phi, lam, tau, eps;
 };
 enum { k32x32, k64x32, k64x64, k64x96, k128x64_load, k128x64, k128x96, k128x128, k128x128_2, k192x128, k256x128, k256x256, kPlainForms };
-constexpr Form kPlain[kPlainForms] = {{32, 32, 2.46f, 0.091f, 0.058f, 0.22f},   {64, 32, 2.60f, 0.111f, 0.126f, 0.34f},   {64, 64, 2.52f, 0.154f, 0.190f, 0.42f},
+inline constexpr Form kPlain[kPlainForms] = {{32, 32, 2.46f, 0.091f, 0.058f, 0.22f},   {64, 32, 2.60f, 0.111f, 0.126f, 0.34f},   {64, 64, 2.52f, 0.154f, 0.190f, 0.42f},
                                       {64, 96, 3.10f, 0.225f, 0.240f, 1.50f},   {128, 64, 2.53f, 0.250f, 0.322f, 0.76f},  {128, 64, 2.57f, 0.274f, 0.322f, 0.59f},
                                       {128, 96, 3.50f, 0.318f, 0.360f, 2.30f},  {128, 128, 3.95f, 0.356f, 0.529f, 3.18f}, {128, 128, 3.19f, 0.515f, 0.465f, 1.20f},
                                       {192, 128, 4.67f, 0.511f, 0.727f, 4.11f}, {256, 128, 5.03f, 0.656f, 0.839f, 6.17f}, {256, 256, 8.05f, 1.379f, 1.789f, 6.40f}};
 // INT8 weights: the widening makes small steps dearer and the large tiles no better (those above 128 x 128 are not built)
 enum { k8_32x32, k8_64x64, k8_64x96, k8_128x64, k8_128x96, k8_128x128, k8_128x128_2, kPlainW8Forms };
-constexpr Form kPlainW8[kPlainW8Forms] = {{32, 32, 2.47f, 0.155f, 0.049f, 0.33f},
+inline constexpr Form kPlainW8[kPlainW8Forms] = {{32, 32, 2.47f, 0.155f, 0.049f, 0.33f},
                                           {64, 64, 2.75f, 0.209f, 0.187f, 0.80f},
                                           {64, 96, 3.30f, 0.245f, 0.235f, 0.90f},
                                           {128, 64, 3.03f, 0.325f, 0.286f, 1.43f},
@@ -49,10 +49,10 @@ constexpr Form kPlainW8[kPlainW8Forms] = {{32, 32, 2.47f, 0.155f, 0.049f, 0.33f}
                                           {128, 128, 4.03f, 0.420f, 0.562f, 3.98f},
                                           {128, 128, 2.89f, 0.658f, 0.382f, 3.13f}};
 enum { kG64x64, kG128x64_2, kG128x64, kG256x64, kG192x128, kGegluForms };   // output features; the W tile holds twice as many rows
-constexpr Form kGeglu[kGegluForms] = {{64, 64, 2.65f, 0.377f, 0.330f, 1.20f}, {128, 64, 3.66f, 0.648f, 0.496f, 2.09f}, {128, 64, 4.41f, 0.442f, 0.588f, 4.08f},
+inline constexpr Form kGeglu[kGegluForms] = {{64, 64, 2.65f, 0.377f, 0.330f, 1.20f}, {128, 64, 3.66f, 0.648f, 0.496f, 2.09f}, {128, 64, 4.41f, 0.442f, 0.588f, 4.08f},
                                       {256, 64, 5.99f, 0.800f, 0.834f, 8.98f}, {192, 128, 7.00f, 1.200f, 1.250f, 7.00f}};
 enum { kG8_64x64, kG8_128x64_2, kG8_256x64, kG8_192x128, kGegluW8Forms };
-constexpr Form kGegluW8[kGegluW8Forms] = {{64, 64, 3.92f, 0.315f, 0.302f, 1.17f}, {128, 64, 3.92f, 0.653f, 0.429f, 2.93f}, {256, 64, 7.90f, 0.816f, 1.031f, 6.53f},
+inline constexpr Form kGegluW8[kGegluW8Forms] = {{64, 64, 3.92f, 0.315f, 0.302f, 1.17f}, {128, 64, 3.92f, 0.653f, 0.429f, 2.93f}, {256, 64, 7.90f, 0.816f, 1.031f, 6.53f},
                                           {192, 128, 9.30f, 1.290f, 1.500f, 5.50f}};
 
 // 256 x 256 tiles take contractions from 512 on (below, their prologue is most of the launch).
@@ -82,6 +82,19 @@ inline int pick_form(const LinearBatch& batch, int n_problems, bool geglu, int n
     return geglu ? pick_form(kGeglu, kGegluForms, batch, n_problems, n_cu) : pick_form(kPlain, kPlainForms, batch, n_problems, n_cu);
 }
 
+// ── 16-bit and INT8 operands of the layer with an epilogue whose rows do not begin on 128-byte lines ──
+// The tiles with a window per row (linear_pipe.h, OFF) and, where a launch is short or very large, three forms without. Constants fitted to 168 such
+// problems (33 to 4608 rows, contractions of 328 to 15976 elements, fp16): the form taken is 1.3 % slower than the fastest of 28 timed on average,
+// and the launches take 0.90 of what they took on the forms above (0.64 to 1.22, the worst 333 x 1288 x 328).
+enum { kOff32x32, kOff64x32, kOff256x256, kOff64x32_row, kOff64x64_row, kOff64x96_row, kOff128x64_row, kOff128x96_row, kOff128x128_row, kOff192x128_row, kOffForms };
+inline constexpr Form kOff[kOffForms] = {{32, 32, 3.18f, 0.110f, 0.092f, 0.50f},   {64, 32, 3.33f, 0.153f, 0.141f, 0.85f},   {256, 256, 15.88f, 1.237f, 1.753f, 11.05f},
+                                  {64, 32, 3.88f, 0.145f, 0.109f, 1.01f},   {64, 64, 4.29f, 0.172f, 0.172f, 1.00f},   {64, 96, 4.87f, 0.223f, 0.249f, 3.23f},
+                                  {128, 64, 5.09f, 0.258f, 0.298f, 3.39f},  {128, 96, 6.84f, 0.297f, 0.377f, 4.49f},  {128, 128, 7.38f, 0.333f, 0.435f, 5.34f},
+                                  {192, 128, 8.09f, 0.543f, 0.696f, 5.51f}};
+inline bool off_lines(const LinearProblem& p) {
+    return ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | static_cast<uintptr_t>(p.ldx * 2) | static_cast<uintptr_t>(p.ldw * 2)) & 127) != 0;
+}
+
 // ── several work groups for a tile's contraction (the layer with an epilogue, where the caller lends memory for their sums) ──
 // Parts leave FP32 or INT32 sums, a second launch adds them and finishes the layer: 3 to 4 us and the bytes of the parts, written and read at
 // 4 TB/s. Paid where few tiles have a long contraction (us, one part / several, 16-bit; rows x features x contraction): 46 x 368 x 15984 29.5 / 10.8
@@ -89,27 +102,31 @@ inline int pick_form(const LinearBatch& batch, int n_problems, bool geglu, int n
 // 5.7 / 6.4 or 1031 x 1152 x 4608 19.8 / 22.0. Taken where the rule below expects a twentieth less; over 140 such problems of 33 to 1500 rows the time
 // was 0.76 (16-bit), 0.54 (W8A16) and 0.83 (W8A8) of one part's on average, at worst 1.26 (49 x 2616 x 10544 W8A8 12.5 -> 15.6).
 struct Parts { int form, splits; };
-constexpr int kSplitPlain[] = {k32x32, k64x64, k128x64_load, k128x128};
-constexpr int kSplitW8[] = {k8_32x32, k8_64x64, k8_128x64, k8_128x96};
+inline constexpr int kSplitPlain[] = {k32x32, k64x64, k128x64_load, k128x128};
+inline constexpr int kSplitW8[] = {k8_32x32, k8_64x64, k8_128x64, k8_128x96};
+inline constexpr int kSplitOff[] = {kOff32x32, kOff64x64_row, kOff128x64_row, kOff128x128_row};
+// The forms of a problem of the layer with an epilogue, and those with parts
+struct FormTable { const Form* forms; int n; const int* split; };
+inline constexpr FormTable kTables[] = {{kPlain, kPlainForms, kSplitPlain}, {kPlainW8, kPlainW8Forms, kSplitW8}, {kOff, kOffForms, kSplitOff}};
+inline const FormTable& table_of(const LinearProblem& p) { return kTables[p.w_scale && !p.x_scale ? 1 : off_lines(p) ? 2 : 0]; }
 inline long tiles_of(const Form& f, const LinearProblem& p) { return static_cast<long>((p.M + f.bm - 1) / f.bm) * ((p.N + f.bn_out - 1) / f.bn_out); }
 inline long part_bytes(const Form& f, const LinearProblem& p, int splits) { return tiles_of(f, p) * splits * f.bm * f.bn_out * 4; }
-// Rows that do not begin on 128-byte lines make a stage's pieces of a row two lines instead of one and its step longer (436 x 1200 x 6472
-// 33 us on 64 x 64 tiles, 18 by the constants above); steps of INT8 weights are long for their widening, whatever the lines.
-inline Parts pick_parts(const Form* forms, int n_forms, const int (&split_forms)[4], const LinearBatch& b, int n_cu) {
-    const LinearProblem& p = b.p[0];
-    const bool lines = (p.w_scale && !p.x_scale) || (p.ldx * 2 % 128 == 0 && p.ldw * 2 % 128 == 0);
-    const double steps = p.K / 64 * (lines ? 1.0 : 1.25);
+inline Parts pick_parts(const LinearProblem& p, int n_cu) {
+    const FormTable& table = table_of(p);
+    const double steps = p.K / 64;
     auto cost = [&](const Form& f, int splits) {
         const double m = static_cast<double>((tiles_of(f, p) * splits + n_cu - 1) / n_cu), s = steps / splits;
         return f.phi + s * f.lam + (m - 1) * (s * f.tau + f.eps) + (splits > 1 ? 3.0 + 2.0 * part_bytes(f, p, splits) / 4e6 : 0.0);
     };
-    const int whole = pick_form(forms, n_forms, b, 1, n_cu);
+    LinearBatch b{};
+    b.p[0] = p;
+    const int whole = pick_form(table.forms, table.n, b, 1, n_cu);
     Parts best{whole, 1};
-    double best_cost = 0.95 * cost(forms[whole], 1);
-    for (int f : split_forms)
+    double best_cost = 0.95 * cost(table.forms[whole], 1);
+    for (int i = 0; i < 4; ++i)
         for (int splits : {2, 3, 4, 6, 8, 12, 16}) {
             if (splits * 4 > p.K / 64) break;
-            if (const double c = cost(forms[f], splits); c < best_cost) { best_cost = c; best = {f, splits}; }
+            if (const double c = cost(table.forms[table.split[i]], splits); c < best_cost) { best_cost = c; best = {table.split[i], splits}; }
         }
     return best;
 }

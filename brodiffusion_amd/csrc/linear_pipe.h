@@ -114,7 +114,16 @@ struct PipeGeo {
 // zero must be finite, so in both operands where they can hold anything else). A: the type of the operands where it is not that of Y (Int8: both, K and the strides in
 // pairs of elements; a stage is then 128 contraction elements in the same bytes). WL: bytes that a lane loads of W at a time, 4 where the
 // rows of INT8 weights lie on 8-byte addresses only (contractions that are no multiple of 16).
-template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16>
+// OFF: rows that do not begin on 128-byte lines. A load of 128 bytes of each of 8 such rows touches 16 lines and takes twice the time of one
+// that touches 8, so every row is loaded from the line on that it begins in: piece p of line l of a row that begins s pieces into its line is
+// the row's piece 8 l + p - s. A stage's fragments then lie in its ring slot and, those from piece 8 - s on, in the next one, so that the stage
+// behind the one multiplied has to be there too (and the rings are a stage deeper); s is the same for rows 8 apart, so one number for a lane and
+// all of its blocks, and the swizzle is as good: of 8 rows of one parity, i = 0 .. 7, the positions ((a i + b) mod 8) ^ i with a even are 8
+// different ones. Pieces in front of a row or behind it are loaded as copies of the nearest of the row and not used. Measured (us, without / with,
+// fp16): 436 x 1200 x 6472 32.9 / 22.6 on 64 x 64 tiles, 1024 x 1288 x 5128 34.4 / 24.2 on 64 x 96, 300 x 6144 x 4616 41.3 / 29.2 on
+// 128 x 96, 2048 x 2240 x 2248 35.5 / 28.7 on 192 x 128; not for short launches, 77 x 1160 x 1288 5.7 / 6.1 on 32 x 32. INT8 weights with 16-bit
+// rows gain 1 to 3 % from it (their step is the widening) and go without.
+template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16, bool OFF = false>
 __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(const PipeArgs args) {
     using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL, WL>;
     using M = Mma<A>;
@@ -123,6 +132,8 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     constexpr bool A8 = std::is_same_v<A, Int8>;
     static_assert(!ACT || !GEGLU, "the GEGLU form has its own epilogue");
     static_assert(WL == 16 || (W8 && ACT && WL == 4), "whole pieces, or words of INT8 weights");
+    static_assert(!OFF || (ACT && !W8 && S >= 3), "two stages of the ring are read at a time");
+    constexpr int D = OFF ? 1 : 0;               // stages that must have landed behind the one read
     constexpr int BM = G::BM, BN_OUT = G::BN_OUT, MI = G::MI;
     // one block of INT8 weights per wavefront: v_mfma_f32_32x32x16 (see the top)
     constexpr bool ONE = W8 && TM == 1 && TN == 1;
@@ -225,17 +236,41 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
             if ((W8 ? 16 : 8) * piece >= in_last) woff[u] -= piece * 16;
         }
     };
-    if (ACT && stages == 1) shorten();
+    // OFF: how many pieces into a line row `r` of the tile begins (tiles begin at multiples of 8 rows)
+    auto off_line = [](const void* first, unsigned row_bytes, int r) { return (static_cast<int>(reinterpret_cast<uintptr_t>(first) >> 4) + r * static_cast<int>(row_bytes >> 4)) & 7; };
+    // ... and the offsets for line `loading` of every row; xg and wg stand a line in front of it, so that none is negative
+    auto place = [&]() {
+        const int first = 8 * loading, end = ((stages - 1) * kBK + in_last) / 8 - 1, row = lane >> 3;
+        auto at = [&](int r, int s) { return static_cast<unsigned>(min(max(first + ((lane & 7) ^ ((r >> 1) & 7)) - s, 0), end) - first + 8) * 16u; };
+        const int xs = off_line(p.x, p.ldx_b, row), ws = off_line(p.w, p.ldw_b, row);
+#pragma unroll
+        for (int u = 0; u < G::MX; ++u) {
+            const int r = 8 * (lw + G::LW * u) + row;
+            xoff[u] = static_cast<unsigned>(min(r, p.M - 1 - m0)) * p.ldx_b + at(r, xs);
+        }
+#pragma unroll
+        for (int u = 0; u < G::MW; ++u) {
+            const int r = 8 * (lw + G::LW * u) + row;
+            woff[u] = static_cast<unsigned>(min(r, p.N - 1 - n0)) * p.ldw_b + at(r, ws);
+        }
+    };
+    if constexpr (OFF) {
+        xg -= kBK * 2;
+        wg -= kBK * 2;
+        place();
+    } else if (ACT && stages == 1) shorten();
     auto next_stage = [&]() {
         xg += kBK * 2;
         wg += W8 ? kBK : kBK * 2;
-        if constexpr (ACT) {
+        if constexpr (OFF) {
+            if (++loading <= 1 || loading >= stages - 1) place();
+        } else if constexpr (ACT) {
             if (++loading == stages - 1 && in_last < kBK) shorten();
         }
     };
     // Waits until at most `stages` of this wavefront's stages are in flight and its LDS reads have returned, then meets the others.
     auto wait_barrier = [&](int stages) {
-        if (stages == S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2) * MI) : "memory");
+        if (stages == S - 2 - D) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2 - D) * MI) : "memory");
         else {
             [&]<int... I>(std::integer_sequence<int, I...>) {
                 ([&] { if (stages == I) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(I * MI) : "memory"); }(), ...);
@@ -270,9 +305,18 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
 
     // ── fragment reads: a stage is two halves of 32 contraction elements, KS MFMA operands each ──
     unsigned xaddr[2 * KS], waddr[2 * KS];
+    unsigned xover[OFF ? 2 * KS : 1], wover[OFF ? 2 * KS : 1];      // all ones: in the next slot
 #pragma unroll
     for (int c = 0; c < 2 * KS; ++c) {
         const int piece = c * (64 / BS) + lg;       // of 8 contraction elements
+        if constexpr (OFF) {
+            const int xp = piece + off_line(p.x, p.ldx_b, lr), wp = piece + off_line(p.w, p.ldw_b, lr);
+            xover[c] = xp >= 8 ? ~0u : 0u;
+            wover[c] = wp >= 8 ? ~0u : 0u;
+            xaddr[c] = wm * TM * 4096 + lr * 128 + (((xp & 7) ^ ((lr >> 1) & 7)) << 4);
+            waddr[c] = G::X_BYTES + wn * TN * 4096 + lr * 128 + (((wp & 7) ^ ((lr >> 1) & 7)) << 4);
+            continue;
+        }
         xaddr[c] = wm * TM * 4096 + lr * 128 + ((piece ^ ((lr >> 1) & 7)) << 4);
         waddr[c] = G::X_BYTES + wn * TN * 32 * G::WROW +
                    (W8 ? lr * 64 + (((piece >> 1) ^ ((lr >> 2) & 3)) << 4) + 8 * (piece & 1) : lr * 128 + ((piece ^ ((lr >> 1) & 7)) << 4));
@@ -285,16 +329,19 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     constexpr int NR = KS * (TB + FB);
     auto read_pieces = [&](auto half_tag, auto r0_tag, auto r1_tag, unsigned slot) {
         constexpr int H = decltype(half_tag)::value, R0 = decltype(r0_tag)::value, R1 = decltype(r1_tag)::value;
+        const unsigned next = slot + G::STAGE == S * G::STAGE ? 0u : slot + G::STAGE;
+        auto xin = [&](int c) { if constexpr (OFF) return (xover[c] & next) | (~xover[c] & slot); else return slot; };
+        auto win = [&](int c) { if constexpr (OFF) return (wover[c] & next) | (~wover[c] & slot); else return slot; };
         [&]<int... R>(std::integer_sequence<int, R...>) {
             ([&] {
                 constexpr int k = R0 + R;
                 if constexpr (ONE) {
-                    if constexpr (k % 2 == 0) xf[H][k / 2] = *reinterpret_cast<const V8*>(lds + slot + xaddr[2 * H + k / 2]);
-                    else wf[H][k / 2] = *reinterpret_cast<const WRaw*>(lds + slot + waddr[2 * H + k / 2]);
-                } else if constexpr (k >= 2 && k < 2 + FB) wf[H][k - 2] = *reinterpret_cast<const WRaw*>(lds + slot + waddr[H] + (k - 2) * 16 * G::WROW);
+                    if constexpr (k % 2 == 0) xf[H][k / 2] = *reinterpret_cast<const V8*>(lds + xin(2 * H + k / 2) + xaddr[2 * H + k / 2]);
+                    else wf[H][k / 2] = *reinterpret_cast<const WRaw*>(lds + win(2 * H + k / 2) + waddr[2 * H + k / 2]);
+                } else if constexpr (k >= 2 && k < 2 + FB) wf[H][k - 2] = *reinterpret_cast<const WRaw*>(lds + win(H) + waddr[H] + (k - 2) * 16 * G::WROW);
                 else {
                     constexpr int b = k < 2 ? k : k - FB;
-                    xf[H][b] = *reinterpret_cast<const V8*>(lds + slot + xaddr[H] + b * 2048);
+                    xf[H][b] = *reinterpret_cast<const V8*>(lds + xin(H) + xaddr[H] + b * 2048);
                 }
             }(), ...);
         }(std::make_integer_sequence<int, R1 - R0>{});
@@ -349,7 +396,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     using Half1 = std::integral_constant<int, 1>;
     using Mid = std::integral_constant<int, MI / 2>;
     using All = std::integral_constant<int, MI>;
-    const int n = ACT ? stages : p.K / kBK;
+    const int n = ACT ? stages : p.K / kBK, lines = n + D;      // steps, and stages to load
     unsigned cur = 0, prev = (S - 1) * G::STAGE;      // ring slots of stages t and t - 1
     // Step t. D0: the second part of stage t + S - 1 is loaded, into the slot of stage t - 1; D1: the first part of stage t + S,
     // into the slot of stage t.
@@ -363,7 +410,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
             multiply_half(Half0{}, std::true_type{}, cur, Half0{}, Half0{}, 0u);
         }
         __builtin_amdgcn_sched_barrier(0);
-        wait_barrier(D1 ? S - 2 : (t + S - 1 < n - 1 ? t + S - 1 : n - 1) - (t + 1));
+        wait_barrier(D1 ? S - 2 - D : (t + S - 1 < lines - 1 ? t + S - 1 : lines - 1) - (t + 1 + D));
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (D1) multiply_half(Half1{}, std::true_type{}, nxt, Half0{}, Mid{}, cur);
         else multiply_half(Half1{}, std::true_type{}, nxt, Half0{}, Half0{}, 0u);
@@ -372,7 +419,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
         cur = nxt;
     };
     if constexpr (NL > 0) {
-        const int ahead = n < S ? n : S;
+        const int ahead = lines < S ? lines : S;
         if (wave >= G::NW) {
             unsigned slot = 0;
             auto load_stage = [&]() {
@@ -382,11 +429,11 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
                 slot = slot + G::STAGE == S * G::STAGE ? 0u : slot + G::STAGE;
             };
             for (int s = 0; s < ahead; ++s) load_stage();
-            if (ahead == S) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((S - 1) * MI) : "memory");
-            else wait_barrier(ahead - 1);
+            if (ahead == S) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((S - 1 - D) * MI) : "memory");
+            else wait_barrier(ahead - 1 - D);
             int t = 0;
-            for (; t < n - S; ++t) {       // stage t + 1 has landed, the slot of stage t is free
-                wait_barrier(S - 2);
+            for (; t < lines - S; ++t) {       // stage t + 1 (OFF: and t + 2) has landed, the slot of stage t is free
+                wait_barrier(S - 2 - D);
                 load_stage();
             }
             for (; t < n - 1; ++t) wait_barrier(n - 2 - t);
@@ -408,13 +455,13 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
             __builtin_amdgcn_sched_barrier(0);
             cur = nxt;
         }
-    } else if (n < S) {   // everything fits the ring
-        for (int s = 0; s < n; ++s) {
+    } else if (lines < S) {   // everything fits the ring
+        for (int s = 0; s < lines; ++s) {
 #pragma unroll
             for (int j = 0; j < MI; ++j) dma_piece(j, s * G::STAGE);
             next_stage();
         }
-        wait_barrier(n - 1);
+        wait_barrier(lines - 1 - D);
         read_half(Half0{}, 0);
         for (int t = 0; t < n - 1; ++t) step(std::false_type{}, std::false_type{}, t);
     } else {
@@ -425,11 +472,11 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
         }
 #pragma unroll
         for (int j = 0; j < MI / 2; ++j) dma_piece(j, prev);
-        // stage 0 has landed: behind it are S - 2 stages and the first part of another
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((S - 2) * MI + MI / 2) : "memory");
+        // stage 0 (OFF: and 1) has landed: behind it are S - 2 stages (one less) and the first part of another
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((S - 2 - D) * MI + MI / 2) : "memory");
         read_half(Half0{}, 0);
         int t = 0;
-        for (; t < n - S; ++t) step(std::true_type{}, std::true_type{}, t);
+        for (; t < lines - S; ++t) step(std::true_type{}, std::true_type{}, t);
         step(std::true_type{}, std::false_type{}, t);
         for (++t; t < n - 1; ++t) step(std::false_type{}, std::false_type{}, t);
     }
@@ -630,7 +677,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const PipeArgs args) {
     *reinterpret_cast<V4*>(static_cast<unsigned char*>(p.y) + static_cast<long>(token) * p.ldy_b + feature * 2L) = o;
 }
 
-template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16, bool JOIN = false>
+template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16, bool JOIN = false, bool OFF = false>
 int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st, int splits = 1, void* parts = nullptr) {
     using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL, WL>;
     auto tiles_m = [&](int i) { return (batch.p[i].M + G::BM - 1) / G::BM; };
@@ -641,7 +688,7 @@ int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st, int sp
     if (G::LDS > 64 * 1024) {
         static thread_local bool raised = false;
         if (!raised) {
-            MI_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL>),
+            MI_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL, OFF>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS));
             raised = true;
         }
@@ -669,7 +716,7 @@ int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st, int sp
         p.inv_panel = inverse(p.panel_tiles); p.inv_width = inverse(p.width); p.inv_last = inverse(p.last_width);
         first += tiles_m(i) * tiles_n(i);
     }
-    hipLaunchKernelGGL((linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL>), dim3(static_cast<unsigned>((tiles + 7) / 8 * 8), ACT ? splits : 1), dim3(G::NT + 64 * NL), G::LDS, st, args);
+    hipLaunchKernelGGL((linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL, OFF>), dim3(static_cast<unsigned>((tiles + 7) / 8 * 8), ACT ? splits : 1), dim3(G::NT + 64 * NL), G::LDS, st, args);
     MI_HIP_CHECK(hipGetLastError());
     if constexpr (JOIN) {
         const long waves = tiles * G::BM * G::BN / 256;      // of 4 features x 64 lanes

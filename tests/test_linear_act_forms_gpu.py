@@ -21,16 +21,27 @@ def _form(M, N, K, int8):
     return C.CDLL(build.FORMS_LIB).linear_form((C.c_int * 3)(M, N, K), 1, int8, 0, bd.device_info()["compute_units"])
 
 
+def _off_form(M, N, K, row):
+    if not os.path.exists(build.FORMS_LIB):
+        build.build_host()
+    splits = C.c_int()
+    return C.CDLL(build.FORMS_LIB).linear_parts(M, N, K, row, 0, bd.device_info()["compute_units"], C.byref(splits)), splits.value
+
+
 def _poisoned(t, pad):
     wide = torch.full((t.shape[0], t.shape[1] + pad), 127 if t.dtype == torch.int8 else float("nan"), dtype=t.dtype, device="cuda")
     wide[:, :t.shape[1]] = t
     return wide[:, :t.shape[1]]
 
 
-def _run(kind, M, N, K, dtype, act, what):
+def _run(kind, M, N, K, dtype, act, what, on_lines=False):
     c = make(M + N + K, kind, M, N, K, dtype)
     # (INT8 weights of a contraction that is a multiple of 8 only: rows on 8-byte addresses)
-    c["x"], c["w"] = _poisoned(c["x"], 16 if kind == "w8a8" else 8), _poisoned(c["w"], 16 if kind != "w8" or K % 16 == 0 else 8)
+    pads = 16 if kind == "w8a8" else 8, 16 if kind != "w8" or K % 16 == 0 else 8
+    if on_lines:       # rows of both operands begin on 128-byte lines
+        line = 128 if kind == "w8a8" else 64
+        pads = (line - K % line, line - K % line)
+    c["x"], c["w"] = _poisoned(c["x"], pads[0]), _poisoned(c["w"], pads[1])
     wide = torch.full((M + 1, N + 8), 7.0, dtype=c["dt"], device="cuda")
     out = wide[:M, :N]
     call(c, act, out=out)
@@ -47,9 +58,50 @@ def test_every_ring_form(int8, geglu, form, n, M, N, K):
     dtype, act = ("fp16", "bf16")[K // 64 % 2], ("none", "gelu", "gelu_tanh", "silu")[M % 4]
     for more in (0, 8, 40, 48):       # (a partial stage changes no form: the rule counts whole ones)
         assert _form(M, N, K + more, int8) == form
-        _run("w8" if int8 else "w16", M, N, K + more, dtype, act, f"{form} +{more}")
+        _run("w8" if int8 else "w16", M, N, K + more, dtype, act, f"{form} +{more}", on_lines=not int8)
         if not int8:
-            _run("w8a8", M, N, 2 * (K + more), dtype, act, f"{form} INT8 +{more}")
+            _run("w8a8", M, N, 2 * (K + more), dtype, act, f"{form} INT8 +{more}", on_lines=True)
+
+
+# 16-bit and INT8 operands whose rows begin off lines: every form of that rule, with one to many stages (and as many partial ones), by rows of every
+# distance to a line, aligned to 16 bytes as they must be
+OFF_FORMS = [(0, 70, 328, 200), (0, 37, 1160, 328), (1, 33, 4616, 200), (2, 1500, 8200, 584), (2, 1500, 16392, 1000), (3, 33, 5600, 4616), (4, 33, 8200, 200), (4, 130, 4616, 1288),
+             (5, 77, 8200, 200), (6, 77, 13000, 200), (7, 200, 8200, 200), (7, 200, 8200, 1288), (8, 200, 13000, 200), (8, 200, 13000, 1288), (9, 500, 8200, 200), (9, 500, 8200, 1288)]
+
+
+@pytest.mark.parametrize("form,M,N,K", OFF_FORMS)
+def test_every_form_of_rows_off_lines(form, M, N, K):
+    for i, beyond in enumerate((8, 24, 32, 56)):      # elements of a row stride beyond whole lines
+        k = K + (0, 8, 16, 48)[i]
+        pad = (beyond - k) % 64 or 64
+        assert _off_form(M, N, k, k + pad) == (form, 1)
+        dtype, act = ("fp16", "bf16")[i % 2], ("none", "gelu", "gelu_tanh", "silu")[i]
+        for kind, two in (("w16", 1), ("w8a8", 2)):
+            c = make(M + N + k, kind, M, N, two * k, dtype, residual=i != 2)
+            c["x"], c["w"] = _poisoned(c["x"], two * pad), _poisoned(c["w"], two * pad)
+            wide = torch.full((M + 1, N + 8), 7.0, dtype=c["dt"], device="cuda")
+            call(c, act, out=wide[:M, :N])
+            check(c, act, wide[:M, :N], f"{kind} {form} {k}")
+            assert bool((wide[M:] == 7).all()) and bool((wide[:, N:] == 7).all())
+
+
+@pytest.mark.parametrize("kind,two", [("w16", 1), ("w8a8", 2)])
+def test_rows_off_lines_give_the_bits_of_rows_on_them(kind, two):
+    """The order of the sums does not hang on where rows begin; also with one operand's rows on lines, or both tensors' first bytes off them."""
+    M, N, K = 300, 1160, 712
+    c = make(9, kind, M, N, two * K, "bf16")
+    ref = None
+    for xp, wp, shift in ((56, 56, 0), (8, 8, 0), (56, 16, 0), (16, 56, 0), (56, 56, 8), (24, 40, 24), (0, 0, 0)):
+        def placed(t, pad):
+            wide = torch.full((t.shape[0] * (t.shape[1] + two * pad) + two * shift,), 127 if t.dtype == torch.int8 else float("nan"), dtype=t.dtype, device="cuda")
+            v = wide[two * shift:].view(t.shape[0], t.shape[1] + two * pad)[:, :t.shape[1]]
+            v.copy_(t)
+            return v
+        got = call({**c, "x": placed(c["x"], xp), "w": placed(c["w"], wp)}, "silu")
+        if ref is None:
+            ref = got
+            check(c, "silu", got, "on lines")
+        assert torch.equal(got, ref), (xp, wp, shift)
 
 
 # rows at the ends of each class; features: narrow (also fewer than one work group's), up to 16 per compute unit, three and four blocks, wide

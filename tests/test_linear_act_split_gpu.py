@@ -18,7 +18,7 @@ def _parts(M, N, K, int8):
     if not os.path.exists(build.FORMS_LIB):
         build.build_host()
     splits = C.c_int()
-    form = C.CDLL(build.FORMS_LIB).linear_parts(M, N, K, int8, bd.device_info()["compute_units"], C.byref(splits))
+    form = C.CDLL(build.FORMS_LIB).linear_parts(M, N, K, K, int8, bd.device_info()["compute_units"], C.byref(splits))
     return form, splits.value
 
 
@@ -38,7 +38,7 @@ def _args(c, act, out):
 
 
 # rows, features, contraction of 16-bit operands, and the form and parts that the rule gives them on 256 compute units
-PLAIN = [(33, 72, 4608, 0, 16), (33, 520, 4608, 0, 6), (130, 520, 6400, 0, 3), (33, 704, 6400, 2, 12), (33, 2248, 9000, 2, 6), (100, 2248, 9000, 2, 3), (33, 6144, 16384, 2, 2),
+PLAIN = [(33, 72, 4608, 0, 16), (33, 520, 4608, 0, 6), (130, 520, 6400, 0, 3), (33, 704, 6400, 2, 12), (33, 2248, 8960, 2, 6), (100, 2248, 8960, 2, 3), (33, 6144, 16384, 2, 2),
          (65, 1640, 16384, 4, 8), (200, 2248, 12800, 4, 3), (65, 6144, 16384, 7, 4), (333, 1000, 16384, 7, 8)]
 W8 = [(33, 72, 3200, 0, 12), (33, 1000, 3200, 0, 4), (33, 360, 9000, 1, 16), (33, 6144, 6400, 1, 2), (65, 2248, 6400, 1, 3), (65, 1640, 12800, 3, 8), (65, 2248, 9000, 3, 6), (65, 3600, 9000, 4, 6),
       (130, 6144, 16384, 4, 2)]
@@ -47,10 +47,10 @@ W8 = [(33, 72, 3200, 0, 12), (33, 1000, 3200, 0, 4), (33, 360, 9000, 1, 16), (33
 @pytest.mark.parametrize("kind,M,N,K,form,splits", [("w16", *p) for p in PLAIN] + [("w8a8", *p) for p in PLAIN] + [("w8", *p) for p in W8])
 def test_parts(kind, M, N, K, form, splits):
     assert _parts(M, N, K, kind == "w8") == (form, splits)
-    # (whole stages, a partial last one, INT8 weights on 8-byte rows; twice the contraction of INT8 operands is the same stages)
+    # (whole stages, a partial last one and rows off lines, INT8 weights on 8-byte rows; twice the contraction of INT8 operands is the same stages)
     for more in (0, 8, 40):
         k = 2 * (K + more) if kind == "w8a8" else K + more
-        splits = _parts(M, N, K + more, kind == "w8")[1]       # (rows off 128-byte lines: more parts)
+        splits = _parts(M, N, K + more, kind == "w8")[1]       # (rows off 128-byte lines: a table of their own)
         assert splits > 1
         c = make(M + N + K + more, kind, M, N, k, "bf16" if more else "fp16", residual=more != 8)
         act = ("none", "gelu", "silu")[more % 3]
@@ -103,6 +103,21 @@ def test_captured_parts_replay_like_eager_calls():
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert torch.equal(o, w), i
+
+
+def test_two_streams_at_once():
+    cs = [make(s, "w8", 46, 368, 16000, "fp16") for s in (3, 4)]
+    want = [call(c, "silu") for c in cs]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for c, s, g in zip(cs, streams, got):
+            with torch.cuda.stream(s):
+                g.append(call(c, "silu"))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in g)
 
 
 def test_no_scratch_for_calls_that_use_none():
