@@ -83,14 +83,15 @@ inline int pick_form(const LinearBatch& batch, int n_problems, bool geglu, int n
 }
 
 // ── 16-bit and INT8 operands of the layer with an epilogue whose rows do not begin on 128-byte lines ──
-// The tiles with a window per row (linear_pipe.h, OFF) and, where a launch is short or very large, three forms without. Constants fitted to 168 such
-// problems (33 to 4608 rows, contractions of 328 to 15976 elements, fp16): the form taken is 1.3 % slower than the fastest of 28 timed on average,
-// and the launches take 0.90 of what they took on the forms above (0.64 to 1.22, the worst 333 x 1288 x 328).
-enum { kOff32x32, kOff64x32, kOff256x256, kOff64x32_row, kOff64x64_row, kOff64x96_row, kOff128x64_row, kOff128x96_row, kOff128x128_row, kOff192x128_row, kOffForms };
-inline constexpr Form kOff[kOffForms] = {{32, 32, 3.18f, 0.110f, 0.092f, 0.50f},   {64, 32, 3.33f, 0.153f, 0.141f, 0.85f},   {256, 256, 15.88f, 1.237f, 1.753f, 11.05f},
-                                  {64, 32, 3.88f, 0.145f, 0.109f, 1.01f},   {64, 64, 4.29f, 0.172f, 0.172f, 1.00f},   {64, 96, 4.87f, 0.223f, 0.249f, 3.23f},
-                                  {128, 64, 5.09f, 0.258f, 0.298f, 3.39f},  {128, 96, 6.84f, 0.297f, 0.377f, 4.49f},  {128, 128, 7.38f, 0.333f, 0.435f, 5.34f},
-                                  {192, 128, 8.09f, 0.543f, 0.696f, 5.51f}};
+// The tiles that load by lines (linear_pipe.h, OFF) and, where a launch is short or very large, four that do not. Constants fitted to 216 such
+// problems (33 to 4608 rows, contractions of 328 to 15976 elements, fp16, launches of one form for 10 ms and more, as the power limit moves the
+// large ones): the form taken is 0.6 % slower than the fastest of 13 on average, 17 % at worst (33 x 6144 x 4616, 64 x 32). Against the forms
+// and constants of rows on lines: 0.90 of the time.
+enum { kOff32x32, kOff64x32, kOff256x128, kOff256x256, kOff64x32_row, kOff64x64_row, kOff64x96_row, kOff128x64_row, kOff128x96_row, kOff128x128_row, kOff192x128_row, kOffForms };
+inline constexpr Form kOff[kOffForms] = {{32, 32, 3.12f, 0.108f, 0.091f, 0.47f},   {64, 32, 3.08f, 0.153f, 0.149f, 0.77f},   {256, 128, 7.31f, 0.909f, 1.062f, 5.97f},
+                                         {256, 256, 13.75f, 1.377f, 1.789f, 10.60f}, {64, 32, 3.70f, 0.143f, 0.120f, 0.90f}, {64, 64, 4.01f, 0.171f, 0.181f, 1.00f},
+                                         {64, 96, 4.62f, 0.221f, 0.259f, 2.99f},   {128, 64, 4.73f, 0.269f, 0.332f, 2.99f},  {128, 96, 5.83f, 0.320f, 0.420f, 4.09f},
+                                         {128, 128, 6.72f, 0.366f, 0.502f, 5.04f}, {192, 128, 7.67f, 0.579f, 0.730f, 6.08f}};
 inline bool off_lines(const LinearProblem& p) {
     return ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | static_cast<uintptr_t>(p.ldx * 2) | static_cast<uintptr_t>(p.ldw * 2)) & 127) != 0;
 }
