@@ -651,10 +651,17 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const PipeArgs args) {
     if (token >= p.M || feature >= p.N) return;
     const Sum* const parts = static_cast<const Sum*>(args.parts);
     Sum sum = parts[part_of<NW, GROUPS>(tile, args.splits, 0, wave, group, lane)];
-    for (int s = 1; s < args.splits; ++s) {
-        const Sum next = parts[part_of<NW, GROUPS>(tile, args.splits, s, wave, group, lane)];
+    // (five at a time on their way: one by one, each was waited for before the next was asked for)
+    for (int s = 1; s < args.splits; s += 5) {
+        Sum next[5];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] += next[i];
+        for (int j = 0; j < 5; ++j) next[j] = parts[part_of<NW, GROUPS>(tile, args.splits, min(s + j, args.splits - 1), wave, group, lane)];
+#pragma unroll
+        for (int j = 0; j < 5; ++j)
+            if (s + j < args.splits) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += next[j][i];
+            }
     }
     V4 bias{}, res{};
     if (p.bias) bias = *reinterpret_cast<const V4*>(static_cast<const T*>(p.bias) + feature);
