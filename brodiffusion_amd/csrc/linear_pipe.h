@@ -118,8 +118,8 @@ struct PipeGeo {
 // that touches 8, so every row is loaded from the line on that it begins in: piece p of line l of a row that begins s pieces into its line is
 // the row's piece 8 l + p - s. A stage's fragments then lie in its ring slot and, those from piece 8 - s on, in the next one, so that the stage
 // behind the one multiplied has to be there too (and the rings are a stage deeper); s is the same for rows 8 apart, so one number for a lane and
-// all of its blocks, and the swizzle is as good: of 8 rows of one parity, i = 0 .. 7, the positions ((a i + b) mod 8) ^ i with a even are 8
-// different ones. Pieces in front of a row or behind it are loaded as copies of the nearest of the row and not used. Measured (us, without / with,
+// all of its blocks. In its slot a piece lies where it would lie in a row on a line, the swizzle is of 8 l + p - s: reads are free of conflicts
+// as there (swizzled by p, 1031 x 4608 x 1160 had conflicts in all of its LDS cycles). Pieces in front of a row or behind it are loaded as copies of the nearest of the row and not used. Measured (us, without / with,
 // fp16): 436 x 1200 x 6472 32.9 / 22.6 on 64 x 64 tiles, 1024 x 1288 x 5128 34.4 / 24.2 on 64 x 96, 300 x 6144 x 4616 41.3 / 29.2 on
 // 128 x 96, 2048 x 2240 x 2248 35.5 / 28.7 on 192 x 128; not for short launches, 77 x 1160 x 1288 5.7 / 6.1 on 32 x 32. INT8 weights with 16-bit
 // rows gain 1 to 3 % from it (their step is the widening) and go without.
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     // ... and the offsets for line `loading` of every row; xg and wg stand a line in front of it, so that none is negative
     auto place = [&]() {
         const int first = 8 * loading, end = ((stages - 1) * kBK + in_last) / 8 - 1, row = lane >> 3;
-        auto at = [&](int r, int s) { return static_cast<unsigned>(min(max(first + ((lane & 7) ^ ((r >> 1) & 7)) - s, 0), end) - first + 8) * 16u; };
+        auto at = [&](int r, int s) { return static_cast<unsigned>(min(max(first + ((((lane & 7) ^ ((r >> 1) & 7)) + s) & 7) - s, 0), end) - first + 8) * 16u; };
         const int xs = off_line(p.x, p.ldx_b, row), ws = off_line(p.w, p.ldw_b, row);
 #pragma unroll
         for (int u = 0; u < G::MX; ++u) {
@@ -310,12 +310,8 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     for (int c = 0; c < 2 * KS; ++c) {
         const int piece = c * (64 / BS) + lg;       // of 8 contraction elements
         if constexpr (OFF) {
-            const int xp = piece + off_line(p.x, p.ldx_b, lr), wp = piece + off_line(p.w, p.ldw_b, lr);
-            xover[c] = xp >= 8 ? ~0u : 0u;
-            wover[c] = wp >= 8 ? ~0u : 0u;
-            xaddr[c] = wm * TM * 4096 + lr * 128 + (((xp & 7) ^ ((lr >> 1) & 7)) << 4);
-            waddr[c] = G::X_BYTES + wn * TN * 4096 + lr * 128 + (((wp & 7) ^ ((lr >> 1) & 7)) << 4);
-            continue;
+            xover[c] = piece + off_line(p.x, p.ldx_b, lr) >= 8 ? ~0u : 0u;
+            wover[c] = piece + off_line(p.w, p.ldw_b, lr) >= 8 ? ~0u : 0u;
         }
         xaddr[c] = wm * TM * 4096 + lr * 128 + ((piece ^ ((lr >> 1) & 7)) << 4);
         waddr[c] = G::X_BYTES + wn * TN * 32 * G::WROW +
