@@ -49,7 +49,7 @@ int launch_off(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
         case kOff64x96_row: return launch_pipe<T, false, false, 2, 3, 1, 1, 5, 4, Int8, true, 16, false, true>(b, 1, st);
         case kOff128x96_row: return launch_pipe<T, false, false, 2, 3, 2, 1, 4, 4, Int8, true, 16, false, true>(b, 1, st);
         case kOff192x128_row: return launch_pipe<T, false, false, 2, 4, 3, 1, 4, 0, Int8, true, 16, false, true>(b, 1, st);
-        case kOff256x128: return launch_pipe<T, false, false, 4, 2, 2, 2, 3, 0, Int8, true>(b, 1, st);
+        case kOff128x128_2: return launch_pipe<T, false, false, 2, 2, 2, 2, 2, 0, Int8, true>(b, 1, st);
         case kOff256x256: return gemm_dma::launch_t<T, gemm::Int8, true>(b, 1, st);
     }
     return fail("linear: no kernel for form %d", s.form);      // (not asked for)

@@ -29,11 +29,32 @@ int launch_split(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
         default: return launch_pipe<T, true, false, 2, 3, 2, 1, 3, 2, T, true, WL, true>(b, 1, st, s.splits, parts);
     }
 }
+// ... of rows that do not begin on lines (kOff8), in one part or, with memory for them, several
+template <typename T, int WL, bool JOIN>
+int launch_off(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
+    switch (s.form) {
+        case kOff8_32x32: return launch_pipe<T, true, false, 1, 1, 1, 1, 6, 2, T, true, WL, JOIN>(b, 1, st, s.splits, parts);
+        case kOff8_64x64: return launch_pipe<T, true, false, 2, 2, 1, 1, 4, 4, T, true, WL, JOIN>(b, 1, st, s.splits, parts);
+        case kOff8_128x64_row: return launch_pipe<T, true, false, 2, 2, 2, 1, 4, 4, T, true, 16, JOIN, true>(b, 1, st, s.splits, parts);
+        case kOff8_128x96_row: return launch_pipe<T, true, false, 2, 3, 2, 1, 4, 2, T, true, 16, JOIN, true>(b, 1, st, s.splits, parts);
+    }
+    if constexpr (!JOIN) switch (s.form) {
+        case kOff8_64x96: return launch_pipe<T, true, false, 2, 3, 1, 1, WL == 16 ? 5 : 4, 2, T, true, WL>(b, 1, st);
+        case kOff8_128x96: return launch_pipe<T, true, false, 2, 3, 2, 1, 3, 2, T, true, WL>(b, 1, st);
+        case kOff8_128x128_2_row: return launch_pipe<T, true, false, 2, 2, 2, 2, 3, 0, T, true, 16, false, true>(b, 1, st);
+        case kOff8_128x128_row: return launch_pipe<T, true, false, 2, 4, 2, 1, 5, 0, T, true, 16, false, true>(b, 1, st);
+    }
+    return fail("linear: no kernel for form %d", s.form);      // (not asked for)
+}
 template <typename T, int WL>
 int launch_words(const LinearBatch& b, const LinearScratch& lent, hipStream_t st) {
-    const Parts s = pick_parts(b.p[0], device_cu_count());
-    if (s.splits > 1 && lent.bytes >= static_cast<size_t>(part_bytes(kPlainW8[s.form], b.p[0], s.splits))) return launch_split<T, WL>(b, s, lent.p, st);
-    return launch_form<T, WL>(b, s.splits > 1 ? pick_form(kPlainW8, kPlainW8Forms, b, 1, device_cu_count()) : s.form, st);
+    const LinearProblem& p = b.p[0];
+    const FormTable& table = table_of(p);
+    const bool off = off_lines(p);
+    const Parts s = pick_parts(p, device_cu_count());
+    if (s.splits > 1 && lent.bytes >= static_cast<size_t>(part_bytes(table.forms[s.form], p, s.splits))) return off ? launch_off<T, WL, true>(b, s, lent.p, st) : launch_split<T, WL>(b, s, lent.p, st);
+    const int form = s.splits > 1 ? pick_form(table.forms, table.n, b, 1, device_cu_count()) : s.form;
+    return off ? launch_off<T, WL, false>(b, {form, 1}, nullptr, st) : launch_form<T, WL>(b, form, st);
 }
 template <typename T>
 int launch_any(const LinearBatch& b, const LinearScratch& lent, hipStream_t st) {

@@ -82,18 +82,24 @@ inline int pick_form(const LinearBatch& batch, int n_problems, bool geglu, int n
     return geglu ? pick_form(kGeglu, kGegluForms, batch, n_problems, n_cu) : pick_form(kPlain, kPlainForms, batch, n_problems, n_cu);
 }
 
-// ── 16-bit and INT8 operands of the layer with an epilogue whose rows do not begin on 128-byte lines ──
-// The tiles that load by lines (linear_pipe.h, OFF) and, where a launch is short or very large, four that do not. Constants fitted to 216 such
-// problems (33 to 4608 rows, contractions of 328 to 15976 elements, fp16, launches of one form for 10 ms and more, as the power limit moves the
-// large ones): the form taken is 0.6 % slower than the fastest of 13 on average, 17 % at worst (33 x 6144 x 4616, 64 x 32). Against the forms
-// and constants of rows on lines: 0.90 of the time.
-enum { kOff32x32, kOff64x32, kOff256x128, kOff256x256, kOff64x32_row, kOff64x64_row, kOff64x96_row, kOff128x64_row, kOff128x96_row, kOff128x128_row, kOff192x128_row, kOffForms };
-inline constexpr Form kOff[kOffForms] = {{32, 32, 3.12f, 0.108f, 0.091f, 0.47f},   {64, 32, 3.08f, 0.153f, 0.149f, 0.77f},   {256, 128, 7.31f, 0.909f, 1.062f, 5.97f},
-                                         {256, 256, 13.75f, 1.377f, 1.789f, 10.60f}, {64, 32, 3.70f, 0.143f, 0.120f, 0.90f}, {64, 64, 4.01f, 0.171f, 0.181f, 1.00f},
-                                         {64, 96, 4.62f, 0.221f, 0.259f, 2.99f},   {128, 64, 4.73f, 0.269f, 0.332f, 2.99f},  {128, 96, 5.83f, 0.320f, 0.420f, 4.09f},
-                                         {128, 128, 6.72f, 0.366f, 0.502f, 5.04f}, {192, 128, 7.67f, 0.579f, 0.730f, 6.08f}};
+// ── the layer with an epilogue, rows that do not begin on 128-byte lines ──
+// The tiles that load by lines (linear_pipe.h, OFF; here _row) and, where a launch is short or very large, some that do not. Constants fitted to 216
+// such problems of 16-bit operands (33 to 4608 rows, contractions of 328 to 15976 elements, fp16) and 336 of INT8 weights, with launches of one
+// form for 10 ms, as the power limit moves the large ones: the form taken is 0.4 (INT8 weights: 1.7) % slower than the fastest of 13 (18) on
+// average, 13 (23) % at worst. Against the forms and constants of rows on lines 0.89 (0.98) of the time.
+enum { kOff32x32, kOff64x32, kOff128x128_2, kOff256x256, kOff64x32_row, kOff64x64_row, kOff64x96_row, kOff128x64_row, kOff128x96_row, kOff128x128_row, kOff192x128_row, kOffForms };
+inline constexpr Form kOff[kOffForms] = {{32, 32, 3.09f, 0.108f, 0.097f, 0.46f},   {64, 32, 3.07f, 0.154f, 0.149f, 0.80f},   {128, 128, 6.25f, 0.494f, 0.622f, 1.07f},
+                                         {256, 256, 13.89f, 1.368f, 1.751f, 11.05f}, {64, 32, 3.70f, 0.140f, 0.123f, 0.88f}, {64, 64, 4.02f, 0.161f, 0.175f, 0.89f},
+                                         {64, 96, 4.49f, 0.206f, 0.242f, 3.05f},   {128, 64, 4.70f, 0.268f, 0.322f, 3.01f},  {128, 96, 6.21f, 0.314f, 0.400f, 4.20f},
+                                         {128, 128, 6.77f, 0.360f, 0.484f, 4.72f}, {192, 128, 7.53f, 0.511f, 0.694f, 5.33f}};
+enum { kOff8_32x32, kOff8_64x64, kOff8_64x96, kOff8_128x96, kOff8_128x64_row, kOff8_128x96_row, kOff8_128x128_2_row, kOff8_128x128_row, kOff8Forms };
+inline constexpr Form kOff8[kOff8Forms] = {{32, 32, 3.05f, 0.166f, 0.058f, 0.62f},  {64, 64, 3.80f, 0.215f, 0.208f, 0.93f},  {64, 96, 4.34f, 0.260f, 0.299f, 1.36f},   {128, 96, 5.37f, 0.388f, 0.444f, 2.10f},
+                                           {128, 64, 5.38f, 0.263f, 0.261f, 1.93f}, {128, 96, 6.74f, 0.349f, 0.409f, 5.10f}, {128, 128, 6.50f, 0.611f, 0.407f, 3.38f}, {128, 128, 6.72f, 0.442f, 0.517f, 5.50f}};
+// (INT8 weights: lines of 64 bytes of them; and the last row ends where a piece does, as pieces are loaded whole)
 inline bool off_lines(const LinearProblem& p) {
-    return ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | static_cast<uintptr_t>(p.ldx * 2) | static_cast<uintptr_t>(p.ldw * 2)) & 127) != 0;
+    const auto x = reinterpret_cast<uintptr_t>(p.x) | static_cast<uintptr_t>(p.ldx * 2), w = reinterpret_cast<uintptr_t>(p.w);
+    if (p.w_scale && !p.x_scale) return ((x & 127) || ((w | static_cast<uintptr_t>(p.ldw)) & 63)) && (p.ldw - p.K) % 16 == 0;
+    return ((x | w | static_cast<uintptr_t>(p.ldw * 2)) & 127) != 0;
 }
 
 // ── several work groups for a tile's contraction (the layer with an epilogue, where the caller lends memory for their sums) ──
@@ -106,10 +112,11 @@ struct Parts { int form, splits; };
 inline constexpr int kSplitPlain[] = {k32x32, k64x64, k128x64_load, k128x128};
 inline constexpr int kSplitW8[] = {k8_32x32, k8_64x64, k8_128x64, k8_128x96};
 inline constexpr int kSplitOff[] = {kOff32x32, kOff64x64_row, kOff128x64_row, kOff128x128_row};
+inline constexpr int kSplitOff8[] = {kOff8_32x32, kOff8_64x64, kOff8_128x64_row, kOff8_128x96_row};
 // The forms of a problem of the layer with an epilogue, and those with parts
 struct FormTable { const Form* forms; int n; const int* split; };
-inline constexpr FormTable kTables[] = {{kPlain, kPlainForms, kSplitPlain}, {kPlainW8, kPlainW8Forms, kSplitW8}, {kOff, kOffForms, kSplitOff}};
-inline const FormTable& table_of(const LinearProblem& p) { return kTables[p.w_scale && !p.x_scale ? 1 : off_lines(p) ? 2 : 0]; }
+inline constexpr FormTable kTables[] = {{kPlain, kPlainForms, kSplitPlain}, {kOff, kOffForms, kSplitOff}, {kPlainW8, kPlainW8Forms, kSplitW8}, {kOff8, kOff8Forms, kSplitOff8}};
+inline const FormTable& table_of(const LinearProblem& p) { return kTables[(p.w_scale && !p.x_scale ? 2 : 0) + (off_lines(p) ? 1 : 0)]; }
 inline long tiles_of(const Form& f, const LinearProblem& p) { return static_cast<long>((p.M + f.bm - 1) / f.bm) * ((p.N + f.bn_out - 1) / f.bn_out); }
 inline long part_bytes(const Form& f, const LinearProblem& p, int splits) { return tiles_of(f, p) * splits * f.bm * f.bn_out * 4; }
 inline Parts pick_parts(const LinearProblem& p, int n_cu) {

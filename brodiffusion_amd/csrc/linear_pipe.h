@@ -121,8 +121,8 @@ struct PipeGeo {
 // all of its blocks. In its slot a piece lies where it would lie in a row on a line, the swizzle is of 8 l + p - s: reads are free of conflicts
 // as there (swizzled by p, 1031 x 4608 x 1160 had conflicts in all of its LDS cycles). Pieces in front of a row or behind it are loaded as copies of the nearest of the row and not used. Measured (us, without / with,
 // fp16): 436 x 1200 x 6472 32.9 / 22.6 on 64 x 64 tiles, 1024 x 1288 x 5128 34.4 / 24.2 on 64 x 96, 300 x 6144 x 4616 41.3 / 29.2 on
-// 128 x 96, 2048 x 2240 x 2248 35.5 / 28.7 on 192 x 128; not for short launches, 77 x 1160 x 1288 5.7 / 6.1 on 32 x 32. INT8 weights with 16-bit
-// rows gain 1 to 3 % from it (their step is the widening) and go without.
+// 128 x 96, 2048 x 2240 x 2248 35.5 / 28.7 on 192 x 128; not for short launches, 77 x 1160 x 1288 5.7 / 6.1 on 32 x 32. INT8 weights (lines
+// of 64 bytes, s of them in halves of pieces): 3000 x 3336 x 5000 138 / 122, 333 x 6144 x 4616 36 / 32.
 template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16, bool OFF = false>
 __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(const PipeArgs args) {
     using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL, WL>;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     constexpr bool A8 = std::is_same_v<A, Int8>;
     static_assert(!ACT || !GEGLU, "the GEGLU form has its own epilogue");
     static_assert(WL == 16 || (W8 && ACT && WL == 4), "whole pieces, or words of INT8 weights");
-    static_assert(!OFF || (ACT && !W8 && S >= 3), "two stages of the ring are read at a time");
+    static_assert(!OFF || (ACT && WL == 16 && S >= 3), "two stages of the ring are read at a time");
     constexpr int D = OFF ? 1 : 0;               // stages that must have landed behind the one read
     constexpr int BM = G::BM, BN_OUT = G::BN_OUT, MI = G::MI;
     // one block of INT8 weights per wavefront: v_mfma_f32_32x32x16 (see the top)
@@ -205,14 +205,14 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
         else dma(woff[j < G::MX ? 0 : j - G::MX], wg, lds_base + slot + G::X_BYTES + (lw + G::LW * (j - G::MX)) * 1024);
     };
     // ACT: how many contraction elements the last stage holds, and the stage that xg and wg stand on
-    int stages = 0, in_last = kBK;
+    int stages = 0, in_last = kBK, followed = 0;
     if constexpr (ACT) {
         stages = (p.K + kBK - 1) / kBK;
         in_last = p.K - (stages - 1) * kBK;
         if (args.splits > 1) {      // (this part's stages; the divisions are left to those launches)
             const int all = stages, part = static_cast<int>(blockIdx.y), from = part * all / args.splits, to = (part + 1) * all / args.splits;
             stages = to - from;
-            if (to < all) in_last = kBK;
+            if (to < all) { in_last = kBK; followed = 1; }
             xg += static_cast<long>(from) * (kBK * 2);
             wg += static_cast<long>(from) * (W8 ? kBK : kBK * 2);
         }
@@ -236,27 +236,30 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
             if ((W8 ? 16 : 8) * piece >= in_last) woff[u] -= piece * 16;
         }
     };
-    // OFF: how many pieces into a line row `r` of the tile begins (tiles begin at multiples of 8 rows)
-    auto off_line = [](const void* first, unsigned row_bytes, int r) { return (static_cast<int>(reinterpret_cast<uintptr_t>(first) >> 4) + r * static_cast<int>(row_bytes >> 4)) & 7; };
-    // ... and the offsets for line `loading` of every row; xg and wg stand a line in front of it, so that none is negative
+    // OFF: how many units of 2^UNIT bytes into a line row `r` of the tile begins (tiles begin at multiples of 8 rows)
+    auto off_line = [](const void* first, unsigned row_bytes, int r, int unit) { return (static_cast<int>(reinterpret_cast<uintptr_t>(first) >> unit) + static_cast<int>(r * row_bytes >> unit)) & 7; };
+    // ... and the offsets for line `loading` of every row; xg and wg stand a line in front of it, so that none is negative. (Of INT8 weights that
+    // are no multiple of 16 every second row begins within a piece and ends with one; the others end within one, whose rest is the next row's. So
+    // does a part's last piece, with what comes behind it.)
+    constexpr int WP = G::WROW / 16;              // pieces of a line of W
     auto place = [&]() {
-        const int first = 8 * loading, end = ((stages - 1) * kBK + in_last) / 8 - 1, row = lane >> 3;
-        auto at = [&](int r, int s) { return static_cast<unsigned>(min(max(first + ((((lane & 7) ^ ((r >> 1) & 7)) + s) & 7) - s, 0), end) - first + 8) * 16u; };
-        const int xs = off_line(p.x, p.ldx_b, row), ws = off_line(p.w, p.ldw_b, row);
+        const int k = (stages - 1) * kBK + in_last, x_end = k / 8 - 1, w_end = !W8 ? x_end : followed ? k / 16 : (k + 8) / 16 - 1;
+        auto at = [&](int piece, int s, int of, int end) { return static_cast<unsigned>(min(max(of * loading + ((piece + s) & (of - 1)) - s, 0), end) - of * loading + of) * 16u; };
+        const int xs = off_line(p.x, p.ldx_b, lane >> 3, 4), j = W8 ? lane >> 2 : lane >> 3, ws = off_line(p.w, p.ldw_b, j, 4) & (WP - 1);
 #pragma unroll
         for (int u = 0; u < G::MX; ++u) {
-            const int r = 8 * (lw + G::LW * u) + row;
-            xoff[u] = static_cast<unsigned>(min(r, p.M - 1 - m0)) * p.ldx_b + at(r, xs);
+            const int r = 8 * (lw + G::LW * u) + (lane >> 3);
+            xoff[u] = static_cast<unsigned>(min(r, p.M - 1 - m0)) * p.ldx_b + at((lane & 7) ^ ((r >> 1) & 7), xs, 8, x_end);
         }
 #pragma unroll
         for (int u = 0; u < G::MW; ++u) {
-            const int r = 8 * (lw + G::LW * u) + row;
-            woff[u] = static_cast<unsigned>(min(r, p.N - 1 - n0)) * p.ldw_b + at(r, ws);
+            const int r = (W8 ? 16 : 8) * (lw + G::LW * u) + j;
+            woff[u] = (static_cast<unsigned>(min(r, p.N - 1 - n0)) * p.ldw_b & ~15u) + at(W8 ? (lane & 3) ^ ((r >> 2) & 3) : (lane & 7) ^ ((r >> 1) & 7), ws, WP, w_end);
         }
     };
     if constexpr (OFF) {
         xg -= kBK * 2;
-        wg -= kBK * 2;
+        wg -= G::WROW;
         place();
     } else if (ACT && stages == 1) shorten();
     auto next_stage = [&]() {
@@ -309,13 +312,16 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
 #pragma unroll
     for (int c = 0; c < 2 * KS; ++c) {
         const int piece = c * (64 / BS) + lg;       // of 8 contraction elements
+        int wp = piece;                       // (INT8 weights: halves of pieces, from the piece on that the row begins in)
         if constexpr (OFF) {
-            xover[c] = piece + off_line(p.x, p.ldx_b, lr) >= 8 ? ~0u : 0u;
-            wover[c] = piece + off_line(p.w, p.ldw_b, lr) >= 8 ? ~0u : 0u;
+            const int ws = off_line(p.w, p.ldw_b, lr, W8 ? 3 : 4);
+            xover[c] = piece + off_line(p.x, p.ldx_b, lr, 4) >= 8 ? ~0u : 0u;
+            wover[c] = piece + ws >= 8 ? ~0u : 0u;
+            if constexpr (W8) wp = (piece + (ws & 1)) & 7;
         }
         xaddr[c] = wm * TM * 4096 + lr * 128 + ((piece ^ ((lr >> 1) & 7)) << 4);
         waddr[c] = G::X_BYTES + wn * TN * 32 * G::WROW +
-                   (W8 ? lr * 64 + (((piece >> 1) ^ ((lr >> 2) & 3)) << 4) + 8 * (piece & 1) : lr * 128 + ((piece ^ ((lr >> 1) & 7)) << 4));
+                   (W8 ? lr * 64 + (((wp >> 1) ^ ((lr >> 2) & 3)) << 4) + 8 * (wp & 1) : lr * 128 + ((piece ^ ((lr >> 1) & 7)) << 4));
     }
     using WRaw = std::conditional_t<W8, u32x2, V8>;
     V8 xf[2][KS * TB];

@@ -21,11 +21,11 @@ def _form(M, N, K, int8):
     return C.CDLL(build.FORMS_LIB).linear_form((C.c_int * 3)(M, N, K), 1, int8, 0, bd.device_info()["compute_units"])
 
 
-def _off_form(M, N, K, row):
+def _off_form(M, N, K, row, int8=0):
     if not os.path.exists(build.FORMS_LIB):
         build.build_host()
     splits = C.c_int()
-    return C.CDLL(build.FORMS_LIB).linear_parts(M, N, K, row, 0, bd.device_info()["compute_units"], C.byref(splits)), splits.value
+    return C.CDLL(build.FORMS_LIB).linear_parts(M, N, K, row, int8, bd.device_info()["compute_units"], C.byref(splits)), splits.value
 
 
 def _poisoned(t, pad):
@@ -58,15 +58,15 @@ def test_every_ring_form(int8, geglu, form, n, M, N, K):
     dtype, act = ("fp16", "bf16")[K // 64 % 2], ("none", "gelu", "gelu_tanh", "silu")[M % 4]
     for more in (0, 8, 40, 48):       # (a partial stage changes no form: the rule counts whole ones)
         assert _form(M, N, K + more, int8) == form
-        _run("w8" if int8 else "w16", M, N, K + more, dtype, act, f"{form} +{more}", on_lines=not int8)
+        _run("w8" if int8 else "w16", M, N, K + more, dtype, act, f"{form} +{more}", on_lines=True)
         if not int8:
             _run("w8a8", M, N, 2 * (K + more), dtype, act, f"{form} INT8 +{more}", on_lines=True)
 
 
 # 16-bit and INT8 operands whose rows begin off lines: every form of that rule, with one to many stages (and as many partial ones), by rows of every
 # distance to a line, aligned to 16 bytes as they must be
-OFF_FORMS = [(0, 70, 328, 200), (0, 37, 1160, 328), (1, 33, 4616, 200), (2, 1031, 5600, 200), (3, 1500, 8200, 584), (3, 1500, 16392, 1000), (4, 33, 5600, 4616), (5, 33, 8200, 200), (5, 130, 4616, 1288),
-             (6, 77, 8200, 200), (7, 77, 13000, 200), (8, 200, 8200, 200), (8, 200, 8200, 1288), (9, 200, 13000, 200), (9, 200, 13000, 1288), (10, 500, 8200, 200), (10, 500, 8200, 1288)]
+OFF_FORMS = [(0, 70, 328, 200), (0, 37, 1160, 328), (1, 33, 4616, 200), (2, 200, 13000, 200), (3, 1500, 8200, 584), (3, 1500, 16392, 1000), (4, 33, 5600, 4616), (5, 33, 8200, 200), (5, 130, 4616, 1288),
+             (6, 77, 8200, 200), (7, 77, 13000, 200), (8, 200, 8200, 200), (8, 200, 8200, 1288), (9, 200, 13000, 328), (9, 200, 13000, 1288), (10, 500, 8200, 200), (10, 500, 8200, 1288)]
 
 
 @pytest.mark.parametrize("form,M,N,K", OFF_FORMS)
@@ -82,6 +82,26 @@ def test_every_form_of_rows_off_lines(form, M, N, K):
             wide = torch.full((M + 1, N + 8), 7.0, dtype=c["dt"], device="cuda")
             call(c, act, out=wide[:M, :N])
             check(c, act, wide[:M, :N], f"{kind} {form} {k}")
+            assert bool((wide[M:] == 7).all()) and bool((wide[:, N:] == 7).all())
+
+
+OFF8_FORMS = [(0, 33, 328, 200), (1, 33, 8200, 200), (2, 77, 8200, 200), (3, 200, 8200, 200), (4, 77, 13000, 328), (5, 130, 8200, 4616), (6, 768, 8200, 200), (6, 768, 8200, 584),
+              (7, 200, 13000, 200), (7, 200, 13000, 328)]
+
+
+@pytest.mark.parametrize("form,M,N,K", OFF8_FORMS)
+def test_every_form_of_int8_weights_off_lines(form, M, N, K):
+    """(K is an odd multiple of 8: every second row of the weights begins within a piece of 16 bytes)"""
+    for i, pad in enumerate((0, 16, 32, 64)):
+        for k in (K, K + 8):
+            assert _off_form(M, N, k, k + pad, 1) == (form, 1)
+            c = make(M + N + k + pad, "w8", M, N, k, ("fp16", "bf16")[i % 2], residual=i != 2)
+            if pad:
+                c["x"], c["w"] = _poisoned(c["x"], pad), _poisoned(c["w"], pad)
+            wide = torch.full((M + 1, N + 8), 7.0, dtype=c["dt"], device="cuda")
+            act = ("none", "gelu", "gelu_tanh", "silu")[i]
+            call(c, act, out=wide[:M, :N])
+            check(c, act, wide[:M, :N], f"{form} {k} + {pad}")
             assert bool((wide[M:] == 7).all()) and bool((wide[:, N:] == 7).all())
 
 
