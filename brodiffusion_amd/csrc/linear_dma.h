@@ -1,8 +1,8 @@
-// Y = X W^T + b for large problems on gfx950 (linear_pipe.hip says which): 256 x 256 output tiles, 8 wavefronts, operand blocks moved global -> LDS
+// Y = X W^T + b for large problems on gfx950 (linear_forms.h says which): 256 x 256 output tiles, 8 wavefronts, operand blocks moved global -> LDS
 // by DMA into rings.
 //
 // The work group's 512 threads are 8 wavefronts in a 2 (feature halves) x 4 (token quarters) arrangement; a wavefront owns
-// 128 features x 64 tokens = 8 x 4 accumulator blocks of v_mfma_f32_16x16x32 (128 registers; linear_pipe.hip says why that one). As in linear.hip the product
+// 128 features x 64 tokens = 8 x 4 accumulator blocks of v_mfma_f32_16x16x32 (128 registers; linear_pipe.h says why that one). As in linear.hip the product
 // is computed transposed (MFMA rows = features), so both operands are read along their contiguous contraction index.
 //
 // Operands arrive in blocks of 64 contraction elements: per operand a 256-row x 128-byte tile (32 KB) = 32 LDS-DMA

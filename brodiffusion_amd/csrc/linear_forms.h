@@ -1,4 +1,4 @@
-// Which tile a projection takes: the forms of linear_pipe.hip (and the 256 x 256 tiles of linear_dma.hip) with what a launch on each is
+// Which tile a projection takes: the forms of linear_pipe.h (and the 256 x 256 tiles of linear_dma.h) with what a launch on each is
 // expected to cost. Host code without HIP in it, so that a test can ask which form a problem gets.
 #pragma once
 #include <algorithm>

@@ -1,4 +1,4 @@
-// Pieces shared by the kernels of the projection GEMM (linear.hip, linear_pipe.hip, linear_dma.hip): MFMA wrappers, the exact
+// Pieces shared by the kernels of the projection GEMM (linear.hip, linear_pipe.h, linear_dma.h, linear_few.hip): MFMA wrappers, the exact
 // GELU of the GEGLU epilogue, the widening of INT8 weights and the scaling of their accumulators.
 #pragma once
 #include "internal.h"

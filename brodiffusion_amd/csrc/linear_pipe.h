@@ -19,7 +19,7 @@
 //   multiply half 1 of stage t, between the products read half 0 of stage t + 1
 // and the DMA of stage t + S, which goes into the ring slot of stage t, is dealt out between the MFMAs of the second half of
 // step t and the first half of step t + 1: issued in one burst behind the barrier it made a step of 128 x 128 take 0.57 us
-// on an otherwise empty compute unit, 0.4 dealt out. The accumulation order is the same in every form (and in linear_dma.hip):
+// on an otherwise empty compute unit, 0.4 dealt out. The accumulation order is the same in every form (and in linear_dma.h):
 // a problem gives the same bits whichever one takes it, alone or in a launch with others.
 //
 // Products are v_mfma_f32_16x16x32, two token blocks with one feature block in a row. What bounds the large forms on values of a
@@ -32,7 +32,7 @@
 // widening, far from the power limit, and with the other product it is longer in every order of reads and widening tried (us, 32x32x16 /
 // 16x16x32: fp16 32 x 1280 x 5120 15.5 / 16.7, 512 x 1280 x 5120 19.7 / 21.0; bf16 512 x 1280 x 5120 19.1 / 22.0, 1024 x 1280 x 5120
 // 26.3 / 29.4, 77 x 6720 x 2240 10.5 / 11.6). Such loops of 80 to 100 instructions also take up to 3 % more or less by where they start in a cache line
-// of instructions, so that this file is compiled with its loops aligned to 64 bytes (fp16, 64 x 64 tiles: 3 % faster than before).
+// of instructions, so that the sources of these kernels are compiled with loops aligned to 64 bytes (fp16, 64 x 64 tiles: 3 % faster than before).
 //
 // With NL > 0 the work group has NL further wavefronts that do nothing but load (a whole stage behind the barrier that frees its slot)
 // and the others nothing but read and multiply: an LDS-DMA instruction keeps its wavefront from issuing for 33 clocks, the products of
@@ -119,10 +119,11 @@ struct PipeGeo {
 // the row's piece 8 l + p - s. A stage's fragments then lie in its ring slot and, those from piece 8 - s on, in the next one, so that the stage
 // behind the one multiplied has to be there too (and the rings are a stage deeper); s is the same for rows 8 apart, so one number for a lane and
 // all of its blocks. In its slot a piece lies where it would lie in a row on a line, the swizzle is of 8 l + p - s: reads are free of conflicts
-// as there (swizzled by p, 1031 x 4608 x 1160 had conflicts in all of its LDS cycles). Pieces in front of a row or behind it are loaded as copies of the nearest of the row and not used. Measured (us, without / with,
-// fp16): 436 x 1200 x 6472 32.9 / 22.6 on 64 x 64 tiles, 1024 x 1288 x 5128 34.4 / 24.2 on 64 x 96, 300 x 6144 x 4616 41.3 / 29.2 on
-// 128 x 96, 2048 x 2240 x 2248 35.5 / 28.7 on 192 x 128; not for short launches, 77 x 1160 x 1288 5.7 / 6.1 on 32 x 32. INT8 weights (lines
-// of 64 bytes, s of them in halves of pieces): 3000 x 3336 x 5000 138 / 122, 333 x 6144 x 4616 36 / 32.
+// as there (swizzled by p, 1031 x 4608 x 1160 had conflicts in all of its LDS cycles). Pieces in front of a row or behind it are loaded as
+// copies of the nearest of the row and not used. Measured (us, without / with, fp16, rows x features x contraction): 1024 x 1288 x 5128 34.4 /
+// 24.2 on 64 x 96 tiles, 300 x 6144 x 4616 41.3 / 29.0 on 128 x 96, 4096 x 1152 x 4616 60.5 / 47.5 on 192 x 128 (rows on lines 45.8); not for
+// short launches, 77 x 1160 x 1288 5.7 / 6.1 on 32 x 32. INT8 weights (lines of 64 bytes of them, s in halves of pieces): 3000 x 3336 x 5000
+// 138 / 122, 333 x 6144 x 4616 36 / 32.
 template <typename T, bool W8, bool GEGLU, int WM, int WN, int TM, int TN, int S, int NL, typename A = T, bool ACT = false, int WL = 16, bool OFF = false>
 __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(const PipeArgs args) {
     using G = PipeGeo<T, W8, GEGLU, WM, WN, TM, TN, S, NL, WL>;
