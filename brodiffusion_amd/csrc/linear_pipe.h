@@ -76,7 +76,7 @@ struct PipeArgs {
     PipeProblem p[kMaxLinearProblems];
     int first[kMaxLinearProblems];       // first tile of a problem
     int n_tiles, chunk;
-    int splits;                          // ACT instances: work groups that share a tile's contraction (blockIdx.y), and where each leaves its
+    int splits;                          // ACT instances: work groups that share a tile's contraction, and where each leaves its
     void* parts;                         // sums (PipeParts) if there are several
 };
 // The sums of a tile's parts: per tile and part, every multiplying wavefront's groups of 4 features x BS tokens, 64 lanes of 16 bytes each.
@@ -151,6 +151,12 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
     for (int i = 0; i < kMaxLinearProblems; ++i) asm volatile("" : : "s"(args.p[i].x), "s"(args.p[i].ldx_b));
     asm volatile("" : : "s"(args.first[1]), "s"(args.first[2]), "s"(args.n_tiles), "s"(args.chunk));
     int tile = (static_cast<int>(blockIdx.x) & 7) * args.chunk + (static_cast<int>(blockIdx.x) >> 3);
+    int part = 0;
+    if constexpr (ACT) {
+        // (parts: those of all tiles' first stages in front, so that a run meets the same stages of neighbouring tiles, and every XCD gets as many)
+        if (args.splits > 1) { part = tile / args.n_tiles; tile -= part * args.n_tiles; }
+        if (part >= args.splits) return;
+    }
     if (tile >= args.n_tiles) return;
     const int pi = (tile >= args.first[1] ? 1 : 0) + (tile >= args.first[2] ? 1 : 0);
     const PipeProblem& p = args.p[pi];
@@ -211,7 +217,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
         stages = (p.K + kBK - 1) / kBK;
         in_last = p.K - (stages - 1) * kBK;
         if (args.splits > 1) {      // (this part's stages; the divisions are left to those launches)
-            const int all = stages, part = static_cast<int>(blockIdx.y), from = part * all / args.splits, to = (part + 1) * all / args.splits;
+            const int all = stages, from = part * all / args.splits, to = (part + 1) * all / args.splits;
             stages = to - from;
             if (to < all) { in_last = kBK; followed = 1; }
             xg += static_cast<long>(from) * (kBK * 2);
@@ -536,7 +542,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
                     Sum v;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = acc[a / NG][b][4 * (a % NG) + i];
-                    parts[part_of<G::NW, FB * NG * TB>(tile, args.splits, blockIdx.y, wave, a * TB + b, lane)] = v;
+                    parts[part_of<G::NW, FB * NG * TB>(tile, args.splits, part, wave, a * TB + b, lane)] = v;
                 }
             return;
         }
@@ -708,7 +714,7 @@ int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st, int sp
     args.n_tiles = static_cast<int>(tiles);
     args.splits = splits;
     args.parts = parts;
-    args.chunk = (args.n_tiles + 7) / 8;
+    args.chunk = static_cast<int>((tiles * splits + 7) / 8);
     int first = 0;
     for (int i = 0; i < kMaxLinearProblems; ++i) {
         args.first[i] = i < n_problems ? first : 0x7fffffff;
@@ -726,7 +732,7 @@ int launch_pipe(const LinearBatch& batch, int n_problems, hipStream_t st, int sp
         p.inv_panel = inverse(p.panel_tiles); p.inv_width = inverse(p.width); p.inv_last = inverse(p.last_width);
         first += tiles_m(i) * tiles_n(i);
     }
-    hipLaunchKernelGGL((linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL, OFF>), dim3(static_cast<unsigned>((tiles + 7) / 8 * 8), ACT ? splits : 1), dim3(G::NT + 64 * NL), G::LDS, st, args);
+    hipLaunchKernelGGL((linear_pipe_kernel<T, W8, GEGLU, WM, WN, TM, TN, S, NL, A, ACT, WL, OFF>), dim3(static_cast<unsigned>((tiles * splits + 7) / 8 * 8)), dim3(G::NT + 64 * NL), G::LDS, st, args);
     MI_HIP_CHECK(hipGetLastError());
     if constexpr (JOIN) {
         const long waves = tiles * G::BM * G::BN / 256;      // of 4 features x 64 lanes
