@@ -104,11 +104,11 @@ inline bool off_lines(const LinearProblem& p) {
 
 // ── several work groups for a tile's contraction (the layer with an epilogue, where the caller lends memory for their sums) ──
 // Parts leave FP32 or INT32 sums, a second launch adds them and finishes the layer: 2 us and the bytes of the parts, written and read at
-// 3 TB/s. Paid where few tiles have a long contraction (us, one part / several, 16-bit; rows x features x contraction): 46 x 368 x 15984 29.5 / 8.2
-// (8 parts of 32 x 32 tiles), 382 x 352 x 14856 28.8 / 18.2 (INT8 weights, 6 of 64 x 64); not for 40 x 320 x 1280 5.7 / 6.4 or 1031 x 1152 x 4608
-// 19.8 / 22.0. Taken where the rule below expects a twentieth less. Over 150 problems of rows off lines, each in every form and number of parts, what
-// it takes is 2 % slower than the fastest on average (one part: 19 %); over 140 others of 33 to 1500 rows that it gives parts the time was
-// 0.69 (16-bit), 0.51 (W8A16) and 0.75 (W8A8) of one part's on average, at worst 1.11 (396 x 712 x 12576 W8A8 17.3 -> 19.3).
+// 5 TB/s. Paid where few tiles have a long contraction (us, one part / several; rows x features x contraction): 46 x 368 x 15984 29.5 / 8.2
+// (8 parts of 32 x 32 tiles), 224 x 1320 x 16320 35.3 / 22.3, with INT8 weights 55.4 / 21.4; not for 40 x 320 x 1280 5.7 / 6.4 or 1031 x 1152 x 4608
+// 19.8 / 22.0. Over 150 problems of 16-bit rows off lines, each in every form and number of parts, what the rule takes is 1.1 % slower than the
+// fastest on average (one part: 22 %), over 130 of INT8 weights 1.9 %. Over 280 others of 33 to 1500 rows that it gives parts the time was 0.71 (16-bit),
+// 0.52 (W8A16) and 0.78 (W8A8) of one part's on average, at worst 1.14 (96 x 10144 x 6016 26.9 -> 30.5).
 struct Parts { int form, splits; };
 inline constexpr int kSplitPlain[] = {k32x32, k64x64, k128x64_load, k128x128};
 inline constexpr int kSplitW8[] = {k8_32x32, k8_64x64, k8_128x64, k8_128x96};
@@ -125,13 +125,13 @@ inline Parts pick_parts(const LinearProblem& p, int n_cu) {
     const double steps = p.K / 64;
     auto cost = [&](const Form& f, int splits) {
         const double m = static_cast<double>((tiles_of(f, p) * splits + n_cu - 1) / n_cu), s = steps / splits;
-        return f.phi + s * f.lam + (m - 1) * (s * f.tau + f.eps) + (splits > 1 ? 2.0 + 2.0 * part_bytes(f, p, splits) / 3e6 : 0.0);
+        return f.phi + s * f.lam + (m - 1) * (s * f.tau + f.eps) + (splits > 1 ? 2.0 + 2.0 * part_bytes(f, p, splits) / 5e6 : 0.0);
     };
     LinearBatch b{};
     b.p[0] = p;
     const int whole = pick_form(table.forms, table.n, b, 1, n_cu);
     Parts best{whole, 1};
-    double best_cost = 0.95 * cost(table.forms[whole], 1);
+    double best_cost = 0.97 * cost(table.forms[whole], 1);
     for (int i = 0; i < 4; ++i)
         for (int splits : {2, 3, 4, 6, 8, 12, 16}) {
             if (splits * 4 > p.K / 64) break;

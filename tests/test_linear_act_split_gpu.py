@@ -38,10 +38,10 @@ def _args(c, act, out):
 
 
 # rows, features, contraction of 16-bit operands, and the form and parts that the rule gives them on 256 compute units
-PLAIN = [(33, 72, 4608, 0, 16), (33, 520, 4608, 0, 6), (130, 520, 6400, 0, 3), (33, 704, 6400, 0, 4), (33, 2248, 8960, 2, 6), (100, 2248, 8960, 2, 3), (33, 6144, 16384, 2, 2),
-         (65, 1640, 16384, 2, 4), (200, 2248, 12800, 4, 3), (65, 6144, 16384, 7, 4), (333, 1000, 16384, 4, 4), (200, 648, 16384, 2, 4), (1031, 328, 15936, 4, 4)]
-W8 = [(33, 72, 3200, 0, 12), (33, 1000, 3200, 0, 4), (33, 360, 8960, 1, 16), (33, 6144, 6400, 1, 2), (65, 2248, 6400, 1, 3), (65, 1640, 12800, 1, 4), (65, 2248, 8960, 1, 3), (65, 3600, 8960, 3, 4),
-      (130, 6144, 16384, 4, 2)]
+PLAIN = [(33, 72, 4608, 0, 16), (33, 520, 4608, 0, 6), (130, 520, 6400, 2, 8), (33, 704, 6400, 2, 16), (33, 2248, 8960, 2, 6), (100, 2248, 8960, 2, 3), (33, 6144, 16384, 2, 2),
+         (65, 1640, 16384, 4, 8), (200, 2248, 12800, 7, 6), (65, 6144, 16384, 7, 4), (333, 1000, 16384, 7, 8), (200, 648, 16384, 4, 8), (65, 2240, 15936, 4, 6)]
+W8 = [(33, 72, 3200, 0, 12), (33, 1000, 3200, 0, 4), (33, 360, 8960, 1, 16), (33, 6144, 6400, 1, 2), (65, 2248, 6400, 1, 3), (65, 1640, 12800, 3, 8), (65, 2248, 8960, 3, 6),
+      (65, 3600, 8960, 4, 6), (130, 6144, 16384, 4, 2)]
 
 
 @pytest.mark.parametrize("kind,M,N,K,form,splits", [("w16", *p) for p in PLAIN] + [("w8a8", *p) for p in PLAIN] + [("w8", *p) for p in W8])
