@@ -13,8 +13,10 @@
 // of 16 / G x 16 / G results; the others are waste, and the matrix pipes have it to spare: at G = 4 and 16 rows they take 64 bytes of
 // W per clock and compute unit, memory brings 10. (us, G = 1 / 4, bf16, 1152 x 4608: 1 row 7.0 / 3.9, 16 rows 10.0 / 5.3, 32 rows 13.9 / 7.3.)
 // Weights of 100 MB (INT8, 6144 x 16384), one token: 18.5 to 19.9 us = 5.1 to 5.4 TB/s, what a large copy reaches here.
+#include <algorithm>
 #include <type_traits>
 
+#include "linear_forms.h"
 #include "linear_math.h"
 
 namespace mi {
@@ -232,6 +234,8 @@ int launch_rows(const LinearProblem& p, hipStream_t st) {
     if (!many) return p.M <= 24 ? launch<T, KIND, 2, 2, 3, 1, 8>(p, st) : launch<T, KIND, 2, 2, 4, 1, 8>(p, st);
     if constexpr (KIND != kBoth8) {
         if (p.M <= 24) return three_blocks<8>(p, s.cu) ? launch<T, KIND, 2, 3, 3, 2, 4>(p, st) : launch<T, KIND, 2, 4, 3, 2, 4>(p, st);
+    }
+    if constexpr (KIND == kWeights8) {
         return three_blocks<8>(p, s.cu) ? launch<T, KIND, 2, 3, 4, 2, 4>(p, st) : launch<T, KIND, 2, 4, 4, 2, 4>(p, st);
     }
     return fail("linear: no kernel for %d rows", p.M);      // (linear_few_takes leaves these to others)
@@ -249,21 +253,34 @@ int launch_kind(const LinearProblem& p, hipStream_t st) {
 }  // namespace
 }  // namespace gemm
 
-// Up to which number of rows this kernel is the faster one, by both sides' times (us, this kernel / the rings of linear_pipe.h, bf16, weights of
-// up to 600 MB in turn; features x contraction):
-//   narrow      1152 x 4608: 16-bit 8 rows 4.4 / 9.9, 32 7.2 / 9.8; W8A16 4.0 / 15.3, 7.5 / 15.3; W8A8 32 5.3 / 6.9
+// Which problems this kernel is the faster one for, by both sides' times (us, this kernel / the rings of linear_pipe.h, with parts where those are
+// taken; bf16, weights of up to 500 MB in turn; features x contraction). Its time goes with the rows and the contraction, that of the rings hardly:
+//   narrow      368 x 15984: 16-bit 8 rows 8.2 / 8.1, 16 11.0 / 8.1; W8A16 12 9.8 / 10.1, 20 16.4 / 10.0; W8A8 16 6.9 / 7.5, 20 9.3 / 7.9;
+//               1152 x 4616: 16-bit 16 5.7 / 7.1, 32 7.9 / 7.4; W8A16 32 8.4 / 8.5; W8A8 32 5.4 / 6.8; 1792 x 10488 W8A16 16 8.8 / 11.5, 20 13.0 / 11.7
+//   up to 16 features per compute unit
+//               2240 x 6728: 16-bit 16 9.3 / 9.7, 20 11.3 / 9.9; W8A16 32 10.7 / 11.2; 4096 x 8192: 16-bit 24 17.6 / 18.5, 32 19.3 / 18.7
 //   brief       4608 x 1152: 16-bit 4 rows 4.2 / 4.4, 8 5.1 / 4.4; W8A16 24 5.8 / 5.9, 32 6.3 / 5.9; W8A8 1 5.0 / 4.0;
 //               8192 x 2048: 16-bit 1 row 7.6 / 6.9; W8A16 24 7.3 / 8.6; W8A8 1 5.3 / 5.2
-//   otherwise   6144 x 16384: 16-bit 16 39.8 / 43.6, 32 45.4 / 45.9; W8A16 16 24.4 / 48.9, 32 32.4 / 48.1; W8A8 16 20.6 / 23, 20 22.2 / 23.1;
-//               6144 x 6144: 16-bit 32 19.8 / 20.3; W8A16 15.1 / 20.1; W8A8 16 9.0 / 9.2, 20 10.1 / 9.2; 2240 x 6720: W8A8 32 7.6 / 8.7
-//   wide        16384 x 6144: 16-bit 24 41.6 / 43.2, 32 45.9 / 45.1; W8A16 4 21.2 / 21.8, 16 24.3 / 23.8; W8A8 16 19.8 / 19.8
+//   otherwise   7168 x 4096: 16-bit 8 12.9 / 13.5, 16 16.5 / 13.5; 6144 x 16384: 16-bit 24 41.9 / 43.2, 32 44.9 / 44.8; W8A16 32 32.6 / 37.8; W8A8 16 20.5 / 26.0
+//   wide        16384 x 6144: 16-bit 16 39.3 / 43.0, 24 42.6 / 44.7, rows off lines (6152) 4 36.1 / 35.9, 8 38.4 / 36.0; 9968 x 12808: 16-bit 4
+//               46.0 / 52.7, 8 55.3 / 52.8; W8A16 8 37.2 / 42.1; 16384 x 6144 W8A16 4 21.2 / 24.0, W8A8 16 19.8 / 19.8
 bool linear_few_takes(const LinearProblem& p) {
     const int kind = gemm::kind_of(p);
     const gemm::Shape s(p, kind);
-    if (s.narrow) return p.M <= 32;
-    if (kind == gemm::kSixteen) return s.brief ? p.M <= 4 && p.N <= 24 * s.cu : p.M <= (s.wide ? 24 : 32);
-    if (kind == gemm::kWeights8) return p.M <= (s.wide ? 8 : s.brief ? 24 : 32);
-    return !s.brief && p.M <= (p.N <= 16 * s.cu ? 32 : 16);
+    if (p.M > 32) return false;
+    const long work = static_cast<long>(p.M) * p.K;
+    if (kind == gemm::kSixteen) {
+        if (s.brief) return p.M <= 4 && p.N <= 24 * s.cu;
+        if (s.wide) return p.M <= (gemm::off_lines(p) ? 4 : 24);
+        if (p.N <= 16 * s.cu) return work <= std::max(130000, 60 * p.N);
+        return p.M <= 8 || (p.M <= 24 && p.K >= 5000);
+    }
+    if (kind == gemm::kWeights8) {
+        if (s.narrow) return work <= (p.M <= 16 ? 240000 : 170000);
+        return p.M <= (s.wide ? 8 : s.brief ? 24 : 32);
+    }
+    if (s.narrow) return work <= 150000;
+    return !s.brief && (p.M <= 16 || p.N <= 16 * s.cu);
 }
 
 int launch_linear_few(const LinearProblem& p, int dtype, hipStream_t st) {

@@ -134,7 +134,9 @@ inline Parts pick_parts(const LinearProblem& p, int n_cu) {
     double best_cost = 0.97 * cost(table.forms[whole], 1);
     for (int i = 0; i < 4; ++i)
         for (int splits : {2, 3, 4, 6, 8, 12, 16}) {
-            if (splits * 4 > p.K / 64) break;
+            // (at most two work groups per compute unit: with more, small tiles of large weights, what bounds a launch is the memory, which the
+            //  costs leave out: 16 x 16384 x 6144 W8A16 24.5 us in one part, 33.9 in 3 of 32 x 32 tiles)
+            if (splits * 4 > p.K / 64 || tiles_of(table.forms[table.split[i]], p) * splits > 2 * n_cu) break;
             if (const double c = cost(table.forms[table.split[i]], splits); c < best_cost) { best_cost = c; best = {table.split[i], splits}; }
         }
     return best;

@@ -127,7 +127,7 @@ def test_rows_off_lines_give_the_bits_of_rows_on_them(kind, two):
 # rows at the ends of each class; features: narrow (also fewer than one work group's), up to 16 per compute unit, three and four blocks, wide
 @pytest.mark.parametrize("kind", ["w16", "w8", "w8a8"])
 @pytest.mark.parametrize("N", [24, 2040, 2056, 4096, 6136, 8200, 16392])
-@pytest.mark.parametrize("K", [80, 1168, 4880])
+@pytest.mark.parametrize("K", [80, 1168, 4880, 5184])
 def test_every_shape_of_few_rows(kind, N, K):
     for M in (1, 4, 5, 8, 9, 16, 17, 24, 25, 32):
         _run(kind, M, N, K + (8 if kind == "w8" and M % 2 else 0), ("fp16", "bf16")[M % 2], ("none", "gelu", "gelu_tanh", "silu")[M % 4], f"{M} rows")
