@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(256) rms_norm_wave_kernel(RmsOperands<T> a, Rm
         }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) ss += __shfl_xor(ss, off);
-        const float inv = __builtin_amdgcn_rsqf(ss / static_cast<float>(cols) + eps);
+        const float inv = inverse_root(ss / static_cast<float>(cols) + eps);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const t8 x8 = __builtin_bit_cast(t8, v[i]), g8 = __builtin_bit_cast(t8, g[i]);
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256) rms_norm_rows_kernel(RmsOperands<T> a, Rm
         __syncthreads();                      // the previous row's readers are done with `red`
         if ((tid & 63) == 0) red[tid >> 6] = ss;
         __syncthreads();
-        const float inv = __builtin_amdgcn_rsqf((red[0] + red[1] + red[2] + red[3]) / static_cast<float>(cols) + eps);
+        const float inv = inverse_root((red[0] + red[1] + red[2] + red[3]) / static_cast<float>(cols) + eps);
 #pragma unroll
         for (int i = 0; i < kRmsChunks; ++i) {
             const int c = tid + 256 * i;

@@ -95,6 +95,13 @@ struct SdpaDev {
 __device__ __forceinline__ float rope_re(float a, float b, float c, float s) { return __builtin_fmaf(a, c, -(b * s)); }
 __device__ __forceinline__ float rope_im(float a, float b, float c, float s) { return __builtin_fmaf(a, s, b * c); }
 
+// 1 / sqrt(x) of a row norm. The instruction takes what is below the smallest normal number for zero: a row of bf16 values of 2^-64 without eps came out as
+// infinities. Such means are lifted by an even power of two; elsewhere the bits are the instruction's.
+__device__ __forceinline__ float inverse_root(float x) {
+    const bool small = x < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(small ? x * 0x1p100f : x) * (small ? 0x1p50f : 1.f);
+}
+
 // 0 = pick by problem size, 1 = 128-row kernel, 2 = 256-row ping-pong kernel (mi_sdpa_set_kernel_choice).
 int sdpa_kernel_choice();
 

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) rows_kernel(const RowsA
             asm volatile("" : "+v"(v[i]));
             if constexpr (NORM) asm volatile("" : "+v"(g[i]));
         }
-        const float inv = NORM ? __builtin_amdgcn_rsqf(ss / static_cast<float>(a.cols) + a.eps) : 1.f;
+        const float inv = NORM ? inverse_root(ss / static_cast<float>(a.cols) + a.eps) : 1.f;
         if (NORM && a.out != nullptr) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
