@@ -177,7 +177,8 @@ struct TileMath {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float sum = static_cast<float>(acc[a][b][4 * g + i]), bias = static_cast<float>(braw[a][g][i]);
-                            v[i] = A8 || W8 ? scaled_acc(sum, sx * p.w_scale[f + i], bias) : sum + bias;
+                            if constexpr (A8) v[i] = scaled_acc(sum * p.w_scale[f + i], sx, bias);
+                            else v[i] = W8 ? scaled_acc(sum, p.w_scale[f + i], bias) : sum + bias;
                         }
                         with_activation(p.act, [&](auto act) {
 #pragma unroll

@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_dma_kernel(const LinearBat
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if constexpr (A8) v[j][e] = scaled_acc(static_cast<float>(acc[i][j][e]), xs[j] * sw[e], bv[e]);
+                    if constexpr (A8) v[j][e] = scaled_acc(static_cast<float>(acc[i][j][e]) * sw[e], xs[j], bv[e]);
                     else v[j][e] = acc[i][j][e] + bv[e];
                 }
             with_activation(p.act, [&](auto act) {

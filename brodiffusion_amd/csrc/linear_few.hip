@@ -48,17 +48,18 @@ __global__ void __launch_bounds__(64 * WAVES) linear_few_kernel(const LinearProb
     const int n0 = static_cast<int>(blockIdx.x) * F;
 
     // What the epilogue needs, requested ahead of everything: result i of a thread is number i NT + tid, features running fastest.
-    float bias[OUT], res[OUT], scale[OUT];
+    float bias[OUT], res[OUT], scale[OUT], xs[KIND == kBoth8 ? OUT : 1];
 #pragma unroll
     for (int i = 0; i < OUT; ++i) {
         const int o = i * NT + tid, feat = n0 + o % F, row = o / F;
         bias[i] = res[i] = 0.f;
         scale[i] = 1.f;
+        if constexpr (KIND == kBoth8) xs[i] = 1.f;
         if (row < p.M && feat < p.N) {
             if (p.bias) bias[i] = static_cast<float>(static_cast<const T*>(p.bias)[feat]);
             if (p.residual) res[i] = static_cast<float>(static_cast<const T*>(p.residual)[static_cast<long>(row) * p.ldr + feat]);
             if constexpr (KIND != kSixteen) scale[i] = p.w_scale[feat];
-            if constexpr (KIND == kBoth8) scale[i] *= p.x_scale[row];
+            if constexpr (KIND == kBoth8) xs[i] = p.x_scale[row];
         }
     }
 
@@ -174,7 +175,10 @@ __global__ void __launch_bounds__(64 * WAVES) linear_few_kernel(const LinearProb
 #pragma unroll
             for (int h = 0; h < G; ++h) total += sums[w][f / R * TB + row / R][(h * R + row % R) * R + f % R];
         const float sum = static_cast<float>(total);
-        float v = KIND == kSixteen ? sum + bias[i] : scaled_acc(sum, scale[i], bias[i]);
+        float v;
+        if constexpr (KIND == kSixteen) v = sum + bias[i];
+        else if constexpr (KIND == kWeights8) v = scaled_acc(sum, scale[i], bias[i]);
+        else v = scaled_acc(sum * scale[i], xs[i], bias[i]);
         with_activation(p.act, [&](auto act) { v = act(v); });
         static_cast<T*>(p.y)[static_cast<long>(row) * p.ldy + n0 + f] = static_cast<T>(v + res[i]);
     }

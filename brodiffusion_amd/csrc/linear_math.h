@@ -82,7 +82,8 @@ __device__ __forceinline__ float gelu_erf(float x) {
 // multiply-add with the rounding to T that follows (v_fma_mixlo_f16: one rounding of the exact result) in some places and
 // not in others, and the plain and the GEGLU form of the same layer then disagree by a unit in the last place in about 3
 // outputs of 100 000; as a separate FP32 operation it is the FP32 multiply-add and conversion of the reference's kernel
-// everywhere.
+// everywhere. Sums of INT8 rows meet w_scale first and x_scale here: the product of the two scales can lie below FP32's normal numbers (bf16 rows of
+// 2^-130) where what comes out does not.
 __device__ __forceinline__ float scaled_acc(float acc, float scale, float bias) {
     float r = __builtin_fmaf(acc, scale, bias);
     asm volatile("" : "+v"(r));

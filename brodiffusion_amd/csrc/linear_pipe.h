@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(64 * (WM * WN + NL), 2) linear_pipe_kernel(con
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float bv = static_cast<float>(braw[a][i]), sum = static_cast<float>(acc[a / NG][b][4 * (a % NG) + i]);
-                    if constexpr (A8) v[a][b][i] = scaled_acc(sum, xs[b] * sraw[a][i], bv);
+                    if constexpr (A8) v[a][b][i] = scaled_acc(sum * sraw[a][i], xs[b], bv);
                     else if constexpr (W8) v[a][b][i] = scaled_acc(sum, sraw[a][i], bv);
                     else v[a][b][i] = sum + bv;
                 }
@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const PipeArgs args) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float b = static_cast<float>(bias[i]), s = static_cast<float>(sum[i]);
-        if constexpr (A8) v[i] = scaled_acc(s, p.x_scale[token] * p.w_scale[feature + i], b);
+        if constexpr (A8) v[i] = scaled_acc(s * p.w_scale[feature + i], p.x_scale[token], b);
         else if constexpr (W8) v[i] = scaled_acc(s, p.w_scale[feature + i], b);
         else v[i] = s + b;
     }

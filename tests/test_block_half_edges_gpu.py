@@ -28,3 +28,23 @@ def test_norms_of_rows_whose_mean_square_is_no_normal_number(cols, power):
     assert torch.all((scales.double() - a * inv / 127).abs() <= a * inv / 127 * rel * 1.01)
     if cols <= 16384:      # (the widest that this one takes)
         assert torch.equal(bd.rms_norm_rows(x, gain, 0.0), y)
+
+
+# few rows, both sides of 8 features per compute unit; rings, parts, 256 x 256 tiles; rows too far apart for the rings
+@pytest.mark.parametrize("M,N,K,stride", [(3, 64, 4096, 0), (9, 6144, 8192, 0), (40, 640, 2048, 0), (46, 368, 32000, 0), (600, 264, 1040, 0), (2188, 5392, 1024, 0),
+                                          (40, 72, 1168, 8388608)])
+def test_scales_of_rows_near_the_smallest_numbers(M, N, K, stride):
+    """INT8 rows whose scales are no normal numbers and a result that is one: one rounding to bf16, 2^-8, and FP32 roundings of the sum, its product
+    with a weight's scale and the fused rest, 3 2^-24. (Sums of at least K = 1024 positive products are above 2^20.)"""
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    x, w = (torch.randint(1, 128, s, generator=g, device="cuda", dtype=torch.int8) for s in ((M, K), (N, K)))
+    xs = (torch.randint(600, 1000, (M,), generator=g, device="cuda").double() * 2.0 ** -149).float()
+    ws = (1 + torch.rand(N, generator=g, device="cuda")) / 16
+    if stride:
+        far = torch.zeros((M - 1) * stride + K, dtype=torch.int8, device="cuda").as_strided((M, K), (stride, 1))
+        far.copy_(x)
+        x = far
+    y = bd.linear_act(x, w, x_scales=xs, w_scales=ws, dtype=torch.bfloat16)
+    ref = (x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()
+    assert bool((ref > 2.0 ** -125).all())
+    assert torch.all((y.double() - ref).abs() <= ref * (2.0 ** -8 + 3 * 2.0 ** -24) * 1.001)
