@@ -169,7 +169,9 @@ inline bool runs_share(const void* a, long a_len, const void* b, long b_len) {
     const char *const p = static_cast<const char*>(a), *const q = static_cast<const char*>(b);
     return p && q && p < q + b_len && q < p + a_len;
 }
-constexpr long kMostStride = 1L << 40;      // of rows, in elements: offsets stay within 64 bits whatever the rows
+// Row strides, and rows times stride, in elements: beyond any memory, and within 64 bits as bytes whatever is added
+constexpr long kMostStride = 1L << 40, kMostReach = 1L << 56;
+inline bool reach_too_far(long rows, long stride) { return rows > 1 && stride > 0 && rows - 1 > kMostReach / stride; }
 
 // One Y = X W^T + bias problem: X (M, K), W (N, K), Y (M, N), bias (N) or null; strides in elements.
 struct LinearProblem {

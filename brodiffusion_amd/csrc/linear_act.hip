@@ -49,6 +49,8 @@ int problem_of(const mi_linear_act_args& a, const char* op, LinearProblem& p) {
     if (p.ldx < p.K || p.ldw < p.K || p.ldy < p.N || (p.residual && p.ldr < p.N)) return fail("%s: a row stride is smaller than the row", op);
     for (long s : {p.ldx, p.ldw, p.ldy, p.ldr})
         if (s > kMostStride) return fail("%s: a row stride exceeds 2^40 elements", op);
+    if (reach_too_far(p.M, p.ldx) || reach_too_far(p.N, p.ldw) || reach_too_far(p.M, p.ldy) || reach_too_far(p.M, p.ldr))
+        return fail("%s: rows reach over more than 2^56 elements", op);
     uintptr_t al = 0;
     for (const void* q : {p.x, p.w, p.bias, p.residual, static_cast<const void*>(p.y)}) al |= reinterpret_cast<uintptr_t>(q);
     if (al & 15u) return fail("%s: operands must be 16-byte aligned", op);

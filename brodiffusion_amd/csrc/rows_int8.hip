@@ -217,6 +217,7 @@ int check_operands(const char* op, int rows, int cols, const Operand* ins, int n
             if (o.p == nullptr || bytes == 0) continue;
             if (o.rs % (8 * bytes) != 0 || o.rs < o.len) return fail("%s: the row stride of %s must be a multiple of 8 elements and at least cols", op, o.name);
             if (o.rs > bytes * kMostStride) return fail("%s: the row stride of %s exceeds 2^40 elements", op, o.name);
+            if (reach_too_far(rows, o.rs / bytes)) return fail("%s: the rows of %s reach over more than 2^56 elements", op, o.name);
             if (reinterpret_cast<uintptr_t>(o.p) % (8 * bytes) != 0) return fail("%s: %s must be %ld-byte aligned", op, o.name, 8 * bytes);
         }
     for (int i = 0; i < n_out; ++i) {

@@ -449,7 +449,7 @@ MI_API int mi_rms_norm_pair_forward(const void* x0, const void* gain0, void* out
  * gives, to rounding) in one pass, with the 8-bit operand of mi_linear_act_forward as its output where that is wanted. At least one of
  * out and out_q; out_q and out_scales together; sum_out (h itself) only with a residual and optional. The mean square is an FP32 sum, as
  * in mi_rms_norm_forward: a row whose sum of squares exceeds FP32 becomes zeros.
- * cols a multiple of 8, at most 65536; strides in elements (0 = dense), multiples of 8; 16-bit tensors 16-byte aligned, out_q 8-byte
+ * cols a multiple of 8, at most 65536; strides in elements (0 = dense), multiples of 8, at most 2^40, rows times stride at most 2^56; 16-bit tensors 16-byte aligned, out_q 8-byte
  * aligned. sum_out and out may each be x or residual (same pointer and stride); outputs share no other memory with each other or an
  * input. */
 typedef struct mi_add_rms_norm_args {
@@ -492,7 +492,8 @@ MI_API int mi_quantize_rows_forward(const mi_quantize_rows_args* args);
  * act: MI_ACT_*, GELU with erf, GELU_TANH = x / (1 + exp(-2 sqrt(2 / pi) (x + 0.044715 x^3))), SILU = x / (1 + exp(-x)).
  * in_features and out_features are multiples of 8 (W8A8: in_features of 16); strides in elements (0 = dense), multiples of 8 (INT8 x and
  * its w: of 16); pointers 16-byte aligned. y may be `residual` itself (same pointer and stride); a call whose y shares other memory with an
- * operand is refused, and so are more than 2^30 rows or features. rows may be 0. */
+ * operand is refused, and so are more than 2^30 rows or features, row strides above 2^40 elements and rows that reach over more than 2^56.
+ * rows may be 0. */
 enum { MI_ACT_NONE = 0, MI_ACT_GELU = 1, MI_ACT_GELU_TANH = 2, MI_ACT_SILU = 3 };
 typedef struct mi_linear_act_args {
     uint32_t struct_size;
