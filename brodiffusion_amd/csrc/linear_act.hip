@@ -68,6 +68,18 @@ int problem_of(const mi_linear_act_args& a, const char* op, LinearProblem& p) {
     return 1;
 }
 
+// Lent memory is none of the operands': parts of sums would go over them. (INT8 rows: K and their strides are in pairs by now)
+int check_scratch(const LinearProblem& p, const char* op, const void* scratch, size_t bytes) {
+    if (!scratch || bytes == 0) return 0;
+    const long run = static_cast<long>(bytes < (1ul << 60) ? bytes : 1ul << 60), w_bytes = p.w_scale && !p.x_scale ? 1 : 2, rows = p.M - 1;
+    const struct { const char* name; const void* first; long len; } operands[] = {
+        {"x", p.x, 2 * (rows * p.ldx + p.K)}, {"w", p.w, w_bytes * ((p.N - 1) * p.ldw + p.K)}, {"bias", p.bias, 2L * p.N}, {"residual", p.residual, 2 * (rows * p.ldr + p.N)},
+        {"y", p.y, 2 * (rows * p.ldy + p.N)}, {"w_scales", p.w_scale, 4L * p.N}, {"x_scales", p.x_scale, 4L * p.M}};
+    for (const auto& o : operands)
+        if (runs_share(scratch, run, o.first, o.len)) return fail("%s: scratch overlaps %s", op, o.name);
+    return 0;
+}
+
 size_t scratch_bytes(const LinearProblem& p) {
     if (linear_few_takes(p) || !rings_take(p)) return 0;
     const gemm::Parts s = gemm::pick_parts(p, device_cu_count());
@@ -87,7 +99,9 @@ int mi_linear_act_forward(const mi_linear_act_args* a) {
     if (reinterpret_cast<uintptr_t>(a->scratch) & 15u) return mi::fail("%s: scratch must be 16-byte aligned", op);
     mi::LinearProblem p{};
     const int rc = mi::problem_of(*a, op, p);
-    return rc <= 0 ? rc : mi::launch_linear_act(p, a->dtype, {a->scratch, a->scratch ? a->scratch_bytes : 0}, mi::resolve_stream(a->stream));
+    if (rc <= 0) return rc;
+    if (mi::check_scratch(p, op, a->scratch, a->scratch_bytes)) return -1;
+    return mi::launch_linear_act(p, a->dtype, {a->scratch, a->scratch ? a->scratch_bytes : 0}, mi::resolve_stream(a->stream));
 }
 
 size_t mi_linear_act_scratch_bytes(const mi_linear_act_args* a) {

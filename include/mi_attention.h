@@ -511,7 +511,8 @@ typedef struct mi_linear_act_args {
     void* scratch;           /* device, 16-byte aligned, or NULL: with mi_linear_act_scratch_bytes(args) bytes a launch of few output tiles and a
                                 long contraction gives each tile to several work groups, which leave their sums here for a second
                                 small launch to add in a fixed order. The next call on the stream may use it again; calls that can overlap
-                                on the GPU (two streams, two captured graphs replayed together) must not share one */
+                                on the GPU (two streams, two captured graphs replayed together) must not share one. Memory of its own: a
+                                call whose scratch overlaps an operand is refused */
     size_t scratch_bytes;
     void* stream;
 } mi_linear_act_args;
