@@ -58,8 +58,12 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) rows_kernel(const RowsA
     const T* const gain = static_cast<const T*>(a.gain);
     auto mine = [&](int i) { return lane + LANES * i < cpr; };      // (lanes past the end load the last chunk and leave it out of everything)
     auto at = [&](int i) { return min(lane + LANES * i, cpr - 1) * 8; };
+    // The gain waits in registers for the sums, but of a lane with more than 4 chunks (sixteen wavefronts have 128 registers): 8 chunks of both put 68 to
+    // 72 bytes a lane into memory. There it is read again, from the L2.
+    constexpr bool KEEP = NORM && N <= 4;
     for (long r = first; r < a.rows; r += step) {
-        u32x4 v[N], g[NORM ? N : 1];
+        u32x4 v[N], g[KEEP ? N : 1];
+        auto gain_of = [&](int i) { if constexpr (KEEP) return g[i]; else return *reinterpret_cast<const u32x4*>(gain + at(i)); };
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = *reinterpret_cast<const u32x4*>(x + r * a.x_rs + at(i));
         if constexpr (NORM) {
@@ -67,8 +71,10 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) rows_kernel(const RowsA
                 u32x4 b[N];
 #pragma unroll
                 for (int i = 0; i < N; ++i) b[i] = *reinterpret_cast<const u32x4*>(res + r * a.r_rs + at(i));
+                if constexpr (KEEP) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) g[i] = *reinterpret_cast<const u32x4*>(gain + at(i));
+                    for (int i = 0; i < N; ++i) g[i] = *reinterpret_cast<const u32x4*>(gain + at(i));
+                }
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const t8 p = __builtin_bit_cast(t8, v[i]), s = __builtin_bit_cast(t8, b[i]);
@@ -79,8 +85,10 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) rows_kernel(const RowsA
                     if (a.sum != nullptr && mine(i)) *reinterpret_cast<u32x4*>(static_cast<T*>(a.sum) + r * a.s_rs + at(i)) = v[i];
                 }
             } else {
+                if constexpr (KEEP) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) g[i] = *reinterpret_cast<const u32x4*>(gain + at(i));
+                    for (int i = 0; i < N; ++i) g[i] = *reinterpret_cast<const u32x4*>(gain + at(i));
+                }
             }
         }
         // (the largest magnitude as an integer: of FP32 bit patterns without sign a NaN is the largest)
@@ -90,7 +98,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) rows_kernel(const RowsA
         for (int i = 0; i < N; ++i) {
             const t8 h = __builtin_bit_cast(t8, v[i]);
             t8 w{};
-            if constexpr (NORM) w = __builtin_bit_cast(t8, g[i]);
+            if constexpr (NORM) w = __builtin_bit_cast(t8, gain_of(i));
             float s = 0.f;
             unsigned m = 0;
 #pragma unroll
@@ -119,13 +127,13 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) rows_kernel(const RowsA
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             asm volatile("" : "+v"(v[i]));
-            if constexpr (NORM) asm volatile("" : "+v"(g[i]));
+            if constexpr (KEEP) asm volatile("" : "+v"(g[i]));
         }
         const float inv = NORM ? inverse_root(ss / static_cast<float>(a.cols) + a.eps) : 1.f;
         if (NORM && a.out != nullptr) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const t8 h = __builtin_bit_cast(t8, v[i]), w = __builtin_bit_cast(t8, g[i]);
+                const t8 h = __builtin_bit_cast(t8, v[i]), w = __builtin_bit_cast(t8, gain_of(i));
                 t8 o;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(static_cast<float>(h[e]) * inv * static_cast<float>(w[e]));
@@ -145,7 +153,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) rows_kernel(const RowsA
         for (int i = 0; i < N; ++i) {
             const t8 h = __builtin_bit_cast(t8, v[i]);
             t8 w{};
-            if constexpr (NORM) w = __builtin_bit_cast(t8, g[i]);
+            if constexpr (NORM) w = __builtin_bit_cast(t8, gain_of(i));
             u32x2 o = {0u, 0u};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
