@@ -176,17 +176,16 @@ int launch_rows(const RowsArgs& a, hipStream_t st) {
     return 0;
 }
 
+// (launch_width asks for one chunk with one wavefront only, for four with eight and sixteen, for more with sixteen)
 template <typename T, int W, bool NORM>
 int launch_chunks(const RowsArgs& a, hipStream_t st) {
-    switch ((a.cols / 8 + 64 * W - 1) / (64 * W)) {
-        case 1: return launch_rows<T, 1, W, NORM>(a, st);
-        case 2: return launch_rows<T, 2, W, NORM>(a, st);
-        case 3: return launch_rows<T, 3, W, NORM>(a, st);
-        case 4: return launch_rows<T, 4, W, NORM>(a, st);
-        default:
-            if constexpr (W == 16) return launch_rows<T, 8, W, NORM>(a, st);
-            return fail("rows: no kernel for %d columns", a.cols);      // (not asked for below)
-    }
+    const int n = (a.cols / 8 + 64 * W - 1) / (64 * W);
+    if constexpr (W == 1) if (n == 1) return launch_rows<T, 1, W, NORM>(a, st);
+    if (n == 2) return launch_rows<T, 2, W, NORM>(a, st);
+    if (n == 3) return launch_rows<T, 3, W, NORM>(a, st);
+    if constexpr (W >= 8) if (n == 4) return launch_rows<T, 4, W, NORM>(a, st);
+    if constexpr (W == 16) if (n > 4) return launch_rows<T, 8, W, NORM>(a, st);
+    return fail("rows: no kernel for %d columns", a.cols);
 }
 
 // Wavefronts per row. Where rows fill the GPU (4 for each compute unit) up to 3 chunks per lane: fewer lanes have none, fewer meet at the barrier;
