@@ -48,3 +48,15 @@ def test_scales_of_rows_near_the_smallest_numbers(M, N, K, stride):
     ref = (x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()
     assert bool((ref > 2.0 ** -125).all())
     assert torch.all((y.double() - ref).abs() <= ref * (2.0 ** -8 + 3 * 2.0 ** -24) * 1.001)
+
+
+@pytest.mark.parametrize("kind", ["w16", "w8"])
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_activations_of_infinity(kind, M):
+    """Sums of plus and minus infinity: x times what tends to 0 or 1, so infinity to the right and NaN to the left, in every activation."""
+    x = torch.ones(M, 64, device="cuda", dtype=torch.bfloat16)
+    x[0, 5], x[1, 7], x[2, 9] = float("inf"), float("-inf"), float("nan")
+    w = torch.ones(72, 64, device="cuda", dtype=torch.int8 if kind == "w8" else torch.bfloat16)
+    for act in ("gelu", "gelu_tanh", "silu"):
+        y = bd.linear_act(x, w, activation=act, w_scales=torch.ones(72, device="cuda") if kind == "w8" else None)
+        assert bool((y[0] == float("inf")).all()) and torch.isnan(y[1:3]).all() and torch.isfinite(y[3:]).all(), act
