@@ -13,17 +13,16 @@
 // of 16 / G x 16 / G results; the others are waste, and the matrix pipes have it to spare: at G = 4 and 16 rows they take 64 bytes of
 // W per clock and compute unit, memory brings 10. (us, G = 1 / 4, bf16, 1152 x 4608: 1 row 7.0 / 3.9, 16 rows 10.0 / 5.3, 32 rows 13.9 / 7.3.)
 // Weights of 100 MB (INT8, 6144 x 16384), one token: 18.5 to 19.9 us = 5.1 to 5.4 TB/s, what a large copy reaches here.
-#include <algorithm>
+#include <iterator>
 #include <type_traits>
+#include <utility>
 
-#include "linear_forms.h"
+#include "linear_few_forms.h"
 #include "linear_math.h"
 
 namespace mi {
 namespace gemm {
 namespace {
-
-enum { kSixteen, kWeights8, kBoth8 };      // operands of 16 bits, INT8 weights, both INT8 (then K and strides in pairs of elements)
 
 // a 16-byte piece of a row whose rows are 8-byte aligned (INT8 weights of a contraction that is no multiple of 16)
 typedef unsigned u32x4_a8 __attribute__((ext_vector_type(4), aligned(8)));
@@ -192,100 +191,31 @@ int launch(const LinearProblem& p, hipStream_t st) {
     return 0;
 }
 
-// How a problem stands to the GPU. narrow: up to 8 features per compute unit, so that work groups of 8 features are what there is to spread;
-// wide: over 32; brief: not narrow, with a contraction of at most 4 KB of W's row, of which a wavefront gets a step or two.
-struct Shape {
-    int cu;
-    bool narrow, wide, brief;
-    Shape(const LinearProblem& p, int kind) {
-        cu = device_cu_count();
-        narrow = p.N <= 8 * cu;
-        wide = p.N > 32 * cu;
-        brief = !narrow && p.K * (kind == kWeights8 ? 1L : 2L) <= 4096;
-    }
-};
-int kind_of(const LinearProblem& p) { return p.x_scale ? kBoth8 : p.w_scale ? kWeights8 : kSixteen; }
-
-// Three or four blocks of R features per work group, by which of them the busiest compute unit has less: 6144 features are 256 work groups of 24 or
-// 192 of 32 (us, three / four blocks, 6144 x 16384: 16-bit 16 rows 39.2 / 42.8, W8A16 20 rows 26.7 / 30.7, W8A8 16 rows 20.4 / 24.3).
-template <int R> bool three_blocks(const LinearProblem& p, int cu) {
-    auto share = [&](int blocks) { return (p.N + R * blocks * cu - 1) / (R * blocks * cu) * blocks; };
-    return share(3) <= share(4);
+// the instance of a form: one of the N of the table FORMS
+template <typename T, int KIND, const auto& FORMS, int... I>
+int launch_form(const LinearProblem& p, const FewForm& form, std::integer_sequence<int, I...>, hipStream_t st) {
+    int rc = 1;
+    (void)((form == FORMS[I] ? (rc = launch<T, KIND, FORMS[I].G, FORMS[I].FB, FORMS[I].TB, FORMS[I].U, FORMS[I].wavefronts>(p, st), true) : false) || ...);
+    return rc <= 0 ? rc : fail("linear: no kernel for %d rows", p.M);
 }
-
-template <typename T, int KIND>
-int launch_rows(const LinearProblem& p, hipStream_t st) {
-    const Shape s(p, KIND);
-    // four wavefronts with two steps on their way each where there are work groups enough, else eight (with one, where a step is many loads)
-    const bool many = p.N > 16 * s.cu;
-    if (p.M <= 4) {
-        if constexpr (KIND != kBoth8) if (s.brief) return launch<T, KIND, 4, 4, 1, 1, 8>(p, st);
-        return launch<T, KIND, 4, 2, 1, 2, 8>(p, st);
-    }
-    if (s.narrow) {
-        if (p.M <= 8) return launch<T, KIND, 4, 2, 2, 2, 8>(p, st);
-        if (p.M <= 16) return launch<T, KIND, 4, 2, 4, 2, 8>(p, st);
-        return launch<T, KIND, 4, 2, 8, 1, KIND == kWeights8 ? 4 : 8>(p, st);
-    }
-    if (p.M <= 8) {
-        if (!many) return three_blocks<4>(p, s.cu) ? launch<T, KIND, 4, 3, 2, 2, 8>(p, st) : launch<T, KIND, 4, 4, 2, 2, 8>(p, st);
-        return three_blocks<4>(p, s.cu) ? launch<T, KIND, 4, 3, 2, 2, 4>(p, st) : launch<T, KIND, 4, 4, 2, 2, 4>(p, st);
-    }
-    if (p.M <= 16) {
-        if (!many) return launch<T, KIND, 2, 2, 2, 2, 8>(p, st);
-        return three_blocks<8>(p, s.cu) ? launch<T, KIND, 2, 3, 2, 2, 4>(p, st) : launch<T, KIND, 2, 4, 2, 2, 4>(p, st);
-    }
-    if (!many) return p.M <= 24 ? launch<T, KIND, 2, 2, 3, 1, 8>(p, st) : launch<T, KIND, 2, 2, 4, 1, 8>(p, st);
-    if constexpr (KIND != kBoth8) {
-        if (p.M <= 24) return three_blocks<8>(p, s.cu) ? launch<T, KIND, 2, 3, 3, 2, 4>(p, st) : launch<T, KIND, 2, 4, 3, 2, 4>(p, st);
-    }
-    if constexpr (KIND == kWeights8) {
-        return three_blocks<8>(p, s.cu) ? launch<T, KIND, 2, 3, 4, 2, 4>(p, st) : launch<T, KIND, 2, 4, 4, 2, 4>(p, st);
-    }
-    return fail("linear: no kernel for %d rows", p.M);      // (linear_few_takes leaves these to others)
+template <typename T, int KIND, const auto& FORMS>
+int launch_table(const LinearProblem& p, hipStream_t st) {
+    return launch_form<T, KIND, FORMS>(p, few_form(p, device_cu_count()), std::make_integer_sequence<int, std::size(FORMS)>{}, st);
 }
 
 template <typename T>
 int launch_kind(const LinearProblem& p, hipStream_t st) {
-    switch (kind_of(p)) {
-        case kBoth8: return launch_rows<T, kBoth8>(p, st);
-        case kWeights8: return launch_rows<T, kWeights8>(p, st);
-        default: return launch_rows<T, kSixteen>(p, st);
+    switch (few_kind(p)) {
+        case kBoth8: return launch_table<T, kBoth8, kFewBoth8>(p, st);
+        case kWeights8: return launch_table<T, kWeights8, kFewW8>(p, st);
+        default: return launch_table<T, kSixteen, kFew16>(p, st);
     }
 }
 
 }  // namespace
 }  // namespace gemm
 
-// Which problems this kernel is the faster one for, by both sides' times (us, this kernel / the rings of linear_pipe.h, with parts where those are
-// taken; bf16, weights of up to 500 MB in turn; features x contraction). Its time goes with the rows and the contraction, that of the rings hardly:
-//   narrow      368 x 15984: 16-bit 8 rows 8.2 / 8.1, 16 11.0 / 8.1; W8A16 12 9.8 / 10.1, 20 16.4 / 10.0; W8A8 16 6.9 / 7.5, 20 9.3 / 7.9;
-//               1152 x 4616: 16-bit 16 5.7 / 7.1, 32 7.9 / 7.4; W8A16 32 8.4 / 8.5; W8A8 32 5.4 / 6.8; 1792 x 10488 W8A16 16 8.8 / 11.5, 20 13.0 / 11.7
-//   up to 16 features per compute unit
-//               2240 x 6728: 16-bit 16 9.3 / 9.7, 20 11.3 / 9.9; W8A16 32 10.7 / 11.2; 4096 x 8192: 16-bit 24 17.6 / 18.5, 32 19.3 / 18.7
-//   brief       4608 x 1152: 16-bit 4 rows 4.2 / 4.4, 8 5.1 / 4.4; W8A16 24 5.8 / 5.9, 32 6.3 / 5.9; W8A8 1 5.0 / 4.0;
-//               8192 x 2048: 16-bit 1 row 7.6 / 6.9; W8A16 24 7.3 / 8.6; W8A8 1 5.3 / 5.2
-//   otherwise   7168 x 4096: 16-bit 8 12.9 / 13.5, 16 16.5 / 13.5; 6144 x 16384: 16-bit 24 41.9 / 43.2, 32 44.9 / 44.8; W8A16 32 32.6 / 37.8; W8A8 16 20.5 / 26.0
-//   wide        16384 x 6144: 16-bit 16 39.3 / 43.0, 24 42.6 / 44.7, rows off lines (6152) 4 36.1 / 35.9, 8 38.4 / 36.0; 9968 x 12808: 16-bit 4
-//               46.0 / 52.7, 8 55.3 / 52.8; W8A16 8 37.2 / 42.1; 16384 x 6144 W8A16 4 21.2 / 24.0, W8A8 16 19.8 / 19.8
-bool linear_few_takes(const LinearProblem& p) {
-    const int kind = gemm::kind_of(p);
-    const gemm::Shape s(p, kind);
-    if (p.M > 32) return false;
-    const long work = static_cast<long>(p.M) * p.K;
-    if (kind == gemm::kSixteen) {
-        if (s.brief) return p.M <= 4 && p.N <= 24 * s.cu;
-        if (s.wide) return p.M <= (gemm::off_lines(p) ? 4 : 24);
-        if (p.N <= 16 * s.cu) return work <= std::max(130000, 60 * p.N);
-        return p.M <= 8 || (p.M <= 24 && p.K >= 5000);
-    }
-    if (kind == gemm::kWeights8) {
-        if (s.narrow) return work <= (p.M <= 16 ? 240000 : 170000);
-        return p.M <= (s.wide ? 8 : s.brief ? 24 : 32);
-    }
-    if (s.narrow) return work <= 150000;
-    return !s.brief && (p.M <= 16 || p.N <= 16 * s.cu);
-}
+bool linear_few_takes(const LinearProblem& p) { return gemm::few_takes(p, device_cu_count()); }
 
 int launch_linear_few(const LinearProblem& p, int dtype, hipStream_t st) {
     return dtype == MI_DTYPE_BF16 ? gemm::launch_kind<__bf16>(p, st) : gemm::launch_kind<_Float16>(p, st);
