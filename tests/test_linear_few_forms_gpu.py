@@ -1,6 +1,6 @@
 """linear_act for few rows on every form of that kernel, the form asserted for each call (tests/test_linear_few_rule.py has the rule): rows at both ends of a form's
 class, features that fill the last work group and that leave it a rest, whole and partial steps, rows on 128-byte lines and off them where the rule lets
-both. Operands with poisoned borders; tests/test_linear_act_gpu.py derives the bounds."""
+both. Operands with poisoned borders; tests/test_linear_act_gpu.py derives the bounds. And rows by themselves and among others."""
 import pytest
 import torch
 
@@ -55,3 +55,40 @@ def test_every_form(kind, form, dtype):
         call(c, ACTS[i % 4], out=wide[:M, :N])
         check(c, ACTS[i % 4], wide[:M, :N], f"{M} x {N} x {k}, {'on' if on_lines else 'off'} lines")
         assert bool((wide[M:] == 7).all()) and bool((wide[:, N:] == 7).all())
+
+
+def _rows_of(c, rows):
+    d = {**c, "x": c["x"][rows].contiguous(), "residual": c["residual"][rows].contiguous()}
+    if c["x_scales"] is not None:
+        d["x_scales"] = c["x_scales"][rows].contiguous()
+    return d
+
+
+@pytest.mark.parametrize("kind,K", [("w16", 5184), ("w8", 5184), ("w8a8", 10368)])
+def test_any_number_of_rows_of_a_class_gives_the_same_bits(kind, K):
+    """9 to 16 rows, in any order: one form of the kernel for few rows."""
+    N = 6136
+    c = make(5, kind, 16, N, K, "bf16")
+    whole = call(c, "silu")
+    check(c, "silu", whole)
+    for M in range(9, 17):
+        assert few_form(M, N, K, kind, 0, bd.device_info()["compute_units"]) == (2, 3, 2, 2, 4)
+        rows = torch.randperm(16, generator=torch.Generator().manual_seed(M))[:M].cuda()
+        assert torch.equal(call(_rows_of(c, rows), "silu"), whole[rows]), M
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("M,N,K", [(12, 6136, 5184), (40, 328, 640), (46, 368, 16000), (300, 1160, 1168), (2188, 5392, 1152)])
+def test_other_rows_do_not_change_a_row(kind, M, N, K):
+    """Every third row kept, the others replaced (some by what is not finite): the kept rows' bits."""
+    c, other = make(7, kind, M, N, K, "fp16"), make(8, kind, M, N, K, "fp16")
+    whole = call(c, "gelu")
+    kept = torch.arange(M, device="cuda") % 3 == 0
+    d = {**c, "x": torch.where(kept[:, None], c["x"], other["x"])}
+    if kind == "w8a8":
+        d["x_scales"] = torch.where(kept, c["x_scales"], other["x_scales"])
+        d["x_scales"][1] = float("nan")
+    else:
+        d["x"][1, 3], d["x"][M - 1 if (M - 1) % 3 else M - 2, K - 1] = float("inf"), float("nan")
+    again = call(d, "gelu")
+    assert torch.equal(again[kept], whole[kept]) and not torch.isfinite(again[1]).any()
