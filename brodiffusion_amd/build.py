@@ -63,6 +63,7 @@ HOST_DIR = os.path.join(HERE, "host")
 HOST_LIB = os.path.join(LIB_DIR, "libbrodiffusion_amd_host.so")
 HOST_TEST = os.path.join(LIB_DIR, "test_host_ops")
 BLOCK_TEST = os.path.join(LIB_DIR, "test_block_half")
+SCRATCH_TEST = os.path.join(LIB_DIR, "test_linear_act_scratch")
 SPLIT_TEST = os.path.join(LIB_DIR, "test_split_geo")
 FORMS_LIB = os.path.join(LIB_DIR, "liblinear_forms_test.so")
 WAITING_LIB = os.path.join(LIB_DIR, "libwaiting_test.so")
@@ -82,9 +83,12 @@ def build_host(with_test: bool = True, verbose: bool = False) -> str:
         raise RuntimeError("host library build failed")
     if with_test:
         oracle_dir = os.path.join(ROOT, "oracle")
-        for source, exe in (("test_host_ops.cpp", HOST_TEST), ("test_block_half.cpp", BLOCK_TEST)):
+        rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+        # (the last one captures graphs itself)
+        hip = ["-D__HIP_PLATFORM_AMD__", "-isystem" + os.path.join(rocm, "include"), "-L" + os.path.join(rocm, "lib"), "-lamdhip64"]
+        for source, exe, more in (("test_host_ops.cpp", HOST_TEST, []), ("test_block_half.cpp", BLOCK_TEST, []), ("test_linear_act_scratch.cpp", SCRATCH_TEST, hip)):
             cmd = [*common, os.path.join(ROOT, "tests", "cpp", source), "-o", exe, *rpath,
-                   "-Wl,-rpath,$ORIGIN/../../oracle", "-L" + oracle_dir, "-lbrodiffusion_amd_host", "-lmi_attention", "-loracle"]
+                   "-Wl,-rpath,$ORIGIN/../../oracle", "-L" + oracle_dir, "-lbrodiffusion_amd_host", "-lmi_attention", "-loracle", *more]
             r = subprocess.run(cmd, capture_output=True, text=True)
             if r.returncode != 0:
                 sys.stderr.write(r.stdout + r.stderr)
