@@ -21,7 +21,7 @@ int launch_form(const LinearBatch& b, int form, hipStream_t st) {
 }
 // ... in several parts (the forms of kSplitW8)
 template <typename T, int WL>
-int launch_split(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
+int launch_split(const LinearBatch& b, const ActLaunch& s, void* parts, hipStream_t st) {
     switch (s.form) {
         case k8_32x32: return launch_pipe<T, true, false, 1, 1, 1, 1, 6, 2, T, true, WL, true>(b, 1, st, s.splits, parts);
         case k8_64x64: return launch_pipe<T, true, false, 2, 2, 1, 1, 4, 4, T, true, WL, true>(b, 1, st, s.splits, parts);
@@ -31,7 +31,7 @@ int launch_split(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
 }
 // ... of rows that do not begin on lines (kOff8), in one part or, with memory for them, several
 template <typename T, int WL, bool JOIN>
-int launch_off(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
+int launch_off(const LinearBatch& b, const ActLaunch& s, void* parts, hipStream_t st) {
     switch (s.form) {
         case kOff8_32x32: return launch_pipe<T, true, false, 1, 1, 1, 1, 6, 2, T, true, WL, JOIN>(b, 1, st, s.splits, parts);
         case kOff8_64x64: return launch_pipe<T, true, false, 2, 2, 1, 1, 4, 4, T, true, WL, JOIN>(b, 1, st, s.splits, parts);
@@ -48,13 +48,9 @@ int launch_off(const LinearBatch& b, Parts s, void* parts, hipStream_t st) {
 }
 template <typename T, int WL>
 int launch_words(const LinearBatch& b, const LinearScratch& lent, hipStream_t st) {
-    const LinearProblem& p = b.p[0];
-    const FormTable& table = table_of(p);
-    const bool off = off_lines(p);
-    const Parts s = pick_parts(p, device_cu_count());
-    if (s.splits > 1 && lent.bytes >= static_cast<size_t>(part_bytes(table.forms[s.form], p, s.splits))) return off ? launch_off<T, WL, true>(b, s, lent.p, st) : launch_split<T, WL>(b, s, lent.p, st);
-    const int form = s.splits > 1 ? pick_form(table.forms, table.n, b, 1, device_cu_count()) : s.form;
-    return off ? launch_off<T, WL, false>(b, {form, 1}, nullptr, st) : launch_form<T, WL>(b, form, st);
+    const ActLaunch s = act_launch(b.p[0], lent.bytes, device_cu_count());
+    if (s.splits > 1) return s.off ? launch_off<T, WL, true>(b, s, lent.p, st) : launch_split<T, WL>(b, s, lent.p, st);
+    return s.off ? launch_off<T, WL, false>(b, s, nullptr, st) : launch_form<T, WL>(b, s.form, st);
 }
 template <typename T>
 int launch_any(const LinearBatch& b, const LinearScratch& lent, hipStream_t st) {

@@ -141,6 +141,17 @@ inline Parts pick_parts(const LinearProblem& p, int n_cu) {
         }
     return best;
 }
+// What a call is launched as: in parts where the caller lent the memory for them
+struct ActLaunch { int form, splits; bool off; };
+inline ActLaunch act_launch(const LinearProblem& p, size_t lent_bytes, int n_cu) {
+    const FormTable& table = table_of(p);
+    const Parts s = pick_parts(p, n_cu);
+    const bool off = off_lines(p);
+    if (s.splits == 1 || lent_bytes >= static_cast<size_t>(part_bytes(table.forms[s.form], p, s.splits))) return {s.form, s.splits, off};
+    LinearBatch b{};
+    b.p[0] = p;
+    return {pick_form(table.forms, table.n, b, 1, n_cu), 1, off};
+}
 
 }  // namespace gemm
 }  // namespace mi
