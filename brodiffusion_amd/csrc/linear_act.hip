@@ -3,8 +3,9 @@
 //
 // Few rows (linear_few.hip): bound by the bytes of W, which go to registers once. Otherwise the rings of linear_pipe.h and the 256 x 256 tiles of
 // linear_dma.h with this epilogue, bound by the matrix pipes under the power limit. Rows so far apart that 32-bit offsets do not span a tile: tiles
-// through registers (linear.hip). Measured (us; kernel, epilogue included): 1 x 1152 x 4608 bf16 3.5; 1 x 6144 x 16384 W8A8 17.3 = 5.8 TB/s;
-// 20 x 16384 x 6144 W8A16 22; 1031 x 1160 x 4608 fp16 20.6; 4608 x 6144 x 16384 bf16 764 = 1.21 PFLOP/s, W8A8 413 = 2.25 PTOP/s (rows x contraction x features).
+// through registers (linear.hip). Measured (us; kernel, epilogue included, operands of 1 GiB in turn; rows x contraction x features): 1 x 1152 x 4608 bf16 5.2
+// (weights in the last-level cache: 3.5 to 3.9); 1 x 6144 x 16384 W8A8 19.2 = 5.2 TB/s; 20 x 16384 x 6144 W8A16 27.5; 1031 x 1160 x 4608 fp16 22.9;
+// 4608 x 6144 x 16384 bf16 767 = 1.21 PFLOP/s, W8A8 423 = 2.19 PTOP/s.
 #include "linear_forms.h"
 
 namespace mi {

@@ -11,8 +11,10 @@
 // x 4608 10 us at 16 rows, 22 at 64). So an operand here holds 16 / G rows and G groups of pieces, the groups as neighbouring lanes: G 16 bytes
 // in a run. Row (r, h) of W meets column (t, h') of X, and of the 16 x 16 results those with h = h' are wanted, G partial sums of each
 // of 16 / G x 16 / G results; the others are waste, and the matrix pipes have it to spare: at G = 4 and 16 rows they take 64 bytes of
-// W per clock and compute unit, memory brings 10. (us, G = 1 / 4, bf16, 1152 x 4608: 1 row 7.0 / 3.9, 16 rows 10.0 / 5.3, 32 rows 13.9 / 7.3.)
-// Weights of 100 MB (INT8, 6144 x 16384), one token: 18.5 to 19.9 us = 5.1 to 5.4 TB/s, what a large copy reaches here.
+// W per clock and compute unit, memory brings 10. (us, G = 1 / 4, bf16, 1152 x 4608 in the last-level
+// cache: 1 row 7.0 / 3.9, 16 rows 10.0 / 5.3, 32 rows 13.9 / 7.3.)
+// Weights of 100 MB (INT8, 6144 x 16384), several in turn, one token: 18.5 to 19.9 us = 5.1 to 5.4 TB/s, what a large copy reaches here.
+// Which problems come here and with which work groups: linear_few_forms.h.
 #include <iterator>
 #include <type_traits>
 #include <utility>

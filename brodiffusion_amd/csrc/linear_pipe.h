@@ -1,5 +1,6 @@
-// Y = X W^T + b for problems between the smallest and the 256 x 256-tile kernel's on gfx950 (contractions that are a
-// multiple of 64; 16-bit or INT8 weights; plain or GEGLU).
+// Y = X W^T + b for problems between the smallest and the 256 x 256-tile kernel's on gfx950 (16-bit or INT8 weights, plain or GEGLU, contractions that
+// are a multiple of 64), and the same layer with an epilogue (ACT: any contraction of whole 16-byte pieces, INT8 operands, rows off 128-byte lines, tiles
+// whose contraction several work groups share).
 //
 // Operands go global -> LDS by DMA into a ring of S stages of 64 contraction elements each: no staging registers, no LDS
 // store instructions, and as many steps in flight as the LDS holds (a problem of this size is a chain of memory latencies
@@ -20,7 +21,8 @@
 // and the DMA of stage t + S, which goes into the ring slot of stage t, is dealt out between the MFMAs of the second half of
 // step t and the first half of step t + 1: issued in one burst behind the barrier it made a step of 128 x 128 take 0.57 us
 // on an otherwise empty compute unit, 0.4 dealt out. The accumulation order is the same in every form (and in linear_dma.h):
-// a problem gives the same bits whichever one takes it, alone or in a launch with others.
+// a problem gives the same bits whichever one takes it, alone or in a launch with others. Parts of a contraction are the exception: each is
+// summed so, and their FP32 sums are added (INT32 sums are exact either way).
 //
 // Products are v_mfma_f32_16x16x32, two token blocks with one feature block in a row. What bounds the large forms on values of a
 // real spread is the power limit, and a loop of these keeps up 2.03 PFLOP/s (bf16, N(0, 1); 1.90 fp16) at it, one of

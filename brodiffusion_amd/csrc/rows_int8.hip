@@ -10,9 +10,10 @@
 // quotients whatever the order of the sum of squares. A row of zeros has q = 0 and scale 0, one with a value that is not finite q = 0
 // and scale NaN.
 //
-// Bound: HBM. Each row is read once, held in registers between its sums and what is written, and nothing else passes through memory.
+// Bound: HBM. Each row is read once, held in registers between its sums and what is written, and nothing else passes through memory but the gain.
 // A lane holds N 16-byte chunks; a row belongs to W wavefronts (one: sums by lane exchanges alone, four rows in a work group; more:
-// one exchange through LDS behind a barrier). 4608 rows of 6144: 41.8 us = 5.4 TB/s, a large copy's rate here; to 8 bits 37.9 us (5.2 TB/s).
+// one exchange through LDS behind a barrier). 4608 rows of 6144, several sets in turn: 41.9 us = 5.4 TB/s, a large copy's rate here (5.1 to 5.4);
+// to 8 bits 37.9 us (5.2 TB/s).
 #include "internal.h"
 
 namespace mi {

@@ -448,9 +448,10 @@ MI_API int mi_rms_norm_pair_forward(const void* x0, const void* gain0, void* out
  * The residual stream's step between two projections of a transformer block: mi_add_inplace and mi_rms_norm_forward (whose results it
  * gives, to rounding) in one pass, with the 8-bit operand of mi_linear_act_forward as its output where that is wanted. At least one of
  * out and out_q; out_q and out_scales together; sum_out (h itself) only with a residual and optional. The mean square is an FP32 sum, as
- * in mi_rms_norm_forward: a row whose sum of squares exceeds FP32 becomes zeros.
- * cols a multiple of 8, at most 65536; strides in elements (0 = dense), multiples of 8, at most 2^40, rows times stride at most 2^56; 16-bit tensors 16-byte aligned, out_q 8-byte
- * aligned. sum_out and out may each be x or residual (same pointer and stride); outputs share no other memory with each other or an
+ * in mi_rms_norm_forward: a row whose sum of squares exceeds FP32 becomes zeros, and without eps one whose squares all lie below 2^-149
+ * infinite.
+ * cols a multiple of 8, at most 65536; strides in elements (0 = dense), multiples of 8, at most 2^40, rows times stride at most 2^56; 16-bit
+ * tensors 16-byte aligned, out_q 8-byte aligned. sum_out and out may each be x or residual (same pointer and stride); outputs share no other memory with each other or an
  * input. */
 typedef struct mi_add_rms_norm_args {
     uint32_t struct_size;
@@ -518,7 +519,9 @@ typedef struct mi_linear_act_args {
 } mi_linear_act_args;
 MI_API int mi_linear_act_forward(const mi_linear_act_args* args);
 /* Bytes of scratch that this call would use (the scratch fields are ignored): 0 where it would not, or is one that is refused. With less the
- * call does without; results agree to rounding (INT8 rows: the sums are exact either way, so bit for bit). */
+ * call does without. No result depends on timing or on the other rows of its call, and INT8 rows give the same bits whatever way a call
+ * goes. FP32 sums of 16-bit rows round in the order that sizes and type, the scratch that is lent, and whether rows begin on 128-byte lines
+ * (addresses, strides) lead to. */
 MI_API size_t mi_linear_act_scratch_bytes(const mi_linear_act_args* args);
 
 /* ── attention with its projections ────────────────────────────────────────
