@@ -22,6 +22,7 @@ MI_LINEAR_ATTN_FORM_BY_SIZE = 0
 MI_LINEAR_ATTN_FORM_THREE_LAUNCHES = 1
 MI_LINEAR_ATTN_FORM_ONE_LAUNCH = 2
 MI_ACT_NONE, MI_ACT_GELU, MI_ACT_GELU_TANH, MI_ACT_SILU = 0, 1, 2, 3
+MI_NORM_NONE, MI_NORM_RMS, MI_NORM_LAYER = 0, 1, 2
 MI_LAYOUT_TOKEN_MAJOR = 0
 MI_LAYOUT_CHANNEL_MAJOR = 1
 
@@ -30,7 +31,7 @@ EXPORTS = [
     "mi_malloc", "mi_free", "mi_memcpy_h2d", "mi_memcpy_d2h", "mi_memcpy_d2d_async", "mi_memset_async",
     "mi_sdpa_forward", "mi_sdpa_split_scratch_bytes", "mi_sdpa_supported", "mi_sdpa_set_kernel_choice", "mi_attention_map_avg", "mi_rope_apply", "mi_headnorm_rope", "mi_scale_rows",
     "mi_linear_attn_workspace_bytes", "mi_linear_attn_scratch_bytes", "mi_linear_attn_relu_forward", "mi_linear_attn_supported", "mi_linear_attn_relu_forward_static_scratch",
-    "mi_linear_forward", "mi_linear_forward_n", "mi_linear_geglu_forward", "mi_add_inplace", "mi_add_row_bias", "mi_rms_norm_forward", "mi_rms_norm_pair_forward", "mi_add_rms_norm_forward", "mi_quantize_rows_forward", "mi_linear_act_forward", "mi_linear_act_scratch_bytes", "mi_flash_attention_scratch_bytes", "mi_attn_block_scratch_bytes", "mi_flash_attention_qkvo_forward",
+    "mi_linear_forward", "mi_linear_forward_n", "mi_linear_geglu_forward", "mi_add_inplace", "mi_add_row_bias", "mi_rms_norm_forward", "mi_rms_norm_pair_forward", "mi_add_rms_norm_forward", "mi_quantize_rows_forward", "mi_gate_add_norm_forward", "mi_linear_act_forward", "mi_linear_act_scratch_bytes", "mi_flash_attention_scratch_bytes", "mi_attn_block_scratch_bytes", "mi_flash_attention_qkvo_forward",
     "mi_flash_attention_q_with_kv_cached_forward", "mi_flash_attention_project_kv",
 ]
 
@@ -162,6 +163,19 @@ class MiQuantizeRowsArgs(C.Structure):
     ]
 
 
+class MiGateAddNormArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("x", C.c_void_p), ("branch", C.c_void_p), ("gate", C.c_void_p), ("post_gain", C.c_void_p), ("gain", C.c_void_p), ("scale", C.c_void_p), ("shift", C.c_void_p),
+        ("sum_out", C.c_void_p), ("out", C.c_void_p),
+        ("rows", C.c_int32), ("cols", C.c_int32), ("post_norm", C.c_int32), ("norm", C.c_int32),
+        ("gate_rows", C.c_int32), ("scale_rows", C.c_int32), ("shift_rows", C.c_int32),
+        ("x_row_stride", C.c_int64), ("branch_row_stride", C.c_int64), ("gate_row_stride", C.c_int64), ("scale_row_stride", C.c_int64), ("shift_row_stride", C.c_int64),
+        ("sum_row_stride", C.c_int64), ("out_row_stride", C.c_int64),
+        ("residual_scale", C.c_float), ("post_eps", C.c_float), ("eps", C.c_float), ("stream", C.c_void_p),
+    ]
+
+
 class MiLinearActArgs(C.Structure):
     _fields_ = [
         ("struct_size", C.c_uint32), ("dtype", C.c_int32),
@@ -241,6 +255,7 @@ def lib() -> C.CDLL:
         L.mi_rms_norm_pair_forward.argtypes = [C.c_void_p] * 6 + [C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.c_float, C.c_int32, C.c_void_p]
         L.mi_add_rms_norm_forward.argtypes = [C.POINTER(MiAddRmsNormArgs)]
         L.mi_quantize_rows_forward.argtypes = [C.POINTER(MiQuantizeRowsArgs)]
+        L.mi_gate_add_norm_forward.argtypes = [C.POINTER(MiGateAddNormArgs)]
         L.mi_linear_act_forward.argtypes = [C.POINTER(MiLinearActArgs)]
         L.mi_linear_act_scratch_bytes.argtypes = [C.POINTER(MiLinearActArgs)]
         L.mi_linear_act_scratch_bytes.restype = C.c_size_t

@@ -1,0 +1,259 @@
+// The step between two blocks of a transformer: a block's output, normalised if the model does that, times its gate onto the residual stream, and the norm in
+// front of the next block with that block's modulation, in one pass.
+//
+//   b = post(branch) post_gain                    post: nothing, RMS or layer norm, FP32
+//   h = T(residual_scale x + gate b)              one rounding; everything below is of the stored value
+//   y = T(pre(h) gain (1 + scale) + shift)        FP32 in between, one rounding
+// RMS: v / sqrt(mean v^2 + eps); layer: (v - mean) / sqrt(mean (v - mean)^2 + eps), the squares summed of the differences, in registers, not as a difference of
+// sums. gate, scale and shift are vectors of all rows or one for each run of rows (an image of a batch, a token).
+//
+// Bound: HBM. x and the branch are read once, h and y written once, the row stays in registers between its sums.
+#include "rows_checks.h"
+
+namespace mi {
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// A vector of the columns for each `each` rows
+struct RowVectors {
+    const void* p;       // null: not there
+    long rs;             // elements
+    int each;
+};
+struct GateNorm {
+    const void* x; const void* branch; const void* post_gain; const void* gain;
+    void* sum; void* out;                         // each null: not asked for
+    RowVectors gate, scale, shift;
+    int rows, cols, post, pre;                    // MI_NORM_*
+    long x_rs, b_rs, s_rs, o_rs;                  // elements
+    float alpha, post_eps, eps;
+};
+
+// W wavefronts per row (one: four rows to a work group), N 16-byte chunks per lane, as in rows_int8.hip.
+template <typename T, int N, int W>
+__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) gate_norm_kernel(const GateNorm a) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    constexpr int LANES = 64 * W;
+    // (sixteen wavefronts have 128 registers: the vectors of all chunks at once would put some of them into memory)
+    constexpr bool TIGHT = W == 16 && N >= 4;
+    __shared__ float red[2][4][W];                // [parity of the row][sum of it]: a slot is written again two rows on, a barrier after its last reader
+    const int cpr = a.cols / 8;
+    int lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const long first = W == 1 ? blockIdx.x * 4L + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x, step = gridDim.x * (W == 1 ? 4L : 1L);
+    const float inv_cols = 1.f / static_cast<float>(a.cols);
+    auto mine = [&](int i) { return lane + LANES * i < cpr; };      // (lanes past the end load the last chunk and leave it out of everything)
+    auto at = [&](int i) { return static_cast<unsigned>(min(lane + LANES * i, cpr - 1)) * 16u; };      // bytes
+    auto store = [&](void* p, long row, int i, u32x4 v) { *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(static_cast<T*>(p) + row) + at(i)) = v; };
+    auto load = [&](const void* p, long row) {
+        const char* const base = reinterpret_cast<const char*>(static_cast<const T*>(p) + row);
+        return [=](unsigned byte) { return __builtin_bit_cast(t8, *reinterpret_cast<const u32x4*>(base + byte)); };
+    };
+    // (a chunk is made FP32 anew for each pass over the row: kept, its 8 values would hold twice the registers)
+    auto anew = [](t8 (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            u32x4 bits = __builtin_bit_cast(u32x4, v[i]);
+            asm volatile("" : "+v"(bits));
+            v[i] = __builtin_bit_cast(t8, bits);
+        }
+    };
+    int parity = 0;
+    for (long r = first; r < a.rows; r += step, parity ^= 1) {
+        if constexpr (TIGHT) asm volatile("" : "+v"(lane));      // (nor offsets kept from row to row)
+        int slot = 0;
+        auto total = [&](float s) {
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+            if constexpr (W > 1) {
+                float* const part = red[parity][slot++];
+                if ((lane & 63) == 0) part[lane >> 6] = s;
+                __syncthreads();
+                s = 0.f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) s += part[i];
+            }
+            return s;
+        };
+        // mean (0 for RMS) and factor of a row
+        auto statistics = [&](t8 (&row)[N], int kind, float eps, float& mean, float& inv) {
+            mean = 0.f;
+            if (kind == MI_NORM_LAYER) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const t8 v = row[i];
+                    float c = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) c += static_cast<float>(v[e]);
+                    if (mine(i)) s += c;
+                }
+                mean = total(s) * inv_cols;
+                anew(row);
+            }
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const t8 v = row[i];
+                float c = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float d = static_cast<float>(v[e]) - mean;
+                    c = __builtin_fmaf(d, d, c);
+                }
+                if (mine(i)) s += c;
+            }
+            inv = inverse_root(total(s) / static_cast<float>(a.cols) + eps);
+            anew(row);
+        };
+        auto vectors = [&](const RowVectors& v) { return load(v.p, r / v.each * v.rs); };
+
+        t8 h[N];
+        const auto x_at = load(a.x, r * a.x_rs);
+        constexpr bool LATE = N == 8;                 // (x behind the branch's sums: both together leave no registers for them)
+        if (!LATE || a.branch == nullptr) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = x_at(at(i));
+        }
+        if (a.branch != nullptr) {
+            t8 b[N];
+            const auto b_at = load(a.branch, r * a.b_rs), pg_at = load(a.post_gain, 0), gate_at = vectors(a.gate);
+#pragma unroll
+            for (int i = 0; i < N; ++i) b[i] = b_at(at(i));
+            float mean = 0.f, inv = 1.f;
+            if (a.post != MI_NORM_NONE) statistics(b, a.post, a.post_eps, mean, inv);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = (static_cast<float>(b[i][e]) - mean) * inv;
+                if constexpr (LATE) h[i] = x_at(at(i));
+                if (a.post_gain != nullptr) {
+                    const t8 g = pg_at(at(i));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] *= static_cast<float>(g[e]);
+                }
+                if (a.gate.p != nullptr) {
+                    const t8 g = gate_at(at(i));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] *= static_cast<float>(g[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[i][e] = static_cast<T>(__builtin_fmaf(a.alpha, static_cast<float>(h[i][e]), f[e]));
+                if (a.sum != nullptr && mine(i)) store(a.sum, r * a.s_rs, i, __builtin_bit_cast(u32x4, h[i]));
+                if constexpr (TIGHT) asm volatile("" ::: "memory");
+            }
+        }
+        if (a.out == nullptr) continue;
+        float mean, inv;
+        statistics(h, a.pre, a.eps, mean, inv);
+        const auto gain_at = load(a.gain, 0), scale_at = vectors(a.scale), shift_at = vectors(a.shift);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = (static_cast<float>(h[i][e]) - mean) * inv;
+            if (a.gain != nullptr) {
+                const t8 g = gain_at(at(i));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= static_cast<float>(g[e]);
+            }
+            if (a.scale.p != nullptr) {
+                const t8 g = scale_at(at(i));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= 1.f + static_cast<float>(g[e]);
+            }
+            if (a.shift.p != nullptr) {
+                const t8 g = shift_at(at(i));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] += static_cast<float>(g[e]);
+            }
+            t8 o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(f[e]);
+            if (mine(i)) store(a.out, r * a.o_rs, i, __builtin_bit_cast(u32x4, o));
+            if constexpr (TIGHT) asm volatile("" ::: "memory");
+        }
+    }
+}
+
+template <typename T, int N, int W>
+int launch_rows(const GateNorm& a, hipStream_t st) {
+    const long groups = W == 1 ? (a.rows + 3L) / 4 : a.rows;
+    hipLaunchKernelGGL((gate_norm_kernel<T, N, W>), dim3(static_cast<unsigned>(groups < (1L << 20) ? groups : 1L << 20)), dim3(W == 1 ? 256 : 64 * W), 0, st, a);
+    MI_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+template <typename T, int W>
+int launch_chunks(const GateNorm& a, hipStream_t st) {
+    const int n = (a.cols / 8 + 64 * W - 1) / (64 * W);
+    if constexpr (W == 1) if (n == 1) return launch_rows<T, 1, W>(a, st);
+    if (n <= 2) return launch_rows<T, 2, W>(a, st);
+    if constexpr (W < 16) if (n == 3) return launch_rows<T, 3, W>(a, st);
+    if constexpr (W >= 8) if (n <= 4) return launch_rows<T, 4, W>(a, st);
+    if constexpr (W == 16) return launch_rows<T, 8, W>(a, st);
+    return fail("gate_norm: no kernel for %d columns", a.cols);
+}
+
+template <typename T>
+int launch_width(const GateNorm& a, hipStream_t st) {
+    const int chunks = a.cols / 8, each = a.rows >= 4 * device_cu_count() ? 3 : 2;
+    if (chunks <= 64 * each) return launch_chunks<T, 1>(a, st);
+    if (chunks <= 128 * each) return launch_chunks<T, 2>(a, st);
+    if (chunks <= 256 * each) return launch_chunks<T, 4>(a, st);
+    if (chunks <= 512 * (each == 3 ? 4 : 2)) return launch_chunks<T, 8>(a, st);
+    return launch_chunks<T, 16>(a, st);
+}
+
+bool bad_eps(float e) { return e < 0.f || (__builtin_bit_cast(unsigned, e) & 0x7fffffffu) >= 0x7f800000u; }      // (by its bits: compiled without NaN in comparisons)
+
+}  // namespace
+}  // namespace mi
+
+using mi::fail;
+
+extern "C" int mi_gate_add_norm_forward(const mi_gate_add_norm_args* a) {
+    const char* op = "mi_gate_add_norm_forward";
+    mi::clear_error();
+    if (!a) return fail("%s: null args", op);
+    if (a->struct_size != sizeof(*a)) return fail("%s: struct_size %u != %zu (header mismatch)", op, a->struct_size, sizeof(*a));
+    if (mi::check_rows(op, a->dtype, a->rows, a->cols)) return -1;
+    for (const int32_t kind : {a->post_norm, a->norm})
+        if (kind < MI_NORM_NONE || kind > MI_NORM_LAYER) return fail("%s: norm %d is none of MI_NORM_*", op, kind);
+    if (mi::bad_eps(a->eps) || mi::bad_eps(a->post_eps)) return fail("%s: eps must be >= 0 and finite", op);
+    if ((__builtin_bit_cast(unsigned, a->residual_scale) & 0x7fffffffu) >= 0x7f800000u) return fail("%s: residual_scale must be finite", op);
+    if (a->rows == 0) return 0;
+    if (!a->x) return fail("%s: null tensor", op);
+    if (!a->out && !a->sum_out) return fail("%s: neither sum_out nor out is given", op);
+    if ((a->out != nullptr) != (a->norm != MI_NORM_NONE)) return fail("%s: out and a norm must be given together", op);
+    if (!a->out && (a->gain || a->scale || a->shift)) return fail("%s: gain, scale or shift without a norm", op);
+    if (!a->branch && (a->gate || a->post_gain || a->sum_out || a->post_norm != MI_NORM_NONE)) return fail("%s: gate, post norm or sum_out without a branch", op);
+    if (a->post_gain && a->post_norm == MI_NORM_NONE) return fail("%s: post_gain without a post norm", op);
+    const long n = a->cols;
+    auto stride = [&](int64_t s) { return s ? static_cast<long>(s) : n; };
+    mi::GateNorm g{};
+    g.x = a->x; g.branch = a->branch; g.post_gain = a->post_gain; g.gain = a->gain; g.sum = a->sum_out; g.out = a->out;
+    g.rows = a->rows; g.cols = a->cols; g.post = a->post_norm; g.pre = a->norm;
+    g.x_rs = stride(a->x_row_stride); g.b_rs = stride(a->branch_row_stride); g.s_rs = stride(a->sum_row_stride); g.o_rs = stride(a->out_row_stride);
+    g.alpha = a->residual_scale; g.post_eps = a->post_eps; g.eps = a->eps;
+    const mi::Operand ins[] = {{"x", g.x, 2 * g.x_rs, 2 * n}, {"branch", g.branch, 2 * g.b_rs, 2 * n}};
+    const mi::Operand outs[] = {{"sum_out", g.sum, 2 * g.s_rs, 2 * n}, {"out", g.out, 2 * g.o_rs, 2 * n}};
+    const struct { const char* name; const void* p; long rs; int32_t each; mi::RowVectors* to; } vectors[] = {
+        {"gate", a->gate, stride(a->gate_row_stride), a->gate_rows, &g.gate}, {"scale", a->scale, stride(a->scale_row_stride), a->scale_rows, &g.scale},
+        {"shift", a->shift, stride(a->shift_row_stride), a->shift_rows, &g.shift},
+        {"post_gain", a->post_gain, n, 0, nullptr}, {"gain", a->gain, n, 0, nullptr}};
+    auto items = [&](int each) { return each ? (a->rows - 1) / each + 1L : 1L; };
+    for (const auto& v : vectors) {
+        if (v.to) *v.to = {v.p, v.rs, v.each ? v.each : a->rows};
+        if (!v.p) continue;
+        if (v.each < 0) return fail("%s: %s_rows must not be negative", op, v.name);
+        const mi::Operand rows{v.name, v.p, 2 * v.rs, 2 * n};
+        if (mi::check_operands(op, items(v.each), a->cols, &rows, 1, nullptr, 0)) return -1;
+    }
+    if (mi::check_operands(op, a->rows, a->cols, ins, 2, outs, 2)) return -1;
+    for (const auto& v : vectors)
+        for (const mi::Operand& o : outs)
+            if (mi::runs_share(o.p, (a->rows - 1) * o.rs + o.len, v.p, (items(v.each) - 1) * 2 * v.rs + 2 * n)) return fail("%s: %s overlaps %s", op, o.name, v.name);
+    return a->dtype == MI_DTYPE_BF16 ? mi::launch_width<__bf16>(g, mi::resolve_stream(a->stream)) : mi::launch_width<_Float16>(g, mi::resolve_stream(a->stream));
+}

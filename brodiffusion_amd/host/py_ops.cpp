@@ -43,6 +43,7 @@ struct Lib {
     decltype(&mi_rms_norm_pair_forward) rms_norm_pair;
     decltype(&mi_add_rms_norm_forward) add_rms_norm;
     decltype(&mi_quantize_rows_forward) quantize_rows;
+    decltype(&mi_gate_add_norm_forward) gate_add_norm;
     decltype(&mi_linear_act_forward) linear_act;
     decltype(&mi_linear_act_scratch_bytes) linear_act_scratch_bytes;
     decltype(&mi_attn_block_scratch_bytes) block_scratch_bytes;
@@ -338,6 +339,76 @@ NATIVE(quantize_rows, 3)
     p.stream = current_stream();
     run("quantize_rows_int8", [&] { return L.quantize_rows(&p); });
     return tuple_of({given(a[1], y), given(a[2], scales)});
+NATIVE_END
+
+int norm_of(PyObject* o) {
+    need(PyUnicode_Check(o));
+    static const char* const names[] = {"none", "rms", "layer"};      // by MI_NORM_*
+    for (int i = 0; i < 3; ++i)
+        if (PyUnicode_CompareWithASCIIString(o, names[i]) == 0) return i;
+    throw Decline{};
+}
+const void* columns_ptr(PyObject* o, const Tensor& x) {
+    if (none(o)) return nullptr;
+    const Tensor& t = tensor(o);
+    need(t.scalar_type() == x.scalar_type() && t.numel() == x.size(-1) && t.is_contiguous());
+    return t.data_ptr();
+}
+// one vector for all rows, or (items, cols) / (items, 1, cols) with X's leading size, or one that divides a 2-D X's rows, as items
+const void* vectors_ptr(PyObject* o, const Tensor& x, int64_t rows, int32_t& each, int64_t& stride) {
+    if (none(o)) return nullptr;
+    const Tensor& t = tensor(o);
+    const int64_t cols = x.size(-1);
+    need(t.scalar_type() == x.scalar_type() && t.dim() >= 1 && t.dim() <= 3 && t.size(-1) == cols && t.stride(-1) == 1);
+    if (t.dim() == 1) { stride = cols; return t.data_ptr(); }
+    need(t.dim() == 2 || t.size(1) == 1);
+    const int64_t items = t.size(0);
+    need(items > 0 && (items == x.size(0) || x.dim() == 2) && x.dim() >= 2 && rows % items == 0);
+    if (items > 1) {
+        need(t.stride(0) >= cols && rows > 0);
+        each = static_cast<int32_t>(rows / items);
+    }
+    stride = items > 1 ? t.stride(0) : cols;
+    return t.data_ptr();
+}
+// X, branch, gate, post, post_gain, post_eps, residual_scale, norm, gain, scale, shift, eps, sum_out, out
+NATIVE(gate_add_norm, 14)
+    need(L.gate_add_norm != nullptr);
+    const Tensor& x = tensor(a[0]);
+    mi_gate_add_norm_args p;
+    std::memset(&p, 0, sizeof(p));
+    p.struct_size = sizeof(p);
+    p.dtype = dtype_code(x);
+    p.x_row_stride = row_stride(x, x.scalar_type());
+    p.rows = rows32(x.numel() / x.size(-1)); p.cols = rows32(x.size(-1));
+    p.post_norm = norm_of(a[3]); p.norm = norm_of(a[7]);
+    p.eps = static_cast<float>(number(a[11]));
+    p.post_eps = none(a[5]) ? p.eps : static_cast<float>(number(a[5]));
+    p.residual_scale = static_cast<float>(number(a[6]));
+    p.post_gain = columns_ptr(a[4], x); p.gain = columns_ptr(a[8], x);
+    p.gate = vectors_ptr(a[2], x, p.rows, p.gate_rows, p.gate_row_stride);
+    p.scale = vectors_ptr(a[9], x, p.rows, p.scale_rows, p.scale_row_stride);
+    p.shift = vectors_ptr(a[10], x, p.rows, p.shift_rows, p.shift_row_stride);
+    Tensor sum = x, y;
+    if (none(a[1])) need(none(a[12]) && !p.gate && !p.post_gain && p.post_norm == MI_NORM_NONE && p.norm != MI_NORM_NONE);
+    else {
+        const Tensor& b = tensor(a[1]);
+        need(b.sizes() == x.sizes());
+        p.branch = b.data_ptr(); p.branch_row_stride = row_stride(b, x.scalar_type());
+        sum = rows_like(a[12], x, x.size(-1), x.scalar_type());
+        p.sum_out = sum.data_ptr(); p.sum_row_stride = row_stride(sum, x.scalar_type());
+    }
+    if (p.norm == MI_NORM_NONE) need(!p.gain && !p.scale && !p.shift && none(a[13]));
+    else {
+        y = rows_like(a[13], x, x.size(-1), x.scalar_type());
+        p.out = y.data_ptr(); p.out_row_stride = row_stride(y, x.scalar_type());
+    }
+    p.x = x.data_ptr();
+    p.stream = current_stream();
+    run("gate_add_norm", [&] { return L.gate_add_norm(&p); });
+    PyObject* const h = none(a[1]) ? given(a[0], x) : given(a[12], sum);
+    if (p.norm == MI_NORM_NONE) { Py_INCREF(Py_None); return tuple_of({h, Py_None}); }
+    return tuple_of({h, given(a[13], y)});
 NATIVE_END
 
 int activation_of(PyObject* o) {
@@ -802,7 +873,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     if (!ok) return PyErr_Format(PyExc_RuntimeError, "%s does not export every function of mi_attention.h: build the library again", path);
     // (a library without these binds all the same: their calls decline, and the Python code says what is missing)
     get(L.add_rms_norm, "mi_add_rms_norm_forward"); get(L.quantize_rows, "mi_quantize_rows_forward"); get(L.linear_act, "mi_linear_act_forward");
-    get(L.linear_act_scratch_bytes, "mi_linear_act_scratch_bytes");
+    get(L.linear_act_scratch_bytes, "mi_linear_act_scratch_bytes"); get(L.gate_add_norm, "mi_gate_add_norm_forward");
     Py_INCREF(lend);
     Py_XSETREF(lend_scratch, lend);
     bound = true;
@@ -810,7 +881,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(linear), FAST(geglu), FAST(add_inplace), FAST(rms_norm), FAST(add_rms_norm), FAST(quantize_rows), FAST(linear_act), FAST(rope), FAST(headnorm_rope),
+PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(linear), FAST(geglu), FAST(add_inplace), FAST(rms_norm), FAST(add_rms_norm), FAST(quantize_rows), FAST(gate_add_norm), FAST(linear_act), FAST(rope), FAST(headnorm_rope),
                          FAST(sdpa), FAST(joint), FAST(attn_block), FAST(mha), FAST(linear_attn), FAST(sana), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native host path of brodiffusion_amd.ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

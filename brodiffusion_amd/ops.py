@@ -20,6 +20,7 @@ Names, argument order and error behaviour follow the brotensor operators the ref
     flash_attention_project_kv(ctx, Wk, bk, Wv, bv, K_out, V_out)            src/unet.cpp:476-480
     linear_batched(W, bias, X, Y)                                            include/brodiffusion/detail/compute.h:52
     add_rms_norm, add_rms_norm_int8, quantize_rows_int8, linear_act          no counterpart: 8-bit rows and projections with an epilogue
+    gate_add_norm                                                            no counterpart: a block's gated residual with its norms
     fused_linear_geglu(X, W, b, Y), add_inplace_vec(Y, X), add_inplace_row_bias(Y, bias)
                                                                              include/brodiffusion/fused_transformer.h:20-61
 
@@ -1211,6 +1212,88 @@ def quantize_rows_int8(X, out: Optional[torch.Tensor] = None, scales: Optional[t
     a.stream = _stream()
     capi.check(capi.lib().mi_quantize_rows_forward(C.byref(a)), op)
     return out, scales
+
+
+_NORMS = {"none": capi.MI_NORM_NONE, "rms": capi.MI_NORM_RMS, "layer": capi.MI_NORM_LAYER}
+
+
+def _vectors_of(op: str, v, name: str, X, rows: int):
+    """A vector of X's columns for all rows, or one for each run of rows: (cols), X's leading sizes or the first of them (with ones behind them) before
+    cols, or, for a 2-D X, (items, cols) with items dividing its rows. Returns (address, rows that share one or 0 for all, row stride)."""
+    _dev(op, v)
+    cols = X.shape[-1]
+    if v.dtype != X.dtype or v.dim() < 1 or v.shape[-1] != cols:
+        _fail(op, f"{name} must hold X's dtype and {cols} columns")
+    lead = list(v.shape[:-1])
+    while lead and lead[-1] == 1:
+        lead.pop()
+    items = math.prod(lead)
+    if lead != list(X.shape[:len(lead)]) and not (X.dim() == 2 and len(lead) == 1 and rows % max(items, 1) == 0) or len(lead) >= X.dim():
+        _fail(op, f"{name} is {tuple(v.shape)}: neither ({cols},) nor one vector for each of X's leading sizes, {tuple(X.shape)}")
+    if items == 1:
+        if v.stride(-1) != 1 and cols > 1:
+            _fail(op, f"{name} must be contiguous along columns")
+        return v.data_ptr(), 0, cols
+    if items == 0:
+        return v.data_ptr(), 0, cols
+    return v.data_ptr(), rows // items, _rows_of(op, v.reshape(items, cols) if v.is_contiguous() else v.squeeze(1) if v.dim() == 3 else v, name, X.dtype)[1]
+
+
+def gate_add_norm(X, branch, *, gate=None, post: str = "none", post_gain=None, post_eps: Optional[float] = None, residual_scale: float = 1.0, norm: str = "rms",
+                  gain=None, scale=None, shift=None, eps: float = 1e-6, sum_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """(h, y): a block's output into the residual stream and the norm in front of the next block (mi_gate_add_norm_forward),
+        h = residual_scale * X + gate * post(branch) * post_gain, rounded to X's dtype,   y = norm(h) * gain * (1 + scale) + shift.
+    post and norm: "none", "rms" or "layer" (without weights of their own), eps of either (post_eps None: eps). X (..., cols), branch of its shape, or None:
+    h is X. gate, scale and shift: (cols), or one vector for each of X's leading sizes, (batch, cols) or (batch, 1, cols) of a (batch, tokens, cols) X, any row
+    stride; for a 2-D X (items, cols), each for rows / items rows. norm "none": y is None. sum_out and out may be X or branch."""
+    op = "gate_add_norm"
+    r = _native.gate_add_norm(X, branch, gate, post, post_gain, post_eps, residual_scale, norm, gain, scale, shift, eps, sum_out, out)
+    if r is not None:
+        return r
+    _dev(op, X, branch, gate, post_gain, gain, scale, shift, sum_out, out)
+    for kind in (post, norm):
+        if kind not in _NORMS:
+            _fail(op, f"norm {kind!r} is none of {', '.join(_NORMS)}")
+    a = capi.MiGateAddNormArgs()
+    a.struct_size = C.sizeof(a)
+    a.dtype = _dtype_code(op, X)
+    a.rows, a.x_row_stride = _rows_of(op, X, "X", X.dtype)
+    a.cols = X.shape[-1]
+    a.x, a.post_norm, a.norm = X.data_ptr(), _NORMS[post], _NORMS[norm]
+    a.residual_scale, a.eps, a.post_eps = residual_scale, eps, eps if post_eps is None else post_eps
+    for name, v in (("post_gain", post_gain), ("gain", gain)):
+        if v is not None:
+            if v.dtype != X.dtype or v.numel() != X.shape[-1] or not v.is_contiguous():
+                _fail(op, f"{name} must hold one value of X's dtype per column")
+            setattr(a, name, v.data_ptr())
+    for name, v in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if v is not None:
+            address, each, stride = _vectors_of(op, v, name, X, a.rows)
+            setattr(a, name, address)
+            setattr(a, name + "_rows", each)
+            setattr(a, name + "_row_stride", stride)
+    if branch is None:
+        for name, there in (("sum_out", sum_out is not None), ("gate", gate is not None), ("post_gain", post_gain is not None), ("post", post != "none")):
+            if there:
+                _fail(op, f"{name} without a branch")
+        if norm == "none":
+            _fail(op, "neither a branch nor a norm")
+        sum_out = X
+    else:
+        a.branch, a.branch_row_stride = branch.data_ptr(), _rows_of(op, branch, "branch", X.dtype, X.shape)[1]
+        if sum_out is None:
+            sum_out = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+        a.sum_out, a.sum_row_stride = sum_out.data_ptr(), _rows_of(op, sum_out, "sum_out", X.dtype, X.shape)[1]
+    if norm == "none":
+        if any(v is not None for v in (gain, scale, shift, out)):
+            _fail(op, "gain, scale, shift or out without a norm")
+    else:
+        if out is None:
+            out = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+        a.out, a.out_row_stride = out.data_ptr(), _rows_of(op, out, "out", X.dtype, X.shape)[1]
+    a.stream = _stream()
+    capi.check(capi.lib().mi_gate_add_norm_forward(C.byref(a)), op)
+    return sum_out, out
 
 
 _ACTIVATIONS = {"none": capi.MI_ACT_NONE, "gelu": capi.MI_ACT_GELU, "gelu_tanh": capi.MI_ACT_GELU_TANH, "silu": capi.MI_ACT_SILU}

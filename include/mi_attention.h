@@ -483,6 +483,41 @@ typedef struct mi_quantize_rows_args {
 } mi_quantize_rows_args;
 MI_API int mi_quantize_rows_forward(const mi_quantize_rows_args* args);
 
+/* ── the step between two blocks ───────────────────────────────────────────
+ *   b = post(branch) * post_gain                       post_norm: MI_NORM_NONE, _RMS (v / sqrt(mean v^2 + post_eps)) or _LAYER
+ *                                                      ((v - mean) / sqrt(mean (v - mean)^2 + post_eps)); FP32
+ *   h = T(residual_scale * x + gate * b)               one rounding to the tensor type T; without a branch h = x (residual_scale is not used)
+ *   out = T(norm(h) * gain * (1 + scale) + shift)      norm: as post_norm, with eps; FP32 in between, one rounding
+ * A block's output into the residual stream with the modulated norm in front of the next block, which the reference does in three to five
+ * operators (LN + modulate and the gated residual of its DiT blocks, src/dit/flux.cpp; factors of the stream, norms behind a block). All of
+ * gate, post_gain, gain, scale and shift may be NULL (a factor of 1, nothing added). gate, scale and shift hold one vector of `cols` for each
+ * `..._rows` rows (0: one for all rows): an image's rows of a batch, or a row each. norm MI_NORM_NONE and out NULL go together (the last
+ * block: h alone); sum_out (h) only with a branch, optional beside out. Sums are FP32: squares that exceed it make zeros of a row.
+ * cols a multiple of 8, at most 65536; strides in elements (0 = dense), multiples of 8, at most 2^40, rows times stride at most 2^56; 16-byte
+ * aligned. sum_out and out may each be x or branch (same pointer and stride); outputs share no other memory with each other or an input. */
+enum { MI_NORM_NONE = 0, MI_NORM_RMS = 1, MI_NORM_LAYER = 2 };
+typedef struct mi_gate_add_norm_args {
+    uint32_t struct_size;
+    int32_t dtype;
+    const void* x;           /* (rows, cols): the residual stream */
+    const void* branch;      /* (rows, cols) or NULL */
+    const void* gate;        /* ((rows - 1) / gate_rows + 1, cols) or NULL; scale and shift likewise */
+    const void* post_gain;   /* (cols) or NULL */
+    const void* gain;        /* (cols) or NULL */
+    const void* scale;
+    const void* shift;
+    void* sum_out;           /* (rows, cols) or NULL */
+    void* out;               /* (rows, cols) or NULL */
+    int32_t rows, cols;
+    int32_t post_norm, norm; /* MI_NORM_* */
+    int32_t gate_rows, scale_rows, shift_rows;
+    int64_t x_row_stride, branch_row_stride, gate_row_stride, scale_row_stride, shift_row_stride, sum_row_stride, out_row_stride;
+    float residual_scale;    /* as it stands: 1 for a plain sum */
+    float post_eps, eps;
+    void* stream;
+} mi_gate_add_norm_args;
+MI_API int mi_gate_add_norm_forward(const mi_gate_add_norm_args* args);
+
 /* ── linear layer with an epilogue ─────────────────────────────────────────
  * Y = act(X W^T [* w_scales] [* x_scales] + bias) + residual, everything behind the product in FP32, one rounding to `dtype`.
  * Three kinds of operands:
