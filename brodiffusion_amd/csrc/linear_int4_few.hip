@@ -1,0 +1,180 @@
+// The linear layer with 4-bit weights for few rows (linear_int4.h): a token of a serving step, a draft, a short prompt.
+//
+// Bound: the bytes of the packed weights, each used once per 16 * TB rows of X. They go from memory straight to the registers of the wavefront that multiplies
+// them, in whole kilobytes. A work group owns 16 FB features and 16 TB rows; its wavefronts take the blocks of 128 contraction elements in turn, each with its
+// next block on its way while it multiplies, and their sums meet in LDS, added in the order of the wavefronts: no result depends on timing. One launch, no
+// workspace, no atomics.
+#include "linear_int4.h"
+
+namespace mi {
+namespace gemm {
+namespace {
+
+template <typename T, int P, int FB, int TB, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4Problem p) {
+    using M = Mma<T>;
+    using V8 = typename M::v8;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    constexpr int F = 16 * FB, NT = 64 * WAVES, OUT = (F * 16 * TB + NT - 1) / NT;
+    __shared__ __attribute__((aligned(16))) float sums[WAVES][FB * TB][16 * 16];      // [row][feature] of a block
+
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = static_cast<int>(blockIdx.x) * F, m0 = static_cast<int>(blockIdx.y) * 16 * TB;
+    const int last_block = (p.N + 15) / 16 - 1;
+
+    const unsigned char* wrow[FB];
+    const T* scale[FB];
+    const unsigned char* zero[FB];
+#pragma unroll
+    for (int a = 0; a < FB; ++a) {
+        wrow[a] = static_cast<const unsigned char*>(p.w) + static_cast<long>(min(n0 / 16 + a, last_block)) * p.KB * 1024 + lane * 16;
+        const int f = min(n0 + 16 * a + 4 * lg, p.N - 4);      // (features come in eights)
+        scale[a] = static_cast<const T*>(p.scales) + f;
+        zero[a] = p.zeros + f;
+    }
+    const T* xrow[TB];
+#pragma unroll
+    for (int b = 0; b < TB; ++b) xrow[b] = static_cast<const T*>(p.x) + static_cast<long>(min(m0 + 16 * b + lr, p.M - 1)) * p.ldx;
+
+    struct Block { u32x4 w[FB]; V8 x[TB][4]; t4 s[FB][P]; unsigned z[FB][P]; };
+    auto load = [&](Block& c, int kb) {
+#pragma unroll
+        for (int a = 0; a < FB; ++a) c.w[a] = *reinterpret_cast<const u32x4*>(wrow[a] + static_cast<long>(kb) * 1024);
+#pragma unroll
+        for (int g = 0; g < P; ++g) {
+            const long row = static_cast<long>(min(P == 1 ? kb / p.span : kb * P + g, p.groups - 1)) * p.N;
+#pragma unroll
+            for (int a = 0; a < FB; ++a) {
+                c.s[a][g] = *reinterpret_cast<const t4*>(scale[a] + row);
+                c.z[a][g] = p.zeros ? *reinterpret_cast<const unsigned*>(zero[a] + row) : 0x08080808u;
+            }
+        }
+        const int k0 = kb * 128 + 8 * lg;
+        if (kb * 128 + 128 <= p.K) {
+#pragma unroll
+            for (int b = 0; b < TB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c.x[b][j] = *reinterpret_cast<const V8*>(xrow[b] + k0 + 32 * j);
+        } else {
+#pragma unroll
+            for (int b = 0; b < TB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {       // (pieces past the end: the row's first one, as zeros)
+                    const bool there = k0 + 32 * j < p.K;
+                    const V8 v = *reinterpret_cast<const V8*>(xrow[b] + (there ? k0 + 32 * j : 0));
+                    c.x[b][j] = there ? v : V8{};
+                }
+        }
+    };
+    f32x4 acc[FB][TB];
+#pragma unroll
+    for (int a = 0; a < FB; ++a)
+#pragma unroll
+        for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Block& c) {
+        f32x4 sx[TB][P];
+#pragma unroll
+        for (int b = 0; b < TB; ++b)
+#pragma unroll
+            for (int g = 0; g < P; ++g) {
+                sx[b][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) sx[b][g] = M::run16(ones<T>(), c.x[b][j], sx[b][g]);
+            }
+#pragma unroll
+        for (int a = 0; a < FB; ++a) {
+            V8 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = nibbles<T>(c.w[a][j]);
+#pragma unroll
+            for (int g = 0; g < P; ++g) {
+                float z[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] = zero_point(c.z[a][g], e);
+#pragma unroll
+                for (int b = 0; b < TB; ++b) {
+                    f32x4 t;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t[e] = -z[e] * sx[b][g][e];
+#pragma unroll
+                    for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) t = M::run16(w[j], c.x[b][j], t);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[a][b][e] = __builtin_fmaf(t[e], static_cast<float>(c.s[a][g][e]), acc[a][b][e]);
+                }
+            }
+        }
+    };
+
+    if (wave < p.KB) {
+        Block c[2];
+        load(c[0], wave);
+        int i = wave;
+        for (; i + WAVES < p.KB; i += 2 * WAVES) {
+            load(c[1], i + WAVES);
+            multiply(c[0]);
+            if (i + 2 * WAVES < p.KB) load(c[0], i + 2 * WAVES);
+            multiply(c[1]);
+        }
+        if (i < p.KB) multiply(c[0]);
+    }
+
+#pragma unroll
+    for (int a = 0; a < FB; ++a)
+#pragma unroll
+        for (int b = 0; b < TB; ++b) *reinterpret_cast<f32x4*>(&sums[wave][a * TB + b][lr * 16 + 4 * lg]) = acc[a][b];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) {
+        const int o = i * NT + tid, f = o % F, row = o / F;
+        if (row >= 16 * TB || m0 + row >= p.M || n0 + f >= p.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += sums[w][f / 16 * TB + row / 16][row % 16 * 16 + f % 16];
+        if (p.bias) v += static_cast<float>(static_cast<const T*>(p.bias)[n0 + f]);
+        with_activation(p.act, [&](auto act) { v = act(v); });
+        if (p.residual) v += static_cast<float>(static_cast<const T*>(p.residual)[static_cast<long>(m0 + row) * p.ldr + n0 + f]);
+        static_cast<T*>(p.y)[static_cast<long>(m0 + row) * p.ldy + n0 + f] = static_cast<T>(v);
+    }
+}
+
+template <typename T, int P, int FB, int TB>
+int launch(const Int4Problem& p, hipStream_t st) {
+    constexpr int WAVES = 8;
+    hipLaunchKernelGGL((linear_int4_few_kernel<T, P, FB, TB, WAVES>), dim3((p.N + 16 * FB - 1) / (16 * FB), (p.M + 16 * TB - 1) / (16 * TB)), dim3(64 * WAVES), 0, st, p);
+    MI_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+template <typename T, int P>
+int launch_form(const Int4Problem& p, hipStream_t st) {
+    const int cu = device_cu_count();
+    if (p.M <= 16) {
+        if (p.N >= 64 * cu) return launch<T, P, 4, 1>(p, st);
+        if (p.N >= 32 * cu) return launch<T, P, 2, 1>(p, st);
+        return launch<T, P, 1, 1>(p, st);
+    }
+    if (p.M <= 32) {
+        if (p.N >= 64 * cu) return launch<T, P, 4, 2>(p, st);
+        if (p.N >= 32 * cu) return launch<T, P, 2, 2>(p, st);
+        return launch<T, P, 1, 2>(p, st);
+    }
+    if (p.N >= 32 * cu) return launch<T, P, 2, 4>(p, st);
+    return launch<T, P, 1, 4>(p, st);
+}
+
+template <typename T>
+int launch_parts(const Int4Problem& p, int parts, hipStream_t st) {
+    return parts == 1 ? launch_form<T, 1>(p, st) : parts == 2 ? launch_form<T, 2>(p, st) : launch_form<T, 4>(p, st);
+}
+
+}  // namespace
+}  // namespace gemm
+
+bool int4_few_takes(const Int4Problem& p) { return p.M <= 64 || p.ldx * 2 * 512 >= (1L << 31); }
+
+int launch_int4_few(const Int4Problem& p, int dtype, int parts, hipStream_t st) {
+    return dtype == MI_DTYPE_BF16 ? gemm::launch_parts<__bf16>(p, parts, st) : gemm::launch_parts<_Float16>(p, parts, st);
+}
+
+}  // namespace mi

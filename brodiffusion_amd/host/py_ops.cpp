@@ -44,6 +44,8 @@ struct Lib {
     decltype(&mi_add_rms_norm_forward) add_rms_norm;
     decltype(&mi_quantize_rows_forward) quantize_rows;
     decltype(&mi_gate_add_norm_forward) gate_add_norm;
+    decltype(&mi_int4_packed_bytes) int4_packed_bytes;
+    decltype(&mi_linear_int4_forward) linear_int4;
     decltype(&mi_linear_act_forward) linear_act;
     decltype(&mi_linear_act_scratch_bytes) linear_act_scratch_bytes;
     decltype(&mi_attn_block_scratch_bytes) block_scratch_bytes;
@@ -478,6 +480,42 @@ NATIVE(linear_act, 9)
     return given(a[8], y);
 NATIVE_END
 
+// X, packed, scales, zeros, out_features, in_features, group, bias, activation, residual, out
+NATIVE(linear_int4, 11)
+    need(L.linear_int4 != nullptr && L.int4_packed_bytes != nullptr);
+    const Tensor &x = tensor(a[0]), &w = tensor(a[1]), &s = tensor(a[2]);
+    mi_linear_int4_args p;
+    std::memset(&p, 0, sizeof(p));
+    p.struct_size = sizeof(p);
+    p.dtype = dtype_code(x);
+    const at::ScalarType dt = x.scalar_type();
+    p.out_features = int32(a[4]); p.in_features = int32(a[5]); p.group = int32(a[6]);
+    p.activation = activation_of(a[8]);
+    need(p.out_features > 0 && p.in_features > 0 && p.group > 0 && x.dim() >= 1 && x.size(-1) == p.in_features);
+    const int64_t groups = (p.in_features + static_cast<int64_t>(p.group) - 1) / p.group;
+    need(w.scalar_type() == at::kByte && w.is_contiguous() && w.numel() == static_cast<int64_t>(L.int4_packed_bytes(p.out_features, p.in_features)));
+    auto per_group = [&](const Tensor& t, at::ScalarType type) {
+        need(t.scalar_type() == type && t.dim() == 2 && t.size(0) == groups && t.size(1) == p.out_features && t.is_contiguous());
+        return t.data_ptr();
+    };
+    p.scales = per_group(s, dt);
+    if (!none(a[3])) p.zeros = per_group(tensor(a[3]), at::kByte);
+    p.x_row_stride = row_stride(x, dt);
+    p.rows = rows32(x.numel() / x.size(-1));
+    p.bias = bias_ptr(a[7], dt, p.out_features);
+    const Tensor y = rows_like(a[10], x, p.out_features, dt);
+    p.y_row_stride = row_stride(y, dt);
+    if (!none(a[9])) {
+        const Tensor& r = tensor(a[9]);
+        need(r.sizes() == y.sizes());
+        p.residual = r.data_ptr(); p.residual_row_stride = row_stride(r, dt);
+    }
+    p.x = x.data_ptr(); p.w = w.data_ptr(); p.y = y.data_ptr();
+    p.stream = current_stream();
+    run("linear_int4", [&] { return L.linear_int4(&p); });
+    return given(a[10], y);
+NATIVE_END
+
 // ── RoPE ──
 const float* table(PyObject* o, int64_t rows, int64_t half) {
     const Tensor& t = tensor(o);
@@ -874,6 +912,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     // (a library without these binds all the same: their calls decline, and the Python code says what is missing)
     get(L.add_rms_norm, "mi_add_rms_norm_forward"); get(L.quantize_rows, "mi_quantize_rows_forward"); get(L.linear_act, "mi_linear_act_forward");
     get(L.linear_act_scratch_bytes, "mi_linear_act_scratch_bytes"); get(L.gate_add_norm, "mi_gate_add_norm_forward");
+    get(L.int4_packed_bytes, "mi_int4_packed_bytes"); get(L.linear_int4, "mi_linear_int4_forward");
     Py_INCREF(lend);
     Py_XSETREF(lend_scratch, lend);
     bound = true;
@@ -881,7 +920,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(linear), FAST(geglu), FAST(add_inplace), FAST(rms_norm), FAST(add_rms_norm), FAST(quantize_rows), FAST(gate_add_norm), FAST(linear_act), FAST(rope), FAST(headnorm_rope),
+PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr}, FAST(linear), FAST(geglu), FAST(add_inplace), FAST(rms_norm), FAST(add_rms_norm), FAST(quantize_rows), FAST(gate_add_norm), FAST(linear_act), FAST(linear_int4), FAST(rope), FAST(headnorm_rope),
                          FAST(sdpa), FAST(joint), FAST(attn_block), FAST(mha), FAST(linear_attn), FAST(sana), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native host path of brodiffusion_amd.ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

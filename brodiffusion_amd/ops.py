@@ -20,7 +20,7 @@ Names, argument order and error behaviour follow the brotensor operators the ref
     flash_attention_project_kv(ctx, Wk, bk, Wv, bv, K_out, V_out)            src/unet.cpp:476-480
     linear_batched(W, bias, X, Y)                                            include/brodiffusion/detail/compute.h:52
     add_rms_norm, add_rms_norm_int8, quantize_rows_int8, linear_act          no counterpart: 8-bit rows and projections with an epilogue
-    gate_add_norm                                                            no counterpart: a block's gated residual with its norms
+    gate_add_norm, pack_int4, linear_int4                                    no counterpart: a block's gated residual with its norms, 4-bit weights
     fused_linear_geglu(X, W, b, Y), add_inplace_vec(Y, X), add_inplace_row_bias(Y, bias)
                                                                              include/brodiffusion/fused_transformer.h:20-61
 
@@ -1355,6 +1355,87 @@ def linear_act(X, W, bias=None, *, activation: str = "none", residual: Optional[
         scratch = torch.empty(need, dtype=torch.uint8, device=X.device)
         a.scratch, a.scratch_bytes = scratch.data_ptr(), need
     capi.check(capi.lib().mi_linear_act_forward(C.byref(a)), op)
+    return out
+
+
+@dataclass(frozen=True)
+class Int4Weight:
+    """A linear layer's 4-bit weights as linear_int4 takes them (pack_int4 makes them). packed: bytes in the library's own order; scales and zeros: (groups,
+    out_features), zeros None where every zero point is 8."""
+    packed: torch.Tensor
+    scales: torch.Tensor
+    zeros: Optional[torch.Tensor]
+    out_features: int
+    in_features: int
+    group: int
+
+
+def pack_int4(q, scales, zeros=None, group: int = 128) -> Int4Weight:
+    """Lays 4-bit weights out for linear_int4, once (mi_pack_int4). q (out_features, in_features / 2) uint8, element 2 j of a row in the low half of byte j and
+    element 2 j + 1 in the high half, each 0 .. 15; scales (out_features, groups) float16 / bfloat16, groups = ceil(in_features / group); zeros the same shape in
+    uint8, or None: 8. The weight is (q - zero) * scale. group: 32, 64 or a multiple of 128."""
+    op = "pack_int4"
+    _dev(op, q, scales, zeros)
+    if q.dtype != torch.uint8 or q.dim() != 2 or q.shape[0] == 0 or q.shape[1] == 0 or (q.stride(1) != 1 and q.shape[1] > 1):
+        _fail(op, "q must be uint8 (out_features, in_features / 2), contiguous along columns")
+    n, k = q.shape[0], 2 * q.shape[1]
+    if group not in (32, 64) and (group <= 0 or group % 128):
+        _fail(op, f"group {group} is neither 32, 64 nor a multiple of 128")
+    _dtype_code(op, scales)
+    shape = (n, -(-k // group))
+    if tuple(scales.shape) != shape:
+        _fail(op, f"scales are {tuple(scales.shape)}, expected {shape}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != shape):
+        _fail(op, f"zeros must be uint8 {shape}")
+    a = capi.MiPackInt4Args()
+    a.struct_size = C.sizeof(a)
+    packed = torch.empty(int(capi.lib().mi_int4_packed_bytes(n, k)), dtype=torch.uint8, device=q.device)
+    a.q, a.packed, a.out_features, a.in_features = q.data_ptr(), packed.data_ptr(), n, k
+    a.q_row_stride = q.stride(0) if n > 1 else k // 2
+    a.stream = _stream()
+    capi.check(capi.lib().mi_pack_int4(C.byref(a)), op)
+    return Int4Weight(packed, scales.t().contiguous(), None if zeros is None else zeros.t().contiguous(), n, k, group)
+
+
+def linear_int4(X, W: Int4Weight, bias=None, *, activation: str = "none", residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """act(X W^T + bias) + residual with 4-bit weights (mi_linear_int4_forward): X (..., in_features), W of pack_int4 with scales of X's dtype, bias
+    (out_features), residual (..., out_features); activations as linear_act. FP32 behind the operands, one rounding; no weight is rounded to 16 bits. A row of X
+    with a value that is not finite gives NaN. `out` may be the residual itself."""
+    op = "linear_int4"
+    if not isinstance(W, Int4Weight):
+        _fail(op, "W must be what pack_int4 returns")
+    r = _native.linear_int4(X, W.packed, W.scales, W.zeros, W.out_features, W.in_features, W.group, bias, activation, residual, out)
+    if r is not None:
+        return r
+    _dev(op, X, W.packed, W.scales, W.zeros, bias, residual, out)
+    if activation not in _ACTIVATIONS:
+        _fail(op, f"activation {activation!r} is none of {', '.join(_ACTIVATIONS)}")
+    a = capi.MiLinearInt4Args()
+    a.struct_size = C.sizeof(a)
+    a.dtype = _dtype_code(op, X)
+    n, k, dtype = W.out_features, W.in_features, X.dtype
+    if X.dim() < 1 or X.shape[-1] != k:
+        _fail(op, f"X is {tuple(X.shape)}, W has {k} in_features")
+    groups = -(-k // W.group) if W.group > 0 else 0
+    if W.packed.dtype != torch.uint8 or not W.packed.is_contiguous() or W.packed.numel() != int(capi.lib().mi_int4_packed_bytes(n, k)):
+        _fail(op, "W.packed is not of W's sizes")
+    if W.scales.dtype != dtype or tuple(W.scales.shape) != (groups, n) or not W.scales.is_contiguous():
+        _fail(op, f"W.scales must be contiguous ({groups}, {n}) of X's dtype, {dtype}")
+    if W.zeros is not None and (W.zeros.dtype != torch.uint8 or tuple(W.zeros.shape) != (groups, n) or not W.zeros.is_contiguous()):
+        _fail(op, f"W.zeros must be contiguous uint8 ({groups}, {n})")
+    shape = (*X.shape[:-1], n)
+    a.rows, a.x_row_stride = _rows_of(op, X, "X", dtype)
+    a.in_features, a.out_features, a.group = k, n, W.group
+    a.bias = _bias(op, bias, "bias", dtype, n)
+    if residual is not None:
+        a.residual, a.residual_row_stride = residual.data_ptr(), _rows_of(op, residual, "residual", dtype, shape)[1]
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=X.device)
+    a.x, a.w, a.scales, a.y, a.y_row_stride = X.data_ptr(), W.packed.data_ptr(), W.scales.data_ptr(), out.data_ptr(), _rows_of(op, out, "out", dtype, shape)[1]
+    a.zeros = None if W.zeros is None else W.zeros.data_ptr()
+    a.activation = _ACTIVATIONS[activation]
+    a.stream = _stream()
+    capi.check(capi.lib().mi_linear_int4_forward(C.byref(a)), op)
     return out
 
 

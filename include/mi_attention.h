@@ -559,6 +559,47 @@ MI_API int mi_linear_act_forward(const mi_linear_act_args* args);
  * (addresses, strides) lead to. */
 MI_API size_t mi_linear_act_scratch_bytes(const mi_linear_act_args* args);
 
+/* ── linear layer with 4-bit weights ───────────────────────────────────────
+ * Y = act(X W^T + bias) + residual with W[n][k] = (q[n][k] - zeros[g][n]) * scales[g][n], g = k / group: 4-bit integers q of 0 .. 15 with a scale, and where
+ * there are zeros a zero point (else 8), for each group of the contraction. Weights are not rounded to 16 bits: a group's product is summed in FP32 and meets its
+ * scale there; bias, activation and residual follow in FP32, one rounding to `dtype`. A row of x with a value that is not finite gives NaN. Results do not
+ * depend on timing. From one row to thousands.
+ *
+ * mi_pack_int4 lays weights out once for that. q: (out_features, in_features / 2) bytes, element 2 j of a row in the low half of byte j, element 2 j + 1
+ * in the high half; packed: mi_int4_packed_bytes(out_features, in_features) bytes of device memory, an order of its own (about half a byte for each weight:
+ * features come in blocks of 16, in_features in blocks of 128). q row stride in bytes (0 = dense), a multiple of 4. scales and zeros are (groups, out_features)
+ * with groups = ceil(in_features / group): a checkpoint's (out_features, groups) transposed.
+ *
+ * in_features and out_features are multiples of 8, group is 32, 64 or a multiple of 128 (the last one may be shorter); strides in elements (0 = dense), multiples
+ * of 8, at most 2^40, rows times stride at most 2^56; operands 16-byte aligned, zeros 8-byte, q 4-byte. y may be `residual` itself (same pointer and stride); a
+ * call whose y shares other memory with an operand is refused. rows may be 0. */
+typedef struct mi_pack_int4_args {
+    uint32_t struct_size;
+    const void* q;
+    void* packed;
+    int32_t out_features, in_features;
+    int64_t q_row_stride;
+    void* stream;
+} mi_pack_int4_args;
+MI_API size_t mi_int4_packed_bytes(int32_t out_features, int32_t in_features);
+MI_API int mi_pack_int4(const mi_pack_int4_args* args);
+typedef struct mi_linear_int4_args {
+    uint32_t struct_size;
+    int32_t dtype;           /* of x, scales, bias, residual, y */
+    const void* x;           /* (rows, in_features) */
+    const void* w;           /* packed, as mi_pack_int4 writes it */
+    const void* scales;      /* (groups, out_features) */
+    const void* zeros;       /* bytes (groups, out_features), or NULL: 8 */
+    const void* bias;        /* (out_features) or NULL */
+    const void* residual;    /* (rows, out_features) or NULL */
+    void* y;                 /* (rows, out_features) */
+    int32_t rows, in_features, out_features, group;
+    int64_t x_row_stride, residual_row_stride, y_row_stride;
+    int32_t activation;      /* MI_ACT_* */
+    void* stream;
+} mi_linear_int4_args;
+MI_API int mi_linear_int4_forward(const mi_linear_int4_args* args);
+
 /* ── attention with its projections ────────────────────────────────────────
  * The three operators the U-Net spatial transformer calls (src/unet_blocks.cpp:255-327,
  * src/unet.cpp:470-480; also the VAE mid blocks, src/vae.cpp:268):
