@@ -16,56 +16,61 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
     using V8 = typename M::v8;
     typedef T t4 __attribute__((ext_vector_type(4)));
     constexpr int F = 16 * FB, NT = 64 * WAVES, OUT = (F * 16 * TB + NT - 1) / NT;
-    __shared__ __attribute__((aligned(16))) float sums[WAVES][FB * TB][16 * 16];      // [row][feature] of a block
+    constexpr int kTokens = TB * 16 * 256, kSums = FB * TB * 1024;      // bytes of a wavefront: a block's rows of X, its sums
+    __shared__ __attribute__((aligned(16))) unsigned char lds[WAVES * (kTokens > kSums ? kTokens : kSums)];
 
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n0 = static_cast<int>(blockIdx.x) * F, m0 = static_cast<int>(blockIdx.y) * 16 * TB;
     const int last_block = (p.N + 15) / 16 - 1;
 
+    // (addresses as a uniform base and an offset of the lane)
     const unsigned char* wrow[FB];
-    const T* scale[FB];
-    const unsigned char* zero[FB];
+    unsigned foff[FB];
 #pragma unroll
     for (int a = 0; a < FB; ++a) {
-        wrow[a] = static_cast<const unsigned char*>(p.w) + static_cast<long>(min(n0 / 16 + a, last_block)) * p.KB * 1024 + lane * 16;
-        const int f = min(n0 + 16 * a + 4 * lg, p.N - 4);      // (features come in eights)
-        scale[a] = static_cast<const T*>(p.scales) + f;
-        zero[a] = p.zeros + f;
+        wrow[a] = static_cast<const unsigned char*>(p.w) + static_cast<long>(min(n0 / 16 + a, last_block)) * p.KB * 1024;
+        foff[a] = static_cast<unsigned>(min(n0 + 16 * a + 4 * lg, p.N - 4));      // (features come in eights)
     }
-    const T* xrow[TB];
+    // X comes in loads of 4 rows of 256 bytes, piece `lr` of row 4 u + lg, and goes through this wavefront's part of LDS: as operands are wanted, a row per
+    // lane, a load's neighbouring lanes would lie in 4 rows, and such loads were the time of more than a few rows (20 x 16384 x 6144: 48 us)
+    constexpr int XU = 4 * TB;
+    const T* xrow[XU];
 #pragma unroll
-    for (int b = 0; b < TB; ++b) xrow[b] = static_cast<const T*>(p.x) + static_cast<long>(min(m0 + 16 * b + lr, p.M - 1)) * p.ldx;
+    for (int u = 0; u < XU; ++u) xrow[u] = static_cast<const T*>(p.x) + static_cast<long>(min(m0 + 4 * u + lg, p.M - 1)) * p.ldx;
+    const int rows = p.M - m0;                              // (loads of rows that are all past the end are left out: their columns of the product are not stored)
 
-    struct Block { u32x4 w[FB]; V8 x[TB][4]; t4 s[FB][P]; unsigned z[FB][P]; };
+    struct Block { u32x4 w[FB]; V8 x[XU]; t4 s[FB][P]; unsigned z[FB][P]; };
     auto load = [&](Block& c, int kb) {
 #pragma unroll
-        for (int a = 0; a < FB; ++a) c.w[a] = *reinterpret_cast<const u32x4*>(wrow[a] + static_cast<long>(kb) * 1024);
+        for (int a = 0; a < FB; ++a) c.w[a] = *reinterpret_cast<const u32x4*>(wrow[a] + static_cast<long>(kb) * 1024 + lane * 16u);
 #pragma unroll
         for (int g = 0; g < P; ++g) {
             const long row = static_cast<long>(min(P == 1 ? kb / p.span : kb * P + g, p.groups - 1)) * p.N;
 #pragma unroll
             for (int a = 0; a < FB; ++a) {
-                c.s[a][g] = *reinterpret_cast<const t4*>(scale[a] + row);
-                c.z[a][g] = p.zeros ? *reinterpret_cast<const unsigned*>(zero[a] + row) : 0x08080808u;
+                c.s[a][g] = *reinterpret_cast<const t4*>(reinterpret_cast<const unsigned char*>(static_cast<const T*>(p.scales) + row) + foff[a] * 2u);
+                c.z[a][g] = p.zeros ? *reinterpret_cast<const unsigned*>(p.zeros + row + foff[a]) : 0x08080808u;
             }
         }
-        const int k0 = kb * 128 + 8 * lg;
-        if (kb * 128 + 128 <= p.K) {
+        const int k0 = kb * 128 + 8 * lr;
+        const bool there = k0 < p.K;                        // (pieces past the end: the row's first one, as zeros)
 #pragma unroll
-            for (int b = 0; b < TB; ++b)
+        for (int u = 0; u < XU; ++u)
+            if (4 * u < rows) {
+                const V8 v = *reinterpret_cast<const V8*>(xrow[u] + (there ? k0 : 0));
+                c.x[u] = there ? v : V8{};
+            }
+    };
+    unsigned char* const tokens = lds + wave * kTokens;
+    auto stage = [&](const Block& c) {
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
 #pragma unroll
-                for (int j = 0; j < 4; ++j) c.x[b][j] = *reinterpret_cast<const V8*>(xrow[b] + k0 + 32 * j);
-        } else {
-#pragma unroll
-            for (int b = 0; b < TB; ++b)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {       // (pieces past the end: the row's first one, as zeros)
-                    const bool there = k0 + 32 * j < p.K;
-                    const V8 v = *reinterpret_cast<const V8*>(xrow[b] + (there ? k0 + 32 * j : 0));
-                    c.x[b][j] = there ? v : V8{};
-                }
-        }
+        for (int u = 0; u < XU; ++u)
+            if (4 * u < rows) *reinterpret_cast<V8*>(tokens + (4 * u + lg) * 256 + ((lr ^ ((4 * u + lg) & 15)) << 4)) = c.x[u];
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
     };
     f32x4 acc[FB][TB];
 #pragma unroll
@@ -73,15 +78,19 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
 #pragma unroll
         for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](const Block& c) {
+        V8 x[TB][4];
         f32x4 sx[TB][P];
 #pragma unroll
-        for (int b = 0; b < TB; ++b)
+        for (int b = 0; b < TB; ++b) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[b][j] = *reinterpret_cast<const V8*>(tokens + (16 * b + lr) * 256 + (((4 * j + lg) ^ lr) << 4));
 #pragma unroll
             for (int g = 0; g < P; ++g) {
                 sx[b][g] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) sx[b][g] = M::run16(ones<T>(), c.x[b][j], sx[b][g]);
+                for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) sx[b][g] = M::run16(ones<T>(), x[b][j], sx[b][g]);
             }
+        }
 #pragma unroll
         for (int a = 0; a < FB; ++a) {
             V8 w[4];
@@ -98,7 +107,7 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
 #pragma unroll
                     for (int e = 0; e < 4; ++e) t[e] = -z[e] * sx[b][g][e];
 #pragma unroll
-                    for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) t = M::run16(w[j], c.x[b][j], t);
+                    for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) t = M::run16(w[j], x[b][j], t);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[a][b][e] = __builtin_fmaf(t[e], static_cast<float>(c.s[a][g][e]), acc[a][b][e]);
                 }
@@ -111,18 +120,25 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
         load(c[0], wave);
         int i = wave;
         for (; i + WAVES < p.KB; i += 2 * WAVES) {
+            stage(c[0]);
             load(c[1], i + WAVES);
             multiply(c[0]);
+            stage(c[1]);
             if (i + 2 * WAVES < p.KB) load(c[0], i + 2 * WAVES);
             multiply(c[1]);
         }
-        if (i < p.KB) multiply(c[0]);
+        if (i < p.KB) {
+            stage(c[0]);
+            multiply(c[0]);
+        }
     }
 
+    __syncthreads();                                        // (the sums go where rows of X were)
+    float* const sums = reinterpret_cast<float*>(lds);      // [wavefront][block][row][feature]
 #pragma unroll
     for (int a = 0; a < FB; ++a)
 #pragma unroll
-        for (int b = 0; b < TB; ++b) *reinterpret_cast<f32x4*>(&sums[wave][a * TB + b][lr * 16 + 4 * lg]) = acc[a][b];
+        for (int b = 0; b < TB; ++b) *reinterpret_cast<f32x4*>(sums + ((wave * FB + a) * TB + b) * 256 + lr * 16 + 4 * lg) = acc[a][b];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < OUT; ++i) {
@@ -130,7 +146,7 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
         if (row >= 16 * TB || m0 + row >= p.M || n0 + f >= p.N) continue;
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) v += sums[w][f / 16 * TB + row / 16][row % 16 * 16 + f % 16];
+        for (int w = 0; w < WAVES; ++w) v += sums[((w * FB + f / 16) * TB + row / 16) * 256 + row % 16 * 16 + f % 16];
         if (p.bias) v += static_cast<float>(static_cast<const T*>(p.bias)[n0 + f]);
         with_activation(p.act, [&](auto act) { v = act(v); });
         if (p.residual) v += static_cast<float>(static_cast<const T*>(p.residual)[static_cast<long>(m0 + row) * p.ldr + n0 + f]);
@@ -140,7 +156,7 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
 
 template <typename T, int P, int FB, int TB>
 int launch(const Int4Problem& p, hipStream_t st) {
-    constexpr int WAVES = 8;
+    constexpr int WAVES = TB == 4 ? 4 : 8;
     hipLaunchKernelGGL((linear_int4_few_kernel<T, P, FB, TB, WAVES>), dim3((p.N + 16 * FB - 1) / (16 * FB), (p.M + 16 * TB - 1) / (16 * TB)), dim3(64 * WAVES), 0, st, p);
     MI_HIP_CHECK(hipGetLastError());
     return 0;
@@ -171,7 +187,7 @@ int launch_parts(const Int4Problem& p, int parts, hipStream_t st) {
 }  // namespace
 }  // namespace gemm
 
-bool int4_few_takes(const Int4Problem& p) { return p.M <= 64 || p.ldx * 2 * 512 >= (1L << 31); }
+bool int4_few_takes(const Int4Problem& p) { return p.M <= 64 || p.ldx * 2 * 512 >= (1L << 31) || p.N > 1 << 24; }      // (tiles have 32-bit offsets)
 
 int launch_int4_few(const Int4Problem& p, int dtype, int parts, hipStream_t st) {
     return dtype == MI_DTYPE_BF16 ? gemm::launch_parts<__bf16>(p, parts, st) : gemm::launch_parts<_Float16>(p, parts, st);
