@@ -30,13 +30,13 @@ struct TileForm {
     static_assert(kBytes <= 160 * 1024, "LDS of a compute unit");
 };
 
-template <typename T, int P, bool ZEROS, int TB, int FB, int WM, int WN, int S>
+template <typename T, int P, bool ZEROS, int TB, int FB, int WM, int WN, int S, bool TURNS>
 __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const Int4Problem p) {
     using M = Mma<T>;
     using V8 = typename M::v8;
     using L = TileForm<P, ZEROS, TB, FB, WM, WN, S>;
     typedef T t4 __attribute__((ext_vector_type(4)));
-    constexpr int NW = L::NW, TM = L::TM, TN = L::TN;
+    constexpr int TM = L::TM, TN = L::TN;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     float* const sums = reinterpret_cast<float*>(lds + L::kSums);      // [P][TM]
 
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
     const int m0 = (logical / tiles_n) * TM, n0 = (logical % tiles_n) * TN;
 
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = TURNS ? wave / WN : wave % WM, wn = TURNS ? wave % WN : wave / WM;      // (wavefronts w and w + 4 share a SIMD)
     const int nw = n0 + wn * 16 * FB, last_block = (p.N + 15) / 16 - 1;
 
     // ── DMA: addresses as a uniform base and an offset per lane ──
@@ -119,63 +119,65 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) request(i);
     int reading = 0;
-    for (int kb = 0; kb < p.KB; ++kb) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2) * L::NI) : "memory");
-        request(kb + S - 1);
-        const unsigned char* const stage = lds + reading * L::kStage;
+    bool short_block = false;
+    const unsigned char* stage = lds;
+    V8 w[FB][4];
+    // scales and zero points of a wavefront's features wait in registers, but for groups of 32, whose 16 FB values a lane would put others into memory:
+    // those are read again for each 16 tokens
+    constexpr bool AGAIN = P == 4;
+    float scale[FB][P][4];
+    unsigned zero[FB][P];
+    auto factors = [&](int g) {
+#pragma unroll
+        for (int a = 0; a < FB; ++a) {
+            const int f = g * TN + (wn * FB + a) * 16 + 4 * lg;
+            const t4 v = *reinterpret_cast<const t4*>(stage + L::kS + f * 2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) scale[a][g][e] = static_cast<float>(v[e]);
+            if constexpr (ZEROS) zero[a][g] = *reinterpret_cast<const unsigned*>(stage + L::kZ + f);
+        }
+    };
+    auto tokens = [&](V8 (&x)[4], int row16) {      // operands of 16 tokens, block `row16` of the tile
+        const unsigned char* const at = stage + row16 * 4096 + lr * 256;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const V8*>(at + (((4 * j + lg) ^ lr) << 4));
+        if (short_block) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (4 * j + lg >= left) x[j] = V8{};
+        }
+    };
+    // part 3 of a step: the sums of the 16-token blocks that the WN wavefronts of these tokens share out
+    auto prepare = [&](int kb) {
+        stage = lds + reading * L::kStage;
         reading = reading + 1 == S ? 0 : reading + 1;
-        const bool short_block = kb == p.KB - 1 && left < 16;
-        auto tokens = [&](V8 (&x)[4], int row16) {      // operands of 16 tokens, block `row16` of the tile
-            const unsigned char* const at = stage + row16 * 4096 + lr * 256;
+        short_block = kb == p.KB - 1 && left < 16;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const V8*>(at + (((4 * j + lg) ^ lr) << 4));
-            if (short_block) {
+        for (int i = 0; i < ceil_div(TB, WN); ++i) {
+            const int b = i * WN + wn;
+            if (TB % WN != 0 && b >= TB) break;
+            V8 x[4];
+            tokens(x, wm * TB + b);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (4 * j + lg >= left) x[j] = V8{};
+            for (int g = 0; g < P; ++g) {
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) s = M::run16(ones<T>(), x[j], s);
+                if (lg == 0) sums[g * TM + 16 * (wm * TB + b) + lr] = s[0];
             }
-        };
-        V8 w[FB][4];
+        }
 #pragma unroll
         for (int a = 0; a < FB; ++a) {
             const u32x4 packed = *reinterpret_cast<const u32x4*>(stage + L::kW + (wn * FB + a) * 1024 + lane * 16);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[a][j] = nibbles<T>(packed[j]);
         }
-#pragma unroll
-        for (int i = 0; i < ceil_div(TM / 16, NW); ++i) {
-            const int b = i * NW + wave;
-            if (TM / 16 % NW != 0 && b >= TM / 16) break;
-            V8 x[4];
-            tokens(x, b);
-#pragma unroll
-            for (int g = 0; g < P; ++g) {
-                f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) s = M::run16(ones<T>(), x[j], s);
-                if (lg == 0) sums[g * TM + 16 * b + lr] = s[0];
-            }
-        }
-        // scales and zero points of a wavefront's features wait in registers, but for groups of 32, whose 16 FB values a lane would put others into memory:
-        // those are read again for each 16 tokens
-        constexpr bool AGAIN = P == 4;
-        float scale[FB][P][4];
-        unsigned zero[FB][P];
-        auto factors = [&](int g) {
-#pragma unroll
-            for (int a = 0; a < FB; ++a) {
-                const int f = g * TN + (wn * FB + a) * 16 + 4 * lg;
-                const t4 v = *reinterpret_cast<const t4*>(stage + L::kS + f * 2);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) scale[a][g][e] = static_cast<float>(v[e]);
-                if constexpr (ZEROS) zero[a][g] = *reinterpret_cast<const unsigned*>(stage + L::kZ + f);
-            }
-        };
         if constexpr (!AGAIN) {
 #pragma unroll
             for (int g = 0; g < P; ++g) factors(g);
         }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto products = [&] {
 #pragma unroll
         for (int b = 0; b < TB; ++b) {
             V8 x[4];
@@ -198,6 +200,32 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
                     for (int e = 0; e < 4; ++e) acc[a][b][e] = __builtin_fmaf(t[e], scale[a][g][e], acc[a][b][e]);
                 }
             }
+        }
+    };
+    if constexpr (TURNS) {
+        // The two wavefronts of a SIMD take turns: while one multiplies the other makes its weights. Wavefronts of wm = 1 are a part of a step behind; a step's
+        // loads are requested where the first of them multiply and the others prepare, and waited for at the end of that.
+        static_assert(WM == 2 && WN == 4);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2) * L::NI) : "memory");
+        if (wm == 1) asm volatile("s_barrier" ::: "memory");
+        for (int kb = 0; kb < p.KB; ++kb) {
+            if (wm == 1) request(kb + S - 1);
+            prepare(kb);
+            if (wm == 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((S - 2) * L::NI) : "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (wm == 0) request(kb + S - 1);
+            products();
+            if (wm == 0) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((S - 2) * L::NI) : "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+        if (wm == 0) asm volatile("s_barrier" ::: "memory");
+    } else {
+        for (int kb = 0; kb < p.KB; ++kb) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2) * L::NI) : "memory");
+            request(kb + S - 1);
+            prepare(kb);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            products();
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (no DMA into LDS that is given back)
@@ -234,11 +262,11 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
     }
 }
 
-template <typename T, int P, bool ZEROS, int TB, int FB, int WM, int WN, int S>
+template <typename T, int P, bool ZEROS, int TB, int FB, int WM, int WN, int S, bool TURNS>
 int launch(const Int4Problem& p, hipStream_t st) {
     using L = TileForm<P, ZEROS, TB, FB, WM, WN, S>;
     constexpr int TM = L::TM, TN = L::TN, bytes = L::kBytes;
-    const auto kernel = &linear_int4_tile_kernel<T, P, ZEROS, TB, FB, WM, WN, S>;
+    const auto kernel = &linear_int4_tile_kernel<T, P, ZEROS, TB, FB, WM, WN, S, TURNS>;
     if constexpr (bytes > 64 * 1024) {
         int device = 0;
         MI_HIP_CHECK(hipGetDevice(&device));
@@ -257,8 +285,8 @@ int launch(const Int4Problem& p, hipStream_t st) {
 template <typename T, int P, bool ZEROS>
 int launch_form(const Int4Problem& p, hipStream_t st) {
     const long big = static_cast<long>((p.M + 127) / 128) * ((p.N + 255) / 256);
-    if (big >= device_cu_count()) return launch<T, P, ZEROS, 4, 4, 2, 4, 3>(p, st);      // 128 x 256
-    return launch<T, P, ZEROS, 2, 2, 2, 2, 3>(p, st);                                    // 64 x 64
+    if (big >= device_cu_count()) return launch<T, P, ZEROS, 4, 4, 2, 4, 3, true>(p, st);      // 128 x 256
+    return launch<T, P, ZEROS, 2, 2, 2, 2, 3, false>(p, st);                                    // 64 x 64
 }
 template <typename T, int P>
 int launch_zeros(const Int4Problem& p, hipStream_t st) { return p.zeros ? launch_form<T, P, true>(p, st) : launch_form<T, P, false>(p, st); }
