@@ -10,6 +10,7 @@
 // word lies in bits [8 i, 8 i + 4), element 4 + i above it: two ANDs and a shift leave bytes 0 .. 15, which as FP8 (E4M3) are multiples of 2^-9, the smallest
 // subnormal numbers and the first binade behind them, and v_cvt_scalef32_pk_*_fp8 makes two of them 16-bit at 2^9 each: 7 instructions for 8 weights.
 #pragma once
+#include "linear_int4_forms.h"
 #include "linear_math.h"
 
 namespace mi {
@@ -27,9 +28,8 @@ struct Int4Problem {
 // scale groups in a block: 4, 2, 1 (of 32, 64, 128 and more elements)
 inline int int4_parts(int group) { return group >= 128 ? 1 : 128 / group; }
 
-bool int4_few_takes(const Int4Problem& p);
-int launch_int4_few(const Int4Problem& p, int dtype, int parts, hipStream_t st);
-int launch_int4_tile(const Int4Problem& p, int dtype, int parts, hipStream_t st);
+int launch_int4_few(const Int4Problem& p, int dtype, int parts, int form, hipStream_t st);
+int launch_int4_tile(const Int4Problem& p, int dtype, int parts, int form, hipStream_t st);
 
 namespace gemm {
 
@@ -49,7 +49,9 @@ template <> struct Nibbles<_Float16> {
 };
 // a word of packed weights -> 8 values of T, exactly
 template <typename T> __device__ __forceinline__ typename Mma<T>::v8 nibbles(unsigned w) {
-    const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    unsigned mask = 0x0f0f0f0fu;
+    asm("" : "+s"(mask));                         // (a literal would double the instruction's length)
+    const unsigned lo = w & mask, hi = (w >> 4) & mask;
     using N = Nibbles<T>;
     const u32x4 r = {N::template two<false>(lo), N::template two<true>(lo), N::template two<false>(hi), N::template two<true>(hi)};
     return __builtin_bit_cast(typename Mma<T>::v8, r);

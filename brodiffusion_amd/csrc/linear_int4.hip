@@ -1,5 +1,5 @@
 // Y = act(X W^T + bias) + residual with 4-bit weights: the entries, the packing of weights and the choice between the kernels of linear_int4_few.hip and
-// linear_int4_tile.hip. Formulas and layout: linear_int4.h.
+// linear_int4_tile.hip (linear_int4_forms.h). Formulas and layout: linear_int4.h.
 #include "linear_int4.h"
 
 namespace mi {
@@ -62,8 +62,8 @@ int problem_of(const mi_linear_int4_args& a, const char* op, Int4Problem& p) {
     if (runs_share(p.y, y_run, p.scales, 2 * per_group)) return fail("%s: y overlaps scales", op);
     if (runs_share(p.y, y_run, p.zeros, per_group)) return fail("%s: y overlaps zeros", op);
     if (runs_share(p.y, y_run, p.bias, 2L * p.N)) return fail("%s: y overlaps the bias", op);
-    // (the smallest tiles are 64 x 64; work groups of few rows take 16 features and at least 16 rows, those in the second grid dimension)
-    if ((p.M + 63L) / 64 * ((p.N + 63L) / 64) > 0x7ffffff0L || (int4_few_takes(p) && p.M > 65535L * 16)) return fail("%s: problem too large for one launch", op);
+    // (work groups of 16 rows lie in the second grid dimension)
+    if ((p.M + 31L) / 32 * ((p.N + 63L) / 64) > 0x7ffffff0L || (int4_far_apart(p.N, p.ldx) && p.M > 65535L * 16)) return fail("%s: problem too large for one launch", op);
     return 1;
 }
 
@@ -106,7 +106,9 @@ int mi_linear_int4_forward(const mi_linear_int4_args* a) {
     const int rc = mi::problem_of(*a, op, p);
     if (rc <= 0) return rc;
     const int parts = mi::int4_parts(a->group);
-    return mi::int4_few_takes(p) ? mi::launch_int4_few(p, a->dtype, parts, mi::resolve_stream(a->stream)) : mi::launch_int4_tile(p, a->dtype, parts, mi::resolve_stream(a->stream));
+    const int form = mi::int4_form(p.M, p.N, p.KB, p.ldx, parts, mi::device_cu_count());
+    const hipStream_t st = mi::resolve_stream(a->stream);
+    return form < mi::kTile32x64 ? mi::launch_int4_few(p, a->dtype, parts, form, st) : mi::launch_int4_tile(p, a->dtype, parts, form, st);
 }
 
 }  // extern "C"

@@ -1,27 +1,29 @@
 // The linear layer with 4-bit weights for few rows (linear_int4.h): a token of a serving step, a draft, a short prompt.
 //
-// Bound: the bytes of the packed weights, each used once per 16 * TB rows of X. They go from memory straight to the registers of the wavefront that multiplies
-// them, in whole kilobytes. A work group owns 16 FB features and 16 TB rows; its wavefronts take the blocks of 128 contraction elements in turn, each with its
+// Bound: the bytes of the packed weights, each used once per 16 rows of X. They go from memory straight to the registers of the wavefront that multiplies
+// them, in whole kilobytes. A work group owns 16 FB features and 16 rows; its 8 wavefronts take the blocks of 128 contraction elements in turn, each with its
 // next block on its way while it multiplies, and their sums meet in LDS, added in the order of the wavefronts: no result depends on timing. One launch, no
-// workspace, no atomics.
+// workspace, no atomics. (32 and 64 rows to a work group were slower than two and four of them, or than tiles, at every size; so were two blocks on their way.)
 #include "linear_int4.h"
 
 namespace mi {
 namespace gemm {
 namespace {
 
-template <typename T, int P, int FB, int TB, int WAVES>
+constexpr int WAVES = 8;
+
+template <typename T, int P, int FB>
 __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4Problem p) {
     using M = Mma<T>;
     using V8 = typename M::v8;
     typedef T t4 __attribute__((ext_vector_type(4)));
-    constexpr int F = 16 * FB, NT = 64 * WAVES, OUT = (F * 16 * TB + NT - 1) / NT;
-    constexpr int kTokens = TB * 16 * 256, kSums = FB * TB * 1024;      // bytes of a wavefront: a block's rows of X, its sums
+    constexpr int F = 16 * FB, NT = 64 * WAVES, OUT = (F * 16 + NT - 1) / NT;
+    constexpr int kTokens = 16 * 256, kSums = FB * 1024;      // bytes of a wavefront: a block's rows of X, its sums
     __shared__ __attribute__((aligned(16))) unsigned char lds[WAVES * (kTokens > kSums ? kTokens : kSums)];
 
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n0 = static_cast<int>(blockIdx.x) * F, m0 = static_cast<int>(blockIdx.y) * 16 * TB;
+    const int n0 = static_cast<int>(blockIdx.x) * F, m0 = static_cast<int>(blockIdx.y) * 16;
     const int last_block = (p.N + 15) / 16 - 1;
 
     // (addresses as a uniform base and an offset of the lane)
@@ -34,7 +36,7 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
     }
     // X comes in loads of 4 rows of 256 bytes, piece `lr` of row 4 u + lg, and goes through this wavefront's part of LDS: as operands are wanted, a row per
     // lane, a load's neighbouring lanes would lie in 4 rows, and such loads were the time of more than a few rows (20 x 16384 x 6144: 48 us)
-    constexpr int XU = 4 * TB;
+    constexpr int XU = 4;
     const T* xrow[XU];
 #pragma unroll
     for (int u = 0; u < XU; ++u) xrow[u] = static_cast<const T*>(p.x) + static_cast<long>(min(m0 + 4 * u + lg, p.M - 1)) * p.ldx;
@@ -72,24 +74,19 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
         __builtin_amdgcn_wave_barrier();
         asm volatile("" ::: "memory");
     };
-    f32x4 acc[FB][TB];
+    f32x4 acc[FB];
 #pragma unroll
-    for (int a = 0; a < FB; ++a)
-#pragma unroll
-        for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int a = 0; a < FB; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](const Block& c) {
-        V8 x[TB][4];
-        f32x4 sx[TB][P];
+        V8 x[4];
+        f32x4 sx[P];
 #pragma unroll
-        for (int b = 0; b < TB; ++b) {
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const V8*>(tokens + lr * 256 + (((4 * j + lg) ^ lr) << 4));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[b][j] = *reinterpret_cast<const V8*>(tokens + (16 * b + lr) * 256 + (((4 * j + lg) ^ lr) << 4));
+        for (int g = 0; g < P; ++g) {
+            sx[g] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int g = 0; g < P; ++g) {
-                sx[b][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) sx[b][g] = M::run16(ones<T>(), x[b][j], sx[b][g]);
-            }
+            for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) sx[g] = M::run16(ones<T>(), x[j], sx[g]);
         }
 #pragma unroll
         for (int a = 0; a < FB; ++a) {
@@ -98,19 +95,13 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
             for (int j = 0; j < 4; ++j) w[j] = nibbles<T>(c.w[a][j]);
 #pragma unroll
             for (int g = 0; g < P; ++g) {
-                float z[4];
+                f32x4 t;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[e] = zero_point(c.z[a][g], e);
+                for (int e = 0; e < 4; ++e) t[e] = -zero_point(c.z[a][g], e) * sx[g][e];
 #pragma unroll
-                for (int b = 0; b < TB; ++b) {
-                    f32x4 t;
+                for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) t = M::run16(w[j], x[j], t);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) t[e] = -z[e] * sx[b][g][e];
-#pragma unroll
-                    for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) t = M::run16(w[j], x[b][j], t);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[a][b][e] = __builtin_fmaf(t[e], static_cast<float>(c.s[a][g][e]), acc[a][b][e]);
-                }
+                for (int e = 0; e < 4; ++e) acc[a][e] = __builtin_fmaf(t[e], static_cast<float>(c.s[a][g][e]), acc[a][e]);
             }
         }
     };
@@ -134,19 +125,17 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
     }
 
     __syncthreads();                                        // (the sums go where rows of X were)
-    float* const sums = reinterpret_cast<float*>(lds);      // [wavefront][block][row][feature]
+    float* const sums = reinterpret_cast<float*>(lds);      // [wavefront][block of features][row][feature]
 #pragma unroll
-    for (int a = 0; a < FB; ++a)
-#pragma unroll
-        for (int b = 0; b < TB; ++b) *reinterpret_cast<f32x4*>(sums + ((wave * FB + a) * TB + b) * 256 + lr * 16 + 4 * lg) = acc[a][b];
+    for (int a = 0; a < FB; ++a) *reinterpret_cast<f32x4*>(sums + (wave * FB + a) * 256 + lr * 16 + 4 * lg) = acc[a];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < OUT; ++i) {
         const int o = i * NT + tid, f = o % F, row = o / F;
-        if (row >= 16 * TB || m0 + row >= p.M || n0 + f >= p.N) continue;
+        if (row >= 16 || m0 + row >= p.M || n0 + f >= p.N) continue;
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) v += sums[((w * FB + f / 16) * TB + row / 16) * 256 + row % 16 * 16 + f % 16];
+        for (int w = 0; w < WAVES; ++w) v += sums[(w * FB + f / 16) * 256 + row * 16 + f % 16];
         if (p.bias) v += static_cast<float>(static_cast<const T*>(p.bias)[n0 + f]);
         with_activation(p.act, [&](auto act) { v = act(v); });
         if (p.residual) v += static_cast<float>(static_cast<const T*>(p.residual)[static_cast<long>(m0 + row) * p.ldr + n0 + f]);
@@ -154,43 +143,31 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
     }
 }
 
-template <typename T, int P, int FB, int TB>
+template <typename T, int P, int FB>
 int launch(const Int4Problem& p, hipStream_t st) {
-    constexpr int WAVES = TB == 4 ? 4 : 8;
-    hipLaunchKernelGGL((linear_int4_few_kernel<T, P, FB, TB, WAVES>), dim3((p.N + 16 * FB - 1) / (16 * FB), (p.M + 16 * TB - 1) / (16 * TB)), dim3(64 * WAVES), 0, st, p);
+    hipLaunchKernelGGL((linear_int4_few_kernel<T, P, FB>), dim3((p.N + 16 * FB - 1) / (16 * FB), (p.M + 15) / 16), dim3(64 * WAVES), 0, st, p);
     MI_HIP_CHECK(hipGetLastError());
     return 0;
 }
 
 template <typename T, int P>
-int launch_form(const Int4Problem& p, hipStream_t st) {
-    const int cu = device_cu_count();
-    if (p.M <= 16) {
-        if (p.N >= 64 * cu) return launch<T, P, 4, 1>(p, st);
-        if (p.N >= 32 * cu) return launch<T, P, 2, 1>(p, st);
-        return launch<T, P, 1, 1>(p, st);
+int launch_form(const Int4Problem& p, int form, hipStream_t st) {
+    switch (form) {
+        case kFew16: return launch<T, P, 1>(p, st);
+        case kFew32: return launch<T, P, 2>(p, st);
+        default: return launch<T, P, P == 4 ? 2 : 4>(p, st);      // (kFew64; not asked for with groups of 32)
     }
-    if (p.M <= 32) {
-        if (p.N >= 64 * cu) return launch<T, P, 4, 2>(p, st);
-        if (p.N >= 32 * cu) return launch<T, P, 2, 2>(p, st);
-        return launch<T, P, 1, 2>(p, st);
-    }
-    if (p.N >= 32 * cu) return launch<T, P, 2, 4>(p, st);
-    return launch<T, P, 1, 4>(p, st);
 }
-
 template <typename T>
-int launch_parts(const Int4Problem& p, int parts, hipStream_t st) {
-    return parts == 1 ? launch_form<T, 1>(p, st) : parts == 2 ? launch_form<T, 2>(p, st) : launch_form<T, 4>(p, st);
+int launch_parts(const Int4Problem& p, int parts, int form, hipStream_t st) {
+    return parts == 1 ? launch_form<T, 1>(p, form, st) : parts == 2 ? launch_form<T, 2>(p, form, st) : launch_form<T, 4>(p, form, st);
 }
 
 }  // namespace
 }  // namespace gemm
 
-bool int4_few_takes(const Int4Problem& p) { return p.M <= 64 || p.ldx * 2 * 512 >= (1L << 31) || p.N > 1 << 24; }      // (tiles have 32-bit offsets)
-
-int launch_int4_few(const Int4Problem& p, int dtype, int parts, hipStream_t st) {
-    return dtype == MI_DTYPE_BF16 ? gemm::launch_parts<__bf16>(p, parts, st) : gemm::launch_parts<_Float16>(p, parts, st);
+int launch_int4_few(const Int4Problem& p, int dtype, int parts, int form, hipStream_t st) {
+    return dtype == MI_DTYPE_BF16 ? gemm::launch_parts<__bf16>(p, parts, form, st) : gemm::launch_parts<_Float16>(p, parts, form, st);
 }
 
 }  // namespace mi

@@ -1,14 +1,20 @@
 // The linear layer with 4-bit weights for many rows (linear_int4.h).
 //
-// A work group owns a tile of tokens x features, 16 TB WM x 16 FB WN, of WM x WN wavefronts with TB x FB blocks of v_mfma_f32_16x16x32 each. All operands
-// come by LDS DMA in steps of 128 contraction elements (a block of packed weights) into a ring of S stages: X in rows of 256 bytes, the piece of 16 bytes at
-// position c of row r being piece c ^ (r % 16), so that the 16 rows of an operand read lie in 16 different bank groups; packed weights, operands already, a kilobyte
-// each; scales and zero points. A step:
+// A work group of 4 wavefronts owns a tile of 16 TB tokens x 64 FB features, each wavefront all the tokens and 16 FB features: TB x FB blocks of
+// v_mfma_f32_16x16x32. All operands come by LDS DMA in steps of 128 contraction elements (a block of packed weights) into a ring of S stages: X in rows of 256
+// bytes, the piece of 16 bytes at position c of row r being piece c ^ (r % 16), so that the 16 rows of an operand read lie in 16 different bank groups; packed
+// weights, operands already, a kilobyte for 16 features; scales and zero points. A step:
 //   1. wait until all but the youngest S - 2 steps' loads of this wavefront have landed; barrier (and the stage before the ring's next is free)
-//   2. request step + S - 1
-//   3. the sums of x of the step, each 16 tokens by one wavefront, into LDS; the wavefront's weights to 16 bits, in registers for all its tokens; barrier
-//   4. products: 16 tokens at a time against all the wavefront's features, a chain of matrix instructions per group from -z times the sum of x, scaled into the
-//      accumulators
+//   2. the sums of x of the step, each 16 tokens by one wavefront, into LDS; the wavefront's weights to 16 bits, in registers for all tokens; barrier. With OWN a
+//      wavefront sums for itself, along with its products, and the second barrier is gone: faster where a step is short
+//   3. products: 16 tokens at a time against all the wavefront's features, a chain of matrix instructions per group from -z times the sum of x, scaled into the
+//      accumulators; between them the loads of step + S - 1, dealt out: a request waits for those ahead of it (60 bytes a clock and compute unit)
+// Bound: what a SIMD issues. Beside 64 products, 64 tokens x 64 features x 128 elements are 112 instructions of the weights, 64 that scale sums and about 60 others;
+// a 16 x 16 product takes the issue 12 of its 16 clocks, another vector instruction 4 (measured: one product and 1 to 4 others, two wavefronts, 17, 19.5,
+// 24.4, 27.9 clocks), so the matrix pipes are busy half of the time. 32 x 32 products leave more room (32.3 clocks with 1, 33.5 with 6 others), but their
+// accumulators came out slower at every size (4608 x 6144 x 16384: 970 us instead of 870), and so did wavefronts that take turns at products and weights (890).
+#include <utility>
+
 #include "linear_int4.h"
 
 namespace mi {
@@ -18,9 +24,10 @@ namespace {
 constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // Sizes of a form: bytes of a stage's parts in LDS, DMA instructions of a wavefront for each (all wavefronts issue the same number: the wait counts them)
-template <int P, bool ZEROS, int TB, int FB, int WM, int WN, int S>
+constexpr int kWaves = 4;
+template <int P, bool ZEROS, int TB, int FB, int S>
 struct TileForm {
-    static constexpr int NW = WM * WN, TM = 16 * TB * WM, TN = 16 * FB * WN;
+    static constexpr int NW = kWaves, TM = 16 * TB, TN = 16 * FB * NW;
     static constexpr int XI = TM / 4 / NW, WI = ceil_div(TN / 16, NW);
     static constexpr int SD = ceil_div(TN * P, 128), ZD = ZEROS ? ceil_div(TN * P, 256) : 0;      // instructions of 256 bytes
     static constexpr int SI = ceil_div(SD, NW), ZI = ceil_div(ZD, NW), NI = XI + WI + SI + ZI;
@@ -30,13 +37,13 @@ struct TileForm {
     static_assert(kBytes <= 160 * 1024, "LDS of a compute unit");
 };
 
-template <typename T, int P, bool ZEROS, int TB, int FB, int WM, int WN, int S, bool TURNS>
-__global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const Int4Problem p) {
+template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN>
+__global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(const Int4Problem p) {
     using M = Mma<T>;
     using V8 = typename M::v8;
-    using L = TileForm<P, ZEROS, TB, FB, WM, WN, S>;
+    using L = TileForm<P, ZEROS, TB, FB, S>;
     typedef T t4 __attribute__((ext_vector_type(4)));
-    constexpr int TM = L::TM, TN = L::TN;
+    constexpr int NW = L::NW, TM = L::TM, TN = L::TN;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     float* const sums = reinterpret_cast<float*>(lds + L::kSums);      // [P][TM]
 
@@ -48,8 +55,8 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
     const int m0 = (logical / tiles_n) * TM, n0 = (logical % tiles_n) * TN;
 
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = TURNS ? wave / WN : wave % WM, wn = TURNS ? wave % WN : wave / WM;      // (wavefronts w and w + 4 share a SIMD)
-    const int nw = n0 + wn * 16 * FB, last_block = (p.N + 15) / 16 - 1;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int last_block = (p.N + 15) / 16 - 1;
 
     // ── DMA: addresses as a uniform base and an offset per lane ──
     const unsigned char* const xg = static_cast<const unsigned char*>(p.x) + static_cast<long>(m0) * p.ldx * 2;
@@ -87,27 +94,38 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
     }
     const unsigned lds_base = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) unsigned char*)lds));
     const int left = (p.K - (p.KB - 1) * 128) / 8;      // pieces of the last block's rows
-    // (the LDS destination travels in m0; the s_nop is the wait state an LDS-DMA instruction needs behind a write of m0)
-    auto dma16 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory"); };
-    auto dma4 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory"); };
-    int filling = 0;                                    // the stage that the next request fills
-    auto request = [&](int step) {
+    // (the LDS destination travels in m0; the s_nop is the wait state an LDS-DMA instruction needs behind a write of m0. No memory clobber: what is read of
+    // LDS between two barriers is another stage, and the barriers have one)
+    auto dma16 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst)); };
+    auto dma4 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "{m0}"(dst)); };
+    int filling = 0, group = 0, of_group = 0;           // the stage that the next request fills; its group, of blocks and more, and which block of it
+    // requests FROM .. TO - 1 of a step's L::NI
+    auto request = [&]<int FROM, int TO>(int step, std::integer_sequence<int, FROM, TO>) {
         const int kb = min(step, p.KB - 1);             // (past the end the last step again, into a stage that nobody reads: the wait counts instructions)
         const unsigned at = lds_base + filling * L::kStage;
-        filling = filling + 1 == S ? 0 : filling + 1;
         const int most = kb == p.KB - 1 ? left - 1 : 15;      // (pieces past the end: the last one, left out of the products)
-        const unsigned char* const base = xg + static_cast<long>(kb) * 256;
-#pragma unroll
-        for (int u = 0; u < L::WI; ++u) dma16(lane * 16u, wg[u] + static_cast<long>(kb) * 1024, at + L::kW + wi[u] * 1024);
-        const int g0 = P == 1 ? kb / p.span : kb * P, most_g = p.groups - 1 - g0;
-        const unsigned char* const sbase = static_cast<const unsigned char*>(p.scales) + static_cast<long>(g0) * p.N * 2;
-#pragma unroll
-        for (int u = 0; u < L::SI; ++u) dma4(soff[u] + (P == 1 ? 0u : static_cast<unsigned>(min(sg[u], most_g)) * (static_cast<unsigned>(p.N) * 2u)), sbase, at + L::kS + si[u] * 256);
-#pragma unroll
-        for (int u = 0; u < L::ZI; ++u)
-            dma4(zoff[u] + (P == 1 ? 0u : static_cast<unsigned>(min(zg[u], most_g)) * static_cast<unsigned>(p.N)), p.zeros + static_cast<long>(g0) * p.N, at + L::kZ + zi[u] * 256);
-#pragma unroll
-        for (int u = 0; u < L::XI; ++u) dma16(xoff[u] + static_cast<unsigned>(min(piece[u], most)) * 16u, base, at + (wave * L::XI + u) * 1024);
+        const int g0 = P == 1 ? min(group, p.groups - 1) : kb * P, most_g = p.groups - 1 - g0;
+        [&]<int... I>(std::integer_sequence<int, I...>) {
+            ([&] {
+                constexpr int i = FROM + I;
+                if constexpr (i < L::WI) dma16(lane * 16u, wg[i] + static_cast<long>(kb) * 1024, at + L::kW + wi[i] * 1024);
+                else if constexpr (i < L::WI + L::SI) {
+                    constexpr int u = i - L::WI;
+                    dma4(soff[u] + (P == 1 ? 0u : static_cast<unsigned>(min(sg[u], most_g)) * (static_cast<unsigned>(p.N) * 2u)), static_cast<const unsigned char*>(p.scales) + static_cast<long>(g0) * p.N * 2,
+                         at + L::kS + si[u] * 256);
+                } else if constexpr (i < L::WI + L::SI + L::ZI) {
+                    constexpr int u = i - L::WI - L::SI;
+                    dma4(zoff[u] + (P == 1 ? 0u : static_cast<unsigned>(min(zg[u], most_g)) * static_cast<unsigned>(p.N)), p.zeros + static_cast<long>(g0) * p.N, at + L::kZ + zi[u] * 256);
+                } else {
+                    constexpr int u = i - L::WI - L::SI - L::ZI;
+                    dma16(xoff[u] + static_cast<unsigned>(min(piece[u], most)) * 16u, xg + static_cast<long>(kb) * 256, at + (wave * L::XI + u) * 1024);
+                }
+            }(), ...);
+        }(std::make_integer_sequence<int, TO - FROM>{});
+        if constexpr (TO == L::NI && FROM < TO) {
+            filling = filling + 1 == S ? 0 : filling + 1;
+            if (++of_group == p.span) { of_group = 0; ++group; }
+        }
     };
 
     f32x4 acc[FB][TB];
@@ -117,122 +135,118 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
         for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) request(i);
+    for (int i = 0; i < S - 1; ++i) request(i, std::integer_sequence<int, 0, L::NI>{});
     int reading = 0;
-    bool short_block = false;
-    const unsigned char* stage = lds;
-    V8 w[FB][4];
-    // scales and zero points of a wavefront's features wait in registers, but for groups of 32, whose 16 FB values a lane would put others into memory:
-    // those are read again for each 16 tokens
-    constexpr bool AGAIN = P == 4;
-    float scale[FB][P][4];
-    unsigned zero[FB][P];
-    auto factors = [&](int g) {
-#pragma unroll
-        for (int a = 0; a < FB; ++a) {
-            const int f = g * TN + (wn * FB + a) * 16 + 4 * lg;
-            const t4 v = *reinterpret_cast<const t4*>(stage + L::kS + f * 2);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) scale[a][g][e] = static_cast<float>(v[e]);
-            if constexpr (ZEROS) zero[a][g] = *reinterpret_cast<const unsigned*>(stage + L::kZ + f);
-        }
-    };
-    auto tokens = [&](V8 (&x)[4], int row16) {      // operands of 16 tokens, block `row16` of the tile
-        const unsigned char* const at = stage + row16 * 4096 + lr * 256;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const V8*>(at + (((4 * j + lg) ^ lr) << 4));
-        if (short_block) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (4 * j + lg >= left) x[j] = V8{};
-        }
-    };
-    // part 3 of a step: the sums of the 16-token blocks that the WN wavefronts of these tokens share out
-    auto prepare = [&](int kb) {
-        stage = lds + reading * L::kStage;
+    for (int kb = 0; kb < p.KB; ++kb) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2) * L::NI) : "memory");
+        unsigned char* const stage = lds + reading * L::kStage;
         reading = reading + 1 == S ? 0 : reading + 1;
-        short_block = kb == p.KB - 1 && left < 16;
+        auto tokens = [&](V8 (&x)[4], int row16) {      // operands of 16 tokens, block `row16` of the tile
+            const unsigned char* const at = stage + row16 * 4096 + lr * 256;
 #pragma unroll
-        for (int i = 0; i < ceil_div(TB, WN); ++i) {
-            const int b = i * WN + wn;
-            if (TB % WN != 0 && b >= TB) break;
+            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const V8*>(at + (((4 * j + lg) ^ lr) << 4));
+        };
+        if (kb == p.KB - 1 && left < 16) {              // zeros behind the end of the rows: every wavefront those of the tokens that it sums
+#pragma unroll
+            for (int i = 0; i < ceil_div(TM / 16, NW); ++i) {
+                const int b = i * NW + wave;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (b < TM / 16 && lr >= left) *reinterpret_cast<u32x4*>(stage + (16 * b + 4 * u + lg) * 256 + ((lr ^ (4 * u + lg)) << 4)) = u32x4{0u, 0u, 0u, 0u};
+            }
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("" ::: "memory");
+            if constexpr (OWN) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < (OWN ? 0 : ceil_div(TM / 16, NW)); ++i) {
+            const int b = i * NW + wave;
+            if (TM / 16 % NW != 0 && b >= TM / 16) break;
             V8 x[4];
-            tokens(x, wm * TB + b);
+            tokens(x, b);
 #pragma unroll
             for (int g = 0; g < P; ++g) {
                 f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) s = M::run16(ones<T>(), x[j], s);
-                if (lg == 0) sums[g * TM + 16 * (wm * TB + b) + lr] = s[0];
+                if (lg == 0) sums[g * TM + 16 * b + lr] = s[0];
             }
         }
+        V8 w[FB][4];
 #pragma unroll
         for (int a = 0; a < FB; ++a) {
-            const u32x4 packed = *reinterpret_cast<const u32x4*>(stage + L::kW + (wn * FB + a) * 1024 + lane * 16);
+            const u32x4 packed = *reinterpret_cast<const u32x4*>(stage + L::kW + (wave * FB + a) * 1024 + lane * 16);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[a][j] = nibbles<T>(packed[j]);
         }
+        // scales and zero points of a wavefront's features wait in registers; where they would be 32 a lane and more they are read again for each 16 tokens
+        constexpr bool AGAIN = P * FB >= 8;
+        float scale[FB][P][4];
+        unsigned zero[FB][P];
+        auto factors = [&](int g) {
+#pragma unroll
+            for (int a = 0; a < FB; ++a) {
+                const int f = g * TN + (wave * FB + a) * 16 + 4 * lg;
+                const t4 v = *reinterpret_cast<const t4*>(stage + L::kS + f * 2);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) scale[a][g][e] = static_cast<float>(v[e]);
+                if constexpr (ZEROS) zero[a][g] = *reinterpret_cast<const unsigned*>(stage + L::kZ + f);
+            }
+        };
         if constexpr (!AGAIN) {
 #pragma unroll
             for (int g = 0; g < P; ++g) factors(g);
         }
-    };
-    auto products = [&] {
+        if constexpr (!OWN) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        V8 x[2][4];
+        float sx[2][P];
+        auto fetch = [&](int b) {
+            tokens(x[b & 1], b);
 #pragma unroll
-        for (int b = 0; b < TB; ++b) {
-            V8 x[4];
-            tokens(x, wm * TB + b);
+            for (int g = 0; g < (OWN ? 0 : P); ++g) sx[b & 1][g] = sums[g * TM + 16 * b + lr];
+        };
+        fetch(0);
+        [&]<int... B>(std::integer_sequence<int, B...>) {
+            ([&] {
+                constexpr int b = B;
+                if constexpr (b + 1 < TB) fetch(b + 1);
+                request(kb + S - 1, std::integer_sequence<int, b * L::NI / TB, (b + 1) * L::NI / TB>{});
 #pragma unroll
-            for (int g = 0; g < P; ++g) {
-                const float sx = sums[g * TM + 16 * (wm * TB + b) + lr];
-                if constexpr (AGAIN) {
-                    asm volatile("" ::: "memory");
-                    factors(g);
+                for (int g = 0; g < P; ++g) {
+                    if constexpr (AGAIN) {
+                        asm volatile("" ::: "memory");
+                        factors(g);
+                    }
+                    f32x4 t[FB];
+#pragma unroll
+                    for (int a = 0; a < FB; ++a)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) t[a][e] = OWN ? 0.f : -(ZEROS ? zero_point(zero[a][g], e) : 8.f) * sx[b & 1][g];
+                    f32x4 total = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (OWN) {
+#pragma unroll
+                        for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) total = M::run16(ones<T>(), x[b & 1][j], total);
+                    }
+#pragma unroll
+                    for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j)
+#pragma unroll
+                        for (int a = 0; a < FB; ++a) t[a] = M::run16(w[a][j], x[b & 1][j], t[a]);
+#pragma unroll
+                    for (int a = 0; a < FB; ++a)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (OWN) t[a][e] = __builtin_fmaf(ZEROS ? -zero_point(zero[a][g], e) : -8.f, total[e], t[a][e]);
+                            acc[a][b][e] = __builtin_fmaf(t[a][e], scale[a][g][e], acc[a][b][e]);
+                        }
                 }
-#pragma unroll
-                for (int a = 0; a < FB; ++a) {
-                    f32x4 t;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) t[e] = -(ZEROS ? zero_point(zero[a][g], e) : 8.f) * sx;
-#pragma unroll
-                    for (int j = g * 4 / P; j < (g + 1) * 4 / P; ++j) t = M::run16(w[a][j], x[j], t);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[a][b][e] = __builtin_fmaf(t[e], scale[a][g][e], acc[a][b][e]);
-                }
-            }
-        }
-    };
-    if constexpr (TURNS) {
-        // The two wavefronts of a SIMD take turns: while one multiplies the other makes its weights. Wavefronts of wm = 1 are a part of a step behind; a step's
-        // loads are requested where the first of them multiply and the others prepare, and waited for at the end of that.
-        static_assert(WM == 2 && WN == 4);
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2) * L::NI) : "memory");
-        if (wm == 1) asm volatile("s_barrier" ::: "memory");
-        for (int kb = 0; kb < p.KB; ++kb) {
-            if (wm == 1) request(kb + S - 1);
-            prepare(kb);
-            if (wm == 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((S - 2) * L::NI) : "memory");
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (wm == 0) request(kb + S - 1);
-            products();
-            if (wm == 0) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((S - 2) * L::NI) : "memory");
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        }
-        if (wm == 0) asm volatile("s_barrier" ::: "memory");
-    } else {
-        for (int kb = 0; kb < p.KB; ++kb) {
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2) * L::NI) : "memory");
-            request(kb + S - 1);
-            prepare(kb);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            products();
-        }
+            }(), ...);
+        }(std::make_integer_sequence<int, TB>{});
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (no DMA into LDS that is given back)
 
 #pragma unroll
     for (int a = 0; a < FB; ++a) {
-        const int f = nw + 16 * a + 4 * lg;
+        const int f = n0 + (wave * FB + a) * 16 + 4 * lg;
         if (f >= p.N) continue;
         f32x4 bias = {0.f, 0.f, 0.f, 0.f};
         if (p.bias) {
@@ -242,7 +256,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
         }
 #pragma unroll
         for (int b = 0; b < TB; ++b) {
-            const int m = m0 + 16 * (wm * TB + b) + lr;
+            const int m = m0 + 16 * b + lr;
             if (m >= p.M) continue;
             f32x4 v = acc[a][b] + bias;
             with_activation(p.act, [&](auto act) {
@@ -262,11 +276,11 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_int4_tile_kernel(const In
     }
 }
 
-template <typename T, int P, bool ZEROS, int TB, int FB, int WM, int WN, int S, bool TURNS>
+template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN>
 int launch(const Int4Problem& p, hipStream_t st) {
-    using L = TileForm<P, ZEROS, TB, FB, WM, WN, S>;
+    using L = TileForm<P, ZEROS, TB, FB, S>;
     constexpr int TM = L::TM, TN = L::TN, bytes = L::kBytes;
-    const auto kernel = &linear_int4_tile_kernel<T, P, ZEROS, TB, FB, WM, WN, S, TURNS>;
+    const auto kernel = &linear_int4_tile_kernel<T, P, ZEROS, TB, FB, S, SIMD, OWN>;
     if constexpr (bytes > 64 * 1024) {
         int device = 0;
         MI_HIP_CHECK(hipGetDevice(&device));
@@ -277,29 +291,32 @@ int launch(const Int4Problem& p, hipStream_t st) {
         }
     }
     const long tiles = static_cast<long>((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), bytes, st, p);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(64 * kWaves), bytes, st, p);
     MI_HIP_CHECK(hipGetLastError());
     return 0;
 }
 
 template <typename T, int P, bool ZEROS>
-int launch_form(const Int4Problem& p, hipStream_t st) {
-    const long big = static_cast<long>((p.M + 127) / 128) * ((p.N + 255) / 256);
-    if (big >= device_cu_count()) return launch<T, P, ZEROS, 4, 4, 2, 4, 3, true>(p, st);      // 128 x 256
-    return launch<T, P, ZEROS, 2, 2, 2, 2, 3, false>(p, st);                                    // 64 x 64
+int launch_form(const Int4Problem& p, int form, hipStream_t st) {
+    switch (form) {
+        case kTile32x64: return launch<T, P, ZEROS, 2, 1, 3, 4, true>(p, st);
+        case kTile32x128: return launch<T, P, ZEROS, 2, 2, 3, 3, true>(p, st);
+        case kTile64x128: return launch<T, P, ZEROS, 4, 2, 2, 2, false>(p, st);
+        default: return launch<T, P, ZEROS, 4, 4, 2, 2, false>(p, st);
+    }
 }
 template <typename T, int P>
-int launch_zeros(const Int4Problem& p, hipStream_t st) { return p.zeros ? launch_form<T, P, true>(p, st) : launch_form<T, P, false>(p, st); }
+int launch_zeros(const Int4Problem& p, int form, hipStream_t st) { return p.zeros ? launch_form<T, P, true>(p, form, st) : launch_form<T, P, false>(p, form, st); }
 template <typename T>
-int launch_parts(const Int4Problem& p, int parts, hipStream_t st) {
-    return parts == 1 ? launch_zeros<T, 1>(p, st) : parts == 2 ? launch_zeros<T, 2>(p, st) : launch_zeros<T, 4>(p, st);
+int launch_parts(const Int4Problem& p, int parts, int form, hipStream_t st) {
+    return parts == 1 ? launch_zeros<T, 1>(p, form, st) : parts == 2 ? launch_zeros<T, 2>(p, form, st) : launch_zeros<T, 4>(p, form, st);
 }
 
 }  // namespace
 }  // namespace gemm
 
-int launch_int4_tile(const Int4Problem& p, int dtype, int parts, hipStream_t st) {
-    return dtype == MI_DTYPE_BF16 ? gemm::launch_parts<__bf16>(p, parts, st) : gemm::launch_parts<_Float16>(p, parts, st);
+int launch_int4_tile(const Int4Problem& p, int dtype, int parts, int form, hipStream_t st) {
+    return dtype == MI_DTYPE_BF16 ? gemm::launch_parts<__bf16>(p, parts, form, st) : gemm::launch_parts<_Float16>(p, parts, form, st);
 }
 
 }  // namespace mi

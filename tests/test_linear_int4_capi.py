@@ -1,11 +1,13 @@
 """The C entries of the linear layer with 4-bit weights without a GPU: struct layouts, sizes, and refusals ahead of any launch (what is passed as a tensor is never read)."""
 import ctypes as C
 import os
+import re
 import subprocess
 
 import pytest
 
 from brodiffusion_amd import _capi as capi
+from brodiffusion_amd import build
 from test_kernel_resources import kernels  # noqa: F401
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -72,3 +74,30 @@ def test_pack_refusals(fields, said):
 
 def test_no_rows_is_no_error():
     assert capi.lib().mi_linear_int4_forward(C.byref(_linear(rows=0, x=None))) == 0
+
+
+def test_instances_are_those_that_calls_reach(kernels):  # noqa: F811
+    """Work groups by the rule (csrc/linear_int4_forms.h), over sizes and kinds of groups, against what is in the library"""
+    if not os.path.exists(build.FORMS_LIB):
+        build.build_host()
+    form = C.CDLL(build.FORMS_LIB).int4_form_test
+    sizes = [(m, n, k) for m in (1, 16, 40, 200, 333, 777, 2049, 3000) for n in (8, 264, 1160, 2056, 4104, 8200) for k in (8, 264, 1160, 2056, 3088, 8200)]
+    reached = {(p, form(m, n, k, C.c_long(k), 128 // p, 256)) for p in (1, 2, 4) for m, n, k in sizes}
+    assert reached == {(p, f) for p in (1, 2, 4) for f in range(7)} - {(4, 2)}
+    few = {(p, 1 << f) for p, f in reached if f < 3}
+    tiles = {(p, z, *((2, 1), (2, 2), (4, 2), (4, 4))[f - 3]) for p, f in reached if f >= 3 for z in (0, 1)}
+    for t in ("DF16_", "DF16b"):
+        assert {tuple(map(int, m.groups())) for name in kernels if (m := re.search(rf"linear_int4_few_kernelI{t}Li(\d+)ELi(\d+)E", name))} == few
+        assert {tuple(map(int, m.groups())) for name in kernels if (m := re.search(rf"linear_int4_tile_kernelI{t}Li(\d+)ELb(\d)ELi(\d+)ELi(\d+)E", name))} == tiles
+
+
+def test_rows_far_apart_and_many_features_get_64_bit_offsets():
+    form = C.CDLL(build.FORMS_LIB).int4_form_test
+    for m in (70, 5000):
+        assert form(m, 1160, 136, C.c_long(1 << 24), 64, 256) < 3 and form(m, (1 << 24) + 8, 136, C.c_long(136), 64, 256) < 3
+        assert form(5000, 1160, 136, C.c_long((1 << 24) - 8), 64, 256) >= 3
+
+
+def test_no_scratch_memory(kernels):  # noqa: F811
+    found = {name: (k[".private_segment_fixed_size"], k[".vgpr_spill_count"]) for name, k in kernels.items() if "linear_int4_" in name or "pack_int4" in name}
+    assert len(found) > 60 and not {name: use for name, use in found.items() if use != (0, 0)}

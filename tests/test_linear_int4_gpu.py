@@ -6,12 +6,14 @@ Tolerance: a group's sum has exact products (4 + 11 bits) and starts at -z sum(x
 elements of a group in a block. Groups, parts of a contraction (8) and bias meet by additions that round to 2^-24 of at most B = sum |q - z| s |x| + |bias|, three
 roundings each. The activations (slopes up to 1.13) are within 2e-5 of their value. The result is rounded to the type once: half a step. Beside that bound, which adds up
 magnitudes, the whole result is held to half a step in its norm: what a rounding of exact values gives is 0.58 of that at most."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 import brodiffusion_amd as bd
+from brodiffusion_amd import build
 from helpers import TORCH_DT
 
 pytestmark = pytest.mark.gpu
@@ -92,6 +94,26 @@ def test_sizes(dtype, m, k, n, group, zeros):
 @pytest.mark.parametrize("m,k,n", [(1, 1152, 16392), (16, 2056, 8200), (20, 1160, 16384), (40, 520, 16392), (1031, 520, 8200), (4608, 264, 2056), (300, 136, 33032)])
 def test_wide_and_long(dtype, m, k, n, group, zeros):
     _case(dtype, m, k, n, group, zeros, bias=True, act="gelu_tanh", residual=True)
+
+
+FEW16, FEW32, FEW64, TILE32x64, TILE32x128, TILE64x128, TILE64x256 = range(7)
+FORMS = {128: {FEW16: (5, 136, 520), FEW32: (17, 264, 2056), FEW64: (40, 520, 4104), TILE32x64: (64, 136, 4104), TILE32x128: (200, 1160, 8200), TILE64x128: (2049, 264, 4104), TILE64x256: (3000, 520, 2056)},
+         64: {FEW16: (1, 264, 264), FEW32: (17, 264, 2056), FEW64: (40, 520, 4104), TILE32x64: (500, 136, 520), TILE32x128: (333, 264, 16392), TILE64x128: (777, 136, 16392), TILE64x256: (3000, 3088, 2056)},
+         32: {FEW16: (1, 264, 264), FEW32: (40, 136, 2056), TILE32x64: (16, 136, 8200), TILE32x128: (333, 1160, 8200), TILE64x128: (2049, 264, 8200), TILE64x256: (3000, 1160, 2056)}}
+
+
+def _form(m, k, n, group, row=0):
+    return C.CDLL(build.FORMS_LIB).int4_form_test(m, n, k, C.c_long(row or k), group, bd.device_info()["compute_units"])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group,form", [(g, f) for g in FORMS for f in FORMS[g]])
+def test_every_form(dtype, zeros, group, form):
+    """Every kernel instance, on problems that end inside its work groups, its steps and their groups"""
+    m, k, n = FORMS[group][form]
+    assert _form(m, k, n, group) == form
+    _case(dtype, m, k, n, group, zeros, bias=True, act="silu", residual=True)
 
 
 @pytest.mark.parametrize("m", [1, 20, 40, 100, 1031])
