@@ -7,7 +7,10 @@
 // RMS: v / sqrt(mean v^2 + eps); layer: (v - mean) / sqrt(mean (v - mean)^2 + eps), the squares summed of the differences, in registers, not as a difference of
 // sums. gate, scale and shift are vectors of all rows or one for each run of rows (an image of a batch, a token).
 //
-// Bound: HBM. x and the branch are read once, h and y written once, the row stays in registers between its sums.
+// Bound: HBM. x and the branch are read once, h and y written once, the row stays in registers between its sums. The vectors come from the caches, which
+// they have to themselves: the rows of x, of the branch and of h are marked as passing through. y, which the next product reads, is not: with it 4608 rows of 6144
+// are 0.7 us faster, a block's norm, two products and norm 19 slower. Measured (us, gate, scale and shift, operands of 1 GiB in turn; without the marks): 4608 rows of 6144
+// 44.6 = 5.1 TB/s, a large copy's rate (51.6), 4608 of 2240 20.9 (24.0), 16384 of 1152 33.4 (38.0), 1000 of 6144 14.3 (16.4), one of 6144 4.4.
 #include "rows_checks.h"
 
 namespace mi {
@@ -30,13 +33,14 @@ struct GateNorm {
     float alpha, post_eps, eps;
 };
 
-// W wavefronts per row (one: four rows to a work group), N 16-byte chunks per lane, as in rows_int8.hip.
+// W wavefronts per row (one: four rows to a work group), N 16-byte chunks per lane, as in rows_int8.hip. (Work groups that stay, with the vectors in registers from row
+// to row and the next row on its way: 46 to 49 us instead of 44.6, their registers leave three wavefronts a SIMD.)
 template <typename T, int N, int W>
 __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) gate_norm_kernel(const GateNorm a) {
     typedef T t8 __attribute__((ext_vector_type(8)));
     constexpr int LANES = 64 * W;
-    // (sixteen wavefronts have 128 registers: the vectors of all chunks at once would put some of them into memory)
-    constexpr bool TIGHT = W == 16 && N >= 4;
+    // (a chunk at a time where a lane has several: the FP32 values of all would cost wavefronts, of sixteen with 128 registers some would go to memory)
+    constexpr bool TIGHT = N >= 2;
     __shared__ float red[2][4][W];                // [parity of the row][sum of it]: a slot is written again two rows on, a barrier after its last reader
     const int cpr = a.cols / 8;
     int lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -49,6 +53,12 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) gate_norm_kernel(const 
         const char* const base = reinterpret_cast<const char*>(static_cast<const T*>(p) + row);
         return [=](unsigned byte) { return __builtin_bit_cast(t8, *reinterpret_cast<const u32x4*>(base + byte)); };
     };
+    // what passes through once: x, the branch, h (which is read again behind a block's products)
+    auto load_once = [&](const void* p, long row) {
+        const char* const base = reinterpret_cast<const char*>(static_cast<const T*>(p) + row);
+        return [=](unsigned byte) { return __builtin_bit_cast(t8, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + byte))); };
+    };
+    auto store_once = [&](void* p, long row, int i, u32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(reinterpret_cast<char*>(static_cast<T*>(p) + row) + at(i))); };
     // (a chunk is made FP32 anew for each pass over the row: kept, its 8 values would hold twice the registers)
     auto anew = [](t8 (&v)[N]) {
 #pragma unroll
@@ -106,10 +116,26 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) gate_norm_kernel(const 
             inv = inverse_root(total(s) / static_cast<float>(a.cols) + eps);
             anew(row);
         };
-        auto vectors = [&](const RowVectors& v) { return load(v.p, r / v.each * v.rs); };
+        auto vectors = [&](const RowVectors& v) { return load(v.p, (v.each == a.rows ? 0u : static_cast<unsigned>(r) / static_cast<unsigned>(v.each)) * v.rs); };
 
+        // The vectors wait in registers for the sums, but of a lane with more than 3 chunks; there they are read behind the sums, from the L2, a latency that every
+        // row then waits for.
+        constexpr bool KEEP = N <= 3;
+        const auto pg_at = load(a.post_gain, 0), gate_at = vectors(a.gate), gain_at = load(a.gain, 0), scale_at = vectors(a.scale), shift_at = vectors(a.shift);
+        t8 pg[KEEP ? N : 1], gate[KEEP ? N : 1], gain[KEEP ? N : 1], scale[KEEP ? N : 1], shift[KEEP ? N : 1];
+        auto keep = [&](t8* to, const void* p, auto from) {
+            // (defined where there is none too: left undefined they cost 36 registers more)
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) to[i] = p != nullptr ? from(at(i)) : t8{};
+            }
+        };
+        auto kept = [&](const t8* v, auto from, int i) {
+            if constexpr (KEEP) return v[i];
+            else return from(at(i));
+        };
         t8 h[N];
-        const auto x_at = load(a.x, r * a.x_rs);
+        const auto x_at = load_once(a.x, r * a.x_rs);
         constexpr bool LATE = N == 8;                 // (x behind the branch's sums: both together leave no registers for them)
         if (!LATE || a.branch == nullptr) {
 #pragma unroll
@@ -117,9 +143,11 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) gate_norm_kernel(const 
         }
         if (a.branch != nullptr) {
             t8 b[N];
-            const auto b_at = load(a.branch, r * a.b_rs), pg_at = load(a.post_gain, 0), gate_at = vectors(a.gate);
+            const auto b_at = load_once(a.branch, r * a.b_rs);
 #pragma unroll
             for (int i = 0; i < N; ++i) b[i] = b_at(at(i));
+            keep(pg, a.post_gain, pg_at);
+            keep(gate, a.gate.p, gate_at);
             float mean = 0.f, inv = 1.f;
             if (a.post != MI_NORM_NONE) statistics(b, a.post, a.post_eps, mean, inv);
 #pragma unroll
@@ -129,42 +157,45 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) gate_norm_kernel(const 
                 for (int e = 0; e < 8; ++e) f[e] = (static_cast<float>(b[i][e]) - mean) * inv;
                 if constexpr (LATE) h[i] = x_at(at(i));
                 if (a.post_gain != nullptr) {
-                    const t8 g = pg_at(at(i));
+                    const t8 g = kept(pg, pg_at, i);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] *= static_cast<float>(g[e]);
                 }
                 if (a.gate.p != nullptr) {
-                    const t8 g = gate_at(at(i));
+                    const t8 g = kept(gate, gate_at, i);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] *= static_cast<float>(g[e]);
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[i][e] = static_cast<T>(__builtin_fmaf(a.alpha, static_cast<float>(h[i][e]), f[e]));
-                if (a.sum != nullptr && mine(i)) store(a.sum, r * a.s_rs, i, __builtin_bit_cast(u32x4, h[i]));
+                if (a.sum != nullptr && mine(i)) store_once(a.sum, r * a.s_rs, i, __builtin_bit_cast(u32x4, h[i]));
                 if constexpr (TIGHT) asm volatile("" ::: "memory");
             }
         }
         if (a.out == nullptr) continue;
+        asm volatile("" ::: "memory");                // (not earlier: all vectors at once would cost wavefronts)
+        keep(gain, a.gain, gain_at);
+        keep(scale, a.scale.p, scale_at);
+        keep(shift, a.shift.p, shift_at);
         float mean, inv;
         statistics(h, a.pre, a.eps, mean, inv);
-        const auto gain_at = load(a.gain, 0), scale_at = vectors(a.scale), shift_at = vectors(a.shift);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = (static_cast<float>(h[i][e]) - mean) * inv;
             if (a.gain != nullptr) {
-                const t8 g = gain_at(at(i));
+                const t8 g = kept(gain, gain_at, i);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] *= static_cast<float>(g[e]);
             }
             if (a.scale.p != nullptr) {
-                const t8 g = scale_at(at(i));
+                const t8 g = kept(scale, scale_at, i);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] *= 1.f + static_cast<float>(g[e]);
             }
             if (a.shift.p != nullptr) {
-                const t8 g = shift_at(at(i));
+                const t8 g = kept(shift, shift_at, i);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] += static_cast<float>(g[e]);
             }
