@@ -31,7 +31,7 @@ EXPORTS = [
     "mi_malloc", "mi_free", "mi_memcpy_h2d", "mi_memcpy_d2h", "mi_memcpy_d2d_async", "mi_memset_async",
     "mi_sdpa_forward", "mi_sdpa_split_scratch_bytes", "mi_sdpa_supported", "mi_sdpa_set_kernel_choice", "mi_attention_map_avg", "mi_rope_apply", "mi_headnorm_rope", "mi_scale_rows",
     "mi_linear_attn_workspace_bytes", "mi_linear_attn_scratch_bytes", "mi_linear_attn_relu_forward", "mi_linear_attn_supported", "mi_linear_attn_relu_forward_static_scratch",
-    "mi_linear_forward", "mi_linear_forward_n", "mi_linear_geglu_forward", "mi_add_inplace", "mi_add_row_bias", "mi_rms_norm_forward", "mi_rms_norm_pair_forward", "mi_add_rms_norm_forward", "mi_quantize_rows_forward", "mi_gate_add_norm_forward", "mi_linear_act_forward", "mi_linear_act_scratch_bytes", "mi_int4_packed_bytes", "mi_pack_int4", "mi_linear_int4_forward", "mi_flash_attention_scratch_bytes", "mi_attn_block_scratch_bytes", "mi_flash_attention_qkvo_forward",
+    "mi_linear_forward", "mi_linear_forward_n", "mi_linear_geglu_forward", "mi_add_inplace", "mi_add_row_bias", "mi_rms_norm_forward", "mi_rms_norm_pair_forward", "mi_add_rms_norm_forward", "mi_quantize_rows_forward", "mi_gate_add_norm_forward", "mi_linear_act_forward", "mi_linear_act_scratch_bytes", "mi_int4_packed_bytes", "mi_pack_int4", "mi_linear_int4_forward", "mi_linear_int4_scratch_bytes", "mi_flash_attention_scratch_bytes", "mi_attn_block_scratch_bytes", "mi_flash_attention_qkvo_forward",
     "mi_flash_attention_q_with_kv_cached_forward", "mi_flash_attention_project_kv",
 ]
 
@@ -198,7 +198,7 @@ class MiLinearInt4Args(C.Structure):
         ("struct_size", C.c_uint32), ("dtype", C.c_int32),
         ("x", C.c_void_p), ("w", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
         ("rows", C.c_int32), ("in_features", C.c_int32), ("out_features", C.c_int32), ("group", C.c_int32),
-        ("x_row_stride", C.c_int64), ("residual_row_stride", C.c_int64), ("y_row_stride", C.c_int64), ("activation", C.c_int32), ("stream", C.c_void_p),
+        ("x_row_stride", C.c_int64), ("residual_row_stride", C.c_int64), ("y_row_stride", C.c_int64), ("activation", C.c_int32), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t), ("stream", C.c_void_p),
     ]
 
 
@@ -279,6 +279,8 @@ def lib() -> C.CDLL:
         L.mi_int4_packed_bytes.restype = C.c_size_t
         L.mi_pack_int4.argtypes = [C.POINTER(MiPackInt4Args)]
         L.mi_linear_int4_forward.argtypes = [C.POINTER(MiLinearInt4Args)]
+        L.mi_linear_int4_scratch_bytes.argtypes = [C.POINTER(MiLinearInt4Args)]
+        L.mi_linear_int4_scratch_bytes.restype = C.c_size_t
         L.mi_flash_attention_scratch_bytes.argtypes = [C.c_int32] * 5
         L.mi_flash_attention_scratch_bytes.restype = C.c_size_t
         L.mi_attn_block_scratch_bytes.argtypes = [C.POINTER(MiAttnBlockArgs)]

@@ -24,7 +24,11 @@ struct Int4Problem {
     int KB, groups, span;          // blocks of 128 contraction elements, groups, blocks that share a group (groups of 128 and more)
     long ldx, ldy, ldr;            // elements
     int act;                       // MI_ACT_*
+    float* parts;                  // null, or (shares, M, N): the contraction in shares, whose sums go here
+    int shares;
 };
+// the blocks of a share of the contraction
+__device__ __forceinline__ int int4_share(const Int4Problem& p, int share) { return static_cast<int>(static_cast<long>(share) * p.KB / p.shares); }
 // scale groups in a block: 4, 2, 1 (of 32, 64, 128 and more elements)
 inline int int4_parts(int group) { return group >= 128 ? 1 : 128 / group; }
 

@@ -21,6 +21,40 @@ __global__ void __launch_bounds__(256) pack_int4_kernel(const unsigned char* q, 
     }
 }
 
+// The sums of the shares of a contraction, added in their order, and what follows them: 4 features per thread
+template <typename T>
+__global__ void __launch_bounds__(256) join_int4_kernel(const Int4Problem p) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const int quads = p.N / 4;
+    const long all = static_cast<long>(p.M) * quads;
+    for (long i = blockIdx.x * 256L + threadIdx.x; i < all; i += gridDim.x * 256L) {
+        const long m = i / quads;
+        const int f = static_cast<int>(i - m * quads) * 4;
+        const float* at = p.parts + 4 * i;
+        gemm::f32x4 v = *reinterpret_cast<const gemm::f32x4*>(at);
+#pragma unroll 4
+        for (int s = 1; s < p.shares; ++s) v += *reinterpret_cast<const gemm::f32x4*>(at + s * 4 * all);
+        if (p.bias) {
+            const t4 b = *reinterpret_cast<const t4*>(static_cast<const T*>(p.bias) + f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += static_cast<float>(b[e]);
+        }
+        gemm::with_activation(p.act, [&](auto act) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = act(v[e]);
+        });
+        if (p.residual) {
+            const t4 r = *reinterpret_cast<const t4*>(static_cast<const T*>(p.residual) + m * p.ldr + f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += static_cast<float>(r[e]);
+        }
+        t4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(v[e]);
+        *reinterpret_cast<t4*>(static_cast<T*>(p.y) + m * p.ldy + f) = o;
+    }
+}
+
 long packed_bytes(long n, long k) { return (n + 15) / 16 * ((k + 127) / 128) * 1024; }
 
 // Features and contraction of a call
@@ -67,6 +101,21 @@ int problem_of(const mi_linear_int4_args& a, const char* op, Int4Problem& p) {
     return 1;
 }
 
+// Lent memory is none of the operands'
+int check_scratch(const Int4Problem& p, const char* op, const void* scratch, size_t bytes) {
+    if (!scratch || bytes == 0) return 0;
+    const long run = static_cast<long>(bytes < (1ul << 60) ? bytes : 1ul << 60), per_group = static_cast<long>(p.groups) * p.N, rows = p.M - 1;
+    const struct { const char* name; const void* first; long len; } operands[] = {
+        {"x", p.x, 2 * (rows * p.ldx + p.K)}, {"w", p.w, packed_bytes(p.N, p.K)}, {"scales", p.scales, 2 * per_group}, {"zeros", p.zeros, per_group}, {"bias", p.bias, 2L * p.N},
+        {"residual", p.residual, 2 * (rows * p.ldr + p.N)}, {"y", p.y, 2 * (rows * p.ldy + p.N)}};
+    for (const auto& o : operands)
+        if (runs_share(scratch, run, o.first, o.len)) return fail("%s: scratch overlaps %s", op, o.name);
+    return 0;
+}
+
+Int4Launch launch_of(const Int4Problem& p, int group, size_t lent) { return int4_launch(p.M, p.N, p.KB, p.ldx, int4_parts(group), device_cu_count(), lent); }
+size_t parts_bytes(const Int4Problem& p, int shares) { return shares > 1 ? sizeof(float) * static_cast<size_t>(shares) * p.M * p.N : 0; }
+
 }  // namespace
 }  // namespace mi
 
@@ -102,13 +151,30 @@ int mi_linear_int4_forward(const mi_linear_int4_args* a) {
     mi::clear_error();
     if (!a) return mi::fail("%s: null args", op);
     if (a->struct_size != sizeof(*a)) return mi::fail("%s: struct_size %u != %zu (header mismatch)", op, a->struct_size, sizeof(*a));
+    if (reinterpret_cast<uintptr_t>(a->scratch) & 15u) return mi::fail("%s: scratch must be 16-byte aligned", op);
     mi::Int4Problem p{};
     const int rc = mi::problem_of(*a, op, p);
     if (rc <= 0) return rc;
+    if (mi::check_scratch(p, op, a->scratch, a->scratch_bytes)) return -1;
     const int parts = mi::int4_parts(a->group);
-    const int form = mi::int4_form(p.M, p.N, p.KB, p.ldx, parts, mi::device_cu_count());
+    const mi::Int4Launch launch = mi::launch_of(p, a->group, a->scratch ? a->scratch_bytes : 0);
+    p.shares = launch.shares;
+    p.parts = launch.shares > 1 ? static_cast<float*>(a->scratch) : nullptr;
     const hipStream_t st = mi::resolve_stream(a->stream);
-    return form < mi::kTile32x64 ? mi::launch_int4_few(p, a->dtype, parts, form, st) : mi::launch_int4_tile(p, a->dtype, parts, form, st);
+    if (launch.form < mi::kTile32x64 ? mi::launch_int4_few(p, a->dtype, parts, launch.form, st) : mi::launch_int4_tile(p, a->dtype, parts, launch.form, st)) return -1;
+    if (launch.shares == 1) return 0;
+    const long groups = (static_cast<long>(p.M) * (p.N / 4) + 255) / 256;
+    const dim3 grid(static_cast<unsigned>(groups < (1L << 20) ? groups : 1L << 20));
+    if (a->dtype == MI_DTYPE_BF16) hipLaunchKernelGGL(mi::join_int4_kernel<__bf16>, grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(mi::join_int4_kernel<_Float16>, grid, dim3(256), 0, st, p);
+    MI_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+size_t mi_linear_int4_scratch_bytes(const mi_linear_int4_args* a) {
+    mi::Int4Problem p{};
+    if (!a || a->struct_size != sizeof(*a) || mi::problem_of(*a, "mi_linear_int4_scratch_bytes", p) != 1) return 0;
+    return mi::parts_bytes(p, mi::launch_of(p, a->group, ~static_cast<size_t>(0)).shares);
 }
 
 }  // extern "C"

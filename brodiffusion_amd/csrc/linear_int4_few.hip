@@ -106,19 +106,20 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
         }
     };
 
-    if (wave < p.KB) {
+    const int share = static_cast<int>(blockIdx.z), end = int4_share(p, share + 1);
+    int i = int4_share(p, share) + wave;
+    if (i < end) {
         Block c[2];
-        load(c[0], wave);
-        int i = wave;
-        for (; i + WAVES < p.KB; i += 2 * WAVES) {
+        load(c[0], i);
+        for (; i + WAVES < end; i += 2 * WAVES) {
             stage(c[0]);
             load(c[1], i + WAVES);
             multiply(c[0]);
             stage(c[1]);
-            if (i + 2 * WAVES < p.KB) load(c[0], i + 2 * WAVES);
+            if (i + 2 * WAVES < end) load(c[0], i + 2 * WAVES);
             multiply(c[1]);
         }
-        if (i < p.KB) {
+        if (i < end) {
             stage(c[0]);
             multiply(c[0]);
         }
@@ -136,6 +137,10 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) v += sums[(w * FB + f / 16) * 256 + row * 16 + f % 16];
+        if (p.parts) {
+            p.parts[(static_cast<long>(share) * p.M + m0 + row) * p.N + n0 + f] = v;
+            continue;
+        }
         if (p.bias) v += static_cast<float>(static_cast<const T*>(p.bias)[n0 + f]);
         with_activation(p.act, [&](auto act) { v = act(v); });
         if (p.residual) v += static_cast<float>(static_cast<const T*>(p.residual)[static_cast<long>(m0 + row) * p.ldr + n0 + f]);
@@ -145,7 +150,7 @@ __global__ void __launch_bounds__(64 * WAVES) linear_int4_few_kernel(const Int4P
 
 template <typename T, int P, int FB>
 int launch(const Int4Problem& p, hipStream_t st) {
-    hipLaunchKernelGGL((linear_int4_few_kernel<T, P, FB>), dim3((p.N + 16 * FB - 1) / (16 * FB), (p.M + 15) / 16), dim3(64 * WAVES), 0, st, p);
+    hipLaunchKernelGGL((linear_int4_few_kernel<T, P, FB>), dim3((p.N + 16 * FB - 1) / (16 * FB), (p.M + 15) / 16, p.shares), dim3(64 * WAVES), 0, st, p);
     MI_HIP_CHECK(hipGetLastError());
     return 0;
 }

@@ -98,10 +98,11 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
     // LDS between two barriers is another stage, and the barriers have one)
     auto dma16 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst)); };
     auto dma4 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "{m0}"(dst)); };
-    int filling = 0, group = 0, of_group = 0;           // the stage that the next request fills; its group, of blocks and more, and which block of it
+    const int share = static_cast<int>(blockIdx.y), begin = int4_share(p, share), end = int4_share(p, share + 1);
+    int filling = 0, group = P == 1 ? begin / p.span : 0, of_group = P == 1 ? begin % p.span : 0;      // the stage that the next request fills; its group, of blocks and more, and which block of it
     // requests FROM .. TO - 1 of a step's L::NI
     auto request = [&]<int FROM, int TO>(int step, std::integer_sequence<int, FROM, TO>) {
-        const int kb = min(step, p.KB - 1);             // (past the end the last step again, into a stage that nobody reads: the wait counts instructions)
+        const int kb = min(step, end - 1);              // (past the end the last step again, into a stage that nobody reads: the wait counts instructions)
         const unsigned at = lds_base + filling * L::kStage;
         const int most = kb == p.KB - 1 ? left - 1 : 15;      // (pieces past the end: the last one, left out of the products)
         const int g0 = P == 1 ? min(group, p.groups - 1) : kb * P, most_g = p.groups - 1 - g0;
@@ -135,9 +136,9 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
         for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) request(i, std::integer_sequence<int, 0, L::NI>{});
+    for (int i = 0; i < S - 1; ++i) request(begin + i, std::integer_sequence<int, 0, L::NI>{});
     int reading = 0;
-    for (int kb = 0; kb < p.KB; ++kb) {
+    for (int kb = begin; kb < end; ++kb) {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((S - 2) * L::NI) : "memory");
         unsigned char* const stage = lds + reading * L::kStage;
         reading = reading + 1 == S ? 0 : reading + 1;
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const V8*>(at + (((4 * j + lg) ^ lr) << 4));
         };
-        if (kb == p.KB - 1 && left < 16) {              // zeros behind the end of the rows: every wavefront those of the tokens that it sums
+        if (__builtin_expect(kb == p.KB - 1 && left < 16, 0)) {      // zeros behind the end of the rows: every wavefront those of the tokens that it sums
 #pragma unroll
             for (int i = 0; i < ceil_div(TM / 16, NW); ++i) {
                 const int b = i * NW + wave;
@@ -179,7 +180,8 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[a][j] = nibbles<T>(packed[j]);
         }
-        // scales and zero points of a wavefront's features wait in registers; where they would be 32 a lane and more they are read again for each 16 tokens
+        // scales and zero points of a wavefront's features wait in registers; where they would be 32 a lane and more they are read again for each 16 tokens,
+        // one group at a time (the scheduling barrier: gathered ahead they do not fit the 256 registers)
         constexpr bool AGAIN = P * FB >= 8;
         float scale[FB][P][4];
         unsigned zero[FB][P];
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
         auto fetch = [&](int b) {
             tokens(x[b & 1], b);
 #pragma unroll
-            for (int g = 0; g < (OWN ? 0 : P); ++g) sx[b & 1][g] = sums[g * TM + 16 * b + lr];
+            for (int g = 0; g < (OWN || AGAIN ? 0 : P); ++g) sx[b & 1][g] = sums[g * TM + 16 * b + lr];
         };
         fetch(0);
         [&]<int... B>(std::integer_sequence<int, B...>) {
@@ -214,8 +216,10 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
 #pragma unroll
                 for (int g = 0; g < P; ++g) {
                     if constexpr (AGAIN) {
+                        __builtin_amdgcn_sched_barrier(0);
                         asm volatile("" ::: "memory");
                         factors(g);
+                        if constexpr (!OWN) sx[b & 1][g] = sums[g * TM + 16 * b + lr];
                     }
                     f32x4 t[FB];
 #pragma unroll
@@ -244,6 +248,17 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (no DMA into LDS that is given back)
 
+    if (p.parts) {
+        float* const to = p.parts + static_cast<long>(share) * p.M * p.N;
+#pragma unroll
+        for (int a = 0; a < FB; ++a)
+#pragma unroll
+            for (int b = 0; b < TB; ++b) {
+                const int f = n0 + (wave * FB + a) * 16 + 4 * lg, m = m0 + 16 * b + lr;
+                if (f < p.N && m < p.M) *reinterpret_cast<f32x4*>(to + static_cast<long>(m) * p.N + f) = acc[a][b];
+            }
+        return;
+    }
 #pragma unroll
     for (int a = 0; a < FB; ++a) {
         const int f = n0 + (wave * FB + a) * 16 + 4 * lg;
@@ -291,7 +306,7 @@ int launch(const Int4Problem& p, hipStream_t st) {
         }
     }
     const long tiles = static_cast<long>((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)), dim3(64 * kWaves), bytes, st, p);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((tiles + 7) / 8 * 8), p.shares), dim3(64 * kWaves), bytes, st, p);
     MI_HIP_CHECK(hipGetLastError());
     return 0;
 }

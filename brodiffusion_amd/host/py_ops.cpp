@@ -46,6 +46,7 @@ struct Lib {
     decltype(&mi_gate_add_norm_forward) gate_add_norm;
     decltype(&mi_int4_packed_bytes) int4_packed_bytes;
     decltype(&mi_linear_int4_forward) linear_int4;
+    decltype(&mi_linear_int4_scratch_bytes) linear_int4_scratch_bytes;
     decltype(&mi_linear_act_forward) linear_act;
     decltype(&mi_linear_act_scratch_bytes) linear_act_scratch_bytes;
     decltype(&mi_attn_block_scratch_bytes) block_scratch_bytes;
@@ -482,7 +483,7 @@ NATIVE_END
 
 // X, packed, scales, zeros, out_features, in_features, group, bias, activation, residual, out
 NATIVE(linear_int4, 11)
-    need(L.linear_int4 != nullptr && L.int4_packed_bytes != nullptr);
+    need(L.linear_int4 != nullptr && L.int4_packed_bytes != nullptr && L.linear_int4_scratch_bytes != nullptr);
     const Tensor &x = tensor(a[0]), &w = tensor(a[1]), &s = tensor(a[2]);
     mi_linear_int4_args p;
     std::memset(&p, 0, sizeof(p));
@@ -512,6 +513,11 @@ NATIVE(linear_int4, 11)
     }
     p.x = x.data_ptr(); p.w = w.data_ptr(); p.y = y.data_ptr();
     p.stream = current_stream();
+    Tensor scratch;      // (as in linear_act)
+    if (const size_t bytes = L.linear_int4_scratch_bytes(&p)) {
+        scratch = at::empty({static_cast<int64_t>(bytes)}, y.options().dtype(at::kByte));
+        p.scratch = scratch.data_ptr(); p.scratch_bytes = bytes;
+    }
     run("linear_int4", [&] { return L.linear_int4(&p); });
     return given(a[10], y);
 NATIVE_END
@@ -912,7 +918,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     // (a library without these binds all the same: their calls decline, and the Python code says what is missing)
     get(L.add_rms_norm, "mi_add_rms_norm_forward"); get(L.quantize_rows, "mi_quantize_rows_forward"); get(L.linear_act, "mi_linear_act_forward");
     get(L.linear_act_scratch_bytes, "mi_linear_act_scratch_bytes"); get(L.gate_add_norm, "mi_gate_add_norm_forward");
-    get(L.int4_packed_bytes, "mi_int4_packed_bytes"); get(L.linear_int4, "mi_linear_int4_forward");
+    get(L.int4_packed_bytes, "mi_int4_packed_bytes"); get(L.linear_int4, "mi_linear_int4_forward"); get(L.linear_int4_scratch_bytes, "mi_linear_int4_scratch_bytes");
     Py_INCREF(lend);
     Py_XSETREF(lend_scratch, lend);
     bound = true;

@@ -1435,6 +1435,11 @@ def linear_int4(X, W: Int4Weight, bias=None, *, activation: str = "none", residu
     a.zeros = None if W.zeros is None else W.zeros.data_ptr()
     a.activation = _ACTIVATIONS[activation]
     a.stream = _stream()
+    # (from the allocator, per call, as in linear_act)
+    need = int(capi.lib().mi_linear_int4_scratch_bytes(C.byref(a)))
+    if need > 0:
+        scratch = torch.empty(need, dtype=torch.uint8, device=X.device)
+        a.scratch, a.scratch_bytes = scratch.data_ptr(), need
     capi.check(capi.lib().mi_linear_int4_forward(C.byref(a)), op)
     return out
 

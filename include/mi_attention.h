@@ -562,8 +562,9 @@ MI_API size_t mi_linear_act_scratch_bytes(const mi_linear_act_args* args);
 /* ── linear layer with 4-bit weights ───────────────────────────────────────
  * Y = act(X W^T + bias) + residual with W[n][k] = (q[n][k] - zeros[g][n]) * scales[g][n], g = k / group: 4-bit integers q of 0 .. 15 with a scale, and where
  * there are zeros a zero point (else 8), for each group of the contraction. Weights are not rounded to 16 bits: a group's product is summed in FP32 and meets its
- * scale there; bias, activation and residual follow in FP32, one rounding to `dtype`. A row of x with a value that is not finite gives NaN. Results do not
- * depend on timing. From one row to thousands.
+ * scale there; bias, activation and residual follow in FP32, one rounding to `dtype`. A row of x with a value that is not finite gives NaN. No result
+ * depends on timing or on what the other rows of its call hold; FP32 sums round in the order that sizes, type and the scratch that is lent lead to. From one row to
+ * thousands.
  *
  * mi_pack_int4 lays weights out once for that. q: (out_features, in_features / 2) bytes, element 2 j of a row in the low half of byte j, element 2 j + 1
  * in the high half; packed: mi_int4_packed_bytes(out_features, in_features) bytes of device memory, an order of its own (about half a byte for each weight:
@@ -596,9 +597,15 @@ typedef struct mi_linear_int4_args {
     int32_t rows, in_features, out_features, group;
     int64_t x_row_stride, residual_row_stride, y_row_stride;
     int32_t activation;      /* MI_ACT_* */
+    void* scratch;           /* device, 16-byte aligned, or NULL: with mi_linear_int4_scratch_bytes(args) bytes a launch of few work groups and a long contraction
+                                gives each share of the contraction work groups of its own, whose sums a second small launch adds in a fixed order; with less the call
+                                does without, or with fewer. As that of mi_linear_act_args: not shared by calls that can overlap on the GPU, no operand's memory */
+    size_t scratch_bytes;
     void* stream;
 } mi_linear_int4_args;
 MI_API int mi_linear_int4_forward(const mi_linear_int4_args* args);
+/* Bytes of scratch that this call would use (the scratch fields are ignored): 0 where it would not, or is one that is refused. */
+MI_API size_t mi_linear_int4_scratch_bytes(const mi_linear_int4_args* args);
 
 /* ── attention with its projections ────────────────────────────────────────
  * The three operators the U-Net spatial transformer calls (src/unet_blocks.cpp:255-327,

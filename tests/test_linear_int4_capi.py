@@ -76,13 +76,17 @@ def test_no_rows_is_no_error():
     assert capi.lib().mi_linear_int4_forward(C.byref(_linear(rows=0, x=None))) == 0
 
 
-def test_instances_are_those_that_calls_reach(kernels):  # noqa: F811
-    """Work groups by the rule (csrc/linear_int4_forms.h), over sizes and kinds of groups, against what is in the library"""
+def _launch(m, n, k, group, row=0, lent=(1 << 64) - 1):
     if not os.path.exists(build.FORMS_LIB):
         build.build_host()
-    form = C.CDLL(build.FORMS_LIB).int4_form_test
+    shares = C.c_int()
+    return C.CDLL(build.FORMS_LIB).int4_form_test(m, n, k, C.c_long(row or k), group, 256, C.c_ulong(lent), C.byref(shares)), shares.value
+
+
+def test_instances_are_those_that_calls_reach(kernels):  # noqa: F811
+    """Work groups by the rule (csrc/linear_int4_forms.h), over sizes and kinds of groups, against what is in the library"""
     sizes = [(m, n, k) for m in (1, 16, 40, 200, 333, 777, 2049, 3000) for n in (8, 264, 1160, 2056, 4104, 8200) for k in (8, 264, 1160, 2056, 3088, 8200)]
-    reached = {(p, form(m, n, k, C.c_long(k), 128 // p, 256)) for p in (1, 2, 4) for m, n, k in sizes}
+    reached = {(p, _launch(m, n, k, 128 // p)[0]) for p in (1, 2, 4) for m, n, k in sizes}
     assert reached == {(p, f) for p in (1, 2, 4) for f in range(7)} - {(4, 2)}
     few = {(p, 1 << f) for p, f in reached if f < 3}
     tiles = {(p, z, *((2, 1), (2, 2), (4, 2), (4, 4))[f - 3]) for p, f in reached if f >= 3 for z in (0, 1)}
@@ -92,10 +96,41 @@ def test_instances_are_those_that_calls_reach(kernels):  # noqa: F811
 
 
 def test_rows_far_apart_and_many_features_get_64_bit_offsets():
-    form = C.CDLL(build.FORMS_LIB).int4_form_test
     for m in (70, 5000):
-        assert form(m, 1160, 136, C.c_long(1 << 24), 64, 256) < 3 and form(m, (1 << 24) + 8, 136, C.c_long(136), 64, 256) < 3
-        assert form(5000, 1160, 136, C.c_long((1 << 24) - 8), 64, 256) >= 3
+        assert _launch(m, 1160, 136, 64, 1 << 24)[0] < 3 and _launch(m, (1 << 24) + 8, 136, 64)[0] < 3
+        assert _launch(5000, 1160, 136, 64, (1 << 24) - 8)[0] >= 3
+
+
+def test_shares_of_the_contraction():
+    """No more than are lent, none of less than four blocks, none where nothing is lent; sizes whose sums pass 64 bits"""
+    for m, n, k in [(1, 264, 16392), (17, 8200, 8200), (200, 1160, 16384), (333, 2056, 4616), (1, 8, 8)]:
+        shares = _launch(m, n, k, 128)[1]
+        assert 1 <= shares <= 16 and -(-k // 128) >= 4 * shares or shares == 1
+        for lent in (0, 1, 4 * m * n, 8 * m * n - 1, 8 * m * n, 4 * shares * m * n - 1, 4 * shares * m * n):
+            got = _launch(m, n, k, 128, lent=lent)[1]
+            assert got == 1 or 4 * got * m * n <= lent
+        assert _launch(m, n, k, 128, lent=4 * shares * m * n)[1] == shares
+    for m, n, k in [(1 << 30, 1 << 30, 1 << 30), (1 << 30, 8, 1 << 30), (1, 1 << 30, 8)]:
+        assert _launch(m, n, k, 128)[1] == 1
+
+
+def test_scratch_bytes():
+    a = _linear(rows=1, in_features=16392, out_features=264, group=128, x=0x1000000, w=0x2000000, scales=0x3000000, zeros=None, residual=None, y=0x5000000)
+    need = capi.lib().mi_linear_int4_scratch_bytes(C.byref(a))
+    assert need > 0 and need % (4 * 264) == 0
+    a.scratch, a.scratch_bytes = 0x2000000, 1 << 20
+    assert capi.lib().mi_linear_int4_scratch_bytes(C.byref(a)) == need
+    assert capi.lib().mi_linear_int4_scratch_bytes(C.byref(_linear())) == 0 and capi.lib().mi_linear_int4_scratch_bytes(None) == 0
+    a.group = 100
+    assert capi.lib().mi_linear_int4_scratch_bytes(C.byref(a)) == 0
+
+
+@pytest.mark.parametrize("name,at", [("x", 0x10000), ("x", 0x10830), ("w", 0x20000), ("w", 0x223f0), ("scales", 0x30180), ("zeros", 0x400c0), ("bias", 0x50040), ("residual", 0x60130), ("y", 0x70000)])
+def test_scratch_that_is_part_of_an_operand(name, at):
+    for scratch, size in ((at, 64), (at - 0x400, 0x410)):
+        assert capi.lib().mi_linear_int4_forward(C.byref(_linear(scratch=scratch, scratch_bytes=size))) == -1
+        assert f"scratch overlaps {name}" in capi.last_error(), capi.last_error()
+    assert capi.lib().mi_linear_int4_forward(C.byref(_linear(scratch=0x80008, scratch_bytes=64))) == -1 and "scratch must be 16-byte" in capi.last_error()
 
 
 def test_no_scratch_memory(kernels):  # noqa: F811

@@ -13,6 +13,7 @@ import pytest
 import torch
 
 import brodiffusion_amd as bd
+from brodiffusion_amd import _capi as capi
 from brodiffusion_amd import build
 from helpers import TORCH_DT
 
@@ -97,23 +98,68 @@ def test_wide_and_long(dtype, m, k, n, group, zeros):
 
 
 FEW16, FEW32, FEW64, TILE32x64, TILE32x128, TILE64x128, TILE64x256 = range(7)
-FORMS = {128: {FEW16: (5, 136, 520), FEW32: (17, 264, 2056), FEW64: (40, 520, 4104), TILE32x64: (64, 136, 4104), TILE32x128: (200, 1160, 8200), TILE64x128: (2049, 264, 4104), TILE64x256: (3000, 520, 2056)},
-         64: {FEW16: (1, 264, 264), FEW32: (17, 264, 2056), FEW64: (40, 520, 4104), TILE32x64: (500, 136, 520), TILE32x128: (333, 264, 16392), TILE64x128: (777, 136, 16392), TILE64x256: (3000, 3088, 2056)},
-         32: {FEW16: (1, 264, 264), FEW32: (40, 136, 2056), TILE32x64: (16, 136, 8200), TILE32x128: (333, 1160, 8200), TILE64x128: (2049, 264, 8200), TILE64x256: (3000, 1160, 2056)}}
+# (rows, contraction, features) by group, work group, and whether the contraction is given in shares
+PROBLEMS = {
+    128: {(FEW16, 0): (5, 520, 136), (FEW16, 1): (17, 16392, 8), (FEW32, 0): (5, 520, 4104), (FEW32, 1): (17, 16392, 264), (FEW64, 0): (500, 264, 264), (FEW64, 1): (1, 16392, 4104),
+          (TILE32x64, 0): (200, 8, 8200), (TILE32x64, 1): (500, 16392, 136), (TILE32x128, 0): (17, 2056, 16392), (TILE32x128, 1): (16, 3088, 16392), (TILE64x128, 0): (500, 264, 8200),
+          (TILE64x128, 1): (100, 16392, 2056), (TILE64x256, 0): (333, 1160, 16392), (TILE64x256, 1): (1031, 4616, 2056)},
+    64: {(FEW16, 0): (1, 264, 1160), (FEW16, 1): (1, 4616, 520), (FEW32, 0): (5, 520, 4104), (FEW32, 1): (17, 16392, 264), (FEW64, 0): (777, 264, 264), (FEW64, 1): (1, 16392, 4104),
+         (TILE32x64, 0): (777, 8, 4104), (TILE32x64, 1): (64, 8200, 1160), (TILE32x128, 0): (200, 1160, 16392), (TILE32x128, 1): (17, 8200, 8200), (TILE64x128, 0): (3000, 136, 4104),
+         (TILE64x128, 1): (100, 16392, 2056), (TILE64x256, 0): (3000, 2056, 2056), (TILE64x256, 1): (2049, 8200, 1160)},
+    32: {(FEW16, 0): (16, 264, 72), (FEW16, 1): (5, 4616, 136), (FEW32, 0): (64, 136, 1160), (FEW32, 1): (17, 8200, 520), (TILE32x64, 0): (64, 136, 4104), (TILE32x64, 1): (100, 4616, 1160),
+         (TILE32x128, 0): (333, 264, 8200), (TILE32x128, 1): (333, 16392, 2056), (TILE64x128, 0): (500, 264, 16392), (TILE64x128, 1): (200, 16392, 1160), (TILE64x256, 0): (1500, 520, 4104),
+         (TILE64x256, 1): (500, 8200, 2056)}}
 
 
-def _form(m, k, n, group, row=0):
-    return C.CDLL(build.FORMS_LIB).int4_form_test(m, n, k, C.c_long(row or k), group, bd.device_info()["compute_units"])
+def _launch(m, k, n, group, lent=(1 << 64) - 1):
+    shares = C.c_int()
+    return C.CDLL(build.FORMS_LIB).int4_form_test(m, n, k, C.c_long(k), group, bd.device_info()["compute_units"], C.c_ulong(lent), C.byref(shares)), shares.value
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("zeros", [False, True])
-@pytest.mark.parametrize("group,form", [(g, f) for g in FORMS for f in FORMS[g]])
-def test_every_form(dtype, zeros, group, form):
-    """Every kernel instance, on problems that end inside its work groups, its steps and their groups"""
-    m, k, n = FORMS[group][form]
-    assert _form(m, k, n, group) == form
+@pytest.mark.parametrize("group,form,shared", [(g, *f) for g in PROBLEMS for f in PROBLEMS[g]])
+def test_every_form(dtype, zeros, group, form, shared):
+    """Every kernel instance, with the contraction whole and in shares, on problems that end inside its work groups, its steps and their groups"""
+    m, k, n = PROBLEMS[group][form, shared]
+    got, shares = _launch(m, k, n, group)
+    assert got == form and (shares > 1) == bool(shared)
     _case(dtype, m, k, n, group, zeros, bias=True, act="silu", residual=True)
+
+
+def _args(x, w, y, scratch=None):
+    a = capi.MiLinearInt4Args()
+    a.struct_size, a.dtype = C.sizeof(a), capi.MI_DTYPE_BF16
+    a.x, a.w, a.scales, a.y = x.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), y.data_ptr()
+    a.rows, a.in_features, a.out_features, a.group = x.shape[0], w.in_features, w.out_features, w.group
+    a.stream = torch.cuda.current_stream().cuda_stream
+    if scratch is not None:
+        a.scratch, a.scratch_bytes = scratch.data_ptr(), scratch.numel()
+    return a
+
+
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_scratch(m):
+    """As much as is asked for, less, none, and more; what lies behind it stays"""
+    g = torch.Generator().manual_seed(m)
+    k, n = 16392, 264
+    q, scales, _ = _checkpoint(g, n, k, 128, False, torch.bfloat16)
+    w = bd.pack_int4(q, scales)
+    x = torch.randn(m, k, generator=g).bfloat16().cuda()
+    ref = _reference(x, q, scales, None, 128, None, "none", None)
+    y = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    need = int(capi.lib().mi_linear_int4_scratch_bytes(C.byref(_args(x, w, y))))
+    assert need == 4 * m * n * _launch(m, k, n, 128)[1] > 4 * m * n
+    memory = torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda")
+    for lent in (need, need - 4, need // 2, 4 * m * n, 0, need + 4096):
+        memory.fill_(77)
+        y.fill_(9)
+        a = _args(x, w, y, memory)
+        a.scratch_bytes = lent
+        assert capi.lib().mi_linear_int4_forward(C.byref(a)) == 0
+        _check(y, *ref)
+        assert torch.all(memory[4 * m * n * _launch(m, k, n, 128, lent)[1] if lent >= 8 * m * n else 0:] == 77)
+    assert torch.equal(bd.linear_int4(x, w), y)
 
 
 @pytest.mark.parametrize("m", [1, 20, 40, 100, 1031])
@@ -159,10 +205,10 @@ def test_strides_and_leading_axes(m):
     assert bd.linear_int4(x[:0], w).shape == (0, n)
 
 
-@pytest.mark.parametrize("m", [4, 50, 90, 300])
-def test_rows_that_are_not_finite_stay_alone(m):
+@pytest.mark.parametrize("m,k", [(4, 520), (50, 520), (90, 520), (300, 520), (4, 8200), (300, 8200)])
+def test_rows_that_are_not_finite_stay_alone(m, k):
     g = torch.Generator().manual_seed(m)
-    k, n = 520, 264
+    n = 264
     q, scales, z = _checkpoint(g, n, k, 128, False, torch.bfloat16)
     w = bd.pack_int4(q, scales, z)
     x = torch.randn(m, k, generator=g).bfloat16().cuda()
@@ -190,10 +236,10 @@ def test_far_rows():
 
 def test_other_stream_and_graphs():
     g = torch.Generator().manual_seed(2)
-    for m in (1, 40, 200):
-        q, scales, z = _checkpoint(g, 520, 1160, 64, True, torch.float16)
+    for m, k in ((1, 1160), (40, 1160), (200, 1160), (1, 8200), (200, 8200)):
+        q, scales, z = _checkpoint(g, 520, k, 64, True, torch.float16)
         w = bd.pack_int4(q, scales, z, group=64)
-        x = torch.randn(m, 1160, generator=g).half().cuda()
+        x = torch.randn(m, k, generator=g).half().cuda()
         want = bd.linear_int4(x, w, activation="gelu")
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
