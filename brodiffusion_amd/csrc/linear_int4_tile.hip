@@ -37,7 +37,9 @@ struct TileForm {
     static_assert(kBytes <= 160 * 1024, "LDS of a compute unit");
 };
 
-template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN>
+// WHOLE: the contraction is never in shares. For the largest form and groups of 128 and more alone, the one where a loop from a computed block to another came out
+// slower (4608 x 6144 x 16384: 937 us against 908; groups of 64, 4096 x 4608 x 1152: 77 against 78)
+template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN, bool WHOLE>
 __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(const Int4Problem p) {
     using M = Mma<T>;
     using V8 = typename M::v8;
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
     // LDS between two barriers is another stage, and the barriers have one)
     auto dma16 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst)); };
     auto dma4 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "{m0}"(dst)); };
-    const int share = static_cast<int>(blockIdx.y), begin = int4_share(p, share), end = int4_share(p, share + 1);
+    const int share = WHOLE ? 0 : static_cast<int>(blockIdx.y), begin = WHOLE ? 0 : int4_share(p, share), end = WHOLE ? p.KB : int4_share(p, share + 1);
     int filling = 0, group = P == 1 ? begin / p.span : 0, of_group = P == 1 ? begin % p.span : 0;      // the stage that the next request fills; its group, of blocks and more, and which block of it
     // requests FROM .. TO - 1 of a step's L::NI
     auto request = [&]<int FROM, int TO>(int step, std::integer_sequence<int, FROM, TO>) {
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (no DMA into LDS that is given back)
 
-    if (p.parts) {
+    if (!WHOLE && p.parts) {
         float* const to = p.parts + static_cast<long>(share) * p.M * p.N;
 #pragma unroll
         for (int a = 0; a < FB; ++a)
@@ -291,11 +293,11 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
     }
 }
 
-template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN>
+template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN, bool WHOLE = false>
 int launch(const Int4Problem& p, hipStream_t st) {
     using L = TileForm<P, ZEROS, TB, FB, S>;
     constexpr int TM = L::TM, TN = L::TN, bytes = L::kBytes;
-    const auto kernel = &linear_int4_tile_kernel<T, P, ZEROS, TB, FB, S, SIMD, OWN>;
+    const auto kernel = &linear_int4_tile_kernel<T, P, ZEROS, TB, FB, S, SIMD, OWN, WHOLE>;
     if constexpr (bytes > 64 * 1024) {
         int device = 0;
         MI_HIP_CHECK(hipGetDevice(&device));
@@ -317,7 +319,10 @@ int launch_form(const Int4Problem& p, int form, hipStream_t st) {
         case kTile32x64: return launch<T, P, ZEROS, 2, 1, 3, 4, true>(p, st);
         case kTile32x128: return launch<T, P, ZEROS, 2, 2, 3, 3, true>(p, st);
         case kTile64x128: return launch<T, P, ZEROS, 4, 2, 2, 2, false>(p, st);
-        default: return launch<T, P, ZEROS, 4, 4, 2, 2, false>(p, st);
+        default:
+            if constexpr (P == 1)
+                if (!p.parts) return launch<T, P, ZEROS, 4, 4, 2, 2, false, true>(p, st);
+            return launch<T, P, ZEROS, 4, 4, 2, 2, false>(p, st);
     }
 }
 template <typename T, int P>
