@@ -336,6 +336,24 @@ void add_rms_norm_impl(const char* op, const Tensor& X, const Tensor* residual, 
 }
 }  // namespace
 
+namespace {
+// Scratch of a linear layer whose contraction several work groups share (outgrown scratch is kept, a captured graph may still write to it; each is twice the one
+// before, so that together they are less than the last)
+template <typename Args> void lend(Args& a, std::size_t need) {
+    struct Grown { std::vector<Tensor> tensors; };
+    if (need == 0) return;
+    auto& scratch = per_stream<Grown, Args>().tensors;
+    if (scratch.empty() || scratch.back().bytes() < need) {
+        const std::size_t bytes = scratch.empty() ? need : std::max(need, 2 * scratch.back().bytes());
+        Tensor next;
+        next.resize(1, static_cast<int>((bytes + 3) / 4), Dtype::FP32, Device::GPU);
+        scratch.push_back(std::move(next));
+    }
+    a.scratch = scratch.back().data;
+    a.scratch_bytes = scratch.back().bytes();
+}
+}  // namespace
+
 void linear_act(const Tensor& X, const Tensor* x_scales, const Tensor& W, const Tensor* w_scales, const Tensor* bias, Activation activation,
                 const Tensor* residual, Tensor& Y) {
     const char* op = "linear_act";
@@ -361,19 +379,7 @@ void linear_act(const Tensor& X, const Tensor* x_scales, const Tensor& W, const 
     a.x = X.data; a.w = W.data; a.y = Y.data;
     a.rows = X.rows; a.in_features = X.cols; a.out_features = W.rows;
     a.activation = static_cast<int>(activation);
-    // (outgrown scratch is kept, a captured graph may still write to it; each is twice the one before, so that together they are less than the last)
-    struct LinearActScratch { std::vector<Tensor> grown; };
-    auto& scratch = per_stream<LinearActScratch, LinearActScratch>().grown;
-    if (const std::size_t need = mi_linear_act_scratch_bytes(&a); need > 0) {
-        if (scratch.empty() || scratch.back().bytes() < need) {
-            const std::size_t bytes = scratch.empty() ? need : std::max(need, 2 * scratch.back().bytes());
-            Tensor next;
-            next.resize(1, static_cast<int>((bytes + 3) / 4), Dtype::FP32, Device::GPU);
-            scratch.push_back(std::move(next));
-        }
-        a.scratch = scratch.back().data;
-        a.scratch_bytes = scratch.back().bytes();
-    }
+    lend(a, mi_linear_act_scratch_bytes(&a));
     check(op, mi_linear_act_forward(&a));
 }
 
@@ -383,6 +389,89 @@ void add_rms_norm(const Tensor& X, const Tensor* residual, const Tensor& gain, f
 void add_rms_norm_int8(const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out, Tensor& scales) {
     add_rms_norm_impl("add_rms_norm_int8", X, residual, gain, eps, sum, out, &scales);
 }
+void gate_add_norm(const Tensor& X, const GateAddNorm& step, Tensor* sum, Tensor* out) {
+    const char* op = "gate_add_norm";
+    need_gpu(op, X);
+    mi_gate_add_norm_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.dtype = dtype_code(op, X.dtype);
+    a.x = X.data; a.rows = X.rows; a.cols = X.cols;
+    if (sum != nullptr) own_tensor(op, "sum", sum, {step.gate, step.post_gain, step.gain, step.scale, step.shift, out});
+    if (out != nullptr) own_tensor(op, "out", out, {step.gate, step.post_gain, step.gain, step.scale, step.shift});
+    if (step.branch != nullptr) {
+        need_gpu(op, *step.branch);
+        if (step.branch->dtype != X.dtype || step.branch->rows != X.rows || step.branch->cols != X.cols) fail(std::string(op) + ": the branch must have X's shape and dtype");
+        a.branch = step.branch->data;
+    }
+    // a vector for all rows, or for each `rows` of them
+    auto vectors = [&](const Tensor* t, const char* name, int* rows) -> const void* {
+        if (t == nullptr) return nullptr;
+        need_gpu(op, *t);
+        const bool one = t->size() == static_cast<std::size_t>(X.cols);
+        if (t->dtype != X.dtype || !(one || (rows != nullptr && t->cols == X.cols && t->rows > 0 && X.rows % t->rows == 0)))
+            fail(std::string(op) + ": " + name + " must hold X's columns in X's dtype" + (rows ? ", once or for equal runs of X's rows" : ""));
+        if (rows != nullptr && !one) *rows = X.rows / t->rows;
+        return t->data;
+    };
+    a.gate = vectors(step.gate, "gate", &a.gate_rows);
+    a.post_gain = vectors(step.post_gain, "post_gain", nullptr);
+    a.gain = vectors(step.gain, "gain", nullptr);
+    a.scale = vectors(step.scale, "scale", &a.scale_rows);
+    a.shift = vectors(step.shift, "shift", &a.shift_rows);
+    a.post_norm = static_cast<int>(step.post_norm); a.norm = static_cast<int>(step.norm);
+    a.post_eps = step.post_eps; a.eps = step.eps; a.residual_scale = step.residual_scale;
+    if (sum != nullptr) { fit(*sum, X.rows, X.cols, X.dtype, X.device); a.sum_out = sum->data; }
+    if (out != nullptr) { fit(*out, X.rows, X.cols, X.dtype, X.device); a.out = out->data; }
+    check(op, mi_gate_add_norm_forward(&a));
+}
+
+void pack_int4(const Tensor& q, Tensor& packed) {
+    const char* op = "pack_int4";
+    need_gpu(op, q);
+    own_tensor(op, "packed", &packed, {&q});
+    const std::size_t bytes = q.cols > 0 && q.cols <= (1 << 30) - 1 ? mi_int4_packed_bytes(q.rows, 2 * q.cols) : 0;
+    const int blocks = (q.rows + 15) / 16;
+    if (q.dtype != Dtype::INT8 || bytes == 0) fail(std::string(op) + ": q must hold (out_features, in_features / 2) bytes (INT8)");
+    fit(packed, blocks, static_cast<int>(bytes / blocks), Dtype::INT8, q.device);
+    mi_pack_int4_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.q = q.data; a.packed = packed.data;
+    a.out_features = q.rows; a.in_features = 2 * q.cols;
+    check(op, mi_pack_int4(&a));
+}
+void linear_int4(const Tensor& X, const Tensor& packed, const Tensor& scales, const Tensor* zeros, int group, const Tensor* bias, Activation activation,
+                 const Tensor* residual, Tensor& Y) {
+    const char* op = "linear_int4";
+    need_gpu(op, X); need_gpu(op, packed); need_gpu(op, scales);
+    own_tensor(op, "Y", &Y, {&X, &packed, &scales, zeros, bias});
+    const int n = scales.cols, groups = group > 0 ? static_cast<int>((static_cast<long long>(X.cols) + group - 1) / group) : 0;
+    if (scales.dtype != X.dtype || scales.rows != groups) fail(std::string(op) + ": scales must be (groups, out_features) of X's dtype");
+    if (packed.dtype != Dtype::INT8 || packed.size() == 0 || packed.size() != mi_int4_packed_bytes(n, X.cols)) fail(std::string(op) + ": the packed weights are not of these sizes");
+    mi_linear_int4_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.dtype = dtype_code(op, X.dtype);
+    if (zeros != nullptr) {
+        need_gpu(op, *zeros);
+        if (zeros->dtype != Dtype::INT8 || zeros->rows != groups || zeros->cols != n) fail(std::string(op) + ": zeros must be (groups, out_features) bytes");
+        a.zeros = zeros->data;
+    }
+    a.bias = bias_ptr(op, bias, "bias", X.dtype, n);
+    if (residual != nullptr) {
+        need_gpu(op, *residual);
+        if (residual->dtype != X.dtype || residual->rows != X.rows || residual->cols != n) fail(std::string(op) + ": the residual must have Y's shape and dtype");
+        a.residual = residual->data;
+    }
+    fit(Y, X.rows, n, X.dtype, X.device);
+    a.x = X.data; a.w = packed.data; a.scales = scales.data; a.y = Y.data;
+    a.rows = X.rows; a.in_features = X.cols; a.out_features = n; a.group = group;
+    a.activation = static_cast<int>(activation);
+    lend(a, mi_linear_int4_scratch_bytes(&a));
+    check(op, mi_linear_int4_forward(&a));
+}
+
 void quantize_rows_int8(const Tensor& X, Tensor& out, Tensor& scales) {
     const char* op = "quantize_rows_int8";
     need_gpu(op, X);

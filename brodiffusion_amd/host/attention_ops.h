@@ -77,6 +77,32 @@ void add_rms_norm(const Tensor& X, const Tensor* residual, const Tensor& gain, f
 void add_rms_norm_int8(const Tensor& X, const Tensor* residual, const Tensor& gain, float eps, Tensor& sum, Tensor& out, Tensor& scales);
 void quantize_rows_int8(const Tensor& X, Tensor& out, Tensor& scales);
 
+// The step between two blocks (mi_gate_add_norm_forward): h = residual_scale * X + gate * post_norm(branch) * post_gain into `sum`, norm(h) * gain * (1 + scale) +
+// shift into `out`; without a branch h is X. Every tensor but X may be null, `sum` and `out` too where nobody wants them (norm None and out null go together; sum
+// only with a branch). gate, scale and shift have one row for all rows of X, or a number of rows that divides X's: one for each X.rows / that many consecutive
+// rows. `sum` and `out` may be X or the branch.
+enum class Norm { None = MI_NORM_NONE, Rms = MI_NORM_RMS, Layer = MI_NORM_LAYER };
+struct GateAddNorm {
+    const Tensor* branch = nullptr;
+    const Tensor* gate = nullptr;
+    Norm post_norm = Norm::None;
+    const Tensor* post_gain = nullptr;
+    float post_eps = 1e-6f, residual_scale = 1.f;
+    Norm norm = Norm::None;
+    const Tensor* gain = nullptr;
+    const Tensor* scale = nullptr;
+    const Tensor* shift = nullptr;
+    float eps = 1e-6f;
+};
+void gate_add_norm(const Tensor& X, const GateAddNorm& step, Tensor* sum, Tensor* out);
+
+// Y = act(X W^T + bias) + residual with 4-bit weights, W[n][k] = (q[n][k] - zeros[g][n]) * scales[g][n], g = k / group (mi_linear_int4_forward). pack_int4 lays q out
+// once: (out_features, in_features / 2) bytes in an INT8 tensor, element 2 j of a row in the low half of byte j. scales (groups, out_features) of X's dtype, zeros
+// the same in bytes (INT8) or null: 8; bias and residual may be null, residual may be Y itself. Scratch as in linear_act.
+void pack_int4(const Tensor& q, Tensor& packed);
+void linear_int4(const Tensor& X, const Tensor& packed, const Tensor& scales, const Tensor* zeros, int group, const Tensor* bias, Activation activation,
+                 const Tensor* residual, Tensor& Y);
+
 // Attention with its projections (the U-Net spatial transformer's operators). Weights are (out_features, in_features),
 // biases may be null, Ctx == nullptr is self-attention. The projections and the attention output live in a scratch
 // tensor owned by the calling thread, grown on demand and kept (no allocation after warm-up, as the reference's

@@ -1394,7 +1394,9 @@ def pack_int4(q, scales, zeros=None, group: int = 128) -> Int4Weight:
     a.q_row_stride = q.stride(0) if n > 1 else k // 2
     a.stream = _stream()
     capi.check(capi.lib().mi_pack_int4(C.byref(a)), op)
-    return Int4Weight(packed, scales.t().contiguous(), None if zeros is None else zeros.t().contiguous(), n, k, group)
+    def transposed(t):      # (a copy, also of a single group, whose transposed view is contiguous already: the weight does not change with the caller's tensor)
+        return t.t().clone(memory_format=torch.contiguous_format)
+    return Int4Weight(packed, transposed(scales), None if zeros is None else transposed(zeros), n, k, group)
 
 
 def linear_int4(X, W: Int4Weight, bias=None, *, activation: str = "none", residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):

@@ -308,6 +308,17 @@ def test_a_block_as_it_is_used():
         assert all(torch.equal(a, b) for a, b in zip(outs, block(x2, att2)))
 
 
+@pytest.mark.parametrize("group", [64, 256])
+def test_packed_weights_are_copies(group):
+    q, scales, z = _checkpoint(torch.Generator().manual_seed(6), 48, 256, group, True, torch.float16)
+    x = torch.randn(5, 256, generator=torch.Generator().manual_seed(7)).half().cuda()
+    w = bd.pack_int4(q, scales, z, group=group)
+    y = bd.linear_int4(x, w)
+    for t in (q, scales, z):
+        t.zero_()
+    assert torch.equal(bd.linear_int4(x, w), y) and y.abs().max() > 0
+
+
 def test_refusals():
     g = torch.Generator().manual_seed(5)
     q, scales, z = _checkpoint(g, 16, 264, 64, True, torch.bfloat16)
