@@ -37,9 +37,7 @@ struct TileForm {
     static_assert(kBytes <= 160 * 1024, "LDS of a compute unit");
 };
 
-// WHOLE: the contraction is never in shares. For the largest form and groups of 128 and more alone, the one where a loop from a computed block to another came out
-// slower (4608 x 6144 x 16384: 937 us against 908; groups of 64, 4096 x 4608 x 1152: 77 against 78)
-template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN, bool WHOLE>
+template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN>
 __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(const Int4Problem p) {
     using M = Mma<T>;
     using V8 = typename M::v8;
@@ -100,7 +98,7 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
     // LDS between two barriers is another stage, and the barriers have one)
     auto dma16 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst)); };
     auto dma4 = [](unsigned off, const unsigned char* base, unsigned dst) { asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "{m0}"(dst)); };
-    const int share = WHOLE ? 0 : static_cast<int>(blockIdx.y), begin = WHOLE ? 0 : int4_share(p, share), end = WHOLE ? p.KB : int4_share(p, share + 1);
+    const int share = static_cast<int>(blockIdx.y), begin = int4_share(p, share), end = int4_share(p, share + 1);
     int filling = 0, group = P == 1 ? begin / p.span : 0, of_group = P == 1 ? begin % p.span : 0;      // the stage that the next request fills; its group, of blocks and more, and which block of it
     // requests FROM .. TO - 1 of a step's L::NI
     auto request = [&]<int FROM, int TO>(int step, std::integer_sequence<int, FROM, TO>) {
@@ -184,7 +182,7 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
         }
         // scales and zero points of a wavefront's features wait in registers; where they would be 32 a lane and more they are read again for each 16 tokens,
         // one group at a time (the scheduling barrier: gathered ahead they do not fit the 256 registers)
-        constexpr bool AGAIN = P * FB >= 8;
+        constexpr bool AGAIN = P * FB >= (SIMD == 3 && !OWN ? 4 : 8);
         float scale[FB][P][4];
         unsigned zero[FB][P];
         auto factors = [&](int g) {
@@ -250,7 +248,7 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (no DMA into LDS that is given back)
 
-    if (!WHOLE && p.parts) {
+    if (p.parts) {
         float* const to = p.parts + static_cast<long>(share) * p.M * p.N;
 #pragma unroll
         for (int a = 0; a < FB; ++a)
@@ -293,11 +291,11 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
     }
 }
 
-template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN, bool WHOLE = false>
+template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN>
 int launch(const Int4Problem& p, hipStream_t st) {
     using L = TileForm<P, ZEROS, TB, FB, S>;
     constexpr int TM = L::TM, TN = L::TN, bytes = L::kBytes;
-    const auto kernel = &linear_int4_tile_kernel<T, P, ZEROS, TB, FB, S, SIMD, OWN, WHOLE>;
+    const auto kernel = &linear_int4_tile_kernel<T, P, ZEROS, TB, FB, S, SIMD, OWN>;
     if constexpr (bytes > 64 * 1024) {
         int device = 0;
         MI_HIP_CHECK(hipGetDevice(&device));
@@ -318,11 +316,11 @@ int launch_form(const Int4Problem& p, int form, hipStream_t st) {
     switch (form) {
         case kTile32x64: return launch<T, P, ZEROS, 2, 1, 3, 4, true>(p, st);
         case kTile32x128: return launch<T, P, ZEROS, 2, 2, 3, 3, true>(p, st);
-        case kTile64x128: return launch<T, P, ZEROS, 4, 2, 2, 2, false>(p, st);
-        default:
-            if constexpr (P == 1)
-                if (!p.parts) return launch<T, P, ZEROS, 4, 4, 2, 2, false, true>(p, st);
-            return launch<T, P, ZEROS, 4, 4, 2, 2, false>(p, st);
+        case kTile64x128: return launch<T, P, ZEROS, 4, 2, 2, 3, false>(p, st);
+        case kTile64x192: return launch<T, P, ZEROS, 4, 3, 2, 2, false>(p, st);
+        case kTile64x256:
+            if constexpr (P < 4) return launch<T, P, ZEROS, 4, 4, 2, 2, false>(p, st);
+        default: return launch<T, P, ZEROS, 6, 3, 2, 2, false>(p, st);
     }
 }
 template <typename T, int P>

@@ -85,11 +85,11 @@ def _launch(m, n, k, group, row=0, lent=(1 << 64) - 1):
 
 def test_instances_are_those_that_calls_reach(kernels):  # noqa: F811
     """Work groups by the rule (csrc/linear_int4_forms.h), over sizes and kinds of groups, against what is in the library"""
-    sizes = [(m, n, k) for m in (1, 16, 40, 200, 333, 777, 2049, 3000) for n in (8, 264, 1160, 2056, 4104, 8200) for k in (8, 264, 1160, 2056, 3088, 8200)]
+    sizes = [(m, n, k) for m in (1, 16, 40, 200, 333, 777, 2049, 3000) for n in (8, 264, 1160, 2056, 4104, 8200, 16392) for k in (8, 264, 1160, 2056, 3088, 8200, 16392)]
     reached = {(p, _launch(m, n, k, 128 // p)[0]) for p in (1, 2, 4) for m, n, k in sizes}
-    assert reached == {(p, f) for p in (1, 2, 4) for f in range(7)} - {(4, 2)}
+    assert reached == {(p, f) for p in (1, 2, 4) for f in range(9)} - {(4, 2), (4, 8)}
     few = {(p, 1 << f) for p, f in reached if f < 3}
-    tiles = {(p, z, *((2, 1), (2, 2), (4, 2), (4, 4))[f - 3]) for p, f in reached if f >= 3 for z in (0, 1)}
+    tiles = {(p, z, *((2, 1), (2, 2), (4, 2), (4, 3), (6, 3), (4, 4))[f - 3]) for p, f in reached if f >= 3 for z in (0, 1)}
     for t in ("DF16_", "DF16b"):
         assert {tuple(map(int, m.groups())) for name in kernels if (m := re.search(rf"linear_int4_few_kernelI{t}Li(\d+)ELi(\d+)E", name))} == few
         assert {tuple(map(int, m.groups())) for name in kernels if (m := re.search(rf"linear_int4_tile_kernelI{t}Li(\d+)ELb(\d)ELi(\d+)ELi(\d+)E", name))} == tiles
@@ -97,8 +97,8 @@ def test_instances_are_those_that_calls_reach(kernels):  # noqa: F811
 
 def test_rows_far_apart_and_many_features_get_64_bit_offsets():
     for m in (70, 5000):
-        assert _launch(m, 1160, 136, 64, 1 << 24)[0] < 3 and _launch(m, (1 << 24) + 8, 136, 64)[0] < 3
-        assert _launch(5000, 1160, 136, 64, (1 << 24) - 8)[0] >= 3
+        assert _launch(m, 1160, 136, 64, 11184816)[0] < 3 and _launch(m, (1 << 24) + 8, 136, 64)[0] < 3
+        assert _launch(5000, 1160, 136, 64, 11184808)[0] >= 3
 
 
 def test_shares_of_the_contraction():
