@@ -9,10 +9,13 @@
 //      wavefront sums for itself, along with its products, and the second barrier is gone: faster where a step is short
 //   3. products: 16 tokens at a time against all the wavefront's features, a chain of matrix instructions per group from -z times the sum of x, scaled into the
 //      accumulators; between them the loads of step + S - 1, dealt out: a request waits for those ahead of it (60 bytes a clock and compute unit)
-// Bound: what a SIMD issues. Beside 64 products, 64 tokens x 64 features x 128 elements are 112 instructions of the weights, 64 that scale sums and about 60 others;
-// a 16 x 16 product takes the issue 12 of its 16 clocks, another vector instruction 4 (measured: one product and 1 to 4 others, two wavefronts, 17, 19.5,
-// 24.4, 27.9 clocks), so the matrix pipes are busy half of the time. 32 x 32 products leave more room (32.3 clocks with 1, 33.5 with 6 others), but their
-// accumulators came out slower at every size (4608 x 6144 x 16384: 970 us instead of 870), and so did wavefronts that take turns at products and weights (890).
+// Bound: what a SIMD issues. 64 tokens x 64 features x 128 elements are 64 products and beside them 112 instructions of the weights, 64 that scale sums and about 60
+// others; a 16 x 16 product takes the issue 12 of its 16 clocks, another vector instruction 4 (measured: one product and 1 to 4 others, two wavefronts, 17, 19.5,
+// 24.4, 27.9 clocks). Tiles of 96 tokens spread the weights' instructions over half as many tokens more. 4608 x 6144 x 16384 bf16 (tokens, contraction, features) takes
+// 0.89 ms, 1.04 PFLOP/s, the matrix pipes busy half of the time; groups of 64 with zero points 1.13 ms. 32 x 32 products leave more room (32.3 clocks with 1, 33.5 with 6
+// others), but their accumulators came out slower at every size (970 us instead of 870 then), and so did wavefronts that take turns at products and weights (890),
+// products, scaling and weights kept apart by scheduling barriers (0 to 3 % slower), and 6-bit conversions of 32 weights at once (as long as 28 instructions); without the
+// sums of x and their barrier it would be 4 % faster, less than a launch that makes the sums ahead costs at most sizes.
 #include <utility>
 
 #include "linear_int4.h"
@@ -313,13 +316,16 @@ int launch(const Int4Problem& p, hipStream_t st) {
 
 template <typename T, int P, bool ZEROS>
 int launch_form(const Int4Problem& p, int form, hipStream_t st) {
+    // Stages, wavefronts a SIMD and who sums x, by measurement. 32 tokens, a step is short: 3 stages and own sums (333 x 2240 x 6720, groups of 64: 29 us;
+    // 2 stages 33, shared sums 36, 4 stages and 2 wavefronts 36; 128 x 4608 x 4608: 23, 29, 30, 24). More tokens: 2 stages and shared sums, so that three work groups of
+    // 64 x 128 fit a compute unit (4096 x 4608 x 1152: 70 us; two of 3 stages 87 to 94, own sums as many) and two of the others.
     switch (form) {
         case kTile32x64: return launch<T, P, ZEROS, 2, 1, 3, 4, true>(p, st);
         case kTile32x128: return launch<T, P, ZEROS, 2, 2, 3, 3, true>(p, st);
         case kTile64x128: return launch<T, P, ZEROS, 4, 2, 2, 3, false>(p, st);
         case kTile64x192: return launch<T, P, ZEROS, 4, 3, 2, 2, false>(p, st);
         case kTile64x256:
-            if constexpr (P < 4) return launch<T, P, ZEROS, 4, 4, 2, 2, false>(p, st);
+            if constexpr (P == 1) return launch<T, P, ZEROS, 4, 4, 2, 2, false>(p, st);
         default: return launch<T, P, ZEROS, 6, 3, 2, 2, false>(p, st);
     }
 }
