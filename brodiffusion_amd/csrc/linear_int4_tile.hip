@@ -262,36 +262,48 @@ __global__ void __launch_bounds__(64 * kWaves, SIMD) linear_int4_tile_kernel(con
             }
         return;
     }
+    // (all of the bias and the residual on their way before the first is used: their latency once, not for each block)
+    t4 bias[FB], res[FB][TB];
+    if (p.bias) {
 #pragma unroll
-    for (int a = 0; a < FB; ++a) {
-        const int f = n0 + (wave * FB + a) * 16 + 4 * lg;
-        if (f >= p.N) continue;
-        f32x4 bias = {0.f, 0.f, 0.f, 0.f};
-        if (p.bias) {
-            const t4 v = *reinterpret_cast<const t4*>(static_cast<const T*>(p.bias) + f);
+        for (int a = 0; a < FB; ++a) bias[a] = *reinterpret_cast<const t4*>(static_cast<const T*>(p.bias) + min(n0 + (wave * FB + a) * 16 + 4 * lg, p.N - 4));
+    }
+    if (p.residual) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) bias[e] = static_cast<float>(v[e]);
+        for (int b = 0; b < TB; ++b) {
+            const T* const row = static_cast<const T*>(p.residual) + static_cast<long>(min(m0 + 16 * b + lr, p.M - 1)) * p.ldr;
+#pragma unroll
+            for (int a = 0; a < FB; ++a) res[a][b] = *reinterpret_cast<const t4*>(row + min(n0 + (wave * FB + a) * 16 + 4 * lg, p.N - 4));
         }
+    }
+    auto finish = [&](auto act) {
 #pragma unroll
         for (int b = 0; b < TB; ++b) {
             const int m = m0 + 16 * b + lr;
-            if (m >= p.M) continue;
-            f32x4 v = acc[a][b] + bias;
-            with_activation(p.act, [&](auto act) {
+            T* const row = static_cast<T*>(p.y) + static_cast<long>(m) * p.ldy;
+#pragma unroll
+            for (int a = 0; a < FB; ++a) {
+                const int f = n0 + (wave * FB + a) * 16 + 4 * lg;
+                f32x4 v = acc[a][b];
+                if (p.bias) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += static_cast<float>(bias[a][e]);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = act(v[e]);
-            });
-            if (p.residual) {
-                const t4 r = *reinterpret_cast<const t4*>(static_cast<const T*>(p.residual) + static_cast<long>(m) * p.ldr + f);
+                if (p.residual) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] += static_cast<float>(r[e]);
+                    for (int e = 0; e < 4; ++e) v[e] += static_cast<float>(res[a][b][e]);
+                }
+                t4 o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(v[e]);
+                if (m < p.M && f < p.N) *reinterpret_cast<t4*>(row + f) = o;
             }
-            t4 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(v[e]);
-            *reinterpret_cast<t4*>(static_cast<T*>(p.y) + static_cast<long>(m) * p.ldy + f) = o;
         }
-    }
+    };
+    if (p.act == MI_ACT_NONE) finish([](float v) { return v; });
+    else with_activation(p.act, finish);
 }
 
 template <typename T, int P, bool ZEROS, int TB, int FB, int S, int SIMD, bool OWN>
