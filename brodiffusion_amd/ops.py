@@ -1125,6 +1125,8 @@ def _rows_of(op: str, t, name: str, dtype, shape=None):
         _fail(op, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dim() < 1 or t.shape[-1] == 0:
         _fail(op, f"{name} must have columns")
+    if t.numel() // t.shape[-1] > 0x7fffffff:      # (a C int, which would take it modulo 2^32)
+        _fail(op, f"{name} has more than 2^31 - 1 rows")
     if t.is_contiguous():
         return t.numel() // t.shape[-1], t.shape[-1]
     if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:

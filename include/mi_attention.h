@@ -494,7 +494,8 @@ MI_API int mi_quantize_rows_forward(const mi_quantize_rows_args* args);
  * `..._rows` rows (0: one for all rows): an image's rows of a batch, or a row each. norm MI_NORM_NONE and out NULL go together (the last
  * block: h alone); sum_out (h) only with a branch, optional beside out. Sums are FP32: squares that exceed it make zeros of a row.
  * cols a multiple of 8, at most 65536; strides in elements (0 = dense), multiples of 8, at most 2^40, rows times stride at most 2^56; 16-byte
- * aligned. sum_out and out may each be x or branch (same pointer and stride); outputs share no other memory with each other or an input. */
+ * aligned. sum_out and out may each be x or branch (same pointer and stride); outputs share no other memory with each other or an input
+ * (to gate, scale and shift belongs what lies between their vectors). */
 enum { MI_NORM_NONE = 0, MI_NORM_RMS = 1, MI_NORM_LAYER = 2 };
 typedef struct mi_gate_add_norm_args {
     uint32_t struct_size;

@@ -193,6 +193,20 @@ def test_no_rows_and_untouched_rows():
     assert torch.all(h[5:] == 9) and torch.all(y[5:] == 9)
 
 
+def test_far_rows():
+    """Rows and vectors 2^30 elements apart: offsets past 32 bits"""
+    cols, apart = 1152, (1 << 30) + 8
+    x, b, vec = _make(6, "bf16", 4, cols)
+    gate, shift = vec(4, cols), vec(2, cols)
+    want = bd.gate_add_norm(x, b, gate=gate, post="rms", norm="layer", shift=shift)
+    ins, outs = (torch.empty(3 * apart + 4 * cols, dtype=x.dtype, device="cuda") for _ in range(2))
+    at = lambda i, rows=4: (ins if i < 4 else outs).as_strided((rows, cols), (apart, 1), i % 4 * cols)
+    for i, t in enumerate((x, b, gate, shift)):
+        at(i, t.shape[0]).copy_(t)
+    h, y = bd.gate_add_norm(at(0), at(1), gate=at(2), post="rms", norm="layer", shift=at(3, 2), sum_out=at(4), out=at(5))
+    assert torch.equal(h, want[0]) and torch.equal(y, want[1])
+
+
 def test_other_stream_and_graph():
     x, b, vec = _make(4, "fp16", 333, 1152)
     gate = vec(1152)

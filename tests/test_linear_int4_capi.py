@@ -95,6 +95,16 @@ def test_instances_are_those_that_calls_reach(kernels):  # noqa: F811
         assert {tuple(map(int, m.groups())) for name in kernels if (m := re.search(rf"linear_int4_tile_kernelI{t}Li(\d+)ELb(\d)ELi(\d+)ELi(\d+)E", name))} == tiles
 
 
+def test_more_rows_than_a_c_int(monkeypatch):
+    import torch
+    from brodiffusion_amd import ops
+    monkeypatch.setattr(ops, "_dev", lambda *a: None)
+    rows = lambda n: torch.empty(n, 8, dtype=torch.float16, device="meta")
+    assert ops._rows_of("op", rows(2 ** 31 - 1), "X", torch.float16) == (2 ** 31 - 1, 8)
+    with pytest.raises(RuntimeError, match="more than 2\\^31 - 1 rows"):
+        ops._rows_of("op", rows(2 ** 32 + 5), "X", torch.float16)
+
+
 def test_rows_far_apart_and_many_features_get_64_bit_offsets():
     for m in (70, 5000):
         assert _launch(m, 1160, 136, 64, 11184816)[0] < 3 and _launch(m, (1 << 24) + 8, 136, 64)[0] < 3

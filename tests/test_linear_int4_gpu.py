@@ -236,6 +236,37 @@ def test_far_rows():
     _check(y.contiguous(), *_reference(x.contiguous(), q, scales, z, 64, None, "none", None))
 
 
+def test_rows_as_far_apart_as_tiles_reach():
+    """The largest row stride whose tiles have 32-bit offsets (csrc/linear_int4_forms.h): 96 rows of it are 512 bytes short of 2^31"""
+    g = torch.Generator().manual_seed(8)
+    k, n, m, apart = 136, 4104, 101, 11184808
+    q, scales, _ = _checkpoint(g, n, k, 128, False, torch.float16)
+    w = bd.pack_int4(q, scales)
+    store = torch.empty((m - 1) * apart + k, dtype=torch.float16, device="cuda")
+    x = store.as_strided((m, k), (apart, 1))
+    x.copy_(torch.randn(m, k, generator=g))
+    _check(bd.linear_int4(x, w), *_reference(x.contiguous(), q, scales, None, 128, None, "none", None))
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls whose contraction is in shares, in turn on two streams without waiting for each other: each has memory of its own"""
+    g = torch.Generator().manual_seed(9)
+    q, scales, z = _checkpoint(g, 264, 16392, 64, True, torch.bfloat16)
+    w = bd.pack_int4(q, scales, z, group=64)
+    xs = [torch.randn(m, 16392, generator=g).bfloat16().cuda() for m in (1, 40, 200, 17)]
+    want = [bd.linear_int4(x, w) for x in xs]
+    assert all(_launch(x.shape[0], 16392, 264, 64)[1] > 1 for x in xs)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(40):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(bd.linear_int4(xs[i % 4 if i < 20 else (i * 7 // 2) % 4], w))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 4 if i < 20 else (i * 7 // 2) % 4])
+
+
 def test_other_stream_and_graphs():
     g = torch.Generator().manual_seed(2)
     for m, k in ((1, 1160), (40, 1160), (200, 1160), (1, 8200), (200, 8200)):
