@@ -100,17 +100,17 @@ def test_wide_and_long(dtype, m, k, n, group, zeros):
 FEW16, FEW32, FEW64, TILE32x64, TILE32x128, TILE64x128, TILE64x192, TILE96x192, TILE64x256 = range(9)
 # (rows, contraction, features) by group, work group, and whether the contraction is given in shares
 PROBLEMS = {
-    128: {(FEW16, 0): (333, 136, 8), (FEW16, 1): (17, 16392, 8), (FEW32, 0): (5, 520, 4104), (FEW32, 1): (17, 16392, 264), (FEW64, 0): (777, 520, 264),
-         (FEW64, 1): (1, 16392, 4104), (TILE32x64, 0): (5, 136, 16392), (TILE32x64, 1): (500, 8200, 264), (TILE32x128, 0): (2049, 136, 1160), (TILE32x128, 1): (16, 3088, 16392),
-         (TILE64x128, 0): (3000, 136, 1160), (TILE64x128, 1): (2049, 16392, 72), (TILE64x192, 0): (200, 264, 16392), (TILE64x192, 1): (3000, 8200, 136), (TILE96x192, 0): (4096, 136, 2056),
-         (TILE96x192, 1): (1031, 16392, 520), (TILE64x256, 0): (777, 264, 16392), (TILE64x256, 1): (500, 4616, 4104)},
-    64: {(FEW16, 0): (1, 264, 1160), (FEW16, 1): (1, 4616, 520), (FEW32, 0): (5, 520, 4104), (FEW32, 1): (17, 16392, 264), (FEW64, 0): (5, 2056, 8200),
-         (FEW64, 1): (1, 16392, 4104), (TILE32x64, 0): (5, 264, 16392), (TILE32x64, 1): (64, 8200, 1160), (TILE32x128, 0): (1031, 136, 2056), (TILE32x128, 1): (100, 2056, 4104),
-         (TILE64x128, 0): (3000, 520, 1160), (TILE64x128, 1): (4096, 16392, 72), (TILE64x192, 0): (4096, 264, 1160), (TILE64x192, 1): (500, 4616, 2056), (TILE96x192, 0): (777, 264, 8200),
-         (TILE96x192, 1): (1031, 4616, 2056)},
-    32: {(FEW16, 0): (16, 264, 72), (FEW16, 1): (5, 4616, 136), (FEW32, 0): (5, 520, 4104), (FEW32, 1): (17, 8200, 520), (TILE32x64, 0): (500, 136, 520),
-         (TILE32x64, 1): (1031, 2056, 264), (TILE32x128, 0): (500, 136, 16392), (TILE32x128, 1): (333, 16392, 2056), (TILE64x128, 0): (1031, 520, 4104), (TILE64x128, 1): (100, 4616, 16392),
-         (TILE64x192, 1): (777, 16392, 520), (TILE96x192, 0): (3000, 136, 4104), (TILE96x192, 1): (2049, 3088, 2056)}}
+    128: {(FEW16, 0): (40, 136, 72), (FEW16, 1): (64, 8200, 8), (FEW32, 0): (40, 136, 2056), (FEW32, 1): (17, 16392, 264), (FEW64, 0): (777, 520, 264),
+         (FEW64, 1): (1, 16392, 4104), (TILE32x64, 0): (333, 8, 4104), (TILE32x64, 1): (500, 8200, 264), (TILE32x128, 0): (40, 1160, 8200), (TILE32x128, 1): (64, 3088, 4104),
+         (TILE64x128, 0): (1500, 520, 2056), (TILE64x128, 1): (2049, 16392, 72), (TILE64x192, 0): (2049, 8, 8200), (TILE64x192, 1): (4096, 8200, 136), (TILE96x192, 0): (2049, 264, 4104),
+         (TILE96x192, 1): (3000, 16392, 136), (TILE64x256, 0): (777, 136, 16392), (TILE64x256, 1): (64, 16392, 8200)},
+    64: {(FEW16, 0): (17, 136, 136), (FEW16, 1): (17, 16392, 8), (FEW32, 0): (40, 136, 2056), (FEW32, 1): (17, 8200, 520), (FEW64, 0): (40, 520, 4104),
+         (FEW64, 1): (1, 16392, 4104), (TILE32x64, 0): (40, 136, 4104), (TILE32x64, 1): (64, 4616, 2056), (TILE32x128, 0): (2049, 136, 1160), (TILE32x128, 1): (17, 3088, 16392),
+         (TILE64x128, 0): (777, 1160, 4104), (TILE64x128, 1): (4096, 16392, 72), (TILE64x192, 0): (500, 136, 16392), (TILE64x192, 1): (4096, 8200, 136), (TILE96x192, 0): (1500, 520, 2056),
+         (TILE96x192, 1): (1031, 8200, 1160)},
+    32: {(FEW16, 0): (1, 264, 1160), (FEW16, 1): (40, 8200, 8), (FEW32, 0): (5, 520, 4104), (FEW32, 1): (17, 8200, 520), (TILE32x64, 0): (64, 136, 4104),
+         (TILE32x64, 1): (500, 8200, 136), (TILE32x128, 0): (100, 520, 16392), (TILE32x128, 1): (333, 16392, 2056), (TILE64x128, 0): (1031, 264, 4104), (TILE64x128, 1): (100, 8200, 8200),
+         (TILE64x192, 1): (40, 16392, 16392), (TILE96x192, 0): (4096, 520, 2056), (TILE96x192, 1): (1031, 3088, 4104)}}
 
 
 def _launch(m, k, n, group, lent=(1 << 64) - 1):
