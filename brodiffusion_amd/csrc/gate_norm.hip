@@ -10,7 +10,7 @@
 // Bound: HBM. x and the branch are read once, h and y written once, the row stays in registers between its sums. The vectors come from the caches, which
 // they have to themselves: the rows of x, of the branch and of h are marked as passing through. y, which the next product reads, is not: with it 4608 rows of 6144
 // are 0.7 us faster, a block's norm, two products and norm 19 slower. Measured (us, gate, scale and shift, operands of 1 GiB in turn; without the marks): 4608 rows of 6144
-// 44.6 = 5.1 TB/s, a large copy's rate (51.6), 4608 of 2240 20.9 (24.0), 16384 of 1152 33.4 (38.0), 1000 of 6144 14.3 (16.4), one of 6144 4.4.
+// 42.5 = 5.3 TB/s, a large copy's rate (51.6), 4608 of 2240 19.6 (24.0), 16384 of 1152 31.1 (38.0), 1000 of 6144 14.6 (16.4), one of 6144 4.4.
 #include "rows_checks.h"
 
 namespace mi {
@@ -34,9 +34,11 @@ struct GateNorm {
 };
 
 // W wavefronts per row (one: four rows to a work group), N 16-byte chunks per lane, as in rows_int8.hip. (Work groups that stay, with the vectors in registers from row
-// to row and the next row on its way: 46 to 49 us instead of 44.6, their registers leave three wavefronts a SIMD.)
+// to row and the next row on its way: 46 to 49 us instead of 44.6, their registers leave three wavefronts a SIMD. Three chunks by
+// themselves take 97 registers, four wavefronts a SIMD; held to five, 4608 rows of 6144 take 42.5 us instead of 43.8, 4608 of 2240 19.6 for 20.8, 16384 of 1152 31.1 for 33.6,
+// but 4096 of 1152, with which four are all there are, 10.8 for 10.1. Two chunks, held to seven for six, were 4 % slower.)
 template <typename T, int N, int W>
-__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) gate_norm_kernel(const GateNorm a) {
+__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W, N == 3 ? 5 : 1) gate_norm_kernel(const GateNorm a) {
     typedef T t8 __attribute__((ext_vector_type(8)));
     constexpr int LANES = 64 * W;
     // (a chunk at a time where a lane has several: the FP32 values of all would cost wavefronts, of sixteen with 128 registers some would go to memory)
