@@ -1380,6 +1380,8 @@ def pack_int4(q, scales, zeros=None, group: int = 128) -> Int4Weight:
     _dev(op, q, scales, zeros)
     if q.dtype != torch.uint8 or q.dim() != 2 or q.shape[0] == 0 or q.shape[1] == 0 or (q.stride(1) != 1 and q.shape[1] > 1):
         _fail(op, "q must be uint8 (out_features, in_features / 2), contiguous along columns")
+    if q.shape[0] > 1 and q.stride(0) < q.shape[1]:
+        _fail(op, "q must be whole rows apart (an expanded row's stride of 0 would mean dense rows)")
     n, k = q.shape[0], 2 * q.shape[1]
     if group not in (32, 64) and (group <= 0 or group % 128):
         _fail(op, f"group {group} is neither 32, 64 nor a multiple of 128")
