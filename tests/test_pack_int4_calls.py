@@ -47,3 +47,22 @@ def test_rows_that_are_one(packed):
     for q in (one, torch.zeros(16 * 32 + 32, dtype=torch.uint8).as_strided((16, 64), (32, 1))):
         with pytest.raises(RuntimeError, match="pack_int4: q must be whole rows apart"):
             packed(q, _scales(16))
+
+
+def test_more_features_than_a_c_int(packed):
+    """2^32 + 16 features would be 16 to the C entry; beyond 2^30 every form refuses"""
+    for n, k, scales in ((2 ** 32 + 16, 8, 1), (16, 2 ** 32 + 8, 1), (2 ** 30 + 8, 8, 1), (16, 2 ** 30 + 8, 1)):
+        q = torch.empty(n, k // 2, dtype=torch.uint8, device="meta")
+        with pytest.raises(RuntimeError, match="pack_int4: more than 2\\^30 features"):
+            packed(q, torch.empty(n, scales, dtype=torch.bfloat16, device="meta"), group=2 ** 33)
+
+
+def test_weights_of_more_features_than_a_c_int(monkeypatch):
+    """... and a weight put together by hand"""
+    monkeypatch.setattr(ops, "_dev", lambda *a: None)
+    monkeypatch.setattr(ops, "_native", type("Declines", (), {"linear_int4": staticmethod(lambda *a: None)}))
+    meta = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="meta")
+    n = 2 ** 32 + 16
+    w = ops.Int4Weight(meta(1024, dtype=torch.uint8), meta(1, n), None, n, 128, 128)
+    with pytest.raises(RuntimeError, match="linear_int4: more than 2\\^30 features"):
+        ops.linear_int4(meta(1, 128), w, out=meta(1, n))
