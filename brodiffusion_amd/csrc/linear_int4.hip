@@ -78,7 +78,7 @@ int problem_of(const mi_linear_int4_args& a, const char* op, Int4Problem& p) {
     if (!a.x || !a.w || !a.scales || !a.y) return fail("%s: null operand", op);
     p.x = a.x; p.w = a.w; p.scales = a.scales; p.zeros = static_cast<const unsigned char*>(a.zeros); p.bias = a.bias; p.residual = a.residual; p.y = a.y;
     p.M = a.rows; p.N = a.out_features; p.K = a.in_features; p.act = a.activation;
-    p.KB = (p.K + 127) / 128; p.groups = (p.K + a.group - 1) / a.group; p.span = a.group > 128 ? a.group / 128 : 1;
+    p.KB = (p.K + 127) / 128; p.groups = static_cast<int>((p.K - 1L + a.group) / a.group); p.span = a.group > 128 ? a.group / 128 : 1;
     p.ldx = a.x_row_stride ? a.x_row_stride : p.K;
     p.ldy = a.y_row_stride ? a.y_row_stride : p.N;
     p.ldr = a.residual_row_stride ? a.residual_row_stride : p.N;

@@ -1360,9 +1360,12 @@ def linear_act(X, W, bias=None, *, activation: str = "none", residual: Optional[
     return out
 
 
-def _int4_features(op: str, n: int, k: int):
-    if max(n, k) > 1 << 30:      # (as the C entries, which would take them modulo 2^32)
+def _int4_sizes(op: str, n: int, k: int, group: int):
+    # (what the C entries would take modulo 2^32)
+    if max(n, k) > 1 << 30:
         _fail(op, "more than 2^30 features are not supported")
+    if group > 0x7fffffff:
+        _fail(op, f"group {group} is more than 2^31 - 1")
 
 
 @dataclass(frozen=True)
@@ -1388,7 +1391,7 @@ def pack_int4(q, scales, zeros=None, group: int = 128) -> Int4Weight:
     if q.shape[0] > 1 and q.stride(0) < q.shape[1]:
         _fail(op, "q must be whole rows apart (an expanded row's stride of 0 would mean dense rows)")
     n, k = q.shape[0], 2 * q.shape[1]
-    _int4_features(op, n, k)
+    _int4_sizes(op, n, k, group)
     if group not in (32, 64) and (group <= 0 or group % 128):
         _fail(op, f"group {group} is neither 32, 64 nor a multiple of 128")
     _dtype_code(op, scales)
@@ -1426,7 +1429,7 @@ def linear_int4(X, W: Int4Weight, bias=None, *, activation: str = "none", residu
     a.struct_size = C.sizeof(a)
     a.dtype = _dtype_code(op, X)
     n, k, dtype = W.out_features, W.in_features, X.dtype
-    _int4_features(op, n, k)
+    _int4_sizes(op, n, k, W.group)
     if X.dim() < 1 or X.shape[-1] != k:
         _fail(op, f"X is {tuple(X.shape)}, W has {k} in_features")
     groups = -(-k // W.group) if W.group > 0 else 0

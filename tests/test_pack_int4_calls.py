@@ -66,3 +66,14 @@ def test_weights_of_more_features_than_a_c_int(monkeypatch):
     w = ops.Int4Weight(meta(1024, dtype=torch.uint8), meta(1, n), None, n, 128, 128)
     with pytest.raises(RuntimeError, match="linear_int4: more than 2\\^30 features"):
         ops.linear_int4(meta(1, 128), w, out=meta(1, n))
+
+
+def test_groups_past_a_c_int(packed, monkeypatch):
+    """2^32 + 128 elements would be groups of 128 to the C entry, of which the scales have only the first"""
+    q = torch.zeros(16, 128, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="pack_int4: group 4294967424 "):
+        packed(q, _scales(16), group=2 ** 32 + 128)
+    monkeypatch.setattr(ops, "_native", type("Declines", (), {"linear_int4": staticmethod(lambda *a: None)}))
+    w = ops.Int4Weight(torch.empty(1024, dtype=torch.uint8), torch.ones(1, 16, dtype=torch.bfloat16), None, 16, 256, 2 ** 32 + 128)
+    with pytest.raises(RuntimeError, match="linear_int4: group 4294967424 "):
+        ops.linear_int4(torch.zeros(1, 256, dtype=torch.bfloat16), w, out=torch.zeros(1, 16, dtype=torch.bfloat16))
