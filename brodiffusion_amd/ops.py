@@ -1230,7 +1230,7 @@ def _vectors_of(op: str, v, name: str, X, rows: int):
     while lead and lead[-1] == 1:
         lead.pop()
     items = math.prod(lead)
-    if lead != list(X.shape[:len(lead)]) and not (X.dim() == 2 and len(lead) == 1 and rows % max(items, 1) == 0) or len(lead) >= X.dim():
+    if lead != list(X.shape[:len(lead)]) and not (X.dim() == 2 and len(lead) == 1 and items > 0 and rows % items == 0) or len(lead) >= X.dim():
         _fail(op, f"{name} is {tuple(v.shape)}: neither ({cols},) nor one vector for each of X's leading sizes, {tuple(X.shape)}")
     if items == 1:
         if v.stride(-1) != 1 and cols > 1:
