@@ -357,21 +357,29 @@ const void* columns_ptr(PyObject* o, const Tensor& x) {
     need(t.scalar_type() == x.scalar_type() && t.numel() == x.size(-1) && t.is_contiguous());
     return t.data_ptr();
 }
-// one vector for all rows, or (items, cols) / (items, 1, cols) with X's leading size, or one that divides a 2-D X's rows, as items
+// one vector for all rows, or one for each of X's leading sizes or the first of them (with ones behind them), or of a 2-D X (items, cols) with a number of items
+// that divides its rows; all equally far apart
 const void* vectors_ptr(PyObject* o, const Tensor& x, int64_t rows, int32_t& each, int64_t& stride) {
     if (none(o)) return nullptr;
     const Tensor& t = tensor(o);
     const int64_t cols = x.size(-1);
-    need(t.scalar_type() == x.scalar_type() && t.dim() >= 1 && t.dim() <= 3 && t.size(-1) == cols && t.stride(-1) == 1);
-    if (t.dim() == 1) { stride = cols; return t.data_ptr(); }
-    need(t.dim() == 2 || t.size(1) == 1);
-    const int64_t items = t.size(0);
-    need(items > 0 && (items == x.size(0) || x.dim() == 2) && x.dim() >= 2 && rows % items == 0);
-    if (items > 1) {
-        need(t.stride(0) >= cols && rows > 0);
-        each = static_cast<int32_t>(rows / items);
+    need(t.scalar_type() == x.scalar_type() && t.dim() >= 1 && t.size(-1) == cols && t.stride(-1) == 1);
+    int64_t lead = t.dim() - 1, items = 1, outer = -1;      // outer: the stride that the next axis outwards has to have
+    while (lead > 0 && t.size(lead - 1) == 1) --lead;
+    need(lead < x.dim());
+    bool alike = true;
+    for (int64_t i = 0; i < lead; ++i) { items *= t.size(i); alike = alike && t.size(i) == x.size(i); }
+    need(items > 0 && (alike || (x.dim() == 2 && lead == 1 && rows % items == 0)));
+    stride = cols;
+    if (items == 1) return t.data_ptr();
+    for (int64_t i = lead - 1; i >= 0; --i) {
+        if (t.size(i) == 1) continue;
+        if (outer < 0) stride = t.stride(i);
+        need(stride >= cols && (outer < 0 || t.stride(i) == outer));
+        outer = t.stride(i) * t.size(i);
     }
-    stride = items > 1 ? t.stride(0) : cols;
+    need(rows > 0);
+    each = static_cast<int32_t>(rows / items);
     return t.data_ptr();
 }
 // X, branch, gate, post, post_gain, post_eps, residual_scale, norm, gain, scale, shift, eps, sum_out, out

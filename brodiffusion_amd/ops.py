@@ -1221,7 +1221,8 @@ _NORMS = {"none": capi.MI_NORM_NONE, "rms": capi.MI_NORM_RMS, "layer": capi.MI_N
 
 def _vectors_of(op: str, v, name: str, X, rows: int):
     """A vector of X's columns for all rows, or one for each run of rows: (cols), X's leading sizes or the first of them (with ones behind them) before
-    cols, or, for a 2-D X, (items, cols) with items dividing its rows. Returns (address, rows that share one or 0 for all, row stride)."""
+    cols, or, for a 2-D X, (items, cols) with items dividing its rows; contiguous along columns, all equally far apart. Returns (address, rows that share one
+    or 0 for all, row stride)."""
     _dev(op, v)
     cols = X.shape[-1]
     if v.dtype != X.dtype or v.dim() < 1 or v.shape[-1] != cols:
@@ -1232,13 +1233,10 @@ def _vectors_of(op: str, v, name: str, X, rows: int):
     items = math.prod(lead)
     if lead != list(X.shape[:len(lead)]) and not (X.dim() == 2 and len(lead) == 1 and items > 0 and rows % items == 0) or len(lead) >= X.dim():
         _fail(op, f"{name} is {tuple(v.shape)}: neither ({cols},) nor one vector for each of X's leading sizes, {tuple(X.shape)}")
-    if items == 1:
-        if v.stride(-1) != 1 and cols > 1:
-            _fail(op, f"{name} must be contiguous along columns")
-        return v.data_ptr(), 0, cols
-    if items == 0:
-        return v.data_ptr(), 0, cols
-    return v.data_ptr(), rows // items, _rows_of(op, v.reshape(items, cols) if v.is_contiguous() else v.squeeze(1) if v.dim() == 3 else v, name, X.dtype)[1]
+    axes = [(n, s) for n, s in zip(lead, v.stride()) if n > 1] if items > 0 else []
+    if (v.stride(-1) != 1 and items > 0) or any(outer[1] != inner[0] * inner[1] for outer, inner in zip(axes, axes[1:])) or (axes and axes[-1][1] < cols):
+        _fail(op, f"{name} must be contiguous along columns, its vectors equally far apart and at least {cols} elements")
+    return v.data_ptr(), rows // items if axes else 0, axes[-1][1] if axes else cols
 
 
 def gate_add_norm(X, branch, *, gate=None, post: str = "none", post_gain=None, post_eps: Optional[float] = None, residual_scale: float = 1.0, norm: str = "rms",
@@ -1246,8 +1244,9 @@ def gate_add_norm(X, branch, *, gate=None, post: str = "none", post_gain=None, p
     """(h, y): a block's output into the residual stream and the norm in front of the next block (mi_gate_add_norm_forward),
         h = residual_scale * X + gate * post(branch) * post_gain, rounded to X's dtype,   y = norm(h) * gain * (1 + scale) + shift.
     post and norm: "none", "rms" or "layer" (without weights of their own), eps of either (post_eps None: eps). X (..., cols), branch of its shape, or None:
-    h is X. gate, scale and shift: (cols), or one vector for each of X's leading sizes, (batch, cols) or (batch, 1, cols) of a (batch, tokens, cols) X, any row
-    stride; for a 2-D X (items, cols), each for rows / items rows. norm "none": y is None. sum_out and out may be X or branch."""
+    h is X. gate, scale and shift: (cols), or one vector for each of X's leading sizes, (batch, cols), (batch, 1, cols) or (batch, tokens, cols) of a
+    (batch, tokens, cols) X; for a 2-D X (items, cols), each for rows / items rows; any row stride that all vectors share (a slice of a
+    modulation's columns). norm "none": y is None. sum_out and out may be X or branch."""
     op = "gate_add_norm"
     r = _native.gate_add_norm(X, branch, gate, post, post_gain, post_eps, residual_scale, norm, gain, scale, shift, eps, sum_out, out)
     if r is not None:
