@@ -98,8 +98,6 @@ int problem_of(const mi_linear_int4_args& a, const char* op, Int4Problem& p) {
     if (runs_share(p.y, y_run, p.scales, 2 * per_group)) return fail("%s: y overlaps scales", op);
     if (runs_share(p.y, y_run, p.zeros, per_group)) return fail("%s: y overlaps zeros", op);
     if (runs_share(p.y, y_run, p.bias, 2L * p.N)) return fail("%s: y overlaps the bias", op);
-    // (work groups of 16 rows lie in the second grid dimension)
-    if ((p.M + 31L) / 32 * ((p.N + 63L) / 64) > 0x7ffffff0L || (int4_far_apart(p.N, p.ldx) && p.M > 65535L * 16)) return fail("%s: problem too large for one launch", op);
     return 1;
 }
 
@@ -160,6 +158,7 @@ int mi_linear_int4_forward(const mi_linear_int4_args* a) {
     if (mi::check_scratch(p, op, a->scratch, a->scratch_bytes)) return -1;
     const int parts = mi::int4_parts(a->group);
     const mi::Int4Launch launch = mi::launch_of(p, a->group, a->scratch ? a->scratch_bytes : 0);
+    if (launch.form < 0) return mi::fail("%s: problem too large for one launch", op);
     p.shares = launch.shares;
     p.parts = launch.shares > 1 ? static_cast<float*>(a->scratch) : nullptr;
     const hipStream_t st = mi::resolve_stream(a->stream);

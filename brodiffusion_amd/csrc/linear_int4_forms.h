@@ -31,11 +31,12 @@ inline constexpr Int4FormRule kInt4Rules[kInt4Forms] = {
     {96, 192, 2, {{2.57f, 1.14f, 0.454f, 0.714f}, {4.03f, 1.17f, 0.738f, 0.0f}, {6.13f, 1.81f, 1.1f, 0.0f}}},    // kTile96x192
     {64, 256, 2, {{3.81f, 1.07f, 0.435f, 0.0598f}, {0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}}},    // kTile64x256
 };
-// A launch: its form, and the shares that the contraction is given in, each to work groups of its own (1: all in one). Shares cost a second launch, which
-// adds them, and what it reads and writes: kJoin us, fitted with the rest, and 1 us for kJoinBytes of sums, half of what a copy moves, as they are written and read
-// (4096 x 4608 x 1152 in two shares of 64 x 192, 38 MB: 74 + 12 us, in one 72)
+// A launch: its form (-1: none, every grid would have 2^32 work-items across or 2^16 work groups down and more), and the shares that the contraction is given in, each
+// to work groups of its own (1: all in one). Shares cost a second launch, which adds them, and what it reads and writes: kJoin us, fitted with the rest, and 1 us for
+// kJoinBytes of sums, half of what a copy moves, as they are written and read (4096 x 4608 x 1152 in two shares of 64 x 192, 38 MB: 74 + 12 us, in one 72)
 struct Int4Launch { int form, shares; };
 constexpr int kInt4Shares[] = {1, 2, 3, 4, 6, 8, 12, 16};
+constexpr long kMostItems = 0xffffffffL;      // work-items of a grid across: 512 for a run of features (few rows), 256 for a tile of a multiple of 8
 constexpr float kJoin = 3.5f, kJoinBytes = 3.0e6f;
 inline Int4Launch int4_launch(int M, int N, int KB, long ldx, int parts, int cu, unsigned long lent) {
     const int which = parts == 1 ? 0 : parts == 2 ? 1 : 2, forms = int4_far_apart(N, ldx) ? kTile32x64 : kInt4Forms;
@@ -43,8 +44,10 @@ inline Int4Launch int4_launch(int M, int N, int KB, long ldx, int parts, int cu,
     float least = 0.f;
     for (int i = 0; i < forms; ++i) {
         const Int4FormRule& f = kInt4Rules[i];
-        if ((parts == 4 && i == kFew64) || (parts > 1 && i == kTile64x256) || (i < kTile32x64 && M > 65535L * 16)) continue;
-        const float whole = static_cast<float>((static_cast<long>(M) + f.rows - 1) / f.rows * ((static_cast<long>(N) + f.features - 1) / f.features));
+        const long down = (static_cast<long>(M) + f.rows - 1) / f.rows, across = (static_cast<long>(N) + f.features - 1) / f.features;
+        if ((parts == 4 && i == kFew64) || (parts > 1 && i == kTile64x256)) continue;
+        if (i < kTile32x64 ? down > 65535 || across > kMostItems / 512 : down * across > kMostItems / 256 - 7) continue;
+        const float whole = static_cast<float>(down * across);
         for (const int shares : kInt4Shares) {
             const float bytes = 4.f * shares * M * N;
             if (shares > 1 && (KB < 4 * shares || whole * shares > 4 * cu || bytes > 1e9f || 4ul * shares * M * N > lent)) break;

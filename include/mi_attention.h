@@ -574,7 +574,8 @@ MI_API size_t mi_linear_act_scratch_bytes(const mi_linear_act_args* args);
  *
  * in_features and out_features are multiples of 8, group is 32, 64 or a multiple of 128 (the last one may be shorter); strides in elements (0 = dense), multiples
  * of 8, at most 2^40, rows times stride at most 2^56; operands 16-byte aligned, zeros 8-byte, q 4-byte. y may be `residual` itself (same pointer and stride); a
- * call whose y shares other memory with an operand is refused. rows may be 0. */
+ * call whose y shares other memory with an operand is refused. rows may be 0. Refused too is what no grid holds: more than 2^28 - 32 out_features (2^29 - 64 with groups of
+ * 64 and more), about 3 * 10^11 results, or 1048560 rows with more than 2^24 out_features or an x row stride beyond 11184810 elements. */
 typedef struct mi_pack_int4_args {
     uint32_t struct_size;
     const void* q;
