@@ -64,6 +64,7 @@ HOST_LIB = os.path.join(LIB_DIR, "libbrodiffusion_amd_host.so")
 HOST_TEST = os.path.join(LIB_DIR, "test_host_ops")
 BLOCK_TEST = os.path.join(LIB_DIR, "test_block_half")
 STEP_TEST = os.path.join(LIB_DIR, "test_gated_step")
+SIZES_TEST = os.path.join(LIB_DIR, "test_int4_sizes")
 SCRATCH_TEST = os.path.join(LIB_DIR, "test_linear_act_scratch")
 SPLIT_TEST = os.path.join(LIB_DIR, "test_split_geo")
 FORMS_LIB = os.path.join(LIB_DIR, "liblinear_forms_test.so")
@@ -88,7 +89,7 @@ def build_host(with_test: bool = True, verbose: bool = False) -> str:
         # (the last one captures graphs itself)
         hip = ["-D__HIP_PLATFORM_AMD__", "-isystem" + os.path.join(rocm, "include"), "-L" + os.path.join(rocm, "lib"), "-lamdhip64"]
         for source, exe, more in (("test_host_ops.cpp", HOST_TEST, []), ("test_block_half.cpp", BLOCK_TEST, []), ("test_gated_step.cpp", STEP_TEST, []),
-                                  ("test_linear_act_scratch.cpp", SCRATCH_TEST, hip)):
+                                  ("test_int4_sizes.cpp", SIZES_TEST, []), ("test_linear_act_scratch.cpp", SCRATCH_TEST, hip)):
             cmd = [*common, os.path.join(ROOT, "tests", "cpp", source), "-o", exe, *rpath,
                    "-Wl,-rpath,$ORIGIN/../../oracle", "-L" + oracle_dir, "-lbrodiffusion_amd_host", "-lmi_attention", "-loracle", *more]
             r = subprocess.run(cmd, capture_output=True, text=True)

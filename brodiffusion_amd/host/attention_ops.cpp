@@ -430,10 +430,12 @@ void pack_int4(const Tensor& q, Tensor& packed) {
     const char* op = "pack_int4";
     need_gpu(op, q);
     own_tensor(op, "packed", &packed, {&q});
-    const std::size_t bytes = q.cols > 0 && q.cols <= (1 << 30) - 1 ? mi_int4_packed_bytes(q.rows, 2 * q.cols) : 0;
+    if (q.dtype != Dtype::INT8 || q.rows <= 0 || q.cols <= 0) fail(std::string(op) + ": q must hold (out_features, in_features / 2) bytes (INT8)");
+    if (q.rows % 8 != 0 || q.cols % 4 != 0) fail(std::string(op) + ": in_features and out_features must be multiples of 8");
+    constexpr int most = (1 << 28) - 128;      // (of whose 16 rows the packed kilobytes, a row of `packed`, are the most that an int counts)
+    if (q.cols > most / 2 || q.rows > 1 << 30) fail(std::string(op) + ": more than 2^28 - 128 in_features or 2^30 out_features are not supported");
     const int blocks = (q.rows + 15) / 16;
-    if (q.dtype != Dtype::INT8 || bytes == 0) fail(std::string(op) + ": q must hold (out_features, in_features / 2) bytes (INT8)");
-    fit(packed, blocks, static_cast<int>(bytes / blocks), Dtype::INT8, q.device);
+    fit(packed, blocks, static_cast<int>(mi_int4_packed_bytes(q.rows, 2 * q.cols) / blocks), Dtype::INT8, q.device);
     mi_pack_int4_args a;
     std::memset(&a, 0, sizeof(a));
     a.struct_size = sizeof(a);

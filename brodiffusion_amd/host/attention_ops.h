@@ -98,7 +98,7 @@ void gate_add_norm(const Tensor& X, const GateAddNorm& step, Tensor* sum, Tensor
 
 // Y = act(X W^T + bias) + residual with 4-bit weights, W[n][k] = (q[n][k] - zeros[g][n]) * scales[g][n], g = k / group (mi_linear_int4_forward). pack_int4 lays q out
 // once: (out_features, in_features / 2) bytes in an INT8 tensor, element 2 j of a row in the low half of byte j. scales (groups, out_features) of X's dtype, zeros
-// the same in bytes (INT8) or null: 8; bias and residual may be null, residual may be Y itself. Scratch as in linear_act.
+// the same in bytes (INT8) or null: 8; bias and residual may be null, residual may be Y itself. in_features at most 2^28 - 128. Scratch as in linear_act.
 void pack_int4(const Tensor& q, Tensor& packed);
 void linear_int4(const Tensor& X, const Tensor& packed, const Tensor& scales, const Tensor* zeros, int group, const Tensor* bias, Activation activation,
                  const Tensor* residual, Tensor& Y);
