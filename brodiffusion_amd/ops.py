@@ -1414,7 +1414,7 @@ def pack_int4(q, scales, zeros=None, group: int = 128) -> Int4Weight:
 def linear_int4(X, W: Int4Weight, bias=None, *, activation: str = "none", residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
     """act(X W^T + bias) + residual with 4-bit weights (mi_linear_int4_forward): X (..., in_features), W of pack_int4 with scales of X's dtype, bias
     (out_features), residual (..., out_features); activations as linear_act. FP32 behind the operands, one rounding; no weight is rounded to 16 bits. A row of X
-    with a value that is not finite gives NaN. `out` may be the residual itself."""
+    with a value that is not finite gives NaN, one with bf16 values beyond 2^112 may. `out` may be the residual itself."""
     op = "linear_int4"
     if not isinstance(W, Int4Weight):
         _fail(op, "W must be what pack_int4 returns")

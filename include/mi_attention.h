@@ -563,7 +563,9 @@ MI_API size_t mi_linear_act_scratch_bytes(const mi_linear_act_args* args);
 /* ── linear layer with 4-bit weights ───────────────────────────────────────
  * Y = act(X W^T + bias) + residual with W[n][k] = (q[n][k] - zeros[g][n]) * scales[g][n], g = k / group: 4-bit integers q of 0 .. 15 with a scale, and where
  * there are zeros a zero point (else 8), for each group of the contraction. Weights are not rounded to 16 bits: a group's product is summed in FP32 and meets its
- * scale there; bias, activation and residual follow in FP32, one rounding to `dtype`. A row of x with a value that is not finite gives NaN. No result
+ * scale there; bias, activation and residual follow in FP32, one rounding to `dtype`. A row of x with a value that is not finite gives NaN. What is summed
+ * ahead of the scale are q x and zeros x, not their difference: (15 + zero point) times the sum of |x| over 128 neighbours has to stay within FP32, as it does for
+ * every fp16 row and for bf16 rows of values up to 2^112; beyond that a finite row can give infinities or NaN. No result
  * depends on timing or on what the other rows of its call hold; FP32 sums round in the order that sizes, type and the scratch that is lent lead to. From one row to
  * thousands.
  *
