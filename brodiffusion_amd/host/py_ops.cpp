@@ -119,9 +119,14 @@ const char* name_of(PyObject* op) {
 const float* f32(const Tensor& t) { return static_cast<const float*>(t.data_ptr()); }
 int rows32(int64_t n) { need(n >= 0 && n <= 0x7fffffff); return static_cast<int>(n); }
 
+// not an expanded tensor: to the C entries a stride of 0 means dense
+void need_apart(const Tensor& t) {
+    for (int64_t i = 0; i < t.dim(); ++i) need(t.stride(i) != 0 || t.size(i) <= 1);
+}
 // (rows, cols) or (batch, rows, cols), contiguous along columns
 struct Mat { int64_t b, rows, cols, rs, bs; };
 Mat as3(const Tensor& t) {
+    need_apart(t);
     if (t.dim() == 2) {
         need(t.stride(1) == 1);
         return {1, t.size(0), t.size(1), t.stride(0), t.stride(0) * t.size(0)};
@@ -241,6 +246,7 @@ NATIVE(rms_norm, 4)
     need(x.dim() == 2 && x.stride(1) == 1 && g.scalar_type() == x.scalar_type() && g.numel() == x.size(1) && g.is_contiguous());
     const Tensor y = none(a[3]) ? at::empty_like(x) : tensor(a[3]);
     need(y.sizes() == x.sizes() && y.scalar_type() == x.scalar_type() && y.stride(1) == 1);
+    need_apart(x); need_apart(y);
     const void *const px = x.data_ptr(), *const pg = g.data_ptr();
     void* const py = y.data_ptr();
     const int rows = rows32(x.size(0)), cols = rows32(x.size(1)), dt = dtype_code(x);
@@ -544,6 +550,7 @@ NATIVE(rope, 9)
     need(hd > 0 && heads > 0 && x.dim() == 2 && x.stride(1) == 1 && x.size(1) == static_cast<int64_t>(hd) * heads);
     const Tensor y = none(a[5]) ? at::empty_like(x) : tensor(a[5]);
     need(y.sizes() == x.sizes() && y.scalar_type() == x.scalar_type() && y.stride(1) == 1);
+    need_apart(x); need_apart(y);
     mi_rope_args p;
     std::memset(&p, 0, sizeof(p));
     p.struct_size = sizeof(p);
@@ -567,6 +574,7 @@ NATIVE(headnorm_rope, 10)
     need(g.scalar_type() == x.scalar_type() && g.numel() == hd && g.is_contiguous());
     const Tensor y = none(a[7]) ? at::empty_like(x) : tensor(a[7]);
     need(y.sizes() == x.sizes() && y.scalar_type() == x.scalar_type() && y.stride(1) == 1);
+    need_apart(x); need_apart(y);
     mi_headnorm_rope_args p;
     std::memset(&p, 0, sizeof(p));
     p.struct_size = sizeof(p);
@@ -581,6 +589,7 @@ NATIVE(headnorm_rope, 10)
     if (!none(a[8])) {
         const Tensor& c = tensor(a[8]);
         need(c.dim() == 2 && c.scalar_type() == x.scalar_type() && c.size(1) == x.size(1) && c.stride(1) == 1 && c.size(0) <= x.size(0));
+        need_apart(c);
         p.out2 = c.data_ptr(); p.out2_rows = rows32(c.size(0)); p.out2_row_stride = c.stride(0);
     }
     p.stream = current_stream();

@@ -110,8 +110,16 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _apart(op: str, **tensors):
+    """No expanded tensors: to the C entries a stride of 0 means dense, and they would read on where the one row or item ends."""
+    for name, t in tensors.items():
+        if t is not None and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+            _fail(op, f"{name} is expanded (one row or item for several): make it contiguous")
+
+
 def _as3(op: str, t: torch.Tensor, name: str):
     """(rows, cols) or (batch, rows, cols) -> (batch, rows, cols, row_stride, batch_stride)."""
+    _apart(op, **{name: t})
     if t.dim() == 2:
         if t.stride(1) != 1:
             _fail(op, f"{name} must be contiguous along columns")
@@ -288,6 +296,7 @@ def sdpa_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: i
         _dev(op, logit_bias)
         if logit_bias.dtype != torch.float32 or logit_bias.dim() != 2 or logit_bias.stride(1) != 1:
             _fail(op, "logit_bias must be a 2-D float32 tensor, contiguous along columns")
+        _apart(op, logit_bias=logit_bias)
         if logit_bias.shape[0] != Lq - bias_q0:
             _fail(op, f"logit_bias must have one row per query row from bias_q0 on ({Lq - bias_q0}), has {logit_bias.shape[0]}")
         a.logit_bias, a.bias_q0, a.bias_cols = logit_bias.data_ptr(), bias_q0, logit_bias.shape[1]
@@ -375,6 +384,7 @@ def flash_attention_varlen_forward(q, k, v, cu_q, cu_k, n_seqs: int, max_q: int,
         out = torch.empty_like(q)
     if out.shape != q.shape or out.dtype != q.dtype or out.stride(1) != 1:
         _fail(op, "out must have q's shape and dtype")
+    _apart(op, q=q, k=k, v=v, out=out)
     a = capi.MiSdpaArgs()
     a.struct_size = C.sizeof(capi.MiSdpaArgs)
     a.dtype = dt
@@ -532,6 +542,7 @@ def add_inplace_row_bias(Y, bias):
     _dev(op, Y, bias)
     if Y.dim() != 2 or Y.stride(1) != 1:
         _fail(op, "Y must be 2-D, contiguous along columns")
+    _apart(op, Y=Y)
     if bias.dtype != Y.dtype or bias.numel() != Y.shape[1] or not bias.is_contiguous():
         _fail(op, f"bias must hold {Y.shape[1]} values of Y's dtype")
     capi.check(capi.lib().mi_add_row_bias(Y.data_ptr(), bias.data_ptr(), Y.shape[0], Y.shape[1], Y.stride(0), _dtype_code(op, Y), _stream()), op)
@@ -711,6 +722,7 @@ def _rope(op: str, X, cos, sin, head_dim, num_heads, out, per_head: bool, split_
         out = torch.empty_like(X)
     if out.shape != X.shape or out.dtype != X.dtype or out.stride(1) != 1:
         _fail(op, "out must have X's shape and dtype")
+    _apart(op, X=X, out=out)
     a = capi.MiRopeArgs()
     a.struct_size = C.sizeof(capi.MiRopeArgs)
     a.dtype = dt
@@ -743,6 +755,7 @@ def scale_rows(X, scale: float = 1.0, row_scale: Optional[torch.Tensor] = None, 
         out = torch.empty_like(X)
     if out.shape != X.shape or out.dtype != X.dtype or out.stride(1) != 1:
         _fail(op, "out must have X's shape and dtype")
+    _apart(op, X=X, out=out)
     a = capi.MiScaleRowsArgs()
     a.struct_size = C.sizeof(a)
     a.dtype = _dtype_code(op, X)
@@ -777,6 +790,7 @@ def headnorm_rope(X, gain, eps: float, cos, sin, head_dim: int, num_heads: int, 
         out = torch.empty_like(X)
     if out.shape != X.shape or out.dtype != X.dtype or out.stride(1) != 1:
         _fail(op, "out must have X's shape and dtype")
+    _apart(op, X=X, out=out)
     a = capi.MiHeadnormRopeArgs()
     a.struct_size = C.sizeof(a)
     a.dtype = _dtype_code(op, X)
@@ -796,6 +810,7 @@ def headnorm_rope(X, gain, eps: float, cos, sin, head_dim: int, num_heads: int, 
         if cache_out.dim() != 2 or cache_out.dtype != X.dtype or cache_out.shape[1] != X.shape[1] or cache_out.stride(1) != 1 \
                 or cache_out.shape[0] > X.shape[0]:
             _fail(op, "cache_out must be (rows <= L, head_dim * num_heads) of X's dtype")
+        _apart(op, cache_out=cache_out)
         a.out2, a.out2_rows, a.out2_row_stride = cache_out.data_ptr(), cache_out.shape[0], cache_out.stride(0)
     a.stream = _stream()
     capi.check(capi.lib().mi_headnorm_rope(C.byref(a)), op)
@@ -838,6 +853,7 @@ def attention_map_avg(q, k, lse, num_heads: int, *, scale: Optional[float] = Non
         out = torch.empty(Lq, Lk, dtype=torch.float32, device=q.device)
     if out.dtype != torch.float32 or tuple(out.shape) != (Lq, Lk) or out.stride(1) != 1:
         _fail(op, "out must be float32 (Lq, Lk)")
+    _apart(op, q=q, k=k, out=out, logit_bias=logit_bias)
     a = capi.MiAttentionMapArgs()
     a.struct_size = C.sizeof(a)
     a.dtype = _dtype_code(op, q)
@@ -1111,6 +1127,7 @@ def rms_norm_rows(X, gain, eps: float, out: Optional[torch.Tensor] = None):
         out = torch.empty_like(X)
     if out.shape != X.shape or out.dtype != X.dtype or out.stride(1) != 1:
         _fail(op, "out must have X's shape and dtype")
+    _apart(op, X=X, out=out)
     capi.check(capi.lib().mi_rms_norm_forward(X.data_ptr(), gain.data_ptr(), out.data_ptr(), X.shape[0], X.shape[1], X.stride(0),
                                               out.stride(0), eps, dt, _stream()), op)
     return out
