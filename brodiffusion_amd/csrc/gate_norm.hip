@@ -10,7 +10,8 @@
 // Bound: HBM. x and the branch are read once, h and y written once, the row stays in registers between its sums. The vectors come from the caches, which
 // they have to themselves: the rows of x, of the branch and of h are marked as passing through. y, which the next product reads, is not: with it 4608 rows of 6144
 // are 0.7 us faster, a block's norm, two products and norm 19 slower. Measured (us, gate, scale and shift, operands of 1 GiB in turn; without the marks): 4608 rows of 6144
-// 42.5 = 5.3 TB/s, a large copy's rate (51.6), 4608 of 2240 19.6 (24.0), 16384 of 1152 31.1 (38.0), 1000 of 6144 14.6 (16.4), one of 6144 4.4.
+// 42.7 = 5.3 TB/s, a large copy's rate (51.6), 4608 of 2240 19.6 (24.0), 16384 of 1152 31.5 (38.0), 1000 of 6144 14.4 (16.4), one of 6144 4.1. 4608 of 6144 without a branch
+// 25.6 = 4.4 TB/s, beside 84 % of the vector instruction slots; the sum alone 28.9 = 5.9 TB/s.
 #include "rows_checks.h"
 
 namespace mi {
@@ -35,8 +36,9 @@ struct GateNorm {
 
 // W wavefronts per row (one: four rows to a work group), N 16-byte chunks per lane, as in rows_int8.hip. (Work groups that stay, with the vectors in registers from row
 // to row and the next row on its way: 46 to 49 us instead of 44.6, their registers leave three wavefronts a SIMD. Three chunks by
-// themselves take 97 registers, four wavefronts a SIMD; held to five, 4608 rows of 6144 take 42.5 us instead of 43.8, 4608 of 2240 19.6 for 20.8, 16384 of 1152 31.1 for 33.6,
-// but 4096 of 1152, with which four are all there are, 10.8 for 10.1. Two chunks, held to seven for six, were 4 % slower.)
+// themselves take 97 registers, four wavefronts a SIMD; held to five, 4608 rows of 6144 take 42.7 us instead of 43.8, 4608 of 2240 19.6 for 20.9, 16384 of 1152 31.5 for 33.9,
+// but rows that are four wavefronts a SIMD or one round of them lose: 4096 of 1152 10.9 for 10.2, 2048 of 2240 10.8 for 10.2, 1024 of 6144 12.9 for 12.4. Two chunks, held to
+// seven for six, were 4 % slower.)
 template <typename T, int N, int W>
 __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W, N == 3 ? 5 : 1) gate_norm_kernel(const GateNorm a) {
     typedef T t8 __attribute__((ext_vector_type(8)));
@@ -230,8 +232,8 @@ int launch_chunks(const GateNorm& a, hipStream_t st) {
 }
 
 // Wavefronts of a row: many for few rows, whose latency a chunk more adds to, few where rows fill the card. Measured (us, 2 / 4 / 8 / 16 wavefronts, three vectors): one row
-// of 2240 4.4 / 3.9 / 4.2, 4608 rows 20.9 / 22.4 / 34.8; one of 6144 - / 4.6 / 4.2 / 5.3, 4608 rows - / 43.9 / 46.7 / 88.2. Over 58 sizes (1 to 16384 rows of 320 to 16384
-// columns) the rule's choice is 0.4 % slower than the fastest on average, 6 % at most.
+// of 2240 4.0 / 3.8 / 4.0, 4608 rows 19.6 / 22.6 / 34.8; one of 6144 - / 4.2 / 4.1 / 5.2, 4608 rows - / 42.7 / 47.2 / 88.5. Over 64 sizes (1 to 16384 rows of 320 to 16384
+// columns) the rule's choice is 0.5 % slower than the fastest on average, 12 % at most (1000 rows of 6144: 14.4, four wavefronts 12.8).
 template <typename T>
 int launch_width(const GateNorm& a, hipStream_t st) {
     const int chunks = a.cols / 8, each = a.rows >= 4 * device_cu_count() ? 3 : 2;

@@ -22,8 +22,8 @@ __global__ void __launch_bounds__(256) pack_int4_kernel(const unsigned char* q, 
 }
 
 // The sums of the shares of a contraction, added in their order, and what follows them: 4 features per thread. Shares put compute units to work that one work group for
-// each piece of Y would leave idle: 20 x 16384 x 6144 (rows x contraction x features) 26.5 -> 19.2 us, 128 x 16384 x 6144 67 -> 43, 1 x 16384 x 128 9.6 -> 6.2; this launch
-// is about 3.5 us of that. The rule for them is int4_launch's.
+// each piece of Y would leave idle: 20 x 16384 x 6144 (rows x contraction x features, operands from memory) 28.7 -> 21.9 us, 128 x 16384 x 6144 70.5 -> 43.6,
+// 1 x 16384 x 128 11.8 -> 6.5; this launch is 3.5 to 4.5 us of that. The rule for them is int4_launch's.
 template <typename T>
 __global__ void __launch_bounds__(256) join_int4_kernel(const Int4Problem p) {
     typedef T t4 __attribute__((ext_vector_type(4)));

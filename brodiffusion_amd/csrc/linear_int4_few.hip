@@ -3,8 +3,9 @@
 // Bound: the bytes of the packed weights, each used once per 16 rows of X. They go from memory straight to the registers of the wavefront that multiplies
 // them, in whole kilobytes. A work group owns 16 FB features and 16 rows; its 8 wavefronts take the blocks of 128 contraction elements in turn, each with its
 // next block on its way while it multiplies, and their sums meet in LDS, added in the order of the wavefronts: no result depends on timing, there are
-// no atomics. Measured (rows x contraction x features, groups): 1 x 6144 x 16384, 128, 12.8 us = 4.0 TB/s; 1 x 1152 x 4608,
-// 128, 3.9; 77 x 4608 x 1152, 32, 9.5. (32 and 64 rows to a work group were slower than two and four of them, or than tiles, at every size; so were two blocks on their way.)
+// no atomics. Measured (rows x contraction x features, groups; operands from memory, in parentheses from the last-level cache): 1 x 6144 x 16384, 128, 14.4 us = 3.6 TB/s
+// (12.8); 1 x 1152 x 4608, 64, 5.3; 77 x 4608 x 1152, 32, 11.3 (9.5). (32 and 64 rows to a work group were slower than two and four of them, or than tiles, at every size; so
+// were two blocks on their way.)
 #include "linear_int4.h"
 
 namespace mi {

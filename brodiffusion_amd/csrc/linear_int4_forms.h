@@ -33,7 +33,8 @@ inline constexpr Int4FormRule kInt4Rules[kInt4Forms] = {
 };
 // A launch: its form (-1: none, every grid would have 2^32 work-items across or 2^16 work groups down and more), and the shares that the contraction is given in, each
 // to work groups of its own (1: all in one). Shares cost a second launch, which adds them, and what it reads and writes: kJoin us, fitted with the rest, and 1 us for
-// kJoinBytes of sums, half of what a copy moves, as they are written and read (4096 x 4608 x 1152 in two shares of 64 x 192, 38 MB: 74 + 12 us, in one 72)
+// kJoinBytes of sums, half of what a copy moves, as they are written and read (4096 x 4608 x 1152, operands from memory, groups of 128: in three shares, 57 MB,
+// which the rule would take if sums cost nothing, 78 us, in one 68; groups of 64: 84 and 75)
 struct Int4Launch { int form, shares; };
 constexpr int kInt4Shares[] = {1, 2, 3, 4, 6, 8, 12, 16};
 constexpr long kMostItems = 0xffffffffL;      // work-items of a grid across: 512 for a run of features (few rows), 256 for a tile of a multiple of 8

@@ -12,10 +12,14 @@
 // Bound: what a SIMD issues. 64 tokens x 64 features x 128 elements are 64 products and beside them 112 instructions of the weights, 64 that scale sums and about 60
 // others; a 16 x 16 product takes the issue 12 of its 16 clocks, another vector instruction 4 (measured: one product and 1 to 4 others, two wavefronts, 17, 19.5,
 // 24.4, 27.9 clocks). Tiles of 96 tokens spread the weights' instructions over half as many tokens more. 4608 x 6144 x 16384 bf16 (tokens, contraction, features) takes
-// 0.89 ms, 1.04 PFLOP/s, the matrix pipes busy half of the time; groups of 64 with zero points 1.13 ms. 32 x 32 products leave more room (32.3 clocks with 1, 33.5 with 6
-// others), but their accumulators came out slower at every size (970 us instead of 870 then), and so did wavefronts that take turns at products and weights (890),
-// products, scaling and weights kept apart by scheduling barriers (0 to 3 % slower), and 6-bit conversions of 32 weights at once (as long as 28 instructions); without the
-// sums of x and their barrier it would be 4 % faster, less than a launch that makes the sums ahead costs at most sizes.
+// 0.89 to 0.93 ms from one GPU to the next, 1.0 PFLOP/s, the matrix pipes busy half of the time; groups of 64 with zero points 1.15 ms; this library's 16-bit layer of that size
+// 0.77 to 0.80. It reads 2570 MiB where operands are 105: the tiles that an XCD has at one time are a strip of 96 tokens, and all weights pass for each strip. Few tiles are
+// bound by latency instead: 4096 x 4608 x 1152, groups of 64, 75 to 83 us from memory (the 16-bit layer 57), one round of 64 x 192 with one step in flight, matrix pipes
+// busy 28 %, vector instructions 43 %.
+// Other ways: 32 x 32 products leave more room (32.3 clocks with 1, 33.5 with 6 others), but their accumulators came out slower at every size (970 us instead of 870 then), and
+// so did wavefronts that take turns at products and weights (890), products, scaling and weights kept apart by scheduling barriers (0 to 3 % slower), and 6-bit conversions of
+// 32 weights at once (as long as 28 instructions); without the sums of x and their barrier it would be 4 % faster, less than a launch that makes the sums ahead costs
+// at most sizes. Neither built nor measured: a launch that writes q - z as 16-bit integers, which are exact, for tiles without conversions and sums of x.
 #include <utility>
 
 #include "linear_int4.h"
@@ -330,7 +334,7 @@ template <typename T, int P, bool ZEROS>
 int launch_form(const Int4Problem& p, int form, hipStream_t st) {
     // Stages, wavefronts a SIMD and who sums x, by measurement. 32 tokens, a step is short: 3 stages and own sums (333 x 2240 x 6720, groups of 64: 29 us;
     // 2 stages 33, shared sums 36, 4 stages and 2 wavefronts 36; 128 x 4608 x 4608: 23, 29, 30, 24). More tokens: 2 stages and shared sums, so that three work groups of
-    // 64 x 128 fit a compute unit (4096 x 4608 x 1152: 70 us; two of 3 stages 87 to 94, own sums as many) and two of the others.
+    // 64 x 128 fit a compute unit (4096 x 4608 x 1152 from the last-level cache: 70 us; two of 3 stages 87 to 94, own sums as many) and two of the others.
     switch (form) {
         case kTile32x64: return launch<T, P, ZEROS, 2, 1, 3, 4, true>(p, st);
         case kTile32x128: return launch<T, P, ZEROS, 2, 2, 3, 3, true>(p, st);
