@@ -1142,8 +1142,9 @@ def _rows_of(op: str, t, name: str, dtype, shape=None):
         _fail(op, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dim() < 1 or t.shape[-1] == 0:
         _fail(op, f"{name} must have columns")
-    if t.numel() // t.shape[-1] > 0x7fffffff:      # (a C int, which would take it modulo 2^32)
-        _fail(op, f"{name} has more than 2^31 - 1 rows")
+    for count, what in ((t.numel() // t.shape[-1], "rows"), (t.shape[-1], "columns")):
+        if count > 0x7fffffff:      # (a C int, which would take it modulo 2^32)
+            _fail(op, f"{name} has more than 2^31 - 1 {what}")
     if t.is_contiguous():
         return t.numel() // t.shape[-1], t.shape[-1]
     if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
@@ -1261,7 +1262,7 @@ def gate_add_norm(X, branch, *, gate=None, post: str = "none", post_gain=None, p
     """(h, y): a block's output into the residual stream and the norm in front of the next block (mi_gate_add_norm_forward),
         h = residual_scale * X + gate * post(branch) * post_gain, rounded to X's dtype,   y = norm(h) * gain * (1 + scale) + shift.
     post and norm: "none", "rms" or "layer" (without weights of their own), eps of either (post_eps None: eps). X (..., cols), branch of its shape, or None:
-    h is X. gate, scale and shift: (cols), or one vector for each of X's leading sizes, (batch, cols), (batch, 1, cols) or (batch, tokens, cols) of a
+    h is X; X, branch and the outputs contiguous, or 2-D with any row stride. gate, scale and shift: (cols), or one vector for each of X's leading sizes, (batch, cols), (batch, 1, cols) or (batch, tokens, cols) of a
     (batch, tokens, cols) X; for a 2-D X (items, cols), each for rows / items rows; any row stride that all vectors share (a slice of a
     modulation's columns). norm "none": y is None. sum_out and out may be X or branch."""
     op = "gate_add_norm"
