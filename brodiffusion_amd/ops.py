@@ -1262,9 +1262,9 @@ def gate_add_norm(X, branch, *, gate=None, post: str = "none", post_gain=None, p
     """(h, y): a block's output into the residual stream and the norm in front of the next block (mi_gate_add_norm_forward),
         h = residual_scale * X + gate * post(branch) * post_gain, rounded to X's dtype,   y = norm(h) * gain * (1 + scale) + shift.
     post and norm: "none", "rms" or "layer" (without weights of their own), eps of either (post_eps None: eps). X (..., cols), branch of its shape, or None:
-    h is X; X, branch and the outputs contiguous, or 2-D with any row stride. gate, scale and shift: (cols), or one vector for each of X's leading sizes, (batch, cols), (batch, 1, cols) or (batch, tokens, cols) of a
-    (batch, tokens, cols) X; for a 2-D X (items, cols), each for rows / items rows; any row stride that all vectors share (a slice of a
-    modulation's columns). norm "none": y is None. sum_out and out may be X or branch."""
+    h is X; X, branch and the outputs contiguous, or 2-D with any row stride. gate, scale and shift: (cols), or one vector for each of X's leading sizes,
+    (batch, cols), (batch, 1, cols) or (batch, tokens, cols) of a (batch, tokens, cols) X; for a 2-D X (items, cols), each for rows / items rows; any row stride
+    that all vectors share (a slice of a modulation's columns). norm "none": y is None. sum_out and out may be X or branch."""
     op = "gate_add_norm"
     r = _native.gate_add_norm(X, branch, gate, post, post_gain, post_eps, residual_scale, norm, gain, scale, shift, eps, sum_out, out)
     if r is not None:
